@@ -293,6 +293,76 @@ int qim_attention_noalloc(const void *q, int64_t ldq, const void *k, int64_t ldk
                           void *o, int64_t ldo, int64_t B, int64_t S, int64_t T, int64_t H, int64_t D,
                           float scale, void *stream);
 
+/* A layer's K/V cache in MXFP8.  B sequences hold C positions each: kc, vc are
+ * (B, C, H, D) E4M3 codes, ks, vs (B, C, H, D/32) E8M0 bytes, all contiguous
+ * and 16-byte aligned; D % 32 == 0.  No reference counterpart: the reference
+ * keeps the prefix K/V of cached decode in bf16 (its layer_cache).
+ *
+ * qim_cache_write quantizes K and V rows as they are written: row s of
+ * sequence b goes to position start[b] + s (first + s where start is NULL).
+ * The codes and exponents are those of qim_mx_quantize on the same values.
+ * k, v: (B, S, H, D) bf16, packed heads, with ldkb / ldvb elements between
+ * sequences and ldk / ldv between tokens (multiples of 8, 16-byte aligned).
+ * start, count: device int32 (B,) or NULL; of sequence b the first
+ * count[b] rows are written (all S where count is NULL).  Rows whose position
+ * is outside [0, C) are not written. */
+int qim_cache_write(const void *k, int64_t ldkb, int64_t ldk, const void *v, int64_t ldvb, int64_t ldv,
+                    void *kc, void *ks, void *vc, void *vs, const int32_t *start, int64_t first,
+                    const int32_t *count, int64_t B, int64_t S, int64_t C, int64_t H, int64_t D, void *stream);
+
+/* The bf16 values of positions [0, rows) of every sequence: ok, ov are
+ * (B, rows, H, D), contiguous.  Exact (a code times a power of two). */
+int qim_cache_read(const void *kc, const void *ks, const void *vc, const void *vs, void *ok, void *ov,
+                   int64_t B, int64_t C, int64_t rows, int64_t H, int64_t D, void *stream);
+
+/* qim_qk_norm_rope_pack with its prefix read from such a cache: positions
+ * [0, P) of each sequence, P <= C, in place of ck, cv.  v and ov are required;
+ * D in {64, 128, 256}. */
+int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, const void *kc, const void *ks,
+                                 const void *vc, const void *vs, int64_t C, const void *wq, const void *wk,
+                                 const void *freqs, void *oq, void *ok, void *ov, int64_t B, int64_t S,
+                                 int64_t P, int64_t H, int64_t D, int64_t ldt, float epsq, float epsk,
+                                 void *stream);
+
+/* Attention of a few tokens over such a cache, D = 128: o[b, i, h] =
+ * softmax(q[b, i, h] K[b]^T * scale) V[b] over the keys t < lengths[b] of K/V
+ * head h / (H / HK).  lengths: device int32 (B,), values outside [0, C] count as
+ * the nearest of the two.  tree: NULL, or truth bytes (0 or 1) with tree_b
+ * bytes between sequences (0: shared by all), (S, S) each: of the last
+ * S keys, at lengths[b] - S + j, query i sees only those with
+ * tree[i * S + j] != 0 (drafted tokens: itself and its ancestors).  A row that
+ * sees no key is zeros.  q: (B, S, H, D) bf16, packed heads, ldqb / ldq elements
+ * between sequences / tokens (multiples of 8, 16-byte aligned); o: (B, S, H,
+ * D) contiguous.  1 <= S <= 64, H % HK == 0, scale > 0.  fp32 scores, softmax and
+ * accumulation; the probabilities are rounded to bf16 for the product with V.
+ * workspace: qim_attention_cached_workspace_bytes(B, S, C, H, HK) bytes,
+ * 16-byte aligned (partial results where the keys are split; may be NULL when
+ * that is 0), not shared by calls that may overlap. */
+int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, const void *kc, const void *ks, const void *vc,
+                         const void *vs, const int32_t *lengths, const void *tree, int64_t tree_b, void *o,
+                         void *workspace, int64_t workspace_bytes, int64_t B, int64_t S, int64_t C, int64_t H,
+                         int64_t HK, int64_t D, float scale, void *stream);
+int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK);
+
+/* Low-rank adapters of several requests beside one projection:
+ *   out[m] = bf16(base[m] + scale[a] * up[a] (down[a] x[m])),  a = index[m / seq]
+ * with the products and their sum in fp32.  x: (M, K) bf16, row stride ldx;
+ * down: (A, parts * R, K) and up: (A, N, R) bf16, contiguous; index: device
+ * int32 of ceil(M / seq) entries, a row whose entry is outside [0, A) has no
+ * adapter; scale: device fp32 (A,) or NULL (1).  parts > 1: N is parts equal
+ * column blocks and block j uses rows [j * R, (j + 1) * R) of down (a stacked
+ * Q/K/V projection in one call).  base: (M, N) bf16, row stride ldb, or NULL
+ * (zeros); out: (M, N), row stride ldo; out may be base.  K, R and N / parts are
+ * multiples of 8, R <= 128; all operands 16-byte aligned.  A request's values
+ * never enter another's rows, whatever they are.  workspace:
+ * qim_low_rank_workspace_bytes(M, K, parts * R) bytes, 16-byte aligned, not
+ * shared by calls that may overlap.  No reference counterpart. */
+int qim_low_rank(const void *x, int64_t ldx, const void *down, const void *up, const int32_t *index,
+                 const float *scale, const void *base, int64_t ldb, void *out, int64_t ldo, void *workspace,
+                 int64_t workspace_bytes, int64_t M, int64_t seq, int64_t K, int64_t N, int64_t R, int64_t parts,
+                 int64_t A, void *stream);
+int64_t qim_low_rank_workspace_bytes(int64_t M, int64_t K, int64_t R);
+
 /* Test hooks: the device conversions every kernel uses, applied elementwise
  * (fp32 -> E4M3 code; fp32 -> bf16 bits), and one scaled MFMA
  * (32x32x64, E4M3 x E4M3) on a single tile: a (32, 64) codes, b (32, 64) codes

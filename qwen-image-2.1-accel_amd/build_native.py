@@ -32,12 +32,13 @@ COMMON = [
 ]
 
 
-# Per-source additions.  qim_attention.hip: MFMA accumulators in architectural
+# Per-source additions.  qim_attention.hip and qim_cache_attention.hip: MFMA accumulators in architectural
 #   VGPRs (the "VGPR form"), operands in AGPRs, so the softmax reads the score
 #   tiles and the lazy O rescale multiplies O in place; the accumulation-
 #   register form copies every tile through v_accvgpr_read/write instead.
 EXTRA = {
     "qim_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "qim_cache_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

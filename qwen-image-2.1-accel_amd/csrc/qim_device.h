@@ -122,6 +122,18 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4_bf16(uint32_t ab, uint32_t cd, fl
     return __builtin_bit_cast(uint32_t, r);
 }
 
+// Eight E4M3 codes of a block with exponent e -> the bf16 values they stand
+// for, code * 2^(e - 127), packed.  Exact: 4 significand bits; a block's
+// smallest code step times its scale is below the smallest bf16 only for codes
+// that no bf16 input gives.
+__device__ __forceinline__ uint4 dequantize8(const uint2 &c, int e) {
+    const float s = mx_scale_operand(e);
+    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, s, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, s, true)));
+}
+
 // Byte offset of the E8M0 exponent of (row r, block kb) of a (rows, K) tensor
 // in the 128x4 swizzled layout (kernels/mxfp8.py:53-56).
 __device__ __forceinline__ int64_t mx_scale_offset(int64_t r, int64_t kb, int64_t K) {

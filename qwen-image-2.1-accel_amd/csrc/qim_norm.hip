@@ -457,6 +457,10 @@ struct NormRopeArgs {
     uint32_t groups;     // head groups of one tensor of one token
     uint32_t main_waves; // waves of the norm/rope part: T * tensors * groups
     int64_t main_blocks; // workgroups of the norm/rope part; the rest copy the prefix
+    // A prefix held in MXFP8 (qim_cache.hip) instead of ck, cv: codes and exponents
+    // of C positions per sequence, the first P of which are read.
+    const uint8_t *kc, *ks, *vc, *vs;
+    int64_t C;
 };
 
 // Head rows per lane of one wave: with V 16-byte vectors of a row per lane, a
@@ -602,6 +606,14 @@ __global__ __launch_bounds__(256) void k_norm_rope(NormRopeArgs p) {
         if (row >= B * PH) return;
         const int64_t bb = row / PH, within = row - bb * PH;
         const int64_t dst = (bb * (p.P + p.S) * p.H + within) * D + cc * 8;
+        if (p.kc) {
+            const int64_t at = (bb * p.C * p.H + within) * D + cc * 8;
+            const uint2 kq = *reinterpret_cast<const uint2 *>(p.kc + at), vq = *reinterpret_cast<const uint2 *>(p.vc + at);
+            const int ke = p.ks[at / 32], ve = p.vs[at / 32];
+            *reinterpret_cast<uint4 *>(p.ok + dst) = dequantize8(kq, ke);
+            *reinterpret_cast<uint4 *>(p.ov + dst) = dequantize8(vq, ve);
+            return;
+        }
         *reinterpret_cast<uint4 *>(p.ok + dst) = *reinterpret_cast<const uint4 *>(p.ck + row * D + cc * 8);
         *reinterpret_cast<uint4 *>(p.ov + dst) = *reinterpret_cast<const uint4 *>(p.cv + row * D + cc * 8);
     }
@@ -716,24 +728,44 @@ extern "C" int qim_rope_qk(const void *q, const void *k, const void *freqs, void
     return rc ? rc : check_launch("qim_rope_qk");
 }
 
+// The checks that both forms of the pack share, and the launch.
+static int norm_rope_pack(const char *who, NormRopeArgs a, int64_t B, int64_t D, bool prefix, void *stream) {
+    QIM_REQUIRE(a.q && a.k && a.wq && a.wk && a.freqs && a.oq && a.ok, QIM_ERR_ARG, "%s: null pointer", who);
+    QIM_REQUIRE(B > 0 && a.S > 0 && a.H > 0 && a.P >= 0, QIM_ERR_SHAPE, "%s: empty input", who);
+    QIM_REQUIRE((a.v == nullptr) == (a.ov == nullptr), QIM_ERR_ARG, "%s: v and ov go together", who);
+    QIM_REQUIRE(a.P == 0 || (prefix && a.v), QIM_ERR_ARG, "%s: a prefix (P > 0) needs its K and V, v and ov", who);
+    QIM_REQUIRE(a.ldt >= a.H * D && a.ldt % 8 == 0, QIM_ERR_LAYOUT, "%s: token stride %lld < H*D or not a multiple of 8",
+                who, (long long)a.ldt);
+    const void *ptrs[] = {a.q, a.k, a.v, a.ck, a.cv, a.wq, a.wk, a.freqs, a.oq, a.ok, a.ov, a.kc, a.ks, a.vc, a.vs};
+    for (const void *pp : ptrs)
+        QIM_REQUIRE(!pp || aligned16(pp), QIM_ERR_LAYOUT, "%s: operands must be 16-byte aligned", who);
+    a.T = B * a.S;
+    int rc = a.v ? launch_norm_rope<true, true, 3>(a, D, B, as_stream(stream))
+                 : launch_norm_rope<true, true, 2>(a, D, B, as_stream(stream));
+    return rc ? rc : check_launch(who);
+}
+
 extern "C" int qim_qk_norm_rope_pack(const void *q, const void *k, const void *v, const void *ck, const void *cv,
                                      const void *wq, const void *wk, const void *freqs, void *oq, void *ok,
                                      void *ov, int64_t B, int64_t S, int64_t P, int64_t H, int64_t D, int64_t ldt,
                                      float epsq, float epsk, void *stream) {
-    QIM_REQUIRE(q && k && wq && wk && freqs && oq && ok, QIM_ERR_ARG, "qim_qk_norm_rope_pack: null pointer");
-    QIM_REQUIRE(B > 0 && S > 0 && H > 0 && P >= 0, QIM_ERR_SHAPE, "qim_qk_norm_rope_pack: empty input");
-    QIM_REQUIRE((v == nullptr) == (ov == nullptr), QIM_ERR_ARG, "qim_qk_norm_rope_pack: v and ov go together");
-    QIM_REQUIRE(P == 0 || (ck && cv && v), QIM_ERR_ARG,
-                "qim_qk_norm_rope_pack: a prefix (P > 0) needs ck, cv, v and ov");
-    QIM_REQUIRE(ldt >= H * D && ldt % 8 == 0, QIM_ERR_LAYOUT, "qim_qk_norm_rope_pack: token stride %lld < H*D or not a multiple of 8",
-                (long long)ldt);
-    const void *ptrs[] = {q, k, v, ck, cv, wq, wk, freqs, oq, ok, ov};
-    for (const void *pp : ptrs)
-        QIM_REQUIRE(!pp || aligned16(pp), QIM_ERR_LAYOUT, "qim_qk_norm_rope_pack: operands must be 16-byte aligned");
     NormRopeArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, (const uint16_t *)ck,
                    (const uint16_t *)cv, (const uint16_t *)wq, (const uint16_t *)wk, (const float *)freqs,
-                   (uint16_t *)oq, (uint16_t *)ok, (uint16_t *)ov, B * S, S, P, H, ldt, epsq, epsk, 0, 0, 0};
-    int rc = v ? launch_norm_rope<true, true, 3>(a, D, B, as_stream(stream))
-               : launch_norm_rope<true, true, 2>(a, D, B, as_stream(stream));
-    return rc ? rc : check_launch("qim_qk_norm_rope_pack");
+                   (uint16_t *)oq, (uint16_t *)ok, (uint16_t *)ov, 0, S, P, H, ldt, epsq, epsk, 0, 0, 0};
+    return norm_rope_pack("qim_qk_norm_rope_pack", a, B, D, ck && cv, stream);
+}
+
+extern "C" int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, const void *kc, const void *ks,
+                                            const void *vc, const void *vs, int64_t C, const void *wq, const void *wk,
+                                            const void *freqs, void *oq, void *ok, void *ov, int64_t B, int64_t S,
+                                            int64_t P, int64_t H, int64_t D, int64_t ldt, float epsq, float epsk,
+                                            void *stream) {
+    QIM_REQUIRE(v && kc && ks && vc && vs, QIM_ERR_ARG, "qim_qk_norm_rope_pack_cached: null pointer");
+    QIM_REQUIRE(P <= C, QIM_ERR_ARG, "qim_qk_norm_rope_pack_cached: %lld rows of a cache of %lld", (long long)P,
+                (long long)C);
+    NormRopeArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, nullptr, nullptr,
+                   (const uint16_t *)wq, (const uint16_t *)wk, (const float *)freqs, (uint16_t *)oq, (uint16_t *)ok,
+                   (uint16_t *)ov, 0, S, P, H, ldt, epsq, epsk, 0, 0, 0, (const uint8_t *)kc, (const uint8_t *)ks,
+                   (const uint8_t *)vc, (const uint8_t *)vs, C};
+    return norm_rope_pack("qim_qk_norm_rope_pack_cached", a, B, D, true, stream);
 }

@@ -69,6 +69,13 @@ SIGNATURES = {
     "qim_attention_workspace_bytes": (_I, [_I, _I, _I, _I, _I]),
     "qim_attention_mxfp8": (_C, [_P, _I, _P, _I, _P, _I, _P, _P, _C, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "qim_attention_noalloc": (_C, [_P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "qim_cache_write": (_C, [_P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P] + [_I] * 5 + [_P]),
+    "qim_cache_read": (_C, [_P] * 6 + [_I] * 5 + [_P]),
+    "qim_qk_norm_rope_pack_cached": (_C, [_P] * 7 + [_I] + [_P] * 6 + [_I] * 6 + [_F, _F, _P]),
+    "qim_attention_cached": (_C, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I] + [_I] * 6 + [_F, _P]),
+    "qim_attention_cached_workspace_bytes": (_I, [_I] * 5),
+    "qim_low_rank": (_C, [_P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I] + [_I] * 7 + [_P]),
+    "qim_low_rank_workspace_bytes": (_I, [_I] * 3),
     "qim_debug_e4m3_encode": (_C, [_P, _P, _I, _P]),
     "qim_debug_e4m3_encode_scaled": (_C, [_P, _C, _P, _I, _P]),
     "qim_debug_bf16_round": (_C, [_P, _P, _I, _P]),
@@ -153,6 +160,25 @@ def stream(device=None):
     if _raw_stream is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def call_on(device, name, *args):
+    """``call`` on the current stream of `device` (appended to the arguments),
+    with `device` current: a launch goes to the current device's queues, and
+    the host side reads that device's properties."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args, stream(device))
+    with torch.cuda.device(device):
+        return call(name, *args, stream(device))
+
+
+def bytes_on(device, name, *args):
+    """The value of a workspace-size entry point for a problem on `device`
+    (sizes depend on that device's CU count)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return getattr(lib(), name)(*args)
+    with torch.cuda.device(device):
+        return getattr(lib(), name)(*args)
 
 
 def loaded_hip_runtimes():

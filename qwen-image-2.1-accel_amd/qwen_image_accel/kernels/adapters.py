@@ -1,0 +1,80 @@
+"""Low-rank adapters of several requests beside one shared projection.
+
+``low_rank`` adds scale[a] * up[a] (down[a] x) to a projection's output, with
+the adapter a chosen per sequence or per row, so that one batch serves
+requests with different adapters over one (bf16 or MXFP8) weight.  The
+reference has no adapters; there is no reference counterpart.  Kernels:
+libqim's ``qim_low_rank``.
+"""
+import torch
+
+from qwen_image_accel import _native
+
+MAX_RANK = 128
+
+
+def _rows(t):
+    """(rows, width, row stride) of a (M, W) or (B, S, W) tensor whose rows lie
+    one stride apart, else None.  An axis of one element may have any stride."""
+    if t.dim() not in (2, 3) or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        return None
+    w = t.shape[-1]
+    if t.dim() == 2:
+        return t.shape[0], w, t.stride(0) if t.shape[0] > 1 else w
+    b, s = t.shape[:2]
+    row = t.stride(1) if s > 1 else t.stride(0) if b > 1 else w
+    if b > 1 and s > 1 and t.stride(0) != s * row:
+        return None
+    return b * s, w, row
+
+
+def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
+    """``base + scale[a] * (x @ down[a].T) @ up[a].T`` per row, a = ``index``.
+
+    x: (M, K) or (B, S, K) bf16.  down: (A, parts * R, K) and up: (A, N, R)
+    bf16, R <= 128.  ``index``: int32 on the GPU, (M,) for (M, K), one per row,
+    or (B,) for (B, S, K), one per sequence; a row whose entry is outside
+    [0, A) (-1 by convention) has no adapter.  ``scale``: None or fp32 (A,).
+    ``base``: the projection's output, (M, N) or (B, S, N) bf16, or None
+    (zeros); ``out``: where the result goes (``base`` itself is fine), by default a new tensor.
+    ``parts``: N is that many equal column blocks, and block j uses rows
+    [j * R, (j + 1) * R) of down: the adapters of a stacked projection (Q/K/V,
+    gate/up) in one call.  The sum is taken in fp32 and rounded once.  K, R and
+    N / parts are multiples of 8; rows may lie any multiple of 8 elements apart.
+    A row's result depends on its own x, base and adapter only."""
+    def refuse(why):
+        raise _native.Unsupported("low_rank", _native.QIM_ERR_LAYOUT, why)
+    device = x.device
+    if not x.is_cuda:
+        refuse("expects tensors on the GPU")
+    xr = _rows(x)
+    if x.dtype != torch.bfloat16 or xr is None:
+        refuse("x is a bf16 (M, K) or (B, S, K) tensor with rows one stride apart")
+    m, k, ldx = xr
+    if (down.dim() != 3 or up.dim() != 3 or down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16
+            or not down.is_contiguous() or not up.is_contiguous() or down.device != device or up.device != device
+            or down.shape[0] != up.shape[0] or down.shape[2] != k or parts < 1 or down.shape[1] != parts * up.shape[2]):
+        refuse(f"down (A, {parts} * R, {k}) and up (A, N, R) are contiguous bf16 tensors on {device}")
+    a, n, r = up.shape
+    if (index.dtype != torch.int32 or index.device != device or index.shape != x.shape[:1] or not index.is_contiguous()):
+        refuse(f"index is a contiguous int32 ({x.shape[0]},) tensor on {device}")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (a,) or scale.device != device
+                              or not scale.is_contiguous()):
+        refuse(f"scale is a contiguous fp32 ({a},) tensor on {device}")
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    strides = []
+    for t in (base, out):
+        rows = None if t is None else _rows(t)
+        if t is not None and (t.dtype != torch.bfloat16 or t.shape != shape or t.device != device or rows is None):
+            refuse(f"base and out are bf16 {tuple(shape)} tensors on {device} with rows one stride apart")
+        strides.append(rows[2] if rows else 0)
+    if m == 0 or n == 0:
+        return out
+    nbytes = _native.bytes_on(device, "qim_low_rank_workspace_bytes", m, k, parts * r)
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    _native.call_on(device, "qim_low_rank", x.data_ptr(), ldx, down.data_ptr(), up.data_ptr(), index.data_ptr(),
+                    _native.ptr(scale), _native.ptr(base), strides[0], out.data_ptr(), strides[1], ws.data_ptr(), nbytes,
+                    m, x.shape[1] if x.dim() == 3 else 1, k, n, r, parts, a)
+    return out

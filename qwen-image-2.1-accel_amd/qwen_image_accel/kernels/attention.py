@@ -10,7 +10,7 @@ across calls.
 import torch
 
 from qwen_image_accel import _native
-from qwen_image_accel.kernels import mxfp8
+from qwen_image_accel.kernels import kv_cache, mxfp8
 from qwen_image_accel.kernels.bf16 import HEAD_DIMS
 
 
@@ -20,41 +20,122 @@ def _norm_ok(norm, d, device):
             and w.dtype == torch.bfloat16 and w.device == device and w.is_contiguous())
 
 
-def prepare_attention_inputs(q, k, v, norm_q, norm_k, freqs, cached_k, cached_v):
-    """Return fused Q/K/V, or None when the original operators should be used."""
+def _prepare_layout(q, k, v, norm_q, norm_k, freqs):
+    """(b, s, h, d, token stride) of the step's own operands, or None where the
+    kernel does not take them."""
     if (q.ndim != 4 or q.shape[-1] not in HEAD_DIMS or q.shape[1] == 0
             or k.shape != q.shape or v.shape != q.shape
             or freqs is None or freqs.dtype != torch.complex64
             or freqs.shape != (q.shape[1], q.shape[-1] // 2) or not freqs.is_contiguous()
-            or freqs.device != q.device
-            or cached_k.ndim != 4 or cached_k.shape[0] != q.shape[0]
-            or cached_k.shape[2:] != q.shape[2:] or cached_v.shape != cached_k.shape):
+            or freqs.device != q.device):
         return None
-    for t in (q, k, v, cached_k, cached_v):
-        if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != q.device:
-            return None
-    for t in (cached_k, cached_v):
-        if not t.is_contiguous():
-            return None
     # q, k, v: contiguous, or column blocks of one fused QKV output -- packed
     # heads and one token stride shared by the three (the kernel's ldt).
     b, s, h, d = q.shape
     ldt = q.stride(1)
     for t in (q, k, v):
-        if t.stride() != (s * ldt, ldt, d, 1):
+        if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != q.device or t.stride() != (s * ldt, ldt, d, 1):
             return None
     if not (_norm_ok(norm_q, d, q.device) and _norm_ok(norm_k, d, q.device)):
         return None
-    p = cached_k.shape[1]
+    return b, s, h, d, ldt
+
+
+def _prepare_outputs(q, prefix):
+    b, s, h, d = q.shape
     oq = torch.empty((b, s, h, d), device=q.device, dtype=q.dtype)
-    ok = torch.empty((b, s + p, h, d), device=q.device, dtype=q.dtype)
-    ov = torch.empty_like(ok)
+    ok = torch.empty((b, s + prefix, h, d), device=q.device, dtype=q.dtype)
+    return oq, ok, torch.empty_like(ok)
+
+
+def prepare_attention_inputs(q, k, v, norm_q, norm_k, freqs, cached_k, cached_v):
+    """Return fused Q/K/V, or None when the original operators should be used."""
+    if (q.ndim != 4 or cached_k.ndim != 4 or cached_k.shape[0] != q.shape[0]
+            or cached_k.shape[2:] != q.shape[2:] or cached_v.shape != cached_k.shape):
+        return None
+    for t in (cached_k, cached_v):
+        if t.dtype != torch.bfloat16 or not t.is_cuda or t.device != q.device or not t.is_contiguous():
+            return None
+    layout = _prepare_layout(q, k, v, norm_q, norm_k, freqs)
+    if layout is None:
+        return None
+    b, s, h, d, ldt = layout
+    p = cached_k.shape[1]
+    oq, ok, ov = _prepare_outputs(q, p)
     _native.call("qim_qk_norm_rope_pack", _native.ptr(q), _native.ptr(k), _native.ptr(v),
                  _native.ptr(cached_k) if p else None, _native.ptr(cached_v) if p else None,
                  _native.ptr(norm_q.weight), _native.ptr(norm_k.weight), _native.complex_ptr(freqs),
                  _native.ptr(oq), _native.ptr(ok), _native.ptr(ov), b, s, p, h, d, ldt,
                  float(norm_q.eps), float(norm_k.eps), _native.stream(q.device))
     return oq, ok, ov
+
+
+def prepare_attention_inputs_quantized(q, k, v, norm_q, norm_k, freqs, cache, prefix=None):
+    """``prepare_attention_inputs`` with the prefix in an MXFP8 cache
+    (``kv_cache.QuantizedCache``, of which the first ``prefix`` positions, by
+    default all, are the prefix): its values go in front of k and v as
+    ``kv_cache.read_cache`` gives them, without that copy.  None where the
+    kernel does not take the step's own operands."""
+    b, c, h, d = kv_cache.check_cache("prepare_attention_inputs_quantized", cache)
+    p = c if prefix is None else int(prefix)
+    if not 0 <= p <= c:
+        raise ValueError(f"a prefix of {p} in a cache of {c} positions")
+    layout = _prepare_layout(q, k, v, norm_q, norm_k, freqs)
+    if layout is None or cache.k.device != q.device or (b, h, d) != (layout[0], layout[2], layout[3]):
+        return None
+    s, ldt = layout[1], layout[4]
+    oq, ok, ov = _prepare_outputs(q, p)
+    _native.call_on(q.device, "qim_qk_norm_rope_pack_cached", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                    cache.k.data_ptr(), cache.k_exponent.data_ptr(), cache.v.data_ptr(), cache.v_exponent.data_ptr(), c,
+                    norm_q.weight.data_ptr(), norm_k.weight.data_ptr(), _native.complex_ptr(freqs), oq.data_ptr(),
+                    ok.data_ptr(), ov.data_ptr(), b, s, p, h, d, ldt, float(norm_q.eps), float(norm_k.eps))
+    return oq, ok, ov
+
+
+def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
+    """softmax(q K^T * scale) V of a few tokens over an MXFP8 cache, read in
+    place: libqim's ``qim_attention_cached``.
+
+    q: (B, S, H, 128) bf16, S <= 64, packed heads, any token and batch
+    stride; ``cache``: B sequences of C positions with HK heads, H a
+    multiple of HK (query head h reads K/V head h // (H // HK)).  ``lengths``:
+    int32 (B,) device tensor, the keys of each sequence, its own S tokens
+    among them when they attend to themselves (write them with
+    ``kv_cache.write_cache`` first); values outside [0, C] count as the nearest
+    of the two.  ``tree``: None (every key is seen), or bool (B, S, S) or
+    (S, S): of the last S keys, query i sees key j only where tree[..., i, j]
+    (drafted tokens: itself and its ancestors; a causal step: the lower
+    triangle).  A row that sees no key is zeros.  scale defaults to
+    1/sqrt(128).  Returns (B, S, H, 128) bf16.  For the queries of a whole image,
+    stage the prefix (``prepare_attention_inputs_quantized``) and use
+    ``attention``."""
+    b, c, kv, d = kv_cache.check_cache("attention_cached", cache)
+    device = cache.k.device
+    if (q.dim() != 4 or q.dtype != torch.bfloat16 or q.device != device or q.shape[0] != b or q.shape[3] != d
+            or kv_cache.token_strides(q) is None):
+        raise _native.Unsupported("attention_cached", _native.QIM_ERR_LAYOUT,
+                                  f"q is a bf16 ({b}, S, H, {d}) tensor with packed heads on {device}")
+    s, h = q.shape[1], q.shape[2]
+    size = kv_cache.per_sequence("attention_cached", "lengths", lengths, b, device)
+    mask, mask_b = None, 0
+    if tree is not None:
+        if tree.dtype != torch.bool or tree.device != device or tree.shape not in ((s, s), (b, s, s)) or not tree.is_contiguous():
+            raise _native.Unsupported("attention_cached", _native.QIM_ERR_LAYOUT,
+                                      f"tree is a contiguous bool ({b}, {s}, {s}) or ({s}, {s}) tensor on {device}")
+        mask, mask_b = tree.data_ptr(), s * s if tree.dim() == 3 else 0
+    if out is None:
+        out = torch.empty((b, s, h, d), dtype=torch.bfloat16, device=device)
+    elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} tensor on {device}")
+    if out.numel() == 0:
+        return out
+    nbytes = _native.bytes_on(device, "qim_attention_cached_workspace_bytes", b, s, c, h, kv)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _native.call_on(device, "qim_attention_cached", q.data_ptr(), *kv_cache.token_strides(q), cache.k.data_ptr(),
+                    cache.k_exponent.data_ptr(), cache.v.data_ptr(), cache.v_exponent.data_ptr(), size, mask, mask_b,
+                    out.data_ptr(), _native.ptr(ws), nbytes, b, s, c, h, kv, d,
+                    float(scale if scale is not None else d ** -0.5))
+    return out
 
 
 def workspace(b, s, t, h, device, d=128):

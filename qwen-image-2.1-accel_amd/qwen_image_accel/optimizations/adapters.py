@@ -1,0 +1,178 @@
+"""Low-rank adapters on the block linears, chosen per request.
+
+``install_adapters`` puts any number of named adapters beside the (bf16 or
+MXFP8) linears of a transformer, after ``install_hot_path``; each batch then
+names the adapter of every sequence with ``AdapterRoute.select``, so that one
+model serves requests with different adapters (or none) together, without
+merging weights.  The reference has no adapters; there is no reference
+counterpart.
+"""
+import torch
+from torch import nn
+
+from qwen_image_accel.kernels.adapters import MAX_RANK, low_rank
+from qwen_image_accel.optimizations.mxfp8 import LAYER_GROUPS, MXFP8Linear
+from qwen_image_accel.weights import ADAPTED_BASE
+
+NO_ADAPTER = -1
+
+
+class AdapterRoute:
+    """Which adapter each sequence of the batch uses: ``index``, int32 (B,), an
+    adapter's number or -1, or None while nothing is selected (no adapter
+    anywhere).  The tensor keeps its place from one ``select`` of the same
+    batch size to the next, so a captured step follows the selection."""
+
+    def __init__(self, names, device):
+        self.names, self.device, self.index = tuple(names), torch.device(device), None
+
+    def select(self, names):
+        """``names``: one adapter name (or None) per sequence of the batch;
+        or None to switch the adapters off."""
+        if names is None:
+            self.index = None
+            return
+        numbers = []
+        for name in names:
+            if name is not None and name not in self.names:
+                raise ValueError(f"unknown adapter {name!r}; installed: {list(self.names)}")
+            numbers.append(NO_ADAPTER if name is None else self.names.index(name))
+        new = torch.tensor(numbers, dtype=torch.int32, device=self.device)
+        if self.index is not None and self.index.shape == new.shape:
+            self.index.copy_(new)
+        else:
+            self.index = new
+
+
+class AdapterStack(nn.Module):
+    """The adapters of one projection, stacked: down (A, parts * R, K), up (A, N,
+    R), scale (A,).  An adapter of a smaller rank is padded with zeros, one that
+    does not touch this projection is zeros with scale 0."""
+
+    def __init__(self, down, up, scale, parts=1):
+        super().__init__()
+        self.parts = parts
+        self.register_buffer("down", down, persistent=False)
+        self.register_buffer("up", up, persistent=False)
+        self.register_buffer("scale", scale, persistent=False)
+
+    @classmethod
+    def of(cls, triples, out_features, in_features, device):
+        """``triples``: per adapter (down (r, K), up (N, r), scale) or None."""
+        ranks = [t[0].shape[0] for t in triples if t is not None]
+        r = (max(ranks) + 7) // 8 * 8
+        if r > MAX_RANK:
+            raise ValueError(f"adapter rank {max(ranks)} is above {MAX_RANK}")
+        down = torch.zeros(len(triples), r, in_features, dtype=torch.bfloat16, device=device)
+        up = torch.zeros(len(triples), out_features, r, dtype=torch.bfloat16, device=device)
+        scale = torch.zeros(len(triples), dtype=torch.float32, device=device)
+        for i, t in enumerate(triples):
+            if t is None:
+                continue
+            d, u, s = t
+            if d.dim() != 2 or u.dim() != 2 or d.shape[1] != in_features or u.shape != (out_features, d.shape[0]):
+                raise ValueError(f"adapter of shapes {tuple(d.shape)}, {tuple(u.shape)} beside a "
+                                 f"({out_features}, {in_features}) linear")
+            down[i, :d.shape[0]] = d.to(device=device, dtype=torch.bfloat16)
+            up[i, :, :d.shape[0]] = u.to(device=device, dtype=torch.bfloat16)
+            scale[i] = float(s)
+        return cls(down, up, scale)
+
+    def add(self, x, y, index):
+        """y (B, S, N) + the adapters' share of x (B, S, K); y is overwritten on the GPU."""
+        if x.dim() != 3 or x.shape[0] != index.shape[0]:
+            raise ValueError(f"the route names {index.shape[0]} sequences, the batch is {tuple(x.shape)}")
+        if x.is_cuda and x.dtype == torch.bfloat16 and y.dtype == torch.bfloat16:
+            return low_rank(x, self.down, self.up, index, scale=self.scale, base=y, out=y, parts=self.parts)
+        out, r = y.float(), self.up.shape[2]
+        for i, a in enumerate(index.tolist()):
+            if a >= 0:
+                h = (x[i].float() @ self.down[a].float().t()).unflatten(-1, (self.parts, r))
+                up = self.up[a].float().unflatten(0, (self.parts, -1))
+                out[i] += self.scale[a] * torch.einsum("spr,pnr->spn", h, up).flatten(1)
+        return out.to(y.dtype)
+
+
+class AdaptedLinear(nn.Module):
+    """A linear (nn.Linear or MXFP8Linear) with adapters beside it."""
+
+    def __init__(self, base, stack, route):
+        super().__init__()
+        self.add_module(ADAPTED_BASE, base)
+        self.stack, self.route = stack, route
+        self.in_features, self.out_features = base.in_features, base.out_features
+
+    @property
+    def base(self):
+        return getattr(self, ADAPTED_BASE)
+
+    def forward(self, x):
+        y = self.base(x)
+        return y if self.route.index is None else self.stack.add(x, y, self.route.index)
+
+
+def _stacked_qkv(linears):
+    """One AdapterStack over the stacked Q/K/V projection, or None where the
+    three do not stack."""
+    if not all(isinstance(m, AdaptedLinear) and isinstance(m.base, MXFP8Linear) for m in linears):
+        return None
+    stacks = [m.stack for m in linears]
+    if len({s.up.shape for s in stacks}) != 1 or not all(torch.equal(s.scale, stacks[0].scale) for s in stacks):
+        return None
+    return AdapterStack(torch.cat([s.down for s in stacks], 1), torch.cat([s.up for s in stacks], 1), stacks[0].scale,
+                        parts=3)
+
+
+def install_adapters(transformer, adapters):
+    """Put named adapters beside the block linears, once, after
+    ``install_hot_path``.
+
+    ``adapters``: {name: {path: (down (r, K), up (N, r), scale)}}, ``path`` as
+    ``quantize_transformer`` returns them ("transformer_blocks.<i>.attn.to_q";
+    any of LAYER_GROUPS["all"]), scale the factor on up @ down (alpha / rank).
+    Ranks up to 128 may differ.  Returns the ``AdapterRoute``; until its
+    ``select`` names adapters the model runs without them."""
+    if getattr(transformer, "_qw_adapters", None) is not None:
+        raise RuntimeError("adapters are installed once per transformer; remove_adapters first")
+    if not adapters:
+        raise ValueError("no adapters given")
+    names = list(adapters)
+    blocks = transformer.transformer_blocks
+    known = {f"transformer_blocks.{i}.{p}": (i, p) for i in range(len(blocks)) for p in LAYER_GROUPS["all"]}
+    paths = sorted({p for a in adapters.values() for p in a})
+    unknown = [p for p in paths if p not in known]
+    if unknown:
+        raise ValueError(f"adapters for unknown linears {unknown}")
+    plan, route = [], None
+    for path in paths:  # everything is checked before anything is replaced
+        block, rel = blocks[known[path][0]], known[path][1]
+        base = block.get_submodule(rel)
+        if not isinstance(base, (nn.Linear, MXFP8Linear)):
+            raise ValueError(f"{path} is a {type(base).__name__}, not a linear")
+        device = base.weight_tiled.device if isinstance(base, MXFP8Linear) else base.weight.device
+        route = route or AdapterRoute(names, device)
+        stack = AdapterStack.of([adapters[n].get(path) for n in names], base.out_features, base.in_features, device)
+        plan.append((block, rel, AdaptedLinear(base, stack, route)))
+    for block, rel, module in plan:
+        parent, _, leaf = rel.rpartition(".")
+        setattr(block.get_submodule(parent), leaf, module)
+    for block in blocks:
+        attn = block.attn
+        attn._adapter_qkv = _stacked_qkv((attn.to_q, attn.to_k, attn.to_v))
+    transformer._qw_adapters = route
+    return route
+
+
+def remove_adapters(transformer):
+    """Undo ``install_adapters``."""
+    for block in transformer.transformer_blocks:
+        for rel in LAYER_GROUPS["all"]:
+            m = block.get_submodule(rel)
+            if isinstance(m, AdaptedLinear):
+                parent, _, leaf = rel.rpartition(".")
+                setattr(block.get_submodule(parent), leaf, m.base)
+        block.attn._adapter_qkv = None
+    transformer._qw_adapters = None
+
+
+__all__ = ["AdapterRoute", "AdapterStack", "AdaptedLinear", "install_adapters", "remove_adapters"]

@@ -16,8 +16,9 @@ stacked Q/K/V and interleaved gate/up weights were built):
                                                 consumer is MXFP8 (one shared activation)
     qkv        to_q / to_k / to_v               one stacked GEMM, or three GEMMs on the
                                                 shared activation
-    prepare    prepare_attention_inputs (fused RMSNorm + RoPE + prefix pack), else the
-               eager RMSNorm, RoPE and concatenation
+    prepare    prepare_attention_inputs (fused RMSNorm + RoPE + prefix pack; its
+               _quantized form for an MXFP8 prefix, prefix_cache.QuantizedLayerCache),
+               else the eager RMSNorm, RoPE and concatenation
     attention  Diffusers' dispatch, or this build's core (QW21_ATTENTION_BACKEND=qim),
                which also writes an MXFP8 out-projection's input
     mlp        img_mlp (SwiGLU hook)            gate/up GEMM with the SwiGLU -> MXFP8
@@ -29,7 +30,8 @@ forward and the attention processor it replaced.
 """
 import torch
 
-from qwen_image_accel.kernels.attention import attention_mxfp8, prepare_attention_inputs
+from qwen_image_accel.kernels.attention import (attention_mxfp8, prepare_attention_inputs,
+                                                prepare_attention_inputs_quantized)
 from qwen_image_accel.kernels.bf16 import swiglu
 from qwen_image_accel.kernels.elementwise import residual, rope_qk
 from qwen_image_accel.kernels.epilogue import layer_norm_scale_quantize, swiglu_quantize
@@ -38,6 +40,7 @@ from qwen_image_accel.kernels.layernorm import layer_norm_scale
 from qwen_image_accel.kernels.mxfp8 import Quantized, quantize
 from qwen_image_accel.optimizations.attention_call import attention, qim_backend
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
+from qwen_image_accel.optimizations.prefix_cache import QuantizedLayerCache
 from qwen_image_accel.weights import fuse_gate_up, fuse_qkv
 
 # Keyword arguments of a block call that the attention module does not take.
@@ -85,6 +88,9 @@ def project_qkv(attn, x, quantized):
     linears = (attn.to_q, attn.to_k, attn.to_v)
     shared = shared_activation(x, linears) if quantized else None
     if shared is None:
+        adapted = _adapted_qkv(attn, x) if quantized else None
+        if adapted is not None:
+            return adapted
         return tuple(p(x).unflatten(-1, (attn.heads, -1)) for p in linears)
     lead = shared.shape[:-1]
     stacked = getattr(attn, "_mx_qkv", None)
@@ -93,6 +99,20 @@ def project_qkv(attn, x, quantized):
     # One GEMM over the stacked weight; q, k, v are column blocks of its output
     # (one token stride), which the fused norm + RoPE + pack reads in place.
     return mx_matmul(shared, *stacked, weight_tiled=True).view(*lead, 3, attn.heads, -1).unbind(-3)
+
+
+def _adapted_qkv(attn, x):
+    """Q, K, V of MXFP8 projections with adapters beside all three
+    (optimizations/adapters.py): the stacked GEMM on x quantized once, and the
+    three adapters in one call on its output.  None where that does not apply."""
+    adapters, stacked = getattr(attn, "_adapter_qkv", None), getattr(attn, "_mx_qkv", None)
+    if adapters is None or stacked is None or x.dim() != 3 or not x.is_contiguous():
+        return None
+    index = attn.to_q.route.index
+    y = mx_matmul(quantize(x.reshape(-1, x.shape[-1]), tiled=True), *stacked, weight_tiled=True).view(*x.shape[:2], -1)
+    if index is not None:
+        y = adapters.add(x, y, index)
+    return y.unflatten(-1, (3, attn.heads, -1)).unbind(-3)
 
 
 def _eager_rope(q, k, freqs):
@@ -107,6 +127,10 @@ def _eager_rope(q, k, freqs):
 
 def attention_inputs(attn, q, k, v, freqs, layer_cache):
     """Q/K RMSNorm + RoPE, and the cached prefix K/V in front of k and v."""
+    if isinstance(layer_cache, QuantizedLayerCache):
+        fused = prepare_attention_inputs_quantized(q, k, v, attn.norm_q, attn.norm_k, freqs, layer_cache.quantized)
+        if fused is not None:
+            return fused
     prefix_k, prefix_v = layer_cache.get()
     fused = prepare_attention_inputs(q, k, v, attn.norm_q, attn.norm_k, freqs, prefix_k, prefix_v)
     if fused is not None:

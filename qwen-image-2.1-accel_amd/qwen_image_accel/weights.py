@@ -100,6 +100,10 @@ def fuse_qkv(attn):
 
 _FUSED = ("_mx_gate_up", "_mx_qkv")
 
+# The name under which a linear with adapters beside it holds the linear
+# (optimizations/adapters.py); it is no part of a saved path.
+ADAPTED_BASE = "shared_linear"
+
 
 def _modules(transformer):
     """(path, module) over the DiT blocks, paths as quantize_transformer names
@@ -122,12 +126,14 @@ def _set(transformer, path, module):
 
 def save_mxfp8(transformer, path):
     """Write every ``MXFP8Linear`` of ``transformer`` (tiled codes, scales,
-    bias) and every interleaved gate/up weight to a safetensors file."""
+    bias) and every interleaved gate/up weight to a safetensors file.  Adapters
+    installed beside them are not written."""
     from safetensors.torch import save_file
     tensors, layers, fused = {}, {}, []
     for name, m in _modules(transformer):
         if not isinstance(m, MXFP8Linear):
             continue
+        name = name.removesuffix("." + ADAPTED_BASE)
         tensors[f"{name}.codes"] = m.weight_tiled.view(torch.uint8).cpu().contiguous()
         tensors[f"{name}.scales"] = m.weight_scale.view(torch.uint8).cpu().contiguous()
         if m.bias is not None:
