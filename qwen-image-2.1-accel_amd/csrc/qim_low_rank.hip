@@ -33,171 +33,352 @@ struct LowRankArgs {
     const float *scale;
     uint16_t *out;
     float *h;  // (chunks, M, PR)
-    int64_t ldx, ldb, ldo, M, seq;
+    int64_t ldx, ldb, ldo, M;
+    uint32_t seq;
     int K, N, R, PR, parts, A;
     int chunks, kchunk;  // K chunks of kchunk values
-    int ncols;           // columns of a block of `out` per workgroup (k_lr_up)
-    int nchunk;          // workgroups per part
+    int ncols, nchunk;   // k_lr_up: columns of a part per wave; workgroups per part
 };
 
 // The adapter of row m, -1 for none.
 __device__ __forceinline__ int lr_adapter(const LowRankArgs &p, int64_t m) {
     if (m >= p.M) return -1;
-    const int a = p.index[p.seq == 1 ? m : m / p.seq];
+    const int a = p.index[p.seq == 1 ? (uint32_t)m : (uint32_t)m / p.seq];
     return a >= 0 && a < p.A ? a : -1;
 }
 
-// Calls f(a) for each distinct adapter a >= 0 among the lanes' values.
-template <class F>
-__device__ __forceinline__ void lr_each(int mine, F &&f) {
-    uint64_t todo = __builtin_amdgcn_ballot_w64(mine >= 0);
-    while (todo) {
-        const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(todo));
-        f(a);
-        todo &= ~__builtin_amdgcn_ballot_w64(mine == a);
+// Calls f(a) for each distinct adapter a >= 0 among the rows of MT tiles whose
+// rank in that order is `slot` modulo `slots`.
+template <int MT, class F>
+__device__ __forceinline__ void lr_each(const int (&mine)[MT], int slot, int slots, F &&f) {
+    uint64_t todo[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) todo[t] = __builtin_amdgcn_ballot_w64(mine[t] >= 0);
+    int rank = slot;
+    for (;;) {
+        int a = -1;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            if (a < 0 && todo[t]) a = __builtin_amdgcn_readlane(mine[t], (int)__builtin_ctzll(todo[t]));
+        if (a < 0) return;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) todo[t] &= ~__builtin_amdgcn_ballot_w64(mine[t] == a);
+        if (rank == 0) f(a);
+        rank = rank == 0 ? slots - 1 : rank - 1;
     }
 }
 
-// h of one 16-row tile, one K chunk and 16 * RT rows of down: the 4 waves take
-// 32-value steps of the chunk in turn and join in LDS.
-template <int RT>
-__global__ __launch_bounds__(256) void k_lr_down(LowRankArgs p) {
-    __shared__ f32x4_t sum[4][RT][64];
+// h of 16 * MT rows, one K chunk and 16 * RT rows of down.  The 8 waves take
+// steps of 32 * S values of the chunk in turn (S = 2: whole 128-byte lines of x;
+// 1 where RT = 8 leaves no registers), with the next step's loads in flight,
+// and join in LDS.
+constexpr int LR_WAVES = 8;
+template <int RT, int MT>
+__global__ __launch_bounds__(64 * LR_WAVES, 2) void k_lr_down(LowRankArgs p, int rblocks) {
+    constexpr int S = RT == 8 ? 1 : 2;
+    extern __shared__ f32x4_t sum[];  // [LR_WAVES][MT][RT][64]
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t m = (int64_t)blockIdx.x * 16 + lr;
-    const int r0 = blockIdx.z * (16 * RT);
-    const int mine = lr_adapter(p, m);
-    const int64_t mc = m < p.M ? m : p.M - 1;
-    const int k0 = blockIdx.y * p.kchunk, k1 = k0 + p.kchunk < p.K ? k0 + p.kchunk : p.K;
-    const uint16_t *xr = p.x + mc * p.ldx;
-    f32x4_t keep[RT] = {};
-    lr_each(mine, [&](int a) {
-        f32x4_t acc[RT] = {};
-        const uint16_t *dn = p.down + (int64_t)a * p.PR * p.K;
-        for (int k = k0 + 32 * wave + 8 * kg; k - 8 * kg < k1; k += 128) {
-            const bool in = k < k1;
-            const u32x4_t zero = {0, 0, 0, 0};
-            const u32x4_t xv = in ? *reinterpret_cast<const u32x4_t *>(xr + k) : zero;
+    // Neighbouring workgroups take neighbouring chunks of the same rows: what is
+    // in flight covers whole rows.
+    const uint32_t tile = blockIdx.x / (uint32_t)p.chunks, chunk = blockIdx.x - tile * p.chunks;
+    const int64_t m0 = (int64_t)tile * (16 * MT);
+    const int slot = blockIdx.y / rblocks, slots = gridDim.y / rblocks, r0 = (blockIdx.y - slot * rblocks) * (16 * RT);
+    int mine[MT];
+    const uint16_t *xr[MT];
+    uint64_t done[MT];  // the lanes whose rows this workgroup computes
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                int r = r0 + 16 * t + lr;
-                r = r < p.PR ? r : p.PR - 1;
-                const u32x4_t dv = in ? *reinterpret_cast<const u32x4_t *>(dn + (int64_t)r * p.K + k) : zero;
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, dv), __builtin_bit_cast(bf16x8_t, xv),
-                                                                 acc[t], 0, 0, 0);
+    for (int t = 0; t < MT; ++t) {
+        const int64_t m = m0 + 16 * t + lr;
+        mine[t] = lr_adapter(p, m);
+        xr[t] = p.x + (m < p.M ? m : p.M - 1) * p.ldx + 8 * kg;
+        done[t] = 0;
+    }
+    const int k0 = chunk * p.kchunk, k1 = k0 + p.kchunk < p.K ? k0 + p.kchunk : p.K;
+    lr_each<MT>(mine, slot, slots, [&](int a) {
+        const uint16_t *dn[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            int row = r0 + 16 * r + lr;
+            row = row < p.PR ? row : p.PR - 1;
+            dn[r] = p.down + ((int64_t)a * p.PR + row) * p.K + 8 * kg;
+        }
+        f32x4_t acc[MT][RT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[t][r] = f32x4_t{};
+        u32x4_t xc[MT][S], dc[RT][S], xn[MT][S], dnx[RT][S];
+        auto load = [&](int k, u32x4_t (&xv)[MT][S], u32x4_t (&dv)[RT][S]) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const bool in = k + 32 * s + 8 * kg < k1;  // K % 8 == 0: 8 values are all in or all out
+                const u32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < MT; ++t) xv[t][s] = in ? *reinterpret_cast<const u32x4_t *>(xr[t] + k + 32 * s) : zero;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) dv[r][s] = in ? *reinterpret_cast<const u32x4_t *>(dn[r] + k + 32 * s) : zero;
+            }
+        };
+        int k = k0 + 32 * S * wave;
+        load(k, xc, dc);
+        for (; k < k1; k += 32 * S * LR_WAVES) {
+            if (k + 32 * S * LR_WAVES < k1) load(k + 32 * S * LR_WAVES, xn, dnx);
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int r = 0; r < RT; ++r)
+                        acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, dc[r][s]),
+                                                                            __builtin_bit_cast(bf16x8_t, xc[t][s]), acc[t][r], 0, 0, 0);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) xc[t][s] = xn[t][s];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) dc[r][s] = dnx[r][s];
             }
         }
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < MT; ++t) {
+            done[t] |= __builtin_amdgcn_ballot_w64(mine[t] == a);
+            if (mine[t] == a) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) keep[t][i] = mine == a ? acc[t][i] : keep[t][i];
+                for (int r = 0; r < RT; ++r) sum[((wave * MT + t) * RT + r) * 64 + lane] = acc[t][r];
+            }
+        }
     });
-#pragma unroll
-    for (int t = 0; t < RT; ++t) sum[wave][t][lane] = keep[t];
     __syncthreads();
-    for (int i = tid; i < RT * 64; i += 256) {
-        const int t = i >> 6, l = i & 63;
-        const f32x4_t s = (sum[0][t][l] + sum[1][t][l]) + (sum[2][t][l] + sum[3][t][l]);
+    for (int i = tid; i < MT * RT * 64; i += 64 * LR_WAVES) {
+        const int t = i / (RT * 64), r = (i >> 6) % RT, l = i & 63;
+        f32x4_t s = sum[i];
+#pragma unroll
+        for (int w = 1; w < LR_WAVES; ++w) s += sum[w * (MT * RT * 64) + i];
         // Lane l of the tile: row l % 16, values 4 (l / 16) .. + 3 of its 16.
-        const int64_t row = (int64_t)blockIdx.x * 16 + (l & 15);
-        const int r = r0 + 16 * t + 4 * (l >> 4);
-        if (row < p.M && r < p.PR)
-            *reinterpret_cast<f32x4_t *>(p.h + ((int64_t)blockIdx.y * p.M + row) * p.PR + r) = s;
+        const int row = 16 * t + (l & 15), col = r0 + 16 * r + 4 * (l >> 4);
+        uint64_t rows = done[0];
+#pragma unroll
+        for (int u = 1; u < MT; ++u) rows = t == u ? done[u] : rows;
+        if (((rows >> l) & 1) && col < p.PR)
+            *reinterpret_cast<f32x4_t *>(p.h + ((int64_t)chunk * p.M + m0 + row) * p.PR + col) = s;
     }
 }
 
-// Columns [c0, c0 + ncols) of one part, 16 rows per wave (the workgroup's 4
-// waves take neighbouring rows).  STEPS * 32 operand slots: chunks of 8 of hi, then of
-// lo.  Two MFMA tiles at a time, whose rows are assigned to columns so that a
-// lane's 8 results are 8 neighbouring columns: row i of tile t is column
-// 8 (i / 4) + 4 t + i % 4.
-template <int STEPS>
-__global__ __launch_bounds__(256) void k_lr_up(LowRankArgs p) {
+// 32 rows x 4 * ncols columns of one part: the workgroup sums the K chunks of its
+// rows' h once, into LDS, as MFMA operands; each wave takes 64 columns at a
+// time, with its next 64 columns of base in flight.  SP =
+// ceil(R / 32) operand steps of hi and as many of lo; with PACK (R <= 16) one step holds
+// both (slots of 8: hi, hi, lo, lo).  A tile's 16 result rows are assigned to
+// columns so that a lane's results of two tiles are 8 neighbouring
+// columns: row i of tile t of a pair is column 8 (i / 4) + 4 t + i % 4.
+constexpr int LR_MT = 2;
+template <int SP, bool PACK>
+__global__ __launch_bounds__(256, SP == 4 ? 2 : 3) void k_lr_up(LowRankArgs p) {
+    constexpr int OPS = PACK ? 1 : 2 * SP;
+    __shared__ u32x4_t hs[LR_MT][OPS][64];
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t m = ((int64_t)blockIdx.x * 4 + wave) * 16 + lr;
-    const int part = blockIdx.y / p.nchunk, width = p.N / p.parts;
-    const int c0 = (blockIdx.y - part * p.nchunk) * p.ncols, c1 = c0 + p.ncols < width ? c0 + p.ncols : width;
-    const int mine = lr_adapter(p, m);
-    const float sc = mine >= 0 ? (p.scale ? p.scale[mine] : 1.0f) : 0.0f;
+    // Neighbouring workgroups take neighbouring columns of the same rows, and the
+    // four waves neighbouring 64-column steps: what is in flight covers whole rows.
+    const uint32_t cols = (uint32_t)(p.nchunk * p.parts), tile = blockIdx.x / cols, cb = blockIdx.x - tile * cols;
+    const int64_t m0 = (int64_t)tile * (16 * LR_MT);
+    const int part = cb / p.nchunk, width = p.N / p.parts;
     const int rc = p.R / 8;  // chunks of 8
-    bf16x8_t hop[STEPS];
+    const int g0 = (cb - part * p.nchunk) * 4 * p.ncols;
+    const int c0 = g0 + 64 * wave, c1 = g0 + 4 * p.ncols < width ? g0 + 4 * p.ncols : width;
+    const int64_t n0 = (int64_t)part * width;
+    // Base columns c .. c + 63.
+    auto load_base = [&](int c, uint4 (&y)[LR_MT][2]) {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        const int ch = 4 * s + kg;
-        float f[8] = {};
-        if (ch < 2 * rc && mine >= 0) {
-            const float *src = p.h + m * p.PR + part * p.R + (ch < rc ? ch : ch - rc) * 8;
-            for (int c = 0; c < p.chunks; ++c) {
-                const f32x4_t a = *reinterpret_cast<const f32x4_t *>(src), b = *reinterpret_cast<const f32x4_t *>(src + 4);
+        for (int t = 0; t < LR_MT; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[e] += a[e];
-                    f[4 + e] += b[e];
+            for (int g = 0; g < 2; ++g) {
+                const int64_t m = m0 + 16 * t + lr;
+                const int col = c + 32 * g + 8 * kg;
+                y[t][g] = make_uint4(0, 0, 0, 0);
+                if (p.base && m < p.M && col < c1) y[t][g] = *reinterpret_cast<const uint4 *>(p.base + m * p.ldb + n0 + col);
+            }
+    };
+    int mine[LR_MT];
+#pragma unroll
+    for (int t = 0; t < LR_MT; ++t) mine[t] = lr_adapter(p, m0 + 16 * t + lr);
+    uint4 yc[LR_MT][2];
+    load_base(c0, yc);  // in flight while h is fetched
+    bool again = false;
+    // h of the workgroup's rows.
+    for (int i = tid; i < LR_MT * SP * 64; i += 256) {
+        const int t = i / (SP * 64), s = (i >> 6) % SP, l = i & 63;
+        const int64_t m = m0 + 16 * t + (l & 15);
+        const int ch = PACK ? (l >> 4) & 1 : 4 * s + (l >> 4);
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, lo[8];
+        if (ch < rc && m < p.M) {  // of a row without an adapter: never written, and its results are not used
+            const float *src = p.h + m * p.PR + part * p.R + ch * 8;
+            for (int c = 0; c < p.chunks; c += 4) {  // four chunks' loads at a time
+                f32x4_t a[4], b[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4_t *at = reinterpret_cast<const f32x4_t *>(src + (c + j < p.chunks ? j : 0) * p.M * p.PR);
+                    a[j] = at[0];
+                    b[j] = at[1];
                 }
-                src += p.M * p.PR;
-            }
-        }
-        if (ch >= rc) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float hi = rbf(f[e]);
-                f[e] = __builtin_isfinite(hi) ? f[e] - hi : 0.0f;
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        f[e] += c + j < p.chunks ? a[j][e] : 0.f;
+                        f[4 + e] += c + j < p.chunks ? b[j][e] : 0.f;
+                    }
+                src += 4 * p.M * p.PR;
             }
         }
-        hop[s] = __builtin_bit_cast(bf16x8_t, pack8(f));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float hi = rbf(f[e]);
+            lo[e] = __builtin_isfinite(hi) ? f[e] - hi : 0.0f;
+        }
+        const uint4 uh = pack8(f), ul = pack8(lo);
+        const u32x4_t vh = {uh.x, uh.y, uh.z, uh.w}, vl = {ul.x, ul.y, ul.z, ul.w};
+        if (PACK) {
+            hs[t][0][l] = l < 32 ? vh : vl;
+        } else {
+            hs[t][s][l] = vh;
+            hs[t][OPS / 2 + s][l] = vl;
+        }
     }
-    for (int c = c0; c < c1; c += 32) {
-        f32x4_t keep[2] = {};
-        lr_each(mine, [&](int a) {
-            f32x4_t acc[2] = {};
+    __syncthreads();
+    bf16x8_t hop[LR_MT][OPS];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                int n = c + 8 * (lr >> 2) + 4 * t + (lr & 3);
+    for (int t = 0; t < LR_MT; ++t)
+#pragma unroll
+        for (int s = 0; s < OPS; ++s) hop[t][s] = __builtin_bit_cast(bf16x8_t, hs[t][s][lane]);
+
+    auto store = [&](int a, int c, int t, int g, const uint4 &y) {
+        const int64_t m = m0 + 16 * t + lr;
+        const int col = c + 32 * g + 8 * kg;
+        if (mine[t] == a && m < p.M && col < c1) *reinterpret_cast<uint4 *>(p.out + m * p.ldo + n0 + col) = y;
+    };
+    if (blockIdx.y == 0 && p.base != p.out) {  // rows without an adapter: copied
+        bool none = false;
+#pragma unroll
+        for (int t = 0; t < LR_MT; ++t) none |= mine[t] < 0 && m0 + 16 * t + lr < p.M;
+        if (__builtin_amdgcn_ballot_w64(none)) {
+            for (int c = c0; c < c1; c += 256) {
+                uint4 y[LR_MT][2];
+                load_base(c, y);
+#pragma unroll
+                for (int t = 0; t < LR_MT; ++t)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) store(-1, c, t, g, y[t][g]);
+            }
+        }
+    }
+    lr_each<LR_MT>(mine, blockIdx.y, gridDim.y, [&](int a) {
+        const float sc = p.scale ? p.scale[a] : 1.0f;
+        const uint16_t *up = p.up + ((int64_t)a * p.N + n0) * p.R;
+        uint4 yn[LR_MT][2];
+        if (again) load_base(c0, yc);
+        again = true;
+        u32x4_t uc[4][SP], un[4][SP];
+        auto load_up = [&](int c, u32x4_t (&u)[4][SP]) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                int n = c + 32 * (q >> 1) + 8 * (lr >> 2) + 4 * (q & 1) + (lr & 3);
                 n = n < width ? n : width - 1;
-                const uint16_t *up = p.up + ((int64_t)a * p.N + part * width + n) * p.R;
+                const uint16_t *row = up + (int64_t)n * p.R;
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) {
-                    const int ch = 4 * s + kg;
+                for (int s = 0; s < SP; ++s) {
+                    const int ch = PACK ? kg & 1 : 4 * s + kg;
                     const u32x4_t zero = {0, 0, 0, 0};
-                    const u32x4_t u = ch < 2 * rc ? *reinterpret_cast<const u32x4_t *>(up + (ch < rc ? ch : ch - rc) * 8) : zero;
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, u), hop[s], acc[t], 0, 0, 0);
+                    u[q][s] = ch < rc ? *reinterpret_cast<const u32x4_t *>(row + ch * 8) : zero;
                 }
             }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) keep[t][i] = mine == a ? acc[t][i] : keep[t][i];
-        });
-        const int col = c + 8 * kg;
-        if (m < p.M && col < c1) {
-            const int64_t n = (int64_t)part * width + col;
-            float y[8] = {};
-            if (p.base) unpack8(*reinterpret_cast<const uint4 *>(p.base + m * p.ldb + n), y);
-            if (mine >= 0) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    y[e] = __builtin_fmaf(sc, keep[0][e], y[e]);
-                    y[4 + e] = __builtin_fmaf(sc, keep[1][e], y[4 + e]);
-                }
+        };
+        constexpr bool AHEAD = SP == 1;  // the next columns' operands too, where registers allow
+        if (AHEAD) load_up(c0, uc);
+        for (int c = c0; c < c1; c += 256) {
+            if (!AHEAD) load_up(c, uc);
+            if (c + 256 < c1) {
+                load_base(c + 256, yn);
+                if (AHEAD) load_up(c + 256, un);
             }
-            *reinterpret_cast<uint4 *>(p.out + m * p.ldo + n) = pack8(y);
+            f32x4_t acc[LR_MT][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int t = 0; t < LR_MT; ++t) {
+                    acc[t][q] = f32x4_t{};
+#pragma unroll
+                    for (int s = 0; s < SP; ++s) {
+                        const bf16x8_t u = __builtin_bit_cast(bf16x8_t, uc[q][s]);
+                        acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, hop[t][s], acc[t][q], 0, 0, 0);
+                        if (!PACK) acc[t][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, hop[t][OPS / 2 + s], acc[t][q], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int t = 0; t < LR_MT; ++t)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    float y[8];
+                    unpack8(yc[t][g], y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[e] = __builtin_fmaf(sc, acc[t][2 * g][e], y[e]);
+                        y[4 + e] = __builtin_fmaf(sc, acc[t][2 * g + 1][e], y[4 + e]);
+                    }
+                    store(a, c, t, g, pack8(y));
+                }
+#pragma unroll
+            for (int t = 0; t < LR_MT; ++t)
+#pragma unroll
+                for (int g = 0; g < 2; ++g) yc[t][g] = yn[t][g];
+            if (AHEAD) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int s = 0; s < SP; ++s) uc[q][s] = un[q][s];
+            }
         }
-    }
+    });
 }
 
-// K chunks: as many as bring the first launch to two workgroups per CU, each
-// with at least 128 values (one step per wave).
-static int64_t lr_chunks(int64_t M, int64_t K, int64_t PR) {
+// The launches' shapes.  Row tiles of the first: 64 rows (32 where R is large:
+// registers, or where R and M are small: fewer, longer chunks), 16 for at most 16 rows.
+// K chunks: as many as still fit one round of a workgroup per CU, each with
+// at least 512 values (a step per wave).  Slots: where that is still too few,
+// the distinct adapters of a row tile (at most `distinct` of them) go to
+// different workgroups.
+struct LrPlan {
+    int rt, mt, ncols;
+    int64_t rblocks, tiles, chunks, kchunk, slots, nchunk, up_slots;
+};
+static LrPlan lr_plan(int64_t M, int64_t seq, int64_t K, int64_t PR, int64_t width, int64_t parts, int64_t A) {
     const int64_t cus = device_cus() > 0 ? device_cus() : 256;
-    const int64_t tiles = (M + 15) / 16 * ((PR + 127) / 128);
-    int64_t n = 2 * cus / tiles;
-    const int64_t most = (K + 127) / 128;
-    n = n < most ? n : most;
-    n = n < 16 ? n : 16;
-    return n > 1 ? n : 1;
+    auto upto = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; };
+    auto distinct = [&](int64_t rows) {
+        const int64_t n = seq % rows == 0 ? 1 : (rows < M ? rows : M) / seq + (seq > 1 ? 2 : 0);
+        return upto(n < A ? n : A, 1, 64);
+    };
+    LrPlan pl;
+    pl.rt = PR <= 16 ? 1 : PR <= 32 ? 2 : PR <= 64 ? 4 : 8;
+    pl.mt = M <= 16 ? 1 : pl.rt == 8 || (pl.rt <= 2 && M < 32 * cus) ? 2 : 4;
+    pl.rblocks = (PR + 16 * pl.rt - 1) / (16 * pl.rt);
+    pl.tiles = (M + 16 * pl.mt - 1) / (16 * pl.mt);
+    constexpr int64_t step = 64 * LR_WAVES;
+    const int64_t chunks = upto(cus / (pl.tiles * pl.rblocks), 1, upto((K + step - 1) / step, 1, 16));
+    pl.kchunk = ((K + chunks - 1) / chunks + step - 1) / step * step;
+    pl.chunks = (K + pl.kchunk - 1) / pl.kchunk;  // none empty after rounding
+    pl.slots = upto(upto(cus / (pl.tiles * pl.rblocks * pl.chunks), 2, 64), 1, distinct(16 * pl.mt));
+    const int64_t up_tiles = (M + 16 * LR_MT - 1) / (16 * LR_MT);
+    pl.ncols = 256;
+    for (; pl.ncols > 64 && up_tiles * parts * ((width + 4 * pl.ncols - 1) / (4 * pl.ncols)) < 2 * cus;) pl.ncols /= 2;
+    pl.nchunk = (width + 4 * pl.ncols - 1) / (4 * pl.ncols);
+    pl.up_slots = upto(2 * cus / (up_tiles * parts * pl.nchunk), 1, distinct(16 * LR_MT));
+    return pl;
 }
+
+// The K chunks of a problem do not depend on N or the adapters.
+static int64_t lr_chunks(int64_t M, int64_t K, int64_t PR) { return lr_plan(M, 1, K, PR, 8, 1, 1).chunks; }
 
 }  // namespace qim
 
@@ -224,22 +405,29 @@ extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const 
                     aligned16(x) && aligned16(down) && aligned16(up) && aligned16(base) && aligned16(out) &&
                     aligned16(workspace) && ((reinterpret_cast<uintptr_t>(index) | reinterpret_cast<uintptr_t>(scale)) & 3u) == 0,
                 QIM_ERR_LAYOUT, "%s: rows must be 16-byte aligned", who);
-    const int64_t PR = parts * R, chunks = lr_chunks(M, K, PR);
-    QIM_REQUIRE(workspace_bytes >= chunks * M * PR * 4, QIM_ERR_ARG, "%s: workspace of %lld bytes, this problem needs %lld", who,
-                (long long)workspace_bytes, (long long)(chunks * M * PR * 4));
+    const int64_t PR = parts * R, width = N / parts;
+    const LrPlan pl = lr_plan(M, seq, K, PR, width, parts, A);
+    QIM_REQUIRE(workspace_bytes >= pl.chunks * M * PR * 4, QIM_ERR_ARG, "%s: workspace of %lld bytes, this problem needs %lld", who,
+                (long long)workspace_bytes, (long long)(pl.chunks * M * PR * 4));
+    const int64_t up_tiles = (M + 16 * LR_MT - 1) / (16 * LR_MT);
+    QIM_REQUIRE(up_tiles * pl.nchunk * parts < (1ll << 31) && pl.tiles * pl.chunks < (1ll << 31) && pl.slots * pl.rblocks < 65536, QIM_ERR_SHAPE, "%s: too large", who);
     LowRankArgs a{(const uint16_t *)x, (const uint16_t *)down, (const uint16_t *)up, (const uint16_t *)base, index, scale,
-                  (uint16_t *)out, (float *)workspace, ldx, ldb, ldo, M, seq, (int)K, (int)N, (int)R, (int)PR, (int)parts,
-                  (int)A, (int)chunks, (int)(((K + chunks - 1) / chunks + 127) / 128 * 128), 0, 0};
-    a.chunks = (int)((K + a.kchunk - 1) / a.kchunk);  // none empty after rounding
-    const int64_t width = N / parts;
-    a.ncols = 256;
-    a.nchunk = (int)((width + a.ncols - 1) / a.ncols);
-    QIM_REQUIRE((int64_t)a.nchunk * parts < 65536, QIM_ERR_SHAPE, "%s: too many columns", who);
-    const int64_t rt = PR <= 16 ? 1 : PR <= 32 ? 2 : PR <= 64 ? 4 : 8;
-    void (*const dn)(LowRankArgs) = rt == 1 ? k_lr_down<1> : rt == 2 ? k_lr_down<2> : rt == 4 ? k_lr_down<4> : k_lr_down<8>;
-    launch(dn, dim3((unsigned)((M + 15) / 16), (unsigned)a.chunks, (unsigned)((PR + 16 * rt - 1) / (16 * rt))), dim3(256), 0, as_stream(stream), a);
-    const int steps = R <= 16 ? 1 : R <= 32 ? 2 : R <= 64 ? 4 : 8;
-    void (*const up_fn)(LowRankArgs) = steps == 1 ? k_lr_up<1> : steps == 2 ? k_lr_up<2> : steps == 4 ? k_lr_up<4> : k_lr_up<8>;
-    launch(up_fn, dim3((unsigned)((M + 63) / 64), (unsigned)(a.nchunk * parts)), dim3(256), 0, as_stream(stream), a);
+                  (uint16_t *)out, (float *)workspace, ldx, ldb, ldo, M, (uint32_t)(seq < M ? seq : M), (int)K, (int)N, (int)R,
+                  (int)PR, (int)parts, (int)A, (int)pl.chunks, (int)pl.kchunk, pl.ncols, (int)pl.nchunk};
+    using Down = void (*)(LowRankArgs, int);
+    static const Down downs[4][3] = {{k_lr_down<1, 1>, k_lr_down<1, 2>, k_lr_down<1, 4>},
+                                     {k_lr_down<2, 1>, k_lr_down<2, 2>, k_lr_down<2, 4>},
+                                     {k_lr_down<4, 1>, nullptr, k_lr_down<4, 4>},
+                                     {k_lr_down<8, 1>, k_lr_down<8, 2>, nullptr}};
+    static std::atomic<bool> configured[4][3][QIM_MAX_DEVICES] = {};
+    const int ri = pl.rt == 8 ? 3 : pl.rt / 2, mi = pl.mt / 2, lds = LR_WAVES * pl.mt * pl.rt * 64 * 16;
+    const Down dn = downs[ri][mi];
+    if (lds > 65536)
+        if (const int rc = reserve_lds(reinterpret_cast<const void *>(dn), lds, configured[ri][mi], who)) return rc;
+    launch(dn, dim3((unsigned)(pl.tiles * pl.chunks), (unsigned)(pl.slots * pl.rblocks)), dim3(64 * LR_WAVES), lds, as_stream(stream), a,
+           (int)pl.rblocks);
+    void (*const up_fn)(LowRankArgs) = R <= 16 ? k_lr_up<1, true> : R <= 32 ? k_lr_up<1, false> : R <= 64 ? k_lr_up<2, false> : k_lr_up<4, false>;
+    launch(up_fn, dim3((unsigned)(up_tiles * pl.nchunk * parts), (unsigned)pl.up_slots), dim3(256), 0,
+           as_stream(stream), a);
     return check_launch(who);
 }
