@@ -316,8 +316,10 @@ int qim_cache_read(const void *kc, const void *ks, const void *vc, const void *v
                    int64_t B, int64_t C, int64_t rows, int64_t H, int64_t D, void *stream);
 
 /* qim_qk_norm_rope_pack with its prefix read from such a cache: positions
- * [0, P) of each sequence, P <= C, in place of ck, cv.  v and ov are required;
- * D in {64, 128, 256}. */
+ * [0, P) of each sequence, P <= C, in place of ck, cv.  The rotated rows are
+ * rounded to bf16 once, at their end (the bf16 form rounds after the
+ * normalisation and after its weight too, as the reference's operators do).  v
+ * and ov are required; D in {64, 128, 256}. */
 int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, const void *kc, const void *ks,
                                  const void *vc, const void *vs, int64_t C, const void *wq, const void *wk,
                                  const void *freqs, void *oq, void *ok, void *ov, int64_t B, int64_t S,

@@ -482,7 +482,10 @@ constexpr int NR_ROWS = 3;
 // holds of one head row (chunks c and c + LPR, ... of the row: each 16-byte
 // load instruction of the wave covers whole 8 * LPR-value row segments); LPR
 // lanes share the row (the helpers are in qim_device.h).
-template <int LPR, int V, bool NORM, bool ROPE>
+//
+// ONCE: the normalised, weighted and rotated value is rounded to bf16 once, at
+// the end, where the reference's operators round after each of the first two.
+template <int LPR, int V, bool NORM, bool ROPE, bool ONCE>
 __device__ __forceinline__ void norm_rope_chunks(const uint4 (&xv)[V], uint4 (&out)[V], const float (&w)[V][8],
                                                  float eps, const float4 (&f0)[V], const float4 (&f1)[V]) {
     float x[V][8];
@@ -498,7 +501,14 @@ __device__ __forceinline__ void norm_rope_chunks(const uint4 (&xv)[V], uint4 (&o
         ss = group_sum<LPR>(ss);
         const float r = rstd_of((float)(ss / (double)(LPR * 8 * V)), eps);
 #pragma unroll
-        for (int v = 0; v < V; ++v) head_rmsnorm8_r(x[v], r, w[v]);
+        for (int v = 0; v < V; ++v) {
+            if constexpr (ONCE) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) x[v][t] *= r * w[v][t];
+            } else {
+                head_rmsnorm8_r(x[v], r, w[v]);
+            }
+        }
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -518,7 +528,9 @@ __device__ __forceinline__ void norm_rope_chunks(const uint4 (&xv)[V], uint4 (&o
 // its RoPE row is read from HBM once and from L2 by the others.  Head slots
 // past H are skipped (uniform over the LPR lanes of a row).  v is copied
 // unchanged.
-template <int D, bool NORM, bool ROPE, int NTENS, int U, bool FULL, int V>
+//
+// Q8: the prefix is held in MXFP8 (kc, ks, vc, vs); the rows round once (ONCE).
+template <int D, bool NORM, bool ROPE, int NTENS, int U, bool FULL, int V, bool Q8>
 __global__ __launch_bounds__(256) void k_norm_rope(NormRopeArgs p) {
     constexpr int LPR = D / (8 * V);  // lanes per head row
     constexpr int RPI = 64 / LPR;     // head rows per wave instruction
@@ -590,7 +602,7 @@ __global__ __launch_bounds__(256) void k_norm_rope(NormRopeArgs p) {
             const int h = h0 + u * RPI;
             if (FULL || h < H) {
                 uint4 o[V];
-                norm_rope_chunks<LPR, V, NORM, ROPE>(x[u], o, wt, eps, f0, f1);
+                norm_rope_chunks<LPR, V, NORM, ROPE, Q8>(x[u], o, wt, eps, f0, f1);
 #pragma unroll
                 for (int v = 0; v < V; ++v) st_nt(dst + off + u * RPI * D + v * 8 * LPR, o[v]);
             }
@@ -606,7 +618,7 @@ __global__ __launch_bounds__(256) void k_norm_rope(NormRopeArgs p) {
         if (row >= B * PH) return;
         const int64_t bb = row / PH, within = row - bb * PH;
         const int64_t dst = (bb * (p.P + p.S) * p.H + within) * D + cc * 8;
-        if (p.kc) {
+        if constexpr (Q8) {
             const int64_t at = (bb * p.C * p.H + within) * D + cc * 8;
             const uint2 kq = *reinterpret_cast<const uint2 *>(p.kc + at), vq = *reinterpret_cast<const uint2 *>(p.vc + at);
             const int ke = p.ks[at / 32], ve = p.vs[at / 32];
@@ -619,7 +631,7 @@ __global__ __launch_bounds__(256) void k_norm_rope(NormRopeArgs p) {
     }
 }
 
-template <int D, bool NORM, bool ROPE, int NTENS, int U, bool FULL, int V = 1>
+template <int D, bool NORM, bool ROPE, int NTENS, bool Q8, int U, bool FULL, int V = 1>
 static void launch_norm_rope_shape(NormRopeArgs a, int64_t prefix_blocks, hipStream_t st) {
     const int64_t rows_per_wave = U * (512 * V / D);
     const int64_t groups = (a.H + rows_per_wave - 1) / rows_per_wave;
@@ -627,22 +639,22 @@ static void launch_norm_rope_shape(NormRopeArgs a, int64_t prefix_blocks, hipStr
     a.groups = (uint32_t)groups;
     a.main_waves = (uint32_t)waves;
     a.main_blocks = (waves + 3) / 4;
-    launch((k_norm_rope<D, NORM, ROPE, NTENS, U, FULL, V>), dim3((unsigned)(a.main_blocks + prefix_blocks)),
+    launch((k_norm_rope<D, NORM, ROPE, NTENS, U, FULL, V, Q8>), dim3((unsigned)(a.main_blocks + prefix_blocks)),
                        dim3(256), 0, st, a);
 }
 
-template <int D, bool NORM, bool ROPE, int NTENS>
+template <int D, bool NORM, bool ROPE, int NTENS, bool Q8>
 static void launch_norm_rope_d(const NormRopeArgs &a, int64_t prefix_blocks, hipStream_t st) {
     constexpr int64_t RPI = 512 / D;
     if (D >= 128 && a.H % (2 * RPI) == 0)
-        launch_norm_rope_shape<D, NORM, ROPE, NTENS, 1, true, 2>(a, prefix_blocks, st);
-    else if (a.H % (2 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, 2, true>(a, prefix_blocks, st);
-    else if (a.H % (3 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, 3, true>(a, prefix_blocks, st);
-    else if (a.H % (4 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, 4, true>(a, prefix_blocks, st);
-    else launch_norm_rope_shape<D, NORM, ROPE, NTENS, NR_ROWS, false>(a, prefix_blocks, st);
+        launch_norm_rope_shape<D, NORM, ROPE, NTENS, Q8, 1, true, 2>(a, prefix_blocks, st);
+    else if (a.H % (2 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, Q8, 2, true>(a, prefix_blocks, st);
+    else if (a.H % (3 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, Q8, 3, true>(a, prefix_blocks, st);
+    else if (a.H % (4 * RPI) == 0) launch_norm_rope_shape<D, NORM, ROPE, NTENS, Q8, 4, true>(a, prefix_blocks, st);
+    else launch_norm_rope_shape<D, NORM, ROPE, NTENS, Q8, NR_ROWS, false>(a, prefix_blocks, st);
 }
 
-template <bool NORM, bool ROPE, int NTENS>
+template <bool NORM, bool ROPE, int NTENS, bool Q8 = false>
 static int launch_norm_rope(const NormRopeArgs &a, int64_t D, int64_t B, hipStream_t st) {
     if (D != 64 && D != 128 && D != 256)
         return fail(QIM_ERR_SHAPE, "norm/rope: head dim %lld not in {64, 128, 256}", (long long)D);
@@ -653,9 +665,9 @@ static int launch_norm_rope(const NormRopeArgs &a, int64_t D, int64_t B, hipStre
         (max_waves + 3) / 4 + prefix_blocks >= (1ll << 31))
         return fail(QIM_ERR_SHAPE, "norm/rope: too large (%lld tokens x %lld heads)", (long long)a.T, (long long)a.H);
     switch (D) {
-        case 64: launch_norm_rope_d<64, NORM, ROPE, NTENS>(a, prefix_blocks, st); break;
-        case 128: launch_norm_rope_d<128, NORM, ROPE, NTENS>(a, prefix_blocks, st); break;
-        default: launch_norm_rope_d<256, NORM, ROPE, NTENS>(a, prefix_blocks, st); break;
+        case 64: launch_norm_rope_d<64, NORM, ROPE, NTENS, Q8>(a, prefix_blocks, st); break;
+        case 128: launch_norm_rope_d<128, NORM, ROPE, NTENS, Q8>(a, prefix_blocks, st); break;
+        default: launch_norm_rope_d<256, NORM, ROPE, NTENS, Q8>(a, prefix_blocks, st); break;
     }
     return QIM_OK;
 }
@@ -740,8 +752,9 @@ static int norm_rope_pack(const char *who, NormRopeArgs a, int64_t B, int64_t D,
     for (const void *pp : ptrs)
         QIM_REQUIRE(!pp || aligned16(pp), QIM_ERR_LAYOUT, "%s: operands must be 16-byte aligned", who);
     a.T = B * a.S;
-    int rc = a.v ? launch_norm_rope<true, true, 3>(a, D, B, as_stream(stream))
-                 : launch_norm_rope<true, true, 2>(a, D, B, as_stream(stream));
+    int rc = a.kc  ? launch_norm_rope<true, true, 3, true>(a, D, B, as_stream(stream))
+             : a.v ? launch_norm_rope<true, true, 3>(a, D, B, as_stream(stream))
+                   : launch_norm_rope<true, true, 2>(a, D, B, as_stream(stream));
     return rc ? rc : check_launch(who);
 }
 

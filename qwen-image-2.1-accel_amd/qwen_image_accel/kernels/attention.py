@@ -74,8 +74,10 @@ def prepare_attention_inputs_quantized(q, k, v, norm_q, norm_k, freqs, cache, pr
     """``prepare_attention_inputs`` with the prefix in an MXFP8 cache
     (``kv_cache.QuantizedCache``, of which the first ``prefix`` positions, by
     default all, are the prefix): its values go in front of k and v as
-    ``kv_cache.read_cache`` gives them, without that copy.  None where the
-    kernel does not take the step's own operands."""
+    ``kv_cache.read_cache`` gives them, without that copy.  The rotated q and k
+    are rounded to bf16 once, at their end; ``prepare_attention_inputs`` rounds
+    after the normalisation and after its weight too, as the reference's
+    operators do.  None where the kernel does not take the step's own operands."""
     b, c, h, d = kv_cache.check_cache("prepare_attention_inputs_quantized", cache)
     p = c if prefix is None else int(prefix)
     if not 0 <= p <= c:

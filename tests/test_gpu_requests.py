@@ -200,7 +200,10 @@ def test_block_with_adapters_and_quantized_prefix(dev, profile, monkeypatch):
         pipeline.install_hot_path(t, profile, validate=False)
         bare = _cached(t, inputs, quantized)
         route = install.install_adapters(t, ad)
-        assert torch.equal(_cached(t, inputs, quantized), _cached(t, inputs, values))   # one prefix, read two ways
+        # One prefix read two ways; the quantized pack rounds q and k once where the bf16 one rounds three times:
+        # two roundings of 2^-8 of q and k, a good deal less of the output.
+        both = rel_fro(_cached(t, inputs, quantized).float().cpu().numpy(), _cached(t, inputs, values).float().cpu().numpy())
+        assert both < 2.0 ** -7
         route.select(["b", None, "a"])
         got = _cached(t, inputs, quantized)
         for i, ref in enumerate(refs):
