@@ -9,38 +9,38 @@
 // a key is read once for up to 64 of them.  A row costs 512 flop for a
 // key's 264 bytes; up to about a hundred rows the cache's bytes bound it.
 //
-// Transposed products on v_mfma_f32_32x32x16_bf16, 32 keys at a time: S^T = K Q^T
-// (32 keys x 32 rows) and O^T = V^T P^T (32 head dims x 32 rows), so a lane owns
-// query row lane % 32 in both, m and the sum are lane-local, and the S^T
-// accumulator is already the B operand of the second product (lane (row, hf)
-// holds keys 8(i/4) + 4hf + i%4, i = 0..15).  Codes become bf16 exactly (4
-// significand bits times a power of two), with the block's exponent as the
-// conversion's scale operand.  K goes from memory to the A operand as it is:
-// lane (key, hf) loads the 16 codes [32j + 16hf, +16) for each j, whose two
-// halves are two 8-value operands; Q is held in the same order (an MFMA pairs
-// the K slots of A and B by position).  V is converted into a per-wave LDS tile
-// of 32 keys x 128 and transposed by the LDS reads.
+// Transposed products on v_mfma_f32_16x16x32_bf16, 32 keys at a time: S^T = K Q^T
+// (two tiles of 16 keys x 16 rows) and O^T = V^T P^T (16 head dims x 16 rows per
+// tile), so a lane owns query row lane % 16 in both; with kg = lane / 16 its scores
+// are those of keys 16u + 4kg + i (u = 0, 1; i = 0..3), which is its B operand of one
+// 32-key step of the second product, and a row's maximum is one value exchanged
+// between 4 lanes per block.  Codes become bf16 exactly (4 significand bits times
+// a power of two), the block's exponent being the conversion's scale operand.  K goes
+// from memory to the A operand as it is: a 16-code chunk is two 8-value operands,
+// and Q is held in the same order (an MFMA pairs the K slots of A and B by
+// position).  V is converted into a per-wave LDS tile of 32 keys x 128 and
+// transposed by the LDS reads.
 //
-// Work split: a workgroup is one (sequence, K/V head, row tile, key chunk); its
-// 4 waves take 32-key blocks of the chunk in turn, each with its own running
-// maximum, and join in LDS.  Where there are too few (sequence, head) pairs to
-// fill the chip the keys are cut into nsplit chunks (of the sequence's
-// own length, read on the device) and a second launch joins them.
+// Where there are too few (sequence, head) pairs to fill the chip the keys are
+// cut into chunks and a second launch joins them; a chunk past a sequence's own
+// length (read on the device) ends at once.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
 namespace qim {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16a_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int CA_D = 128;
 constexpr int CA_KB = 32;                        // keys per block
 constexpr int CA_VTILE = CA_KB * CA_D * 2;       // 8 KiB of LDS per wave
-constexpr int CA_OROW = CA_D + 4;                // floats per row of the joining buffer (staggers the banks)
 constexpr int CA_MAX_S = 64;
-constexpr int CA_MAX_SPLIT = 64;
+constexpr int CA_WAVES = 8, CA_MAX = 32;
+// Waves (heads) per workgroup: two per SIMD where the registers of a tile of
+// 16 * nr rows allow, else one.
+constexpr int ca_waves(int nr) { return nr <= 2 ? 8 : 4; }
 
 struct CacheAttnArgs {
     const uint16_t *q;
@@ -50,10 +50,11 @@ struct CacheAttnArgs {
     const uint8_t *tree;
     int64_t tree_b;
     uint16_t *o;
-    float *part_o;   // (item, split, row of the tile, 128), relative to the split's maximum
-    float2 *part_ml; // (item, split, row of the tile): (maximum, sum)
+    float *part_o;   // (sequence, K/V head, chunk, row, 128), relative to the chunk's maximum
+    float2 *part_ml; // (sequence, K/V head, chunk, row): (maximum, sum)
     int64_t C;
-    int S, H, HK, G, rows, ntile, nsplit;
+    int B, S, H, HK, G, rows, ntile, nsplit;
+    int per;  // blocks per key chunk
     float scale_log2e;
 };
 
@@ -65,351 +66,408 @@ __device__ __forceinline__ bf16x8_t ca_operand(uint32_t lo, uint32_t hi, float s
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// 32 keys of K and V as loaded: K of lane (key = lane % 32, hf) chunks 2j + hf;
-// V of lane: key 8 it + lane / 8, chunk lane % 8.
-struct CaRaw {
-    uint4 k[4], v[4];
-    uint32_t ks, vs[4];
-};
-
+__device__ __forceinline__ int64_t ca_length(const CacheAttnArgs &p, int64_t b) {
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : n > p.C ? p.C : n;
+}
 __device__ __forceinline__ float ca_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float ca_swap_max(float x) {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
 }
 
-template <int NT>
-__global__ __launch_bounds__(256) void k_cache_attn(CacheAttnArgs p) {
-    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-    const int tid = threadIdx.x, lane = tid & 63, lq = lane & 31, hf = lane >> 5;
+// The tree's bits of query s: bit j, whether it sees the j-th of the last S keys.
+// Four truth bytes per load (rows of S bytes, any alignment), all loads in flight
+// together; the last load ends at the row's end and repeats bits.
+__device__ __forceinline__ uint64_t ca_tree_bits(const CacheAttnArgs &p, int b, int s) {
+    if (!p.tree) return 0;
+    const uint8_t *row = p.tree + b * p.tree_b + s * p.S;
+    uint64_t bits = 0;
+    if (p.S < 4) {
+        for (int j = 0; j < p.S; ++j) bits |= (uint64_t)(row[j] != 0) << j;
+        return bits;
+    }
+    uint32_t w[CA_MAX_S / 4];
+#pragma unroll
+    for (int i = 0; i < CA_MAX_S / 4; ++i) {
+        w[i] = 0;
+        if (4 * i < p.S) __builtin_memcpy(&w[i], row + (4 * i + 4 <= p.S ? 4 * i : p.S - 4), 4);
+    }
+#pragma unroll
+    for (int i = 0; i < CA_MAX_S / 4; ++i) {
+        // Bytes of 0 or 1 to 4 bits.
+        const uint32_t four = ((w[i] & 0x01010101u) * 0x01020408u) >> 24;
+        bits |= (uint64_t)four << (4 * i + 4 <= p.S ? 4 * i : p.S - 4 > 0 ? p.S - 4 : 0);
+    }
+    return bits;
+}
+
+// The 32 keys from k0 as bits, for the row whose tree bits are `bits`: keys before
+// the tree's (from tree0 > k0 - 32 on) are seen, keys past the last are not.
+__device__ __forceinline__ uint32_t ca_seen(int64_t k0, int64_t len, int64_t tree0, uint64_t bits) {
+    const int64_t s0 = k0 - tree0, left = len - k0;  // s0 > -32, left >= 1
+    uint32_t w = s0 >= 0 ? (uint32_t)(bits >> s0) : ((uint32_t)bits << (uint32_t)-s0) | ((1u << (uint32_t)-s0) - 1u);
+    if (left < 32) w &= (1u << (uint32_t)left) - 1u;
+    return w;
+}
+
+// A key that one row does not see may hold infinities or NaN for another.  Such
+// values leave the operand v (0 * NaN is NaN); ind gets 1 where they were, so that
+// a product of ind and "seen" finds the rows that do see them.  Any in this lane?
+__device__ __forceinline__ bool ca_not_finite(bf16x8_t &v, u32x4_t &ind) {
+    u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = (w[e] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u;
+        const uint32_t hi = (w[e] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+        ind[e] = (lo | hi) & 0x3f803f80u;
+        w[e] &= ~(lo | hi);
+        any |= (lo | hi) != 0;
+    }
+    v = __builtin_bit_cast(bf16x8_t, w);
+    return any;
+}
+
+// Sequence and key chunk of this workgroup, and its place among the `wide`
+// workgroups (heads and row tiles) of that chunk.  Workgroup ids go to the 8
+// XCDs round-robin; the `wide` of one chunk are given to one XCD: a token's
+// exponents of all heads lie in one or two lines (32 heads: 128 bytes), which
+// each L2 would otherwise fetch for its few heads.  Which XCD starts with which
+// sequence changes from chunk to chunk (lengths differ).  False past the end.
+__device__ __forceinline__ bool ca_place(const CacheAttnArgs &p, uint32_t wide, int &b, int &split, uint32_t &at) {
+    const uint32_t q = blockIdx.x >> 3, block = q / wide, group = block * 8 + (blockIdx.x & 7);
+    at = q - block * wide;
+    split = (int)(group / (uint32_t)p.B);
+    b = (int)((group - split * p.B + split) % (uint32_t)p.B);
+    return split < p.nsplit;
+}
+
+// 32 keys of K and V as loaded: K of lane (key, kg) the 16-code chunks 4j + kg of
+// keys key and 16 + key; V of a lane, key 8 it + lane / 8, chunk lane % 8.
+struct CaRaw {
+    uint4 k[2][2], v[4];
+    uint32_t ks[2], vs[4];
+};
+
+// One wave: a (sequence, K/V head, tile of 16 * NR rows, key chunk) of its own;
+// neighbouring waves take neighbouring heads, whose 128-byte pieces are neighbours in
+// memory.  No barrier anywhere.
+template <int NR>
+__global__ __launch_bounds__(64 * ca_waves(NR), NR <= 2 ? 2 : 1) void k_cache_attn(CacheAttnArgs p) {
+    constexpr int WG = ca_waves(NR);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[WG * CA_VTILE];
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Neighbouring workgroups: the row tiles of a head (which share its keys in
-    // L2), then the heads (whose 128-byte pieces are neighbours in memory).
-    const int item = blockIdx.x, split = blockIdx.y;
-    const int tile = item % p.ntile, h = (item / p.ntile) % p.HK, b = item / (p.ntile * p.HK);
-    const int64_t len64 = p.lengths[b];
-    const int64_t len = len64 < 0 ? 0 : len64 > p.C ? p.C : len64;
-    const int64_t nblk = (len + CA_KB - 1) / CA_KB, per = (nblk + p.nsplit - 1) / p.nsplit;
-    const int64_t blk0 = split * per, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
-    const int row0 = tile * 32 * NT;
-    const float c = p.scale_log2e;
-    const float ninf = -__builtin_inff();
+    const uint32_t tasks = (uint32_t)(p.HK * p.ntile);
+    int b, split;
+    uint32_t task;
+    if (!ca_place(p, (tasks + WG - 1) / WG, b, split, task)) return;
+    task = task * WG + wave;
+    if (task >= tasks) return;
+    const int tile = (int)(task / (uint32_t)p.HK), h = (int)(task - tile * (uint32_t)p.HK);
+    const int64_t len = ca_length(p, b);
+    const int64_t nblk = (len + CA_KB - 1) / CA_KB;
+    const int64_t blk0 = (int64_t)split * p.per, blk1 = blk0 + p.per < nblk ? blk0 + p.per : nblk;
+    if (split > 0 && blk0 >= blk1) return;  // nothing there; the join does not look at it
+    const float c = p.scale_log2e, ninf = -__builtin_inff();
 
-    // Q operands, and the tree's bits of each row.
-    bf16x8_t qf[NT][8];
-    uint64_t bits[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        int r = row0 + 32 * t + lq;
-        r = r < p.rows ? r : p.rows - 1;  // rows past the end: computed, not stored
-        const int s = r / p.G, head = h * p.G + (r - s * p.G);
-        const uint16_t *qr = p.q + b * p.ldqb + s * p.ldq + head * CA_D + hf * 16;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            qf[t][2 * j] = *reinterpret_cast<const bf16x8_t *>(qr + 32 * j);
-            qf[t][2 * j + 1] = *reinterpret_cast<const bf16x8_t *>(qr + 32 * j + 8);
-        }
-        bits[t] = 0;
-        if (p.tree) {
-            const uint8_t *mask = p.tree + b * p.tree_b + s * p.S;
-            for (int j = 0; j < p.S; ++j) bits[t] |= (uint64_t)(mask[j] != 0) << j;
-        }
-    }
-
-    f32x16a_t o[NT][4];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = ninf;
-        l[t] = 0.f;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) o[t][dt] = f32x16a_t{};
-    }
-
+    // A block's loads: wave-uniform bases and per-lane 32-bit offsets.  Only a block
+    // that reaches past the cache's end clamps its rows to the last one.  The next
+    // block's are issued as soon as this one's registers have been consumed.
     const int64_t W = (int64_t)p.HK * CA_D;
     const uint8_t *kc = p.kc + b * p.C * W + h * CA_D, *vc = p.vc + b * p.C * W + h * CA_D;
     const uint8_t *ks = p.ks + (b * p.C * W + h * CA_D) / 32, *vs = p.vs + (b * p.C * W + h * CA_D) / 32;
-    auto load = [&](int64_t blk, CaRaw &x) {
+    const uint32_t w32 = (uint32_t)W, ws = (uint32_t)(W / 32);
+    CaRaw cur;
+    auto load_k = [&](int64_t blk) {
         const int64_t k0 = blk * CA_KB;
-        int64_t key = k0 + lq;
-        key = key < p.C ? key : p.C - 1;
-        const uint8_t *at = kc + key * W + hf * 16;
+        const uint8_t *kb = kc + k0 * W, *ksb = ks + k0 * (W / 32);
+        const int last = p.C - k0 < CA_KB ? (int)(p.C - k0) - 1 : CA_KB - 1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.k[j] = *reinterpret_cast<const uint4 *>(at + 32 * j);
-        x.ks = *reinterpret_cast<const uint32_t *>(ks + key * (W / 32));
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t key = 16 * u + lr < last ? 16 * u + lr : last, ko = key * w32 + 16 * kg;
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
-            int64_t vk = k0 + 8 * it + (lane >> 3);
-            vk = vk < p.C ? vk : p.C - 1;
-            x.v[it] = *reinterpret_cast<const uint4 *>(vc + vk * W + (lane & 7) * 16);
-            x.vs[it] = *reinterpret_cast<const uint32_t *>(vs + vk * (W / 32));
+            for (int j = 0; j < 2; ++j) cur.k[u][j] = *reinterpret_cast<const uint4 *>(kb + ko + 64 * j);
+            cur.ks[u] = *reinterpret_cast<const uint32_t *>(ksb + key * ws);
         }
     };
-
-    // This wave's V tile.  Row = key, 16-byte chunk c at chunk c ^ 4 (key % 4).
-    uint8_t *const vt = lds + wave * CA_VTILE;
-    const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)vt;
-    uint32_t vread[4];
-    {
-        const int i = lane & 15;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-            vread[dt] = vbase + (4 * hf + (i >> 2)) * 256 + ((dt ^ (i >> 2)) << 6) + ((lane >> 4) & 1) * 32 + (i & 3) * 8;
-    }
-
-    const int64_t tree0 = p.tree ? len - p.S : len;  // the first key that needs a look at the mask
-    CaRaw cur, nxt;
-    if (blk0 + wave < blk1) load(blk0 + wave, cur);
-    for (int64_t blk = blk0 + wave; blk < blk1; blk += 4) {
+    auto load_v = [&](int64_t blk) {
         const int64_t k0 = blk * CA_KB;
-        if (blk + 4 < blk1) load(blk + 4, nxt);
-        // V rows past the last key are zeros, whatever the cache holds there.
-        const int shift = 8 * ((lane & 7) >> 1);
+        const uint8_t *vb = vc + k0 * W, *vsb = vs + k0 * (W / 32);
+        const int last = p.C - k0 < CA_KB ? (int)(p.C - k0) - 1 : CA_KB - 1;
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-            const int key = 8 * it + (lane >> 3), ch = 2 * (lane & 7);
-            const bool in = k0 + key < len;
-            const float s = mx_scale_operand(in ? (int)((cur.vs[it] >> shift) & 0xffu) : 0);
-            const uint4 x = in ? cur.v[it] : make_uint4(0, 0, 0, 0);
-            uint8_t *row = vt + key * 256;
-            *reinterpret_cast<bf16x8_t *>(row + ((ch ^ ((key & 3) << 2)) << 4)) = ca_operand(x.x, x.y, s);
-            *reinterpret_cast<bf16x8_t *>(row + (((ch + 1) ^ ((key & 3) << 2)) << 4)) = ca_operand(x.z, x.w, s);
+            const uint32_t vk = 8 * it + (lane >> 3) < last ? 8 * it + (lane >> 3) : last;
+            cur.v[it] = *reinterpret_cast<const uint4 *>(vb + (vk * w32 + (lane & 7) * 16));
+            cur.vs[it] = vsb[vk * ws + ((lane & 7) >> 1)];
         }
-        f32x16a_t s[NT];
+    };
+    if (blk0 < blk1) {
+        load_v(blk0);
+        load_k(blk0);
+    }
+
+    // Q operands (step 2j + half: d [64j + 16kg + 8half, +8)) and the tree's bits of
+    // this lane's rows.
+    bf16x8_t qf[NR][4];
+    uint64_t bits[NR];
+    int row[NR];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float sc = mx_scale_operand((int)((cur.ks >> (8 * j)) & 0xffu));
-            const bf16x8_t a = ca_operand(cur.k[j].x, cur.k[j].y, sc), bq = ca_operand(cur.k[j].z, cur.k[j].w, sc);
+    for (int t = 0; t < NR; ++t) {
+        row[t] = (tile * NR + t) * 16 + lr;
+        const int r = row[t] < p.rows ? row[t] : p.rows - 1;  // rows past the end: computed, not stored
+        const int s = r / p.G, head = h * p.G + (r - s * p.G);
+        const uint16_t *qr = p.q + b * p.ldqb + s * p.ldq + head * CA_D + 16 * kg;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, qf[t][2 * j], j == 0 ? f32x16a_t{} : s[t], 0, 0, 0);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bq, qf[t][2 * j + 1], s[t], 0, 0, 0);
+        for (int j = 0; j < 2; ++j) {
+            qf[t][2 * j] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * j);
+            qf[t][2 * j + 1] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * j + 8);
+        }
+        bits[t] = ca_tree_bits(p, b, s);
+    }
+    f32x4_t o[NR][8];
+    float m[NR], l[NR];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        m[t] = ninf;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[t][dt] = f32x4_t{};
+    }
+
+    // This wave's V tile: row = key, 32-byte unit n of key r at unit n ^ (r % 8).
+    // Reads: lane i of a 16-lane group addresses 8 bytes of key 4kg + i / 4 (and 16
+    // keys later), d 16dt + 4 (i % 4), and receives column i of that 4 x 16 block.
+    uint8_t *const vt = lds + wave * CA_VTILE;
+    const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)vt;
+    const int vkey = 4 * kg + (lr >> 2);
+    const uint32_t vrow = vbase + vkey * 256 + (lr & 3) * 8;
+    const int64_t tree0 = p.tree ? len - p.S : len;  // the first key that needs a look at the mask
+
+    for (int64_t blk = blk0; blk < blk1; ++blk) {
+        const int64_t k0 = blk * CA_KB;
+        const bool whole = k0 + CA_KB <= len;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int key = 8 * it + (lane >> 3);
+            uint4 x = cur.v[it];
+            uint32_t e = cur.vs[it];
+            if (!whole) {  // V rows past the last key are zeros, whatever the cache holds there
+                const bool in = k0 + key < len;
+                x = make_uint4(in ? x.x : 0, in ? x.y : 0, in ? x.z : 0, in ? x.w : 0);
+                e = in ? e : 0;
             }
+            const float sc = mx_scale_operand((int)e);
+            uint8_t *at = vt + key * 256 + (((lane & 7) ^ (key & 7)) << 5);
+            *reinterpret_cast<bf16x8_t *>(at) = ca_operand(x.x, x.y, sc);
+            *reinterpret_cast<bf16x8_t *>(at + 16) = ca_operand(x.z, x.w, sc);
         }
+        if (blk + 1 < blk1) load_v(blk + 1);
+        f32x4_t s[NR][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float sc = mx_scale_operand((int)((cur.ks[u] >> (8 * (2 * j + (kg >> 1)))) & 0xffu));
+                const uint4 x = cur.k[u][j];
+                const bf16x8_t k_lo = ca_operand(x.x, x.y, sc), k_hi = ca_operand(x.z, x.w, sc);
+#pragma unroll
+                for (int t = 0; t < NR; ++t) {
+                    s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_lo, qf[t][2 * j], j == 0 ? f32x4_t{} : s[t][u], 0, 0, 0);
+                    s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k_hi, qf[t][2 * j + 1], s[t][u], 0, 0, 0);
+                }
+            }
+        if (blk + 1 < blk1) load_k(blk + 1);
         // Only blocks that reach the tree's keys or the end have anything masked.
         const bool masked = k0 + CA_KB > tree0;
-        uint32_t seen[NT];
+        uint32_t seen[NR];
+        u32x4_t pw[NR];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < NR; ++t) {
             seen[t] = ~0u;
             if (masked) {
-                // The block's 32 keys as bits: keys before the tree's are seen.
-                const int64_t s0 = k0 - tree0, left = len - k0;  // s0 > -32, left >= 1
-                uint32_t w = s0 >= 0 ? (uint32_t)(bits[t] >> s0)
-                                     : ((uint32_t)bits[t] << (uint32_t)-s0) | ((1u << (uint32_t)-s0) - 1u);
-                if (left < 32) w &= (1u << (uint32_t)left) - 1u;
-                seen[t] = w >> (4 * hf);
+                seen[t] = ca_seen(k0, len, tree0, bits[t]) >> (4 * kg);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[t][i] = (seen[t] >> (8 * (i >> 2) + (i & 3))) & 1u ? s[t][i] : ninf;
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][u][i] = (seen[t] >> (16 * u + i)) & 1u ? s[t][u][i] : ninf;
             }
-        }
-        uint32_t pw[NT][8];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float mx = ca_max(s[t][0], s[t][1]);
-#pragma unroll
-            for (int i = 2; i < 16; ++i) mx = ca_max(mx, s[t][i]);
-            mx = ca_swap_max(mx) * c;
+            float mx = ca_max(ca_max(ca_max(s[t][0][0], s[t][0][1]), ca_max(s[t][0][2], s[t][0][3])),
+                              ca_max(ca_max(s[t][1][0], s[t][1][1]), ca_max(s[t][1][2], s[t][1][3])));
+            {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = ca_swap_max(ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1]))) * c;
+            }
             const float mn = ca_max(m[t], mx);
             const float ref = mn == ninf ? 0.f : mn;  // nothing seen yet: every p is 0
             const float alpha = __builtin_amdgcn_exp2f(m[t] - ref);
             m[t] = mn;
-            float e[16], sum = 0.f;
+            float e[8], sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, -ref));
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], c, -ref));
                 sum += e[i];
             }
             l[t] = l[t] * alpha + sum;
-            // p is rounded to bf16 for the matrix product: at most 2^-9 of each
+            // p is rounded to bf16 for the matrix product: at most 2^-8 of each
             // term of a sum that is itself rounded to bf16 at the end.
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pw[t][i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+            pw[t] = u32x4_t{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]), pack_bf16x2(e[6], e[7])};
             if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
 #pragma unroll
-                for (int dt = 0; dt < 4; ++dt) o[t][dt] *= alpha;
+                for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
             }
         }
         // A wave's LDS operations run in order; the compiler must not reorder them.
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
+        for (int dt = 0; dt < 8; ++dt) {
             typedef __attribute__((address_space(3))) i16x4_t *ptr_t;
-            bf16x8_t vf[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t at = vread[dt] + u * (16 * CA_D * 2);
-                const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)at));
-                const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)(at + 8 * CA_D * 2)));
-                vf[u] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            }
+            const uint32_t at = vrow + ((dt ^ (vkey & 7)) << 5);
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)at));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)(at + 16 * CA_D * 2)));
+            bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             if (masked) {
-                // A key that one row does not see may hold infinities or NaN for
-                // another: those values leave the product (0 * NaN is NaN) and make
-                // NaN of the rows that do see their key, by a product of
-                // "not finite" and "seen".
-                typedef unsigned int u4 __attribute__((ext_vector_type(4)));
-                u4 ind[2];
-                bool any = false;
+                u32x4_t ind;
+                if (__builtin_amdgcn_ballot_w64(ca_not_finite(vf, ind))) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    u4 w = __builtin_bit_cast(u4, vf[u]);
+                    for (int t = 0; t < NR; ++t) {
+                        u32x4_t sv;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t lo = (w[e] & 0x7f80u) == 0x7f80u ? 0x3f80u : 0u;
-                        const uint32_t hi = (w[e] & 0x7f800000u) == 0x7f800000u ? 0x3f800000u : 0u;
-                        ind[u][e] = lo | hi;
-                        if (lo) w[e] &= 0xffff0000u;
-                        if (hi) w[e] &= 0x0000ffffu;
-                        any |= ind[u][e] != 0;
-                    }
-                    vf[u] = __builtin_bit_cast(bf16x8_t, w);
-                }
-                if (__builtin_amdgcn_ballot_w64(any)) {
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        f32x16a_t hit{};
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            u4 sv;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t two = seen[t] >> (16 * u + 8 * (e >> 1) + 2 * (e & 1));
-                                sv[e] = ((two & 1u) ? 0x3f80u : 0u) | ((two & 2u) ? 0x3f800000u : 0u);
-                            }
-                            hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, ind[u]),
-                                                                         __builtin_bit_cast(bf16x8_t, sv), hit, 0, 0, 0);
+                        for (int e2 = 0; e2 < 4; ++e2) {
+                            const uint32_t two = seen[t] >> (16 * (e2 >> 1) + 2 * (e2 & 1));
+                            sv[e2] = ((two & 1u) ? 0x3f80u : 0u) | ((two & 2u) ? 0x3f800000u : 0u);
                         }
+                        const f32x4_t hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8_t, ind), __builtin_bit_cast(bf16x8_t, sv), f32x4_t{}, 0, 0, 0);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[t][dt][i] = hit[i] > 0.f ? __builtin_nanf("") : o[t][dt][i];
+                        for (int i = 0; i < 4; ++i) o[t][dt][i] = hit[i] > 0.f ? __builtin_nanf("") : o[t][dt][i];
                     }
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const u32x4_t w = {pw[t][4 * u], pw[t][4 * u + 1], pw[t][4 * u + 2], pw[t][4 * u + 3]};
-                    o[t][dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[u], __builtin_bit_cast(bf16x8_t, w), o[t][dt], 0, 0, 0);
-                }
+            for (int t = 0; t < NR; ++t)
+                o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8_t, pw[t]), o[t][dt], 0, 0, 0);
         }
         asm volatile("" ::: "memory");
-        cur = nxt;
     }
-
-    // Join the four waves: weights 2^(m_w - M), then the sums, a tile at a time.
-    float *const buf = reinterpret_cast<float *>(lds);                        // [4][32][CA_OROW]
-    float2 *const ml = reinterpret_cast<float2 *>(buf + 4 * 32 * CA_OROW);    // [4][32]
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        __syncthreads();  // the V tiles, or the previous tile, are done with
-        const float lt = l[t] + __shfl_xor(l[t], 32, 64);
-        if (hf == 0) ml[wave * 32 + lq] = make_float2(m[t], lt);
-        __syncthreads();
-        float M = ca_max(ca_max(ml[lq].x, ml[32 + lq].x), ca_max(ml[64 + lq].x, ml[96 + lq].x));
-        M = M == ninf ? 0.f : M;
-        const float wgt = __builtin_amdgcn_exp2f(m[t] - M);
-        float *row = buf + (wave * 32 + lq) * CA_OROW;
+    for (int t = 0; t < NR; ++t) {
+        float lt = l[t] + __shfl_xor(l[t], 16, 64);
+        lt += __shfl_xor(lt, 32, 64);
+        if (row[t] >= p.rows) continue;
+        if (p.nsplit == 1) {
+            const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // no visible key: zeros
+            const int s = row[t] / p.G, head = h * p.G + (row[t] - s * p.G);
+            uint16_t *dst = p.o + (((int64_t)b * p.S + s) * p.H + head) * CA_D + 4 * kg;
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+            for (int dt = 0; dt < 8; ++dt)
+                *reinterpret_cast<uint2 *>(dst + 16 * dt) = make_uint2(pack_bf16x2(o[t][dt][0] * inv, o[t][dt][1] * inv),
+                                                                       pack_bf16x2(o[t][dt][2] * inv, o[t][dt][3] * inv));
+        } else {
+            const int64_t at = (((int64_t)b * p.HK + h) * p.nsplit + split) * p.rows + row[t];
+            float *dst = p.part_o + at * CA_D + 4 * kg;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<float4 *>(row + 32 * dt + 8 * g + 4 * hf) =
-                    make_float4(o[t][dt][4 * g] * wgt, o[t][dt][4 * g + 1] * wgt, o[t][dt][4 * g + 2] * wgt, o[t][dt][4 * g + 3] * wgt);
-        __syncthreads();
-        // 8 threads per row, 16 head dims each.
-        const int rl = tid >> 3, d0 = (tid & 7) * 16, r = row0 + 32 * t + rl;
-        float acc[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-        float Mr = ninf, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) Mr = ca_max(Mr, ml[w * 32 + rl].x);
-        const float Mz = Mr == ninf ? 0.f : Mr;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 x = ml[w * 32 + rl];
-            L += x.y * __builtin_amdgcn_exp2f(x.x - Mz);
-            const float *src = buf + (w * 32 + rl) * CA_OROW + d0;
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const float4 f = *reinterpret_cast<const float4 *>(src + e);
-                acc[e] += f.x;
-                acc[e + 1] += f.y;
-                acc[e + 2] += f.z;
-                acc[e + 3] += f.w;
-            }
-        }
-        if (r < p.rows) {
-            if (p.nsplit == 1) {
-                const float inv = L == 0.f ? 0.f : 1.0f / L;  // no visible key: zeros
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[e] *= inv;
-                const int s = r / p.G, head = h * p.G + (r - s * p.G);
-                uint16_t *dst = p.o + (((int64_t)b * p.S + s) * p.H + head) * CA_D + d0;
-                *reinterpret_cast<uint4 *>(dst) = pack8(acc);
-                *reinterpret_cast<uint4 *>(dst + 8) = pack8(acc + 8);
-            } else {
-                const int64_t at = ((int64_t)item * p.nsplit + split) * (32 * NT) + 32 * t + rl;
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<float4 *>(p.part_o + at * CA_D + d0 + e) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-                if ((tid & 7) == 0) p.part_ml[at] = make_float2(Mr, L);
-            }
+            for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4_t *>(dst + 16 * dt) = o[t][dt];
+            if (kg == 0) p.part_ml[at] = make_float2(m[t], lt);
         }
     }
 }
 
-// Join the key chunks: 32 lanes per row, 4 head dims each.
-__global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int tile_rows, int64_t nrows) {
-    const int64_t g = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int d0 = (threadIdx.x & 31) * 4;
-    if (g >= nrows) return;
-    const int64_t item0 = g / p.rows;  // (sequence, K/V head)
-    const int r = (int)(g - item0 * p.rows), tile = r / tile_rows, rl = r - tile * tile_rows;
-    const int64_t first = ((item0 * p.ntile + tile) * p.nsplit) * tile_rows + rl;
-    float M = -__builtin_inff();
-    for (int i = 0; i < p.nsplit; ++i) M = ca_max(M, p.part_ml[first + (int64_t)i * tile_rows].x);
-    M = M == -__builtin_inff() ? 0.f : M;
+// Join the key chunks of a row: GP groups of LANES lanes (4 head dims each) take the
+// chunks of 4 * LANES head dims in turn, four loads at a time, and join in LDS.
+template <int GP, int LANES>
+__global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_t nparts) {
+    constexpr int PARTS = 32 / LANES, NG = 256 / LANES;  // parts of a row; groups of the workgroup
+    __shared__ float4 so[NG][LANES];
+    __shared__ float2 sml[NG];
+    const int grp = threadIdx.x / LANES, ln = threadIdx.x % LANES;
+    const int64_t g = (int64_t)blockIdx.x * (NG / GP) + grp / GP;
+    const bool live = g < nparts;
+    const int64_t row = live ? g / PARTS : 0, item0 = row / p.rows;  // (sequence, K/V head)
+    const int d0 = (int)(g % PARTS) * (4 * LANES) + ln * 4;
+    const int r = (int)(row - item0 * p.rows);
+    const int64_t b = item0 / p.HK;
+    const int64_t blocks = (ca_length(p, b) + CA_KB - 1) / CA_KB;
+    const int n = (int)((blocks + p.per - 1) / p.per);  // chunks of this sequence
+    const int64_t first = item0 * p.nsplit * p.rows + r;
+    const float ninf = -__builtin_inff();
+    float M = ninf, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-    for (int i = 0; i < p.nsplit; ++i) {
-        const int64_t at = first + (int64_t)i * tile_rows;
-        const float2 ml = p.part_ml[at];
-        const float4 f = *reinterpret_cast<const float4 *>(p.part_o + at * CA_D + d0);
-        const float w = __builtin_amdgcn_exp2f(ml.x - M);
-        L += ml.y * w;
-        acc.x += f.x * w;
-        acc.y += f.y * w;
-        acc.z += f.z * w;
-        acc.w += f.w * w;
+    for (int i = grp % GP; i < n; i += 4 * GP) {
+        float2 ml[4];
+        float4 f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t at = first + (int64_t)(i + j * GP < n ? i + j * GP : i) * p.rows;
+            ml[j] = p.part_ml[at];
+            f[j] = *reinterpret_cast<const float4 *>(p.part_o + at * CA_D + d0);
+            if (i + j * GP >= n) ml[j] = make_float2(ninf, 0.f);
+        }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Mn = ca_max(Mn, ml[j].x);
+        const float ref = Mn == ninf ? 0.f : Mn, sc = __builtin_amdgcn_exp2f(M - ref);
+        L *= sc;
+        acc = make_float4(acc.x * sc, acc.y * sc, acc.z * sc, acc.w * sc);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float w = __builtin_amdgcn_exp2f(ml[j].x - ref);
+            if (i + j * GP < n) {  // (a repeated chunk may hold NaN)
+                L += ml[j].y * w;
+                acc = make_float4(acc.x + f[j].x * w, acc.y + f[j].y * w, acc.z + f[j].z * w, acc.w + f[j].w * w);
+            }
+        }
+        M = Mn;
     }
+    if constexpr (GP > 1) {
+        so[grp][ln] = acc;
+        if (ln == 0) sml[grp] = make_float2(M, L);
+        __syncthreads();
+        if (grp % GP) return;
+        M = ninf;
+#pragma unroll
+        for (int j = 0; j < GP; ++j) M = ca_max(M, sml[grp + j].x);
+        const float ref = M == ninf ? 0.f : M;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        L = 0.f;
+#pragma unroll
+        for (int j = 0; j < GP; ++j) {
+            const float w = __builtin_amdgcn_exp2f(sml[grp + j].x - ref);
+            const float4 f = so[grp + j][ln];
+            L += sml[grp + j].y * w;
+            acc = make_float4(acc.x + f.x * w, acc.y + f.y * w, acc.z + f.z * w, acc.w + f.w * w);
+        }
+    }
+    if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     const int h = (int)(item0 % p.HK), s = r / p.G, head = h * p.G + (r - s * p.G);
-    uint16_t *dst = p.o + (((item0 / p.HK) * p.S + s) * p.H + head) * CA_D + d0;
+    uint16_t *dst = p.o + ((b * p.S + s) * p.H + head) * CA_D + d0;
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
-// Row tiles of 32 (one MFMA tile) or 64, and key chunks: as many as bring the
-// launch to two workgroups per CU, each with at least a block for every wave.
+// Row tiles of up to 64 rows, and key chunks of `per` blocks: as many chunks as
+// bring the launch to 8 waves per CU, at most CA_MAX blocks each.
 struct CaPlan {
-    int64_t rows, tile, ntile, items, nsplit;
-    int64_t part_o() const { return nsplit > 1 ? items * nsplit * tile * CA_D * 4 : 0; }
-    int64_t bytes() const { return nsplit > 1 ? part_o() + items * nsplit * tile * 8 : 0; }
+    int64_t rows, nr, ntile, nsplit, per, items;
+    int64_t grid(int64_t B) const {  // ca_place
+        return (B * nsplit + 7) / 8 * 8 * ((items / B * ntile + ca_waves((int)nr) - 1) / ca_waves((int)nr));
+    }
+    int64_t part_o() const { return nsplit > 1 ? items * nsplit * rows * CA_D * 4 : 0; }
+    int64_t bytes() const { return nsplit > 1 ? part_o() + items * nsplit * rows * 8 : 0; }
 };
 static CaPlan ca_plan(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     CaPlan pl;
     pl.rows = S * (H / HK);
-    pl.tile = pl.rows > 32 ? 64 : 32;
-    pl.ntile = (pl.rows + pl.tile - 1) / pl.tile;
-    pl.items = B * HK * pl.ntile;
+    pl.ntile = (pl.rows + 63) / 64;
+    pl.nr = ((pl.rows + pl.ntile - 1) / pl.ntile + 15) / 16;
+    pl.items = B * HK;
     const int64_t cus = device_cus() > 0 ? device_cus() : 256, nblk = (C + CA_KB - 1) / CA_KB;
-    int64_t n = (2 * cus + pl.items - 1) / pl.items;
-    const int64_t most = nblk / 4;
-    n = n < most ? n : most;
-    n = n < CA_MAX_SPLIT ? n : CA_MAX_SPLIT;
-    pl.nsplit = n > 1 ? n : 1;
+    int64_t n = CA_WAVES * cus / (pl.items * pl.ntile);
+    if (n * CA_MAX < nblk) n = (nblk + CA_MAX - 1) / CA_MAX;
+    n = n < 1 ? 1 : n > nblk ? nblk : n;
+    pl.per = (nblk + n - 1) / n;
+    pl.nsplit = (nblk + pl.per - 1) / pl.per;
     return pl;
 }
 
@@ -419,7 +477,7 @@ using namespace qim;
 
 static bool ca_shape(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     return B > 0 && S > 0 && S <= CA_MAX_S && C > 0 && C < (1ll << 31) && HK > 0 && H > 0 && H % HK == 0 && H <= (1 << 16) && B < (1 << 20) &&
-           B * HK * ((S * (H / HK) + 31) / 32) < (1 << 24);
+           B * HK * ((S * (H / HK) + 31) / 32) < (1 << 24) && ca_plan(B, S, C, H, HK).grid(B) < (1ll << 31);
 }
 
 extern "C" int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
@@ -444,18 +502,19 @@ extern "C" int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, co
     QIM_REQUIRE(pl.bytes() == 0 || (workspace && workspace_bytes >= pl.bytes()), QIM_ERR_ARG,
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)pl.bytes());
     QIM_REQUIRE(aligned16(workspace), QIM_ERR_LAYOUT, "%s: workspace must be 16-byte aligned", who);
-    static std::atomic<bool> configured[2][QIM_MAX_DEVICES] = {};
-    constexpr int bytes = (4 * 32 * CA_OROW) * 4 + 4 * 32 * 8;
-    void (*const fn)(CacheAttnArgs) = pl.tile == 64 ? k_cache_attn<2> : k_cache_attn<1>;
-    if (const int rc = reserve_lds(reinterpret_cast<const void *>(fn), bytes, configured[pl.tile == 64], who)) return rc;
+    void (*const fn)(CacheAttnArgs) = pl.nr == 1 ? k_cache_attn<1> : pl.nr == 2 ? k_cache_attn<2> : pl.nr == 3 ? k_cache_attn<3> : k_cache_attn<4>;
     CacheAttnArgs a{(const uint16_t *)q, ldqb, ldq, (const uint8_t *)kc, (const uint8_t *)ks, (const uint8_t *)vc,
                     (const uint8_t *)vs, lengths, (const uint8_t *)tree, tree_b, (uint16_t *)o, (float *)workspace,
-                    (float2 *)((uint8_t *)workspace + pl.part_o()), C, (int)S, (int)H, (int)HK, (int)(H / HK),
-                    (int)pl.rows, (int)pl.ntile, (int)pl.nsplit, scale * 1.4426950408889634f};
-    launch(fn, dim3((unsigned)pl.items, (unsigned)pl.nsplit), dim3(256), bytes, as_stream(stream), a);
+                    (float2 *)((uint8_t *)workspace + pl.part_o()), C, (int)B, (int)S, (int)H, (int)HK, (int)(H / HK),
+                    (int)pl.rows, (int)pl.ntile, (int)pl.nsplit, (int)pl.per, scale * 1.4426950408889634f};
+    launch(fn, dim3((unsigned)pl.grid(B)), dim3(64 * ca_waves((int)pl.nr)), 0, as_stream(stream), a);
     if (pl.nsplit > 1) {
         const int64_t nrows = B * HK * pl.rows;
-        launch(k_cache_attn_join, dim3((unsigned)((nrows + 7) / 8)), dim3(256), 0, as_stream(stream), a, (int)pl.tile, nrows);
+        // Few rows of many chunks: a quarter row per workgroup, 32 chunks at once.
+        const bool many = pl.nsplit > 16 && nrows <= 4 * device_cus();
+        launch(many ? k_cache_attn_join<32, 8> : pl.nsplit > 4 ? k_cache_attn_join<2, 32> : k_cache_attn_join<1, 32>,
+               dim3((unsigned)(many ? nrows * 4 : (nrows * (pl.nsplit > 4 ? 2 : 1) + 7) / 8)), dim3(256), 0, as_stream(stream), a,
+               many ? nrows * 4 : nrows);
     }
     return check_launch(who);
 }
