@@ -6,6 +6,7 @@ and streams are then shared.  There is no CPU fallback here: if the library is
 missing every call raises NativeUnavailable.
 """
 import ctypes
+import functools
 import os
 import threading
 
@@ -172,13 +173,17 @@ def call_on(device, name, *args):
         return call(name, *args, stream(device))
 
 
+@functools.lru_cache(maxsize=4096)
+def _bytes(device_index, name, *args):
+    with torch.cuda.device(device_index):
+        return getattr(lib(), name)(*args)
+
+
 def bytes_on(device, name, *args):
-    """The value of a workspace-size entry point for a problem on `device`
-    (sizes depend on that device's CU count)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return getattr(lib(), name)(*args)
-    with torch.cuda.device(device):
-        return getattr(lib(), name)(*args)
+    """The value of a workspace-size entry point for a problem on `device`: a
+    function of the sizes and of that device's CU count, kept per device and
+    sizes."""
+    return _bytes(torch.cuda.current_device() if device.index is None else device.index, name, *args)
 
 
 def loaded_hip_runtimes():

@@ -16,9 +16,13 @@ MAX_RANK = 128
 def _rows(t):
     """(rows, width, row stride) of a (M, W) or (B, S, W) tensor whose rows lie
     one stride apart, else None.  An axis of one element may have any stride."""
-    if t.dim() not in (2, 3) or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dim() not in (2, 3):
         return None
     w = t.shape[-1]
+    if t.is_contiguous():
+        return t.numel() // w if w else 0, w, w
+    if w > 1 and t.stride(-1) != 1:
+        return None
     if t.dim() == 2:
         return t.shape[0], w, t.stride(0) if t.shape[0] > 1 else w
     b, s = t.shape[:2]

@@ -41,17 +41,17 @@ def empty_cache(batch, capacity, heads, head_dim, device):
 
 def check_cache(name, cache):
     """(B, C, H, D) of a cache the kernels can read, else Unsupported."""
-    codes = cache.k
-    shape, device = codes.shape, codes.device
-    if codes.dim() != 4 or shape[3] % BLOCK or not codes.is_cuda:
+    k, ke, v, ve = cache
+    shape, device = k.shape, k.device
+    if k.dim() != 4 or shape[3] % BLOCK or not k.is_cuda:
         raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT, "the cache holds (B, C, H, D) codes on the GPU")
     blocks = shape[:3] + (shape[3] // BLOCK,)
-    for t, dtype, want in ((codes, torch.float8_e4m3fn, shape), (cache.k_exponent, torch.uint8, blocks),
-                           (cache.v, torch.float8_e4m3fn, shape), (cache.v_exponent, torch.uint8, blocks)):
-        if t.dtype != dtype or t.shape != want or t.device != device or not t.is_contiguous():
-            raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT,
-                                      "codes (B, C, H, D) float8_e4m3fn and exponents (B, C, H, D/32) uint8, contiguous, "
-                                      "on one device")
+    if not (k.dtype == v.dtype == torch.float8_e4m3fn and ke.dtype == ve.dtype == torch.uint8 and v.shape == shape
+            and ke.shape == blocks and ve.shape == blocks and ke.device == v.device == ve.device == device
+            and k.is_contiguous() and ke.is_contiguous() and v.is_contiguous() and ve.is_contiguous()):
+        raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT,
+                                  "codes (B, C, H, D) float8_e4m3fn and exponents (B, C, H, D/32) uint8, contiguous, "
+                                  "on one device")
     return shape
 
 
