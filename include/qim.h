@@ -357,13 +357,14 @@ int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, in
  * (zeros); out: (M, N), row stride ldo; out may be base.  K, R and N / parts are
  * multiples of 8, R <= 128; all operands 16-byte aligned.  A request's values
  * never enter another's rows, whatever they are.  workspace:
- * qim_low_rank_workspace_bytes(M, K, parts * R) bytes, 16-byte aligned, not
- * shared by calls that may overlap.  No reference counterpart. */
+ * qim_low_rank_workspace_bytes(M, seq, K, R, parts) bytes, 16-byte aligned (may
+ * be NULL when that is 0), not shared by calls that may overlap.  No reference
+ * counterpart. */
 int qim_low_rank(const void *x, int64_t ldx, const void *down, const void *up, const int32_t *index,
                  const float *scale, const void *base, int64_t ldb, void *out, int64_t ldo, void *workspace,
                  int64_t workspace_bytes, int64_t M, int64_t seq, int64_t K, int64_t N, int64_t R, int64_t parts,
                  int64_t A, void *stream);
-int64_t qim_low_rank_workspace_bytes(int64_t M, int64_t K, int64_t R);
+int64_t qim_low_rank_workspace_bytes(int64_t M, int64_t seq, int64_t K, int64_t R, int64_t parts);
 
 /* Test hooks: the device conversions every kernel uses, applied elementwise
  * (fp32 -> E4M3 code; fp32 -> bf16 bits), and one scaled MFMA

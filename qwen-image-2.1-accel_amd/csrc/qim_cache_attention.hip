@@ -21,9 +21,8 @@
 // position).  V is converted into a per-wave LDS tile of 32 keys x 128 and
 // transposed by the LDS reads.
 //
-// Where there are too few (sequence, head) pairs to fill the chip the keys are
-// cut into chunks and a second launch joins them; a chunk past a sequence's own
-// length (read on the device) ends at once.
+// Where there are too few (sequence, head) pairs to fill the chip, or their keys are
+// many, the keys are cut into chunks and a second launch joins them.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -37,7 +36,7 @@ constexpr int CA_D = 128;
 constexpr int CA_KB = 32;                        // keys per block
 constexpr int CA_VTILE = CA_KB * CA_D * 2;       // 8 KiB of LDS per wave
 constexpr int CA_MAX_S = 64;
-constexpr int CA_WAVES = 8, CA_MAX = 32;
+constexpr int CA_MAX_ROUNDS = 16;
 // Waves (heads) per workgroup: two per SIMD where the registers of a tile of
 // 16 * nr rows allow, else one.
 constexpr int ca_waves(int nr) { return nr <= 2 ? 8 : 4; }
@@ -50,11 +49,12 @@ struct CacheAttnArgs {
     const uint8_t *tree;
     int64_t tree_b;
     uint16_t *o;
-    float *part_o;   // (sequence, K/V head, chunk, row, 128), relative to the chunk's maximum
-    float2 *part_ml; // (sequence, K/V head, chunk, row): (maximum, sum)
+    float *part_o;   // (chunk, K/V head, row, 128), relative to the chunk's maximum
+    float2 *part_ml; // (chunk, K/V head, row): (maximum, sum)
     int64_t C;
-    int B, S, H, HK, G, rows, ntile, nsplit;
-    int per;  // blocks per key chunk
+    int2 *dir;       // per sequence: its first chunk and their number
+    int B, S, H, HK, G, rows, ntile;
+    int chunks;      // key chunks over all sequences, short of one per sequence; 0: a sequence is one chunk, nothing to join
     float scale_log2e;
 };
 
@@ -129,18 +129,60 @@ __device__ __forceinline__ bool ca_not_finite(bf16x8_t &v, u32x4_t &ind) {
     return any;
 }
 
-// Sequence and key chunk of this workgroup, and its place among the `wide`
-// workgroups (heads and row tiles) of that chunk.  Workgroup ids go to the 8
-// XCDs round-robin; the `wide` of one chunk are given to one XCD: a token's
-// exponents of all heads lie in one or two lines (32 heads: 128 bytes), which
-// each L2 would otherwise fetch for its few heads.  Which XCD starts with which
-// sequence changes from chunk to chunk (lengths differ).  False past the end.
-__device__ __forceinline__ bool ca_place(const CacheAttnArgs &p, uint32_t wide, int &b, int &split, uint32_t &at) {
-    const uint32_t q = blockIdx.x >> 3, block = q / wide, group = block * 8 + (blockIdx.x & 7);
+// Chunk of this workgroup, and its place among the `wide` workgroups (heads and
+// row tiles) of that chunk.  Workgroup ids go to the 8 XCDs round-robin; the `wide`
+// of one chunk are given to one XCD: a token's exponents of all heads lie in one
+// or two lines (32 heads: 128 bytes), which each L2 would otherwise fetch for its
+// few heads.
+__device__ __forceinline__ uint32_t ca_group(uint32_t wide, uint32_t &at) {
+    const uint32_t q = blockIdx.x >> 3, block = q / wide;
     at = q - block * wide;
-    split = (int)(group / (uint32_t)p.B);
-    b = (int)((group - split * p.B + split) % (uint32_t)p.B);
-    return split < p.nsplit;
+    return block * 8 + (blockIdx.x & 7);
+}
+
+// The chunks: all sequences' blocks of 32 keys, whatever their lengths, are cut into
+// pieces of `per` blocks, the smallest of which there are at most p.chunks + B (a
+// sequence's last piece may be shorter): equal shares for the waves in a batch of
+// unequal lengths, and never a few workgroups more than fit.  Finds sequence and
+// piece of chunk `group`; false past the last.  The first workgroup also writes
+// p.dir for the join.  Every lane of the wave takes part.
+__device__ __forceinline__ int ca_scan(int x, int lane) {  // inclusive, over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d, 64);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+__device__ __forceinline__ bool ca_chunk(const CacheAttnArgs &p, uint32_t group, bool writes, int &b, int64_t &blk0, int64_t &per) {
+    if (!p.chunks) {
+        b = (int)group;
+        blk0 = 0;
+        per = p.C;
+        return b < p.B;
+    }
+    const int lane = threadIdx.x & 63;
+    auto blocks = [&](int i) { return i < p.B ? (int)((ca_length(p, i) + CA_KB - 1) / CA_KB) : 0; };
+    int64_t total = 0;
+    for (int i = 0; i < p.B; i += 64) total += __builtin_amdgcn_readlane(ca_scan(blocks(i + lane), lane), 63);
+    const int each = (int)((total + p.chunks - 1) / p.chunks);
+    per = each > 1 ? each : 1;
+    uint32_t first = 0;
+    bool found = false;
+    for (int i = 0; i < p.B && !(found && !writes); i += 64) {
+        const int n = (blocks(i + lane) + (int)per - 1) / (int)per, last = ca_scan(n, lane);
+        const uint32_t from = first + last - n;
+        if (writes && i + lane < p.B) p.dir[i + lane] = make_int2((int)from, n);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(group >= from && group < from + n);
+        if (here) {
+            const int at = (int)__builtin_ctzll(here);
+            b = i + at;
+            blk0 = (int64_t)(group - (uint32_t)__builtin_amdgcn_readlane((int)from, at)) * per;
+            found = true;
+        }
+        first += (uint32_t)__builtin_amdgcn_readlane(last, 63);
+    }
+    return found;
 }
 
 // 32 keys of K and V as loaded: K of lane (key, kg) the 16-code chunks 4j + kg of
@@ -160,16 +202,16 @@ __global__ __launch_bounds__(64 * ca_waves(NR), NR <= 2 ? 2 : 1) void k_cache_at
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t tasks = (uint32_t)(p.HK * p.ntile);
-    int b, split;
     uint32_t task;
-    if (!ca_place(p, (tasks + WG - 1) / WG, b, split, task)) return;
+    const uint32_t group = ca_group((tasks + WG - 1) / WG, task);
+    int b = 0;
+    int64_t blk0 = 0, per = 1;
+    if (!ca_chunk(p, group, blockIdx.x == 0 && wave == 0, b, blk0, per)) return;
     task = task * WG + wave;
     if (task >= tasks) return;
     const int tile = (int)(task / (uint32_t)p.HK), h = (int)(task - tile * (uint32_t)p.HK);
     const int64_t len = ca_length(p, b);
-    const int64_t nblk = (len + CA_KB - 1) / CA_KB;
-    const int64_t blk0 = (int64_t)split * p.per, blk1 = blk0 + p.per < nblk ? blk0 + p.per : nblk;
-    if (split > 0 && blk0 >= blk1) return;  // nothing there; the join does not look at it
+    const int64_t nblk = (len + CA_KB - 1) / CA_KB, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
     const float c = p.scale_log2e, ninf = -__builtin_inff();
 
     // A block's loads: wave-uniform bases and per-lane 32-bit offsets.  Only a block
@@ -356,7 +398,7 @@ __global__ __launch_bounds__(64 * ca_waves(NR), NR <= 2 ? 2 : 1) void k_cache_at
         float lt = l[t] + __shfl_xor(l[t], 16, 64);
         lt += __shfl_xor(lt, 32, 64);
         if (row[t] >= p.rows) continue;
-        if (p.nsplit == 1) {
+        if (!p.chunks) {
             const float inv = lt == 0.f ? 0.f : 1.0f / lt;  // no visible key: zeros
             const int s = row[t] / p.G, head = h * p.G + (row[t] - s * p.G);
             uint16_t *dst = p.o + (((int64_t)b * p.S + s) * p.H + head) * CA_D + 4 * kg;
@@ -365,7 +407,7 @@ __global__ __launch_bounds__(64 * ca_waves(NR), NR <= 2 ? 2 : 1) void k_cache_at
                 *reinterpret_cast<uint2 *>(dst + 16 * dt) = make_uint2(pack_bf16x2(o[t][dt][0] * inv, o[t][dt][1] * inv),
                                                                        pack_bf16x2(o[t][dt][2] * inv, o[t][dt][3] * inv));
         } else {
-            const int64_t at = (((int64_t)b * p.HK + h) * p.nsplit + split) * p.rows + row[t];
+            const int64_t at = ((int64_t)group * p.HK + h) * p.rows + row[t];
             float *dst = p.part_o + at * CA_D + 4 * kg;
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4_t *>(dst + 16 * dt) = o[t][dt];
@@ -388,9 +430,9 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
     const int d0 = (int)(g % PARTS) * (4 * LANES) + ln * 4;
     const int r = (int)(row - item0 * p.rows);
     const int64_t b = item0 / p.HK;
-    const int64_t blocks = (ca_length(p, b) + CA_KB - 1) / CA_KB;
-    const int n = (int)((blocks + p.per - 1) / p.per);  // chunks of this sequence
-    const int64_t first = item0 * p.nsplit * p.rows + r;
+    const int2 dir = p.dir[b];
+    const int n = dir.y;  // chunks of this sequence
+    const int64_t step = (int64_t)p.HK * p.rows, first = dir.x * step + (item0 - b * p.HK) * p.rows + r;
     const float ninf = -__builtin_inff();
     float M = ninf, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -399,7 +441,7 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
         float4 f[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int64_t at = first + (int64_t)(i + j * GP < n ? i + j * GP : i) * p.rows;
+            const int64_t at = first + (i + j * GP < n ? i + j * GP : i) * step;
             ml[j] = p.part_ml[at];
             f[j] = *reinterpret_cast<const float4 *>(p.part_o + at * CA_D + d0);
             if (i + j * GP >= n) ml[j] = make_float2(ninf, 0.f);
@@ -446,28 +488,42 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
-// Row tiles of up to 64 rows, and key chunks of `per` blocks: as many chunks as
-// bring the launch to 8 waves per CU, at most CA_MAX blocks each.
+// Row tiles of up to 64 rows, and key chunks.  A chunk's heads and row tiles are
+// `wide` workgroups of one XCD, one workgroup to a CU, so `cap` chunks run at a time.  The
+// chunks are to fill r such rounds: in blocks of 32 keys a round costs its chunk's
+// blocks, 1 for its start and rows / 8 for writing and joining its partial results.
+// (16 sequences of up to 263 blocks, 32 heads: 2.95 rounds 172 us, 2.1 rounds 200; 2 sequences
+// of 4096 and 3072 blocks, 8 heads: 249 chunks 88 us, 257 chunks 119.)
 struct CaPlan {
-    int64_t rows, nr, ntile, nsplit, per, items;
-    int64_t grid(int64_t B) const {  // ca_place
-        return (B * nsplit + 7) / 8 * 8 * ((items / B * ntile + ca_waves((int)nr) - 1) / ca_waves((int)nr));
-    }
-    int64_t part_o() const { return nsplit > 1 ? items * nsplit * rows * CA_D * 4 : 0; }
-    int64_t bytes() const { return nsplit > 1 ? part_o() + items * nsplit * rows * 8 : 0; }
+    int64_t rows, nr, ntile, wide, chunks, groups, B, HK;
+    int64_t grid() const { return (groups + 7) / 8 * 8 * wide; }  // ca_group
+    int64_t part_o() const { return chunks ? groups * HK * rows * CA_D * 4 : 0; }
+    int64_t part_ml() const { return chunks ? groups * HK * rows * 8 : 0; }
+    int64_t bytes() const { return chunks ? part_o() + part_ml() + B * 8 : 0; }
 };
 static CaPlan ca_plan(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     CaPlan pl;
+    pl.B = B;
+    pl.HK = HK;
     pl.rows = S * (H / HK);
     pl.ntile = (pl.rows + 63) / 64;
     pl.nr = ((pl.rows + pl.ntile - 1) / pl.ntile + 15) / 16;
-    pl.items = B * HK;
+    pl.wide = (HK * pl.ntile + ca_waves((int)pl.nr) - 1) / ca_waves((int)pl.nr);
     const int64_t cus = device_cus() > 0 ? device_cus() : 256, nblk = (C + CA_KB - 1) / CA_KB;
-    int64_t n = CA_WAVES * cus / (pl.items * pl.ntile);
-    if (n * CA_MAX < nblk) n = (nblk + CA_MAX - 1) / CA_MAX;
-    n = n < 1 ? 1 : n > nblk ? nblk : n;
-    pl.per = (nblk + n - 1) / n;
-    pl.nsplit = (nblk + pl.per - 1) / pl.per;
+    const int64_t at_once = cus / 8 / pl.wide, cap = 8 * (at_once > 1 ? at_once : 1);
+    int64_t best = (B + cap - 1) / cap * (nblk + 1);  // a sequence per chunk, nothing to join
+    pl.chunks = 0;
+    pl.groups = B;
+    for (int64_t r = 1; r <= CA_MAX_ROUNDS && nblk > 1; ++r) {
+        const int64_t n = r * cap - B;
+        if (n < 1) continue;
+        const int64_t cost = r * ((B * nblk + n - 1) / n + 1 + pl.rows / 8);
+        if (cost < best) {
+            best = cost;
+            pl.chunks = n;
+            pl.groups = n + B < B * nblk ? n + B : B * nblk;
+        }
+    }
     return pl;
 }
 
@@ -477,7 +533,7 @@ using namespace qim;
 
 static bool ca_shape(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     return B > 0 && S > 0 && S <= CA_MAX_S && C > 0 && C < (1ll << 31) && HK > 0 && H > 0 && H % HK == 0 && H <= (1 << 16) && B < (1 << 20) &&
-           B * HK * ((S * (H / HK) + 31) / 32) < (1 << 24) && ca_plan(B, S, C, H, HK).grid(B) < (1ll << 31);
+           B * HK * ((S * (H / HK) + 31) / 32) < (1 << 24) && ca_plan(B, S, C, H, HK).grid() < (1ll << 31);
 }
 
 extern "C" int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
@@ -503,18 +559,20 @@ extern "C" int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, co
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)pl.bytes());
     QIM_REQUIRE(aligned16(workspace), QIM_ERR_LAYOUT, "%s: workspace must be 16-byte aligned", who);
     void (*const fn)(CacheAttnArgs) = pl.nr == 1 ? k_cache_attn<1> : pl.nr == 2 ? k_cache_attn<2> : pl.nr == 3 ? k_cache_attn<3> : k_cache_attn<4>;
+    uint8_t *const ws = static_cast<uint8_t *>(workspace);
     CacheAttnArgs a{(const uint16_t *)q, ldqb, ldq, (const uint8_t *)kc, (const uint8_t *)ks, (const uint8_t *)vc,
-                    (const uint8_t *)vs, lengths, (const uint8_t *)tree, tree_b, (uint16_t *)o, (float *)workspace,
-                    (float2 *)((uint8_t *)workspace + pl.part_o()), C, (int)B, (int)S, (int)H, (int)HK, (int)(H / HK),
-                    (int)pl.rows, (int)pl.ntile, (int)pl.nsplit, (int)pl.per, scale * 1.4426950408889634f};
-    launch(fn, dim3((unsigned)pl.grid(B)), dim3(64 * ca_waves((int)pl.nr)), 0, as_stream(stream), a);
-    if (pl.nsplit > 1) {
-        const int64_t nrows = B * HK * pl.rows;
+                    (const uint8_t *)vs, lengths, (const uint8_t *)tree, tree_b, (uint16_t *)o, (float *)ws,
+                    (float2 *)(ws + pl.part_o()), C, (int2 *)(ws + pl.part_o() + pl.part_ml()), (int)B, (int)S, (int)H,
+                    (int)HK, (int)(H / HK), (int)pl.rows, (int)pl.ntile, (int)pl.chunks,
+                    scale * 1.4426950408889634f};
+    launch(fn, dim3((unsigned)pl.grid()), dim3(64 * ca_waves((int)pl.nr)), 0, as_stream(stream), a);
+    if (pl.chunks) {
         // Few rows of many chunks: a quarter row per workgroup, 32 chunks at once.
-        const bool many = pl.nsplit > 16 && nrows <= 4 * device_cus();
-        launch(many ? k_cache_attn_join<32, 8> : pl.nsplit > 4 ? k_cache_attn_join<2, 32> : k_cache_attn_join<1, 32>,
-               dim3((unsigned)(many ? nrows * 4 : (nrows * (pl.nsplit > 4 ? 2 : 1) + 7) / 8)), dim3(256), 0, as_stream(stream), a,
-               many ? nrows * 4 : nrows);
+        const int64_t nrows = B * HK * pl.rows, each = pl.groups / B;
+        const bool many = each > 16 && 2 * nrows <= device_cus();
+        const int64_t gp = each > 16 ? 8 : each > 4 ? 2 : 1;
+        launch(many ? k_cache_attn_join<32, 8> : gp == 8 ? k_cache_attn_join<8, 32> : gp == 2 ? k_cache_attn_join<2, 32> : k_cache_attn_join<1, 32>,
+               dim3((unsigned)(many ? nrows * 4 : (nrows * gp + 7) / 8)), dim3(256), 0, as_stream(stream), a, many ? nrows * 4 : nrows);
     }
     return check_launch(who);
 }

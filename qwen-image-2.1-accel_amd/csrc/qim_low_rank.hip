@@ -2,7 +2,7 @@
 //
 //   out[m] = base[m] + scale[a] * up[a] (down[a] x[m]),   a = index[m / seq]
 //
-// in two launches.  k_lr_down: h = down x, (M, parts * R) in fp32, with the K
+// in two launches (in one for a few short rows, k_lr_small).  k_lr_down: h = down x, (M, parts * R) in fp32, with the K
 // axis cut into chunks where there are few rows (each chunk's sums go to the
 // workspace).  k_lr_up: adds the chunks, multiplies by up and adds to base.
 //
@@ -342,6 +342,142 @@ __global__ __launch_bounds__(256, SP == 4 ? 2 : 3) void k_lr_up(LowRankArgs p) {
     });
 }
 
+// At most 16 rows of few values each: both products in one launch.  A workgroup
+// takes 8 * 64 columns of one part for the adapters of its slot, and computes
+// h for them itself: it reads R rows of down (again in every workgroup of that
+// adapter, from L2) and the x of the adapter's own rows, the 8 waves taking
+// steps of 128 values in turn, joins h in LDS, and multiplies by its columns of up.
+// SP, PACK and the operands are k_lr_up's.
+template <int SP, bool PACK>
+__global__ __launch_bounds__(512, 2) void k_lr_small(LowRankArgs p) {
+    constexpr int RT = PACK ? 1 : 2 * SP;  // 16-row tiles of down
+    __shared__ f32x4_t sum[8][RT][64];
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = blockIdx.x / p.nchunk, width = p.N / p.parts, rc = p.R / 8;
+    const int c = (blockIdx.x - part * p.nchunk) * 512 + 64 * wave;
+    const int64_t n0 = (int64_t)part * width;
+    const bool row = lr < p.M;
+    uint4 y[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int col = c + 32 * g + 8 * kg;
+        if (p.base && row && col < width) y[g] = *reinterpret_cast<const uint4 *>(p.base + lr * p.ldb + n0 + col);
+    }
+    const int mine[1] = {lr_adapter(p, lr)};
+    if (blockIdx.y == 0 && p.base != p.out && mine[0] < 0 && row) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int col = c + 32 * g + 8 * kg;
+            if (col < width) *reinterpret_cast<uint4 *>(p.out + lr * p.ldo + n0 + col) = y[g];
+        }
+    }
+    lr_each<1>(mine, blockIdx.y, gridDim.y, [&](int a) {
+        const bool own = mine[0] == a;
+        const uint16_t *xr = p.x + (own ? lr : 0) * p.ldx + 8 * kg, *dn[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int at = 16 * r + lr < p.R ? 16 * r + lr : p.R - 1;
+            dn[r] = p.down + ((int64_t)a * p.PR + part * p.R + at) * p.K + 8 * kg;
+        }
+        f32x4_t acc[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[r] = f32x4_t{};
+        constexpr int S = PACK ? 4 : 2;  // 32-value steps whose loads go together
+        u32x4_t xc[S], dc[RT][S], xn[S], dx[RT][S];
+        auto load = [&](int k, u32x4_t (&xv)[S], u32x4_t (&dv)[RT][S]) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const bool in = k + 32 * s + 8 * kg < p.K;
+                const u32x4_t zero = {0, 0, 0, 0};
+                xv[s] = in && own ? *reinterpret_cast<const u32x4_t *>(xr + k + 32 * s) : zero;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) dv[r][s] = in ? *reinterpret_cast<const u32x4_t *>(dn[r] + k + 32 * s) : zero;
+            }
+        };
+        int k = 32 * S * wave;
+        load(k, xc, dc);
+        for (; k < p.K; k += 256 * S) {
+            if (k + 256 * S < p.K) load(k + 256 * S, xn, dx);
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, dc[r][s]),
+                                                                     __builtin_bit_cast(bf16x8_t, xc[s]), acc[r], 0, 0, 0);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                xc[s] = xn[s];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) dc[r][s] = dx[r][s];
+            }
+        }
+        // up of this wave's columns, in flight over the join.
+        u32x4_t up[4][SP];
+        const uint16_t *ua = p.up + ((int64_t)a * p.N + n0) * p.R;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            int n = c + 32 * (q >> 1) + 8 * (lr >> 2) + 4 * (q & 1) + (lr & 3);
+            n = n < width ? n : width - 1;
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                const int ch = PACK ? kg & 1 : 4 * s + kg;
+                const u32x4_t zero = {0, 0, 0, 0};
+                up[q][s] = ch < rc ? *reinterpret_cast<const u32x4_t *>(ua + (int64_t)n * p.R + ch * 8) : zero;
+            }
+        }
+        __syncthreads();  // the previous adapter's sums have been read
+#pragma unroll
+        for (int r = 0; r < RT; ++r) sum[wave][r][lane] = acc[r];
+        __syncthreads();
+        f32x4_t res[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) res[q] = f32x4_t{};
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+            // Chunk ch of row lr: two lanes' values of tile ch / 2.
+            const int ch = PACK ? kg & 1 : 4 * s + kg, at = (ch & 1) * 32 + lr;
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, hi[8], lo[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                const f32x4_t u = sum[w][ch >> 1][at], v = sum[w][ch >> 1][at + 16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f[e] += u[e];
+                    f[4 + e] += v[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[e] = ch < rc ? f[e] : 0.f;
+                hi[e] = rbf(f[e]);
+                lo[e] = __builtin_isfinite(hi[e]) ? f[e] - hi[e] : 0.f;
+                if (PACK && kg >= 2) hi[e] = lo[e];
+            }
+            const bf16x8_t h0 = __builtin_bit_cast(bf16x8_t, pack8(hi)), h1 = __builtin_bit_cast(bf16x8_t, pack8(lo));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const bf16x8_t u = __builtin_bit_cast(bf16x8_t, up[q][s]);
+                res[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, h0, res[q], 0, 0, 0);
+                if (!PACK) res[q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, h1, res[q], 0, 0, 0);
+            }
+        }
+        const float sc = p.scale ? p.scale[a] : 1.0f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int col = c + 32 * g + 8 * kg;
+            float f[8];
+            unpack8(y[g], f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] = __builtin_fmaf(sc, res[2 * g][e], f[e]);
+                f[4 + e] = __builtin_fmaf(sc, res[2 * g + 1][e], f[4 + e]);
+            }
+            if (own && col < width) *reinterpret_cast<uint4 *>(p.out + lr * p.ldo + n0 + col) = pack8(f);
+        }
+    });
+}
+
 // The launches' shapes.  Row tiles of the first: 64 rows (32 where R is large:
 // registers, or where R and M are small: fewer, longer chunks), 16 for at most 16 rows.
 // K chunks: as many as still fit one round of a workgroup per CU, each with
@@ -377,6 +513,16 @@ static LrPlan lr_plan(int64_t M, int64_t seq, int64_t K, int64_t PR, int64_t wid
     return pl;
 }
 
+// One launch (k_lr_small) for at most 16 rows whose adapter and own rows are few
+// values: every workgroup reads them.  One against two launches, us per call alone
+// on the GPU (N 4096; in a stream of calls the host's share of the second launch
+// adds 2.4): R 8, 8 rows each, K 1024 (16384 values) 4.6 / 6.8; R 16, 1 row, K 4096
+// (69632) 9.1 / 9.3; 4 rows each (81920) 8.8 / 7.8; R 16, 1 row, K 12288 (208896) 17.9 / 10.9.
+constexpr int64_t LR_SMALL = 72 * 1024;
+static bool lr_small(int64_t M, int64_t seq, int64_t K, int64_t R) {
+    return M <= 16 && R <= 64 && (R + (seq < M ? seq : M)) * K <= LR_SMALL;
+}
+
 // The K chunks of a problem do not depend on N or the adapters.
 static int64_t lr_chunks(int64_t M, int64_t K, int64_t PR) { return lr_plan(M, 1, K, PR, 8, 1, 1).chunks; }
 
@@ -384,9 +530,11 @@ static int64_t lr_chunks(int64_t M, int64_t K, int64_t PR) { return lr_plan(M, 1
 
 using namespace qim;
 
-extern "C" int64_t qim_low_rank_workspace_bytes(int64_t M, int64_t K, int64_t R) {
-    if (M <= 0 || K <= 0 || R <= 0 || M >= (1ll << 31) || K >= (1ll << 24) || R >= (1ll << 14)) return 0;
-    return lr_chunks(M, K, R) * M * R * 4;
+extern "C" int64_t qim_low_rank_workspace_bytes(int64_t M, int64_t seq, int64_t K, int64_t R, int64_t parts) {
+    if (M <= 0 || seq <= 0 || K <= 0 || R <= 0 || parts <= 0 || M >= (1ll << 31) || K >= (1ll << 24) || parts >= (1ll << 14) ||
+        R >= (1ll << 14) || parts * R >= (1ll << 14) || lr_small(M, seq, K, R))
+        return 0;
+    return lr_chunks(M, K, parts * R) * M * parts * R * 4;
 }
 
 extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const void *up, const int32_t *index,
@@ -394,7 +542,7 @@ extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const 
                             int64_t workspace_bytes, int64_t M, int64_t seq, int64_t K, int64_t N, int64_t R,
                             int64_t parts, int64_t A, void *stream) {
     const char *who = "qim_low_rank";
-    QIM_REQUIRE(x && down && up && index && out && workspace, QIM_ERR_ARG, "%s: null pointer", who);
+    QIM_REQUIRE(x && down && up && index && out, QIM_ERR_ARG, "%s: null pointer", who);
     QIM_REQUIRE(M > 0 && seq > 0 && K > 0 && N > 0 && R > 0 && parts > 0 && A > 0, QIM_ERR_SHAPE, "%s: empty problem", who);
     QIM_REQUIRE(K % 8 == 0 && R % 8 == 0 && R <= 128 && N % parts == 0 && (N / parts) % 8 == 0, QIM_ERR_SHAPE,
                 "%s: K %lld, rank %lld (at most 128) and N %lld / %lld must be multiples of 8", who, (long long)K,
@@ -407,13 +555,21 @@ extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const 
                 QIM_ERR_LAYOUT, "%s: rows must be 16-byte aligned", who);
     const int64_t PR = parts * R, width = N / parts;
     const LrPlan pl = lr_plan(M, seq, K, PR, width, parts, A);
-    QIM_REQUIRE(workspace_bytes >= pl.chunks * M * PR * 4, QIM_ERR_ARG, "%s: workspace of %lld bytes, this problem needs %lld", who,
-                (long long)workspace_bytes, (long long)(pl.chunks * M * PR * 4));
+    const int64_t need = qim_low_rank_workspace_bytes(M, seq, K, R, parts);
+    QIM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), QIM_ERR_ARG,
+                "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)need);
     const int64_t up_tiles = (M + 16 * LR_MT - 1) / (16 * LR_MT);
     QIM_REQUIRE(up_tiles * pl.nchunk * parts < (1ll << 31) && pl.tiles * pl.chunks < (1ll << 31) && pl.slots * pl.rblocks < 65536, QIM_ERR_SHAPE, "%s: too large", who);
     LowRankArgs a{(const uint16_t *)x, (const uint16_t *)down, (const uint16_t *)up, (const uint16_t *)base, index, scale,
                   (uint16_t *)out, (float *)workspace, ldx, ldb, ldo, M, (uint32_t)(seq < M ? seq : M), (int)K, (int)N, (int)R,
                   (int)PR, (int)parts, (int)A, (int)pl.chunks, (int)pl.kchunk, pl.ncols, (int)pl.nchunk};
+    if (lr_small(M, seq, K, R)) {
+        a.nchunk = (int)((width + 511) / 512);
+        const int64_t slots = seq > 1 ? (M + seq - 1) / seq : M;
+        launch(R <= 16 ? k_lr_small<1, true> : R <= 32 ? k_lr_small<1, false> : k_lr_small<2, false>,
+               dim3((unsigned)(a.nchunk * parts), (unsigned)(slots < A ? slots : A)), dim3(512), 0, as_stream(stream), a);
+        return check_launch(who);
+    }
     using Down = void (*)(LowRankArgs, int);
     static const Down downs[4][3] = {{k_lr_down<1, 1>, k_lr_down<1, 2>, k_lr_down<1, 4>},
                                      {k_lr_down<2, 1>, k_lr_down<2, 2>, k_lr_down<2, 4>},

@@ -76,7 +76,7 @@ SIGNATURES = {
     "qim_attention_cached": (_C, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I] + [_I] * 6 + [_F, _P]),
     "qim_attention_cached_workspace_bytes": (_I, [_I] * 5),
     "qim_low_rank": (_C, [_P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I] + [_I] * 7 + [_P]),
-    "qim_low_rank_workspace_bytes": (_I, [_I] * 3),
+    "qim_low_rank_workspace_bytes": (_I, [_I] * 5),
     "qim_debug_e4m3_encode": (_C, [_P, _P, _I, _P]),
     "qim_debug_e4m3_encode_scaled": (_C, [_P, _C, _P, _I, _P]),
     "qim_debug_bf16_round": (_C, [_P, _P, _I, _P]),

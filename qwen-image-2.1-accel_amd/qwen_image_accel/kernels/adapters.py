@@ -76,9 +76,10 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
         strides.append(rows[2] if rows else 0)
     if m == 0 or n == 0:
         return out
-    nbytes = _native.bytes_on(device, "qim_low_rank_workspace_bytes", m, k, parts * r)
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    seq = x.shape[1] if x.dim() == 3 else 1
+    nbytes = _native.bytes_on(device, "qim_low_rank_workspace_bytes", m, seq, k, r, parts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _native.call_on(device, "qim_low_rank", x.data_ptr(), ldx, down.data_ptr(), up.data_ptr(), index.data_ptr(),
-                    _native.ptr(scale), _native.ptr(base), strides[0], out.data_ptr(), strides[1], ws.data_ptr(), nbytes,
-                    m, x.shape[1] if x.dim() == 3 else 1, k, n, r, parts, a)
+                    _native.ptr(scale), _native.ptr(base), strides[0], out.data_ptr(), strides[1], _native.ptr(ws), nbytes,
+                    m, seq, k, n, r, parts, a)
     return out

@@ -29,6 +29,8 @@ def check(out, *args, **kw):
 @pytest.mark.parametrize("m,k,n,r,a,parts", [
     (1, 8, 8, 8, 1, 1), (1, 4096, 4096, 16, 3, 1), (16, 256, 512, 16, 16, 1), (17, 264, 40, 8, 5, 1), (33, 1000, 96, 24, 2, 3),
     (5, 128, 256, 128, 7, 1), (64, 96, 264, 40, 4, 1), (200, 640, 1152, 32, 6, 3), (1030, 512, 768, 64, 3, 2),
+    # at most 16 rows: one launch up to 72 K values of an adapter and its rows, two above
+    (16, 1024, 1536, 8, 16, 3), (13, 520, 4136, 64, 5, 1), (7, 1000, 72, 40, 2, 1), (2, 4096, 2048, 16, 1, 1), (9, 2000, 1040, 32, 4, 1),
     (3000, 2048, 1024, 16, 20, 1), (129, 4104, 2056, 104, 9, 1), (100, 72, 4096, 128, 3, 4)])
 def test_an_adapter_per_row(dev, m, k, n, r, a, parts):
     say("rows", m, k, n, r, a, parts)
@@ -36,7 +38,7 @@ def test_an_adapter_per_row(dev, m, k, n, r, a, parts):
     check(adapters.low_rank(x, down, up, index, scale=scale, base=base, parts=parts), x, down, up, index, scale, base, parts)
 
 
-@pytest.mark.parametrize("b,s,k,n,r,parts", [(3, 1, 128, 128, 16, 1), (2, 77, 320, 384, 8, 3), (5, 16, 512, 128, 32, 1),
+@pytest.mark.parametrize("b,s,k,n,r,parts", [(3, 1, 128, 128, 16, 1), (5, 3, 1024, 640, 24, 1), (1, 16, 512, 192, 8, 3), (2, 77, 320, 384, 8, 3), (5, 16, 512, 128, 32, 1),
                                              (2, 1024, 1024, 512, 48, 1)])
 def test_an_adapter_per_sequence(dev, b, s, k, n, r, parts):
     say("sequences", b, s, k, n, r, parts)

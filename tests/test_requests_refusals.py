@@ -46,7 +46,7 @@ def adapt(x=16, ldx=256, down=16, index=16, base=16, ldb=512, out=16, ldo=512, w
     (attend(ws=None, c=1 << 20), ARG), (attend(nbytes=16, c=1 << 20), ARG), (attend(d=64), SHAPE), (attend(s=65), SHAPE),
     (attend(s=0), SHAPE), (attend(h=3), SHAPE), (attend(c=0), SHAPE), (attend(q=8), LAYOUT), (attend(ldq=500), LAYOUT),
     (attend(o=8), LAYOUT), (attend(lengths=18), LAYOUT), (attend(ws=8, c=1 << 20), LAYOUT),
-    (adapt(x=None), ARG), (adapt(index=None), ARG), (adapt(ws=None), ARG), (adapt(nbytes=15), ARG), (adapt(m=0), SHAPE),
+    (adapt(x=None), ARG), (adapt(index=None), ARG), (adapt(ws=None, m=40), ARG), (adapt(nbytes=15, m=40), ARG), (adapt(m=0), SHAPE),
     (adapt(seq=0), SHAPE), (adapt(k=260), SHAPE), (adapt(r=12), SHAPE), (adapt(r=136), SHAPE), (adapt(parts=3), SHAPE),
     (adapt(n=516), SHAPE), (adapt(ldx=128), LAYOUT), (adapt(ldb=500), LAYOUT), (adapt(ldo=516), LAYOUT), (adapt(x=8), LAYOUT),
     (adapt(down=24), LAYOUT), (adapt(out=8), LAYOUT), (adapt(index=18), LAYOUT)])
@@ -62,8 +62,9 @@ def test_workspace_sizes():
     assert lib.qim_attention_cached_workspace_bytes(1, 1, 32, 4, 4) == 0          # nothing to split
     assert lib.qim_attention_cached_workspace_bytes(1, 1, 100000, 4, 4) > 0
     assert lib.qim_attention_cached_workspace_bytes(1, 65, 100000, 4, 4) == 0     # not a shape it takes
-    assert lib.qim_low_rank_workspace_bytes(4, 256, 16) >= 4 * 16 * 4
-    assert lib.qim_low_rank_workspace_bytes(0, 256, 16) == 0
+    assert lib.qim_low_rank_workspace_bytes(400, 1, 256, 16, 3) >= 400 * 48 * 4
+    assert lib.qim_low_rank_workspace_bytes(4, 1, 256, 16, 1) == 0                # one launch
+    assert lib.qim_low_rank_workspace_bytes(0, 1, 256, 16, 1) == 0
 
 
 def cpu_cache(b=1, c=8, h=2, d=128):
