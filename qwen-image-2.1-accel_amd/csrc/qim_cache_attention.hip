@@ -5,9 +5,9 @@
 //   o[r] = sum_t p_rt V[t] / sum_t p_rt,  p_rt = 2^(c q_r . K[t] - m_r)
 //
 // in one pass over the keys with a running maximum m_r and sum (fp32).  The
-// S * G query rows that share a K/V head are the columns of the MFMA tiles, so
-// a key is read once for up to 64 of them.  A row costs 512 flop for a
-// key's 264 bytes; up to about a hundred rows the cache's bytes bound it.
+// S * G query rows that share a K/V head are the columns of the MFMA tiles, 16 or 32
+// to a wave.  A row costs 512 flop for a key's 264 bytes: up to 32 rows the cache's
+// bytes bound it, more rows the waves' work on codes and softmax.
 //
 // Transposed products on v_mfma_f32_16x16x32_bf16, 32 keys at a time: S^T = K Q^T
 // (two tiles of 16 keys x 16 rows) and O^T = V^T P^T (16 head dims x 16 rows per
@@ -35,11 +35,9 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 constexpr int CA_D = 128;
 constexpr int CA_KB = 32;                        // keys per block
 constexpr int CA_VTILE = CA_KB * CA_D * 2;       // 8 KiB of LDS per wave
+constexpr int CA_WAVES = 8;                      // (heads) per workgroup: two per SIMD
 constexpr int CA_MAX_S = 64;
 constexpr int CA_MAX_ROUNDS = 16;
-// Waves (heads) per workgroup: two per SIMD where the registers of a tile of
-// 16 * nr rows allow, else one.
-constexpr int ca_waves(int nr) { return nr <= 2 ? 8 : 4; }
 
 struct CacheAttnArgs {
     const uint16_t *q;
@@ -196,18 +194,17 @@ struct CaRaw {
 // neighbouring waves take neighbouring heads, whose 128-byte pieces are neighbours in
 // memory.  No barrier anywhere.
 template <int NR>
-__global__ __launch_bounds__(64 * ca_waves(NR), NR <= 2 ? 2 : 1) void k_cache_attn(CacheAttnArgs p) {
-    constexpr int WG = ca_waves(NR);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[WG * CA_VTILE];
+__global__ __launch_bounds__(64 * CA_WAVES, 2) void k_cache_attn(CacheAttnArgs p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[CA_WAVES * CA_VTILE];
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t tasks = (uint32_t)(p.HK * p.ntile);
     uint32_t task;
-    const uint32_t group = ca_group((tasks + WG - 1) / WG, task);
+    const uint32_t group = ca_group((tasks + CA_WAVES - 1) / CA_WAVES, task);
     int b = 0;
     int64_t blk0 = 0, per = 1;
     if (!ca_chunk(p, group, blockIdx.x == 0 && wave == 0, b, blk0, per)) return;
-    task = task * WG + wave;
+    task = task * CA_WAVES + wave;
     if (task >= tasks) return;
     const int tile = (int)(task / (uint32_t)p.HK), h = (int)(task - tile * (uint32_t)p.HK);
     const int64_t len = ca_length(p, b);
@@ -488,12 +485,16 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
-// Row tiles of up to 64 rows, and key chunks.  A chunk's heads and row tiles are
-// `wide` workgroups of one XCD, one workgroup to a CU, so `cap` chunks run at a time.  The
-// chunks are to fill r such rounds: in blocks of 32 keys a round costs its chunk's
-// blocks, 1 for its start and rows / 8 for writing and joining its partial results.
-// (16 sequences of up to 263 blocks, 32 heads: 2.95 rounds 172 us, 2.1 rounds 200; 2 sequences
-// of 4096 and 3072 blocks, 8 heads: 249 chunks 88 us, 257 chunks 119.)
+// Row tiles (16 or 32 rows a wave) and key chunks.  A chunk's heads and row tiles are `wide`
+// workgroups of one XCD, one workgroup to a CU, so `cap` chunks run at a time; the chunks
+// are to fill whole rounds.  What is weighed, in ns: a block of 32 keys costs a
+// round the time of its bytes, or that of a wave's work where rows share them
+// (8 waves a CU: 2100 with 16 rows, 3000 with 32); a round 1500 for its start; chunks
+// 5000 for the second launch and their partial results, written and read.  (Batches of 5 x
+// 8040 keys with 64 rows a head, 32 heads: 182 us as 16 rows a wave, 118 as 32;
+// 14 x 428: 39 and 48.  Wider tiles gain nothing: 128 and 53 as 64 rows.  16 sequences of
+// up to 263 blocks, 32 heads: 5 rounds of chunks 167 us, 2.95 172, 2.1 200; 2 of 4096
+// and 3072 blocks, 8 heads: 249 chunks 88 us, 257 chunks 119.)
 struct CaPlan {
     int64_t rows, nr, ntile, wide, chunks, groups, B, HK;
     int64_t grid() const { return (groups + 7) / 8 * 8 * wide; }  // ca_group
@@ -506,22 +507,27 @@ static CaPlan ca_plan(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     pl.B = B;
     pl.HK = HK;
     pl.rows = S * (H / HK);
-    pl.ntile = (pl.rows + 63) / 64;
-    pl.nr = ((pl.rows + pl.ntile - 1) / pl.ntile + 15) / 16;
-    pl.wide = (HK * pl.ntile + ca_waves((int)pl.nr) - 1) / ca_waves((int)pl.nr);
     const int64_t cus = device_cus() > 0 ? device_cus() : 256, nblk = (C + CA_KB - 1) / CA_KB;
-    const int64_t at_once = cus / 8 / pl.wide, cap = 8 * (at_once > 1 ? at_once : 1);
-    int64_t best = (B + cap - 1) / cap * (nblk + 1);  // a sequence per chunk, nothing to join
-    pl.chunks = 0;
-    pl.groups = B;
-    for (int64_t r = 1; r <= CA_MAX_ROUNDS && nblk > 1; ++r) {
-        const int64_t n = r * cap - B;
-        if (n < 1) continue;
-        const int64_t cost = r * ((B * nblk + n - 1) / n + 1 + pl.rows / 8);
-        if (cost < best) {
+    int64_t best = -1;
+    for (int64_t nr = 1; nr <= 2 && (nr - 1) * 16 < pl.rows; ++nr) {
+        const int64_t ntile = (pl.rows + 16 * nr - 1) / (16 * nr), wide = (HK * ntile + CA_WAVES - 1) / CA_WAVES;
+        const int64_t at_once = cus / 8 / wide, cap = 8 * (at_once > 1 ? at_once : 1);
+        // r rounds of chunks; 0: a chunk per sequence and nothing to join.
+        for (int64_t r = 0; r <= CA_MAX_ROUNDS && (r == 0 || nblk > 1); ++r) {
+            const int64_t n = r * cap - B;
+            if (r && n < 1) continue;
+            const int64_t groups = r == 0 ? B : n + B < B * nblk ? n + B : B * nblk;
+            const int64_t rounds = r ? r : (B + cap - 1) / cap, blocks = r ? (B * nblk + n - 1) / n : nblk;
+            const int64_t bytes = (groups < cap ? groups : cap) * HK * CA_KB * 2 * (CA_D + CA_D / 32);
+            const int64_t work = nr == 1 ? 2100 : 3000, block = bytes / 5140 > work ? bytes / 5140 : work;
+            const int64_t cost = rounds * (blocks * block + 1500) + (r ? 5000 + groups * HK * pl.rows * CA_D * 8 / 5140 : 0);
+            if (best >= 0 && cost >= best) continue;
             best = cost;
-            pl.chunks = n;
-            pl.groups = n + B < B * nblk ? n + B : B * nblk;
+            pl.nr = nr;
+            pl.ntile = ntile;
+            pl.wide = wide;
+            pl.chunks = r ? n : 0;
+            pl.groups = groups;
         }
     }
     return pl;
@@ -533,7 +539,7 @@ using namespace qim;
 
 static bool ca_shape(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     return B > 0 && S > 0 && S <= CA_MAX_S && C > 0 && C < (1ll << 31) && HK > 0 && H > 0 && H % HK == 0 && H <= (1 << 16) && B < (1 << 20) &&
-           B * HK * ((S * (H / HK) + 31) / 32) < (1 << 24) && ca_plan(B, S, C, H, HK).grid() < (1ll << 31);
+           B * HK * ((S * (H / HK) + 15) / 16) < (1 << 25) && B * C < (1ll << 40) / HK && ca_plan(B, S, C, H, HK).grid() < (1ll << 31);
 }
 
 extern "C" int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
@@ -558,14 +564,14 @@ extern "C" int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, co
     QIM_REQUIRE(pl.bytes() == 0 || (workspace && workspace_bytes >= pl.bytes()), QIM_ERR_ARG,
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)pl.bytes());
     QIM_REQUIRE(aligned16(workspace), QIM_ERR_LAYOUT, "%s: workspace must be 16-byte aligned", who);
-    void (*const fn)(CacheAttnArgs) = pl.nr == 1 ? k_cache_attn<1> : pl.nr == 2 ? k_cache_attn<2> : pl.nr == 3 ? k_cache_attn<3> : k_cache_attn<4>;
+    void (*const fn)(CacheAttnArgs) = pl.nr == 1 ? k_cache_attn<1> : k_cache_attn<2>;
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     CacheAttnArgs a{(const uint16_t *)q, ldqb, ldq, (const uint8_t *)kc, (const uint8_t *)ks, (const uint8_t *)vc,
                     (const uint8_t *)vs, lengths, (const uint8_t *)tree, tree_b, (uint16_t *)o, (float *)ws,
                     (float2 *)(ws + pl.part_o()), C, (int2 *)(ws + pl.part_o() + pl.part_ml()), (int)B, (int)S, (int)H,
                     (int)HK, (int)(H / HK), (int)pl.rows, (int)pl.ntile, (int)pl.chunks,
                     scale * 1.4426950408889634f};
-    launch(fn, dim3((unsigned)pl.grid()), dim3(64 * ca_waves((int)pl.nr)), 0, as_stream(stream), a);
+    launch(fn, dim3((unsigned)pl.grid()), dim3(64 * CA_WAVES), 0, as_stream(stream), a);
     if (pl.chunks) {
         // Few rows of many chunks: a quarter row per workgroup, 32 chunks at once.
         const int64_t nrows = B * HK * pl.rows, each = pl.groups / B;
