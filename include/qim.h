@@ -319,7 +319,7 @@ int qim_cache_read(const void *kc, const void *ks, const void *vc, const void *v
  * [0, P) of each sequence, P <= C, in place of ck, cv.  The rotated rows are
  * rounded to bf16 once, at their end (the bf16 form rounds after the
  * normalisation and after its weight too, as the reference's operators do).  v
- * and ov are required; D in {64, 128, 256}. */
+ * and ov are required, the cache where P > 0; D in {64, 128, 256}. */
 int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, const void *kc, const void *ks,
                                  const void *vc, const void *vs, int64_t C, const void *wq, const void *wk,
                                  const void *freqs, void *oq, void *ok, void *ov, int64_t B, int64_t S,
@@ -335,7 +335,7 @@ int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, co
  * tree[i * S + j] != 0 (drafted tokens: itself and its ancestors).  A row that
  * sees no key is zeros.  q: (B, S, H, D) bf16, packed heads, ldqb / ldq elements
  * between sequences / tokens (multiples of 8, 16-byte aligned); o: (B, S, H,
- * D) contiguous.  1 <= S <= 64, H % HK == 0, scale > 0.  fp32 scores, softmax and
+ * D) contiguous, apart from q.  1 <= S <= 64, H % HK == 0, scale > 0.  fp32 scores, softmax and
  * accumulation; the probabilities are rounded to bf16 for the product with V.
  * workspace: qim_attention_cached_workspace_bytes(B, S, C, H, HK) bytes,
  * 16-byte aligned (partial results where the keys are split; may be NULL when
@@ -354,9 +354,10 @@ int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, in
  * adapter; scale: device fp32 (A,) or NULL (1).  parts > 1: N is parts equal
  * column blocks and block j uses rows [j * R, (j + 1) * R) of down (a stacked
  * Q/K/V projection in one call).  base: (M, N) bf16, row stride ldb, or NULL
- * (zeros); out: (M, N), row stride ldo; out may be base.  K, R and N / parts are
- * multiples of 8, R <= 128; all operands 16-byte aligned.  A request's values
- * never enter another's rows, whatever they are.  workspace:
+ * (zeros); out: (M, N), row stride ldo; out may be base, with its stride, and is else
+ * apart from base and x (other columns of one buffer are).  K, R and N / parts
+ * are multiples of 8, R <= 128; all operands 16-byte aligned.  A request's
+ * values never enter another's rows, whatever they are.  workspace:
  * qim_low_rank_workspace_bytes(M, seq, K, R, parts) bytes, 16-byte aligned (may
  * be NULL when that is 0), not shared by calls that may overlap.  No reference
  * counterpart. */

@@ -564,6 +564,9 @@ extern "C" int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, co
     QIM_REQUIRE(pl.bytes() == 0 || (workspace && workspace_bytes >= pl.bytes()), QIM_ERR_ARG,
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)pl.bytes());
     QIM_REQUIRE(aligned16(workspace), QIM_ERR_LAYOUT, "%s: workspace must be 16-byte aligned", who);
+    // Rows are written while others are still read.
+    const char *q0 = (const char *)q, *q1 = q0 + 2 * ((B - 1) * ldqb + (S - 1) * ldq + H * D), *o0 = (const char *)o;
+    QIM_REQUIRE(q1 <= o0 || o0 + 2 * B * S * H * D <= q0, QIM_ERR_ARG, "%s: o overlaps q", who);
     void (*const fn)(CacheAttnArgs) = pl.nr == 1 ? k_cache_attn<1> : k_cache_attn<2>;
     uint8_t *const ws = static_cast<uint8_t *>(workspace);
     CacheAttnArgs a{(const uint16_t *)q, ldqb, ldq, (const uint8_t *)kc, (const uint8_t *)ks, (const uint8_t *)vc,

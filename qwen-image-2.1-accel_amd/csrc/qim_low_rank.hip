@@ -526,6 +526,16 @@ static bool lr_small(int64_t M, int64_t seq, int64_t K, int64_t R) {
 // The K chunks of a problem do not depend on N or the adapters.
 static int64_t lr_chunks(int64_t M, int64_t K, int64_t PR) { return lr_plan(M, 1, K, PR, 8, 1, 1).chunks; }
 
+// Whether rows of out share memory with the rows of t, (M, W): ranges that meet, other than
+// other columns of one buffer.
+static bool lr_shares(const void *out, int64_t ldo, int64_t N, const void *t, int64_t ldt, int64_t W, int64_t M) {
+    const int64_t d = (int64_t)((intptr_t)t - (intptr_t)out) / 2;  // both 16-byte aligned
+    if (d >= (M - 1) * ldo + N || -d >= (M - 1) * ldt + W) return false;
+    if (M == 1 || ldt != ldo) return true;
+    const int64_t col = (d % ldo + ldo) % ldo;
+    return col < N || col + W > ldo;
+}
+
 }  // namespace qim
 
 using namespace qim;
@@ -560,6 +570,9 @@ extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const 
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)need);
     const int64_t up_tiles = (M + 16 * LR_MT - 1) / (16 * LR_MT);
     QIM_REQUIRE(up_tiles * pl.nchunk * parts < (1ll << 31) && pl.tiles * pl.chunks < (1ll << 31) && pl.slots * pl.rblocks < 65536, QIM_ERR_SHAPE, "%s: too large", who);
+    QIM_REQUIRE(!lr_shares(out, ldo, N, x, ldx, K, M) &&
+                    (!base || (base == out && (ldb == ldo || M == 1)) || !lr_shares(out, ldo, N, base, ldb, N, M)),
+                QIM_ERR_ARG, "%s: out overlaps x, or base other than as the same rows", who);
     LowRankArgs a{(const uint16_t *)x, (const uint16_t *)down, (const uint16_t *)up, (const uint16_t *)base, index, scale,
                   (uint16_t *)out, (float *)workspace, ldx, ldb, ldo, M, (uint32_t)(seq < M ? seq : M), (int)K, (int)N, (int)R,
                   (int)PR, (int)parts, (int)A, (int)pl.chunks, (int)pl.kchunk, pl.ncols, (int)pl.nchunk};

@@ -741,18 +741,18 @@ extern "C" int qim_rope_qk(const void *q, const void *k, const void *freqs, void
 }
 
 // The checks that both forms of the pack share, and the launch.
-static int norm_rope_pack(const char *who, NormRopeArgs a, int64_t B, int64_t D, bool prefix, void *stream) {
+static int norm_rope_pack(const char *who, NormRopeArgs a, int64_t B, int64_t D, bool q8, void *stream) {
     QIM_REQUIRE(a.q && a.k && a.wq && a.wk && a.freqs && a.oq && a.ok, QIM_ERR_ARG, "%s: null pointer", who);
     QIM_REQUIRE(B > 0 && a.S > 0 && a.H > 0 && a.P >= 0, QIM_ERR_SHAPE, "%s: empty input", who);
     QIM_REQUIRE((a.v == nullptr) == (a.ov == nullptr), QIM_ERR_ARG, "%s: v and ov go together", who);
-    QIM_REQUIRE(a.P == 0 || (prefix && a.v), QIM_ERR_ARG, "%s: a prefix (P > 0) needs its K and V, v and ov", who);
+    QIM_REQUIRE(a.P == 0 || (a.v && (q8 ? a.kc && a.ks && a.vc && a.vs : a.ck && a.cv)), QIM_ERR_ARG, "%s: a prefix (P > 0) needs its K and V, v and ov", who);
     QIM_REQUIRE(a.ldt >= a.H * D && a.ldt % 8 == 0, QIM_ERR_LAYOUT, "%s: token stride %lld < H*D or not a multiple of 8",
                 who, (long long)a.ldt);
     const void *ptrs[] = {a.q, a.k, a.v, a.ck, a.cv, a.wq, a.wk, a.freqs, a.oq, a.ok, a.ov, a.kc, a.ks, a.vc, a.vs};
     for (const void *pp : ptrs)
         QIM_REQUIRE(!pp || aligned16(pp), QIM_ERR_LAYOUT, "%s: operands must be 16-byte aligned", who);
     a.T = B * a.S;
-    int rc = a.kc  ? launch_norm_rope<true, true, 3, true>(a, D, B, as_stream(stream))
+    int rc = q8    ? launch_norm_rope<true, true, 3, true>(a, D, B, as_stream(stream))
              : a.v ? launch_norm_rope<true, true, 3>(a, D, B, as_stream(stream))
                    : launch_norm_rope<true, true, 2>(a, D, B, as_stream(stream));
     return rc ? rc : check_launch(who);
@@ -765,7 +765,7 @@ extern "C" int qim_qk_norm_rope_pack(const void *q, const void *k, const void *v
     NormRopeArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, (const uint16_t *)ck,
                    (const uint16_t *)cv, (const uint16_t *)wq, (const uint16_t *)wk, (const float *)freqs,
                    (uint16_t *)oq, (uint16_t *)ok, (uint16_t *)ov, 0, S, P, H, ldt, epsq, epsk, 0, 0, 0};
-    return norm_rope_pack("qim_qk_norm_rope_pack", a, B, D, ck && cv, stream);
+    return norm_rope_pack("qim_qk_norm_rope_pack", a, B, D, false, stream);
 }
 
 extern "C" int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, const void *kc, const void *ks,
@@ -773,7 +773,7 @@ extern "C" int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const 
                                             const void *freqs, void *oq, void *ok, void *ov, int64_t B, int64_t S,
                                             int64_t P, int64_t H, int64_t D, int64_t ldt, float epsq, float epsk,
                                             void *stream) {
-    QIM_REQUIRE(v && kc && ks && vc && vs, QIM_ERR_ARG, "qim_qk_norm_rope_pack_cached: null pointer");
+    QIM_REQUIRE(v, QIM_ERR_ARG, "qim_qk_norm_rope_pack_cached: null pointer");
     QIM_REQUIRE(P <= C, QIM_ERR_ARG, "qim_qk_norm_rope_pack_cached: %lld rows of a cache of %lld", (long long)P,
                 (long long)C);
     NormRopeArgs a{(const uint16_t *)q, (const uint16_t *)k, (const uint16_t *)v, nullptr, nullptr,

@@ -40,20 +40,21 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     or (B,) for (B, S, K), one per sequence; a row whose entry is outside
     [0, A) (-1 by convention) has no adapter.  ``scale``: None or fp32 (A,).
     ``base``: the projection's output, (M, N) or (B, S, N) bf16, or None
-    (zeros); ``out``: where the result goes (``base`` itself is fine), by default a new tensor.
+    (zeros); ``out``: where the result goes, by default a new tensor; ``base`` itself is fine, else it
+    shares no rows with ``base`` or ``x``.
     ``parts``: N is that many equal column blocks, and block j uses rows
     [j * R, (j + 1) * R) of down: the adapters of a stacked projection (Q/K/V,
     gate/up) in one call.  The sum is taken in fp32 and rounded once.  K, R and
     N / parts are multiples of 8; rows may lie any multiple of 8 elements apart.
-    A row's result depends on its own x, base and adapter only."""
+    A row's result depends on its own x, base and adapter only.  No gradient is recorded."""
     def refuse(why):
         raise _native.Unsupported("low_rank", _native.QIM_ERR_LAYOUT, why)
     device = x.device
     if not x.is_cuda:
         refuse("expects tensors on the GPU")
     xr = _rows(x)
-    if x.dtype != torch.bfloat16 or xr is None:
-        refuse("x is a bf16 (M, K) or (B, S, K) tensor with rows one stride apart")
+    if x.dtype != torch.bfloat16 or xr is None or xr[1] == 0:
+        refuse("x is a bf16 (M, K) or (B, S, K) tensor, K > 0, with rows one stride apart")
     m, k, ldx = xr
     if (down.dim() != 3 or up.dim() != 3 or down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16
             or not down.is_contiguous() or not up.is_contiguous() or down.device != device or up.device != device

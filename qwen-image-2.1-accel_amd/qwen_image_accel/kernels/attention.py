@@ -108,7 +108,7 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
     (S, S): of the last S keys, query i sees key j only where tree[..., i, j]
     (drafted tokens: itself and its ancestors; a causal step: the lower
     triangle).  A row that sees no key is zeros.  scale defaults to
-    1/sqrt(128).  Returns (B, S, H, 128) bf16.  For the queries of a whole image,
+    1/sqrt(128).  Returns (B, S, H, 128) bf16 (``out``, if given: contiguous, apart from q).  For the queries of a whole image,
     stage the prefix (``prepare_attention_inputs_quantized``) and use
     ``attention``."""
     b, c, kv, d = kv_cache.check_cache("attention_cached", cache)

@@ -20,11 +20,12 @@ NO_ADAPTER = -1
 class AdapterRoute:
     """Which adapter each sequence of the batch uses: ``index``, int32 (B,), an
     adapter's number or -1, or None while nothing is selected (no adapter
-    anywhere).  The tensor keeps its place from one ``select`` of the same
-    batch size to the next, so a captured step follows the selection."""
+    anywhere).  Each batch size has one tensor, kept from its first ``select``
+    on, so a step captured with a selection follows the later ones of its batch size."""
 
     def __init__(self, names, device):
         self.names, self.device, self.index = tuple(names), torch.device(device), None
+        self._by_batch = {}
 
     def select(self, names):
         """``names``: one adapter name (or None) per sequence of the batch;
@@ -38,15 +39,14 @@ class AdapterRoute:
                 raise ValueError(f"unknown adapter {name!r}; installed: {list(self.names)}")
             numbers.append(NO_ADAPTER if name is None else self.names.index(name))
         new = torch.tensor(numbers, dtype=torch.int32, device=self.device)
-        if self.index is not None and self.index.shape == new.shape:
+        self.index = self._by_batch.setdefault(len(numbers), new)
+        if self.index is not new:
             self.index.copy_(new)
-        else:
-            self.index = new
 
 
 class AdapterStack(nn.Module):
     """The adapters of one projection, stacked: down (A, parts * R, K), up (A, N,
-    R), scale (A,).  An adapter of a smaller rank is padded with zeros, one that
+    R) in bf16, scale (A,).  An adapter of a smaller rank is padded with zeros, one that
     does not touch this projection is zeros with scale 0."""
 
     def __init__(self, down, up, scale, parts=1):
@@ -60,7 +60,7 @@ class AdapterStack(nn.Module):
     def of(cls, triples, out_features, in_features, device):
         """``triples``: per adapter (down (r, K), up (N, r), scale) or None."""
         ranks = [t[0].shape[0] for t in triples if t is not None]
-        r = (max(ranks) + 7) // 8 * 8
+        r = max(8, (max(ranks) + 7) // 8 * 8)
         if r > MAX_RANK:
             raise ValueError(f"adapter rank {max(ranks)} is above {MAX_RANK}")
         down = torch.zeros(len(triples), r, in_features, dtype=torch.bfloat16, device=device)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from qwen_image_accel import _native
 from qwen_image_accel.kernels import attention, kv_cache
 from tests import requests_ref as R
 from tests.helpers import bf16_randn
@@ -69,6 +70,32 @@ def test_tree(dev, b, s, h, hk, c, lengths, shared):
     tree = tree[0].contiguous() if shared else tree
     n = lens(lengths, dev)
     check(attention.attention_cached(q, cache, n, tree=tree.to(dev)), q, cache, n, tree)
+
+
+@pytest.mark.parametrize("b,c", [(70, 600), (130, 1000), (300, 90)])
+def test_batches_of_many_unequal_sequences(dev, b, c):
+    """More sequences than a wave has lanes, of lengths from 0 to all, in chunks or one each."""
+    say("many sequences", b, c)
+    q, cache = make(dev, b, 1, 2, 2, c, seed=b)
+    n = torch.randint(0, c + 1, (b,), generator=torch.Generator().manual_seed(c), dtype=torch.int32)
+    n[::9], n[1], n[-1] = 0, c, c - 31
+    n = n.to(dev)
+    check(attention.attention_cached(q, cache, n), q, cache, n)
+
+
+def test_long_cache_with_more_rows_than_a_tile(dev):
+    say("tiles of 32 rows, chunks")
+    b, s, c = 5, 40, 8000
+    q, cache = make(dev, b, s, 8, 8, c)
+    tree, n = random_tree(b, s, 3), lens([3001, 100, 33, 40, 0], dev)
+    check(attention.attention_cached(q, cache, n, tree=tree.to(dev)), q, cache, n, tree)
+
+
+def test_out_over_q_is_refused(dev):
+    say("out over q")
+    q, cache = make(dev, 2, 3, 2, 2, 64)
+    with pytest.raises(_native.QimError, match="overlaps"):
+        attention.attention_cached(q, cache, lens([64, 5], dev), out=q)
 
 
 def test_causal_equals_one_token_at_a_time(dev):

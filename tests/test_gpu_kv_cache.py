@@ -182,3 +182,18 @@ def test_pack(dev, b, s, p, h, d, view):
         mag = torch.stack([z.real.abs() * f.real.abs() + z.imag.abs() * f.imag.abs(),
                            z.real.abs() * f.imag.abs() + z.imag.abs() * f.real.abs()], -1).flatten(-2)
         assert ((got.double() - want).abs() <= R.HALF * want.abs() + (1 + R.HALF) * 16 * R.F32 * mag).all()
+
+
+def test_pack_without_a_prefix(dev):
+    """No positions of a cache, or a cache of none: the step's own rows, the same values."""
+    say("pack, no prefix")
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (bf16_randn(g, (2, 9, 3, 128)).to(dev) for _ in range(3))
+    norms = [types.SimpleNamespace(weight=bf16_randn(g, (128,)).to(dev), eps=1e-6, bias=None) for _ in range(2)]
+    freqs = torch.polar(torch.ones(9, 64), torch.randn(9, 64, generator=g)).to(dev)
+    some = attention.prepare_attention_inputs_quantized(q, k, v, *norms, freqs, filled(2, 4, 3, 128, dev), prefix=0)
+    none = attention.prepare_attention_inputs_quantized(q, k, v, *norms, freqs, kv_cache.empty_cache(2, 0, 3, 128, dev))
+    whole = attention.prepare_attention_inputs_quantized(q, k, v, *norms, freqs, filled(2, 4, 3, 128, dev))
+    for a, b, c, skip in zip(some, none, whole, (0, 4, 4)):
+        assert torch.equal(a, b) and torch.equal(a, c[:, skip:])
+    assert torch.equal(some[2], v)

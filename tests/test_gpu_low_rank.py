@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from qwen_image_accel import _native
 from qwen_image_accel.kernels import adapters
 from tests import requests_ref as R
 from tests.helpers import bf16_randn
@@ -78,6 +79,25 @@ def test_in_place_strided_and_views(dev):
     assert adapters.low_rank(wide_x[:, 16:272], down, up, index, scale=scale, base=y, out=y) is y
     assert torch.equal(y, want)
     assert (wide[:, :8] == 5).all() and (wide[:, 144:] == 5).all()
+
+
+@pytest.mark.parametrize("m", [9, 90])
+def test_out_beside_x_and_over_other_rows(dev, m):
+    """x, base and out as columns of one buffer; rows of out that are others' rows of x or base are refused."""
+    say("shared buffer", m)
+    x, down, up, scale, base, index = make(dev, m, 128, 128, 8, 3)
+    want = adapters.low_rank(x, down, up, index, scale=scale, base=base)
+    buf = torch.cat([x, base, torch.zeros_like(base)], 1)
+    bx, bb, bo = buf[:, :128], buf[:, 128:256], buf[:, 256:]
+    assert torch.equal(adapters.low_rank(bx, down, up, index, scale=scale, base=bb, out=bo), want)
+    assert torch.equal(bx, x) and torch.equal(bb, base)
+    tall = torch.zeros(m + 1, 128, dtype=torch.bfloat16, device=dev)
+    for kw in (dict(x=x, base=base, out=x), dict(x=x, base=tall[1:], out=tall[:-1]), dict(x=tall[:-1], base=base, out=tall[1:]),
+               dict(x=bx, base=bb, out=buf[:, 64:192])):
+        with pytest.raises(_native.QimError, match="overlaps"):
+            adapters.low_rank(kw["x"], down, up, index, scale=scale, base=kw["base"], out=kw["out"])
+    with pytest.raises(_native.Unsupported):
+        adapters.low_rank(x[:, :0], down[:, :, :0].contiguous(), up, index, base=base)
 
 
 def test_entries_outside_the_adapters_mean_none(dev):

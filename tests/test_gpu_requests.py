@@ -155,6 +155,25 @@ def test_adapters_on_the_cpu_equal_merged_weights():
     assert type(t.transformer_blocks[0].attn.to_q) is torch.nn.Linear
 
 
+def test_each_batch_size_keeps_its_route_tensor():
+    """A step captured at one batch size reads the tensor that later selections of that size write."""
+    route = install.AdapterRoute(("a", "b"), "cpu")
+    route.select(["b", None])
+    two = route.index
+    route.select(["a"] * 3)
+    assert route.index.tolist() == [0, 0, 0]
+    route.select(None)
+    assert route.index is None
+    route.select(["a", "b"])
+    assert route.index is two and two.tolist() == [0, 1]
+
+
+def test_an_adapter_of_rank_zero_adds_nothing():
+    stack = install.AdapterStack.of([(torch.zeros(0, 16), torch.zeros(24, 0), 1.0), None], 24, 16, "cpu")
+    y = torch.randn(2, 3, 24)
+    assert torch.equal(stack.add(torch.randn(2, 3, 16), y.clone(), torch.tensor([0, 1])), y)
+
+
 def test_adapter_refusals():
     t = fq.make_transformer()
     ok = (torch.zeros(4, 256), torch.zeros(256, 4), 1.0)

@@ -49,7 +49,11 @@ def adapt(x=16, ldx=256, down=16, index=16, base=16, ldb=512, out=16, ldo=512, w
     (adapt(x=None), ARG), (adapt(index=None), ARG), (adapt(ws=None, m=40), ARG), (adapt(nbytes=15, m=40), ARG), (adapt(m=0), SHAPE),
     (adapt(seq=0), SHAPE), (adapt(k=260), SHAPE), (adapt(r=12), SHAPE), (adapt(r=136), SHAPE), (adapt(parts=3), SHAPE),
     (adapt(n=516), SHAPE), (adapt(ldx=128), LAYOUT), (adapt(ldb=500), LAYOUT), (adapt(ldo=516), LAYOUT), (adapt(x=8), LAYOUT),
-    (adapt(down=24), LAYOUT), (adapt(out=8), LAYOUT), (adapt(index=18), LAYOUT)])
+    (adapt(down=24), LAYOUT), (adapt(out=8), LAYOUT), (adapt(index=18), LAYOUT),
+    # out over x, over base's rows at another place or stride, and over q
+    (adapt(out=1 << 20, base=1 << 20, x=(1 << 20) + 1024), ARG), (adapt(out=1 << 20, base=(1 << 20) + 1024), ARG),
+    (adapt(out=1 << 20, base=1 << 20, ldb=520), ARG), (adapt(out=1 << 20, ldo=1024, base=(1 << 20) + 1008, ldb=1024), ARG),
+    (attend(o=528), ARG), (attend(q=528, o=16), ARG)])
 def test_entry_points_refuse(call, code):
     name, args = call
     rc = getattr(_native.lib(), name)(*args)
