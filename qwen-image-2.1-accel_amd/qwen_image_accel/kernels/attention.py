@@ -113,11 +113,13 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
     ``attention``."""
     b, c, kv, d = kv_cache.check_cache("attention_cached", cache)
     device = cache.k.device
-    if (q.dim() != 4 or q.dtype != torch.bfloat16 or q.device != device or q.shape[0] != b or q.shape[3] != d
-            or kv_cache.token_strides(q) is None):
+    shape = q.shape
+    strides = (kv_cache.token_strides(q) if len(shape) == 4 and q.dtype == torch.bfloat16 and q.device == device
+               and shape[0] == b and shape[3] == d else None)
+    if strides is None:
         raise _native.Unsupported("attention_cached", _native.QIM_ERR_LAYOUT,
                                   f"q is a bf16 ({b}, S, H, {d}) tensor with packed heads on {device}")
-    s, h = q.shape[1], q.shape[2]
+    s, h = shape[1], shape[2]
     size = kv_cache.per_sequence("attention_cached", "lengths", lengths, b, device)
     mask, mask_b = None, 0
     if tree is not None:
@@ -127,13 +129,13 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
         mask, mask_b = tree.data_ptr(), s * s if tree.dim() == 3 else 0
     if out is None:
         out = torch.empty((b, s, h, d), dtype=torch.bfloat16, device=device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != device or not out.is_contiguous():
+    elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} tensor on {device}")
-    if out.numel() == 0:
+    if not (b and s and h and d):
         return out
     nbytes = _native.bytes_on(device, "qim_attention_cached_workspace_bytes", b, s, c, h, kv)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    _native.call_on(device, "qim_attention_cached", q.data_ptr(), *kv_cache.token_strides(q), cache.k.data_ptr(),
+    _native.call_on(device, "qim_attention_cached", q.data_ptr(), *strides, cache.k.data_ptr(),
                     cache.k_exponent.data_ptr(), cache.v.data_ptr(), cache.v_exponent.data_ptr(), size, mask, mask_b,
                     out.data_ptr(), _native.ptr(ws), nbytes, b, s, c, h, kv, d,
                     float(scale if scale is not None else d ** -0.5))

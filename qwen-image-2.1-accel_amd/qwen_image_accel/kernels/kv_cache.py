@@ -68,10 +68,12 @@ def token_strides(t):
     tensor with packed heads, else None.  The stride of an axis of one element
     says nothing and is not looked at."""
     b, s, h, d = t.shape
-    if (d > 1 and t.stride(3) != 1) or (h > 1 and t.stride(2) != d):
+    batch, token, head, one = t.stride()
+    if (d > 1 and one != 1) or (h > 1 and head != d):
         return None
-    token = t.stride(1) if s > 1 else h * d
-    return (t.stride(0) if b > 1 else s * token), token
+    if s == 1:
+        token = h * d
+    return (batch if b > 1 else s * token), token
 
 
 def write_cache(cache, k, v, start=0, count=None):
@@ -86,22 +88,24 @@ def write_cache(cache, k, v, start=0, count=None):
     any token and batch stride (e.g. views into a fused QKV output)."""
     b, c, h, d = check_cache("write_cache", cache)
     device = cache.k.device
+    shape = k.shape
+    s = shape[1] if len(shape) == 4 else 0
+    strides = ()
     for t in (k, v):
-        if (t.dtype != torch.bfloat16 or t.device != device or t.dim() != 4 or t.shape[0] != b or t.shape[2:] != (h, d)
-                or t.shape[1] != k.shape[1] or token_strides(t) is None):
+        step = token_strides(t) if t.dtype == torch.bfloat16 and t.device == device and t.shape == (b, s, h, d) else None
+        if step is None:
             raise _native.Unsupported("write_cache", _native.QIM_ERR_LAYOUT,
                                       f"k and v are bf16 ({b}, S, {h}, {d}) tensors with packed heads on {device}")
-    s = k.shape[1]
-    if k.numel() == 0:
+        strides += step
+    if not (b and s and h and d):
         return
     counts = None if count is None else per_sequence("write_cache", "count", count, b, device)
     if isinstance(start, torch.Tensor):
         starts, first = per_sequence("write_cache", "start", start, b, device), 0
     else:
         starts, first = None, int(start)
-    _native.call_on(device, "qim_cache_write", k.data_ptr(), *token_strides(k), v.data_ptr(),
-                    *token_strides(v), cache.k.data_ptr(), cache.k_exponent.data_ptr(), cache.v.data_ptr(),
-                    cache.v_exponent.data_ptr(), starts, first, counts, b, s, c, h, d)
+    _native.call_on(device, "qim_cache_write", k.data_ptr(), *strides[:2], v.data_ptr(), *strides[2:],
+                    cache.k.data_ptr(), cache.k_exponent.data_ptr(), cache.v.data_ptr(), cache.v_exponent.data_ptr(), starts, first, counts, b, s, c, h, d)
 
 
 def read_cache(cache, rows=None):
