@@ -16,20 +16,22 @@ MAX_RANK = 128
 def _rows(t):
     """(rows, width, row stride) of a (M, W) or (B, S, W) tensor whose rows lie
     one stride apart, else None.  An axis of one element may have any stride."""
-    if t.dim() not in (2, 3):
+    shape = t.shape
+    if len(shape) not in (2, 3):
         return None
-    w = t.shape[-1]
+    w = shape[-1]
+    rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
     if t.is_contiguous():
-        return t.numel() // w if w else 0, w, w
+        return rows, w, w
     if w > 1 and t.stride(-1) != 1:
         return None
-    if t.dim() == 2:
-        return t.shape[0], w, t.stride(0) if t.shape[0] > 1 else w
-    b, s = t.shape[:2]
+    if len(shape) == 2:
+        return rows, w, t.stride(0) if rows > 1 else w
+    b, s = shape[:2]
     row = t.stride(1) if s > 1 else t.stride(0) if b > 1 else w
     if b > 1 and s > 1 and t.stride(0) != s * row:
         return None
-    return b * s, w, row
+    return rows, w, row
 
 
 def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
@@ -53,34 +55,38 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     if not x.is_cuda:
         refuse("expects tensors on the GPU")
     xr = _rows(x)
-    if x.dtype != torch.bfloat16 or xr is None or xr[1] == 0:
+    bf16, lead = torch.bfloat16, x.shape[:-1]
+    if x.dtype != bf16 or xr is None or xr[1] == 0:
         refuse("x is a bf16 (M, K) or (B, S, K) tensor, K > 0, with rows one stride apart")
     m, k, ldx = xr
-    if (down.dim() != 3 or up.dim() != 3 or down.dtype != torch.bfloat16 or up.dtype != torch.bfloat16
-            or not down.is_contiguous() or not up.is_contiguous() or down.device != device or up.device != device
-            or down.shape[0] != up.shape[0] or down.shape[2] != k or parts < 1 or down.shape[1] != parts * up.shape[2]):
+    if (up.dim() != 3 or down.dtype != bf16 or up.dtype != bf16 or parts < 1
+            or down.shape != (up.shape[0], parts * up.shape[2], k) or not down.is_contiguous() or not up.is_contiguous()
+            or down.device != device or up.device != device):
         refuse(f"down (A, {parts} * R, {k}) and up (A, N, R) are contiguous bf16 tensors on {device}")
     a, n, r = up.shape
-    if (index.dtype != torch.int32 or index.device != device or index.shape != x.shape[:1] or not index.is_contiguous()):
+    if index.dtype != torch.int32 or index.device != device or index.shape != lead[:1] or not index.is_contiguous():
         refuse(f"index is a contiguous int32 ({x.shape[0]},) tensor on {device}")
     if scale is not None and (scale.dtype != torch.float32 or scale.shape != (a,) or scale.device != device
                               or not scale.is_contiguous()):
         refuse(f"scale is a contiguous fp32 ({a},) tensor on {device}")
-    shape = x.shape[:-1] + (n,)
-    if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-    strides = []
-    for t in (base, out):
-        rows = None if t is None else _rows(t)
-        if t is not None and (t.dtype != torch.bfloat16 or t.shape != shape or t.device != device or rows is None):
+    shape = lead + (n,)
+
+    def stride(t):
+        rows = _rows(t)
+        if rows is None or t.dtype != bf16 or t.shape != shape or t.device != device:
             refuse(f"base and out are bf16 {tuple(shape)} tensors on {device} with rows one stride apart")
-        strides.append(rows[2] if rows else 0)
+        return rows[2]
+    ldb = 0 if base is None else stride(base)
+    if out is None:
+        out, ldo = torch.empty(shape, dtype=bf16, device=device), n
+    else:
+        ldo = ldb if out is base else stride(out)
     if m == 0 or n == 0:
         return out
-    seq = x.shape[1] if x.dim() == 3 else 1
+    seq = lead[1] if len(lead) == 2 else 1
     nbytes = _native.bytes_on(device, "qim_low_rank_workspace_bytes", m, seq, k, r, parts)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _native.call_on(device, "qim_low_rank", x.data_ptr(), ldx, down.data_ptr(), up.data_ptr(), index.data_ptr(),
-                    _native.ptr(scale), _native.ptr(base), strides[0], out.data_ptr(), strides[1], _native.ptr(ws), nbytes,
+                    _native.ptr(scale), _native.ptr(base), ldb, out.data_ptr(), ldo, _native.ptr(ws), nbytes,
                     m, seq, k, n, r, parts, a)
     return out
