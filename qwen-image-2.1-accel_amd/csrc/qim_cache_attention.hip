@@ -490,16 +490,16 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
 }
 
-// Row tiles (16 or 32 rows a wave) and key chunks.  A chunk's heads and row tiles are `wide`
-// workgroups of one XCD, one workgroup to a CU, so `cap` chunks run at a time; the chunks
-// are to fill whole rounds.  What is weighed, in ns: a block of 32 keys costs a
-// round the time of its bytes, or that of a wave's work where rows share them
-// (8 waves a CU: 2100 with 16 rows, 3000 with 32); a round 1500 for its start; chunks
-// 5000 for the second launch and their partial results, written and read.  (Batches of 5 x
-// 8040 keys with 64 rows a head, 32 heads: 182 us as 16 rows a wave, 118 as 32;
-// 14 x 428: 39 and 48.  Wider tiles gain nothing: 128 and 53 as 64 rows.  16 sequences of
-// up to 263 blocks, 32 heads: 5 rounds of chunks 167 us, 2.95 172, 2.1 200; 2 of 4096
-// and 3072 blocks, 8 heads: 249 chunks 88 us, 257 chunks 119.)
+// Row tiles (16 or 32 rows a wave) and key chunks.  A chunk's heads and row tiles are
+// `wide` workgroups of one XCD, one workgroup to a CU, so `cap` chunks run at a time;
+// the chunks are to fill whole rounds.  What is weighed, in ns: a block of 32 keys
+// costs a round the time of its bytes, or that of a wave's work where rows share them
+// (8 waves a CU: 2100 with 16 rows, 3000 with 32); a round 1500 for its start;
+// chunks 5000 for the second launch and their partial results, written and read.
+// (5 sequences of up to 8040 keys, 64 rows a head, 32 heads: 182 us as 16 rows a wave,
+// 118 as 32; 14 of up to 428: 39 and 48.  Wider tiles gain nothing: 128 and 53 as 64
+// rows.  16 of up to 8392, one row: 5 rounds of chunks 168 us, 2.95 172, 2.1 200; 2 of up to
+// 131072, 8 heads: 249 chunks 88 us, 257 chunks 119.)
 struct CaPlan {
     int64_t rows, nr, ntile, wide, chunks, groups, B, HK;
     int64_t grid() const { return (groups + 7) / 8 * 8 * wide; }  // ca_group
