@@ -336,7 +336,8 @@ int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, co
  * sees no key is zeros.  q: (B, S, H, D) bf16, packed heads, ldqb / ldq elements
  * between sequences / tokens (multiples of 8, 16-byte aligned); o: (B, S, H,
  * D) contiguous, apart from q.  1 <= S <= 64, H % HK == 0, scale > 0.  fp32 scores, softmax and
- * accumulation; the probabilities are rounded to bf16 for the product with V.
+ * accumulation; the probabilities enter the product with V as two bf16 terms
+ * (16 significand bits).
  * workspace: qim_attention_cached_workspace_bytes(B, S, C, H, HK) bytes,
  * 16-byte aligned (partial results where the keys are split; may be NULL when
  * that is 0), not shared by calls that may overlap. */

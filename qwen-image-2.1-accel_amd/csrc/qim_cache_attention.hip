@@ -26,8 +26,8 @@
 //
 // One row a head: 16 sequences of up to 8392 keys, 32 heads, 168 us (869 MB, 5.2 TB/s); 2 of
 // up to 131072 with 8 K/V heads of 4 rows 88 us (484 MB, 5.5 TB/s); the join 5 us.  24 rows a
-// head, 4 sequences of up to 8392 keys: 58 us (4.0 TB/s), where half the waves' time is
-// the codes' conversion and the softmax; the join of 24 MB 6.6 us.
+// head, 4 sequences of up to 8392 keys: 59 us (3.9 TB/s); the join of 24 MB 6.2 us.
+// The second term of p costs 0.9 us of these 59, nothing with one row a head.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * CA_WAVES, 2) void k_cache_attn(CacheAttnArgs p
         // Only blocks that reach the tree's keys or the end have anything masked.
         const bool masked = k0 + CA_KB > tree0;
         uint32_t seen[NR];
-        u32x4_t pw[NR];
+        u32x4_t pw[NR], pl[NR];
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
             seen[t] = ~0u;
@@ -354,9 +354,14 @@ __global__ __launch_bounds__(64 * CA_WAVES, 2) void k_cache_attn(CacheAttnArgs p
                 sum += e[i];
             }
             l[t] = l[t] * alpha + sum;
-            // p is rounded to bf16 for the matrix product: at most 2^-8 of each
-            // term of a sum that is itself rounded to bf16 at the end.
-            pw[t] = u32x4_t{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]), pack_bf16x2(e[6], e[7])};
+            // p enters the matrix product as two bf16 terms, pw + pl (pl the rounding
+            // error of pw): 16 significand bits, where pw alone would put 2^-8 of each
+            // term into the sum while l keeps all of it.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pw[t][i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+                pl[t][i] = pack_bf16x2(e[2 * i] - bf_lo(pw[t][i]), e[2 * i + 1] - bf_hi(pw[t][i]));
+            }
             if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
@@ -390,8 +395,10 @@ __global__ __launch_bounds__(64 * CA_WAVES, 2) void k_cache_attn(CacheAttnArgs p
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NR; ++t)
+            for (int t = 0; t < NR; ++t) {
+                o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8_t, pl[t]), o[t][dt], 0, 0, 0);
                 o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8_t, pw[t]), o[t][dt], 0, 0, 0);
+            }
         }
         asm volatile("" ::: "memory");
     }
