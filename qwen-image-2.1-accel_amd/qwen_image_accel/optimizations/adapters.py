@@ -10,6 +10,7 @@ counterpart.
 import torch
 from torch import nn
 
+from qwen_image_accel import _native
 from qwen_image_accel.kernels.adapters import MAX_RANK, low_rank
 from qwen_image_accel.optimizations.mxfp8 import LAYER_GROUPS, MXFP8Linear
 from qwen_image_accel.weights import ADAPTED_BASE
@@ -18,30 +19,52 @@ NO_ADAPTER = -1
 
 
 class AdapterRoute:
-    """Which adapter each sequence of the batch uses: ``index``, int32 (B,), an
-    adapter's number or -1, or None while nothing is selected (no adapter
-    anywhere).  Each batch size has one tensor, kept from its first ``select``
-    on, so a step captured with a selection follows the later ones of its batch size."""
+    """Which adapter each sequence of the batch uses, an adapter's number or -1;
+    nothing while nothing is selected (no adapter anywhere).
+
+    A step reads a tensor that its selection wrote before ``select`` returned
+    and that nothing writes again: a step already queued keeps its selection,
+    and one started afterwards, on any stream, has the new one.  A step that is
+    captured into a graph reads ``index`` instead: each batch size has one such
+    tensor, kept from its first ``select`` on and written by the later ones of that batch size
+    on the current stream, as any other input of a graph is
+    (order replays on another stream behind it, and ``select`` behind them)."""
 
     def __init__(self, names, device):
         self.names, self.device, self.index = tuple(names), torch.device(device), None
         self._by_batch = {}
+        self._step, self._streams = None, set()
 
     def select(self, names):
         """``names``: one adapter name (or None) per sequence of the batch;
         or None to switch the adapters off."""
         if names is None:
-            self.index = None
+            self.index = self._step = None
             return
         numbers = []
         for name in names:
             if name is not None and name not in self.names:
                 raise ValueError(f"unknown adapter {name!r}; installed: {list(self.names)}")
             numbers.append(NO_ADAPTER if name is None else self.names.index(name))
-        new = torch.tensor(numbers, dtype=torch.int32, device=self.device)
-        self.index = self._by_batch.setdefault(len(numbers), new)
-        if self.index is not new:
-            self.index.copy_(new)
+        self._step, self._streams = torch.tensor(numbers, dtype=torch.int32, device=self.device), set()
+        self.index = self._by_batch.get(len(numbers))
+        if self.index is None:
+            self.index = self._by_batch[len(numbers)] = self._step.clone()
+        else:
+            self.index.copy_(self._step)
+
+    def step_index(self):
+        """The int32 (B,) tensor that a step started now reads, or None."""
+        step = self._step
+        if step is None or not step.is_cuda:
+            return step
+        if torch.cuda.is_current_stream_capturing():
+            return self.index
+        stream = _native.stream(step.device)
+        if stream not in self._streams:  # its memory outlives what this stream does with it
+            self._streams.add(stream)
+            step.record_stream(torch.cuda.current_stream(step.device))
+        return step
 
 
 class AdapterStack(nn.Module):
@@ -107,8 +130,8 @@ class AdaptedLinear(nn.Module):
         return getattr(self, ADAPTED_BASE)
 
     def forward(self, x):
-        y = self.base(x)
-        return y if self.route.index is None else self.stack.add(x, y, self.route.index)
+        y, index = self.base(x), self.route.step_index()
+        return y if index is None else self.stack.add(x, y, index)
 
 
 def _stacked_qkv(linears):
