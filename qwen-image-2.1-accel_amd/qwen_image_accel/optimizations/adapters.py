@@ -37,9 +37,13 @@ class AdapterRoute:
 
     def select(self, names):
         """``names``: one adapter name (or None) per sequence of the batch;
-        or None to switch the adapters off."""
+        or None to switch the adapters off, in captured steps of every batch
+        size too.  (A step captured while nothing was selected has no adapters in
+        it, whatever is selected later.)"""
         if names is None:
             self.index = self._step = None
+            for kept in self._by_batch.values():
+                kept.fill_(NO_ADAPTER)
             return
         numbers = []
         for name in names:

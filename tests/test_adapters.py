@@ -69,3 +69,45 @@ def test_selections_beside_a_step_on_another_stream(dev):
         torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+def test_switching_off_reaches_captured_steps():
+    """A captured step reads the kept tensor of its batch size: nothing selected means no adapter there either."""
+    route = install.AdapterRoute(("a", "b"), "cpu")
+    route.select(["b", "a", None])
+    three = route.index
+    route.select(["a", "b"])
+    two = route.index
+    route.select(None)
+    assert route.index is None
+    assert three.tolist() == [-1, -1, -1] and two.tolist() == [-1, -1]
+    route.select(["b", "b"])
+    assert route.index is two and two.tolist() == [1, 1] and three.tolist() == [-1, -1, -1]
+
+
+@pytest.mark.gpu
+def test_captured_layer_follows_selections(dev):
+    """Replays of one captured layer across selections, none among them, beside eager calls of the same."""
+    say("captured selections")
+    m, _, route, _ = adapted(k=256, n=256, dtype=torch.bfloat16, device=dev)
+    x = bf16_randn(torch.Generator().manual_seed(1), (2, 40, 256)).to(dev)
+    with torch.no_grad():
+        route.select(["a", "b"])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m(x)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        for names in (["b", None], None, ["a", "a"], None, [None, "b"]):
+            route.select(names)
+            want = m(x)
+            torch.cuda.synchronize()
+            for _ in range(2):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want), names
+    del graph
