@@ -213,7 +213,7 @@ class QuantizedSwiGLU:
         gate, value = mlp.gate_layer.matmul(shared), mlp.proj.matmul(shared)
         act = swiglu_quantize(gate, value, tiled=True) if to_mxfp8 else None
         if act is None:
-            return mlp.out(swiglu(gate, value)).view(*lead, -1)
+            return mlp.out(swiglu(gate, value).view(*lead, -1))
         return mlp.out.matmul(act).view(*lead, -1)
 
 

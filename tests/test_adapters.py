@@ -1,11 +1,16 @@
 """Adapters beside the block linears: selections, and what an adapted linear
 takes, keeps and is saved as."""
+import copy
+import types
+
 import pytest
 import torch
 from torch import nn
 
 from qwen_image_accel import pipeline
 from qwen_image_accel.optimizations import adapters as install
+from qwen_image_accel.optimizations import decode
+from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
 from tests import fake_qwen21 as fq
 from tests.helpers import bf16_randn
 
@@ -111,3 +116,83 @@ def test_captured_layer_follows_selections(dev):
                 torch.cuda.synchronize()
                 assert torch.equal(out, want), names
     del graph
+
+
+# ----------------------------------------------- adapters beside some linears --
+
+class HostMXFP8(MXFP8Linear):
+    """An MXFP8Linear whose product is the bf16 linear's, for hosts without the kernels."""
+
+    def __init__(self, linear):
+        nn.Module.__init__(self)
+        self.linear, self.in_features, self.out_features, self.bias = linear, linear.in_features, linear.out_features, None
+
+    def matmul(self, activation):
+        return self.linear(activation.rows)
+
+    def forward(self, x):
+        return self.linear(x)
+
+
+def test_an_adapter_beside_the_down_projection_alone(monkeypatch):
+    """Gate and value multiply one shared activation into (B * S, F) rows; the adapted down projection still sees
+    sequences."""
+    mlp = fq.SwiGLU(64, 128)
+    plain = copy.deepcopy(mlp)
+    for name in ("gate_layer", "proj", "out"):
+        setattr(mlp, name, HostMXFP8(getattr(mlp, name)))
+    g = torch.Generator().manual_seed(2)
+    down, up = torch.randn(8, 128, generator=g) * 0.1, torch.randn(64, 8, generator=g)
+    route = install.AdapterRoute(("a",), "cpu")
+    mlp.out = install.AdaptedLinear(mlp.out, install.AdapterStack.of([(down, up, 0.5)], 64, 128, "cpu"), route)
+    monkeypatch.setattr(decode, "shared_activation", lambda x, consumers: types.SimpleNamespace(rows=x.reshape(-1, 64), shape=x.shape))
+    monkeypatch.setattr(decode, "swiglu", lambda gate, value: torch.nn.functional.silu(gate) * value)
+    forward, x = decode.QuantizedSwiGLU(mlp), torch.randn(2, 5, 64, generator=g)
+    with torch.no_grad():
+        want = plain(x)
+        assert torch.allclose(forward(x), want, atol=1e-5)      # sums of 128 fp32 products of another order
+        route.select(["a", None])
+        got = forward(x)
+        bf = lambda t: t.bfloat16().float()
+        h = torch.nn.functional.silu(plain.gate_layer(x)) * plain.proj(x)
+        want[0] += 0.5 * (h[0] @ bf(down).T) @ bf(up).T
+        assert torch.allclose(got, want, atol=1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", install.LAYER_GROUPS["all"])
+def test_mxfp8_block_with_adapters_beside_one_linear(dev, path, monkeypatch):
+    """Two requests, one with an adapter on one linear of each block, against the same profile with it merged into the
+    weights.  The merged weight is quantized with the adapter inside, 2^-4 of each weight at most and a random part of
+    that on average; the adapter is half of the weight's size, so the change it makes points the same way."""
+    say("one adapted linear", path)
+    monkeypatch.setenv("QW21_MXFP8_SKIP_BLOCKS", "")
+    t = fq.make_transformer(dim=512, heads=4, ffn=1024, device=dev)
+    ref, ad, g = copy.deepcopy(t), {}, torch.Generator().manual_seed(4)
+    for i, block in enumerate(t.transformer_blocks):
+        m = block.get_submodule(path)
+        down, up = bf16_randn(g, (16, m.in_features), m.in_features ** -0.5), bf16_randn(g, (m.out_features, 16), 0.05)
+        ad[f"transformer_blocks.{i}.{path}"] = (down, up, 1.0)
+        with torch.no_grad():
+            ref.transformer_blocks[i].get_submodule(path).weight.add_((up.float() @ down.float()).to(dev).bfloat16())
+    h, mod, freqs, layer = fq.make_inputs(dim=512, heads=4, tokens=96, prefix=37, batch=2, device=dev)
+    mod.view(-1, 2, 2, 512)[:, :, 1] *= 10      # gates of O(1): what a block adds is well above the rounding of h
+
+    def run(t):
+        x = h
+        for b in t.transformer_blocks:
+            x = b(hidden_states=x, modulation=mod, rotary_emb=freqs, layer_cache=layer, kv_cache_mode="cached")
+        return x.float()
+    with torch.no_grad():
+        pipeline.install_hot_path(t, "mxfp8", validate=False)
+        bare = run(t)
+        route = install.install_adapters(t, {"a": ad})
+        route.select([None, None])
+        none = run(t)
+        route.select([None, "a"])
+        got = run(t)
+        pipeline.install_hot_path(ref, "mxfp8", validate=False)
+        want = run(ref)
+    assert torch.equal(got[0], none[0])         # the request without an adapter
+    delta, change = got[1] - bare[1], want[1] - bare[1]
+    assert float((delta * change).sum() / (delta.norm() * change.norm())) > 0.9
