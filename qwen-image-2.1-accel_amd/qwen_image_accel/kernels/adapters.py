@@ -34,6 +34,13 @@ def _rows(t):
     return rows, w, row
 
 
+def takes_rows(t):
+    """Whether ``low_rank`` takes the rows of t as they lie: one multiple of 8
+    elements apart, 16-byte aligned."""
+    rows = _rows(t)
+    return rows is not None and rows[2] >= rows[1] and rows[2] % 8 == 0 and t.data_ptr() % 16 == 0
+
+
 def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     """``base + scale[a] * (x @ down[a].T) @ up[a].T`` per row, a = ``index``.
 

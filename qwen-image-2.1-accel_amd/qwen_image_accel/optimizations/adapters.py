@@ -11,7 +11,7 @@ import torch
 from torch import nn
 
 from qwen_image_accel import _native
-from qwen_image_accel.kernels.adapters import MAX_RANK, low_rank
+from qwen_image_accel.kernels.adapters import MAX_RANK, low_rank, takes_rows
 from qwen_image_accel.optimizations.mxfp8 import LAYER_GROUPS, MXFP8Linear
 from qwen_image_accel.weights import ADAPTED_BASE
 
@@ -106,18 +106,29 @@ class AdapterStack(nn.Module):
         return cls(down, up, scale)
 
     def add(self, x, y, index):
-        """y (B, S, N) + the adapters' share of x (B, S, K); y is overwritten on the GPU."""
-        if x.dim() != 3 or x.shape[0] != index.shape[0]:
-            raise ValueError(f"the route names {index.shape[0]} sequences, the batch is {tuple(x.shape)}")
-        if x.is_cuda and x.dtype == torch.bfloat16 and y.dtype == torch.bfloat16:
-            return low_rank(x, self.down, self.up, index, scale=self.scale, base=y, out=y, parts=self.parts)
-        out, r = y.float(), self.up.shape[2]
+        """y + the adapters' share of x; y may be overwritten.
+
+        x (..., K), y (..., N): the leading axis is the sequences (so a 2-D x holds a
+        row of each); of a batch of one, x may be its rows alone or one row."""
+        lead, b = x.shape[:-1], index.shape[0]
+        if not (lead[:1] == (b,) or (b == 1 and len(lead) < 2)):
+            raise ValueError(f"the route names {b} sequences, the batch is {tuple(x.shape)}")
+        k, n = x.shape[-1], y.shape[-1]
+        if 0 in lead:
+            return y
+        xs, out = x.reshape(b, -1, k), y.reshape(b, -1, n)
+        if (x.is_cuda and x.dtype == torch.bfloat16 and y.dtype == torch.bfloat16
+                and k % 8 == 0 and n % (8 * self.parts) == 0):
+            # Rows that the kernel does not take as they lie (a slice of a batch) are copied, as the linear does.
+            xs, out = (t if takes_rows(t) else t.clone(memory_format=torch.contiguous_format) for t in (xs, out))
+            return low_rank(xs, self.down, self.up, index, scale=self.scale, base=out, out=out, parts=self.parts).reshape(y.shape)
+        out, r = out.float(), self.up.shape[2]
         for i, a in enumerate(index.tolist()):
             if a >= 0:
-                h = (x[i].float() @ self.down[a].float().t()).unflatten(-1, (self.parts, r))
+                h = (xs[i].float() @ self.down[a].float().t()).unflatten(-1, (self.parts, r))
                 up = self.up[a].float().unflatten(0, (self.parts, -1))
                 out[i] += self.scale[a] * torch.einsum("spr,pnr->spn", h, up).flatten(1)
-        return out.to(y.dtype)
+        return out.to(y.dtype).reshape(y.shape)
 
 
 class AdaptedLinear(nn.Module):

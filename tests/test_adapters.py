@@ -12,6 +12,7 @@ from qwen_image_accel.optimizations import adapters as install
 from qwen_image_accel.optimizations import decode
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
 from tests import fake_qwen21 as fq
+from tests import requests_ref as R
 from tests.helpers import bf16_randn
 
 
@@ -116,6 +117,81 @@ def test_captured_layer_follows_selections(dev):
                 torch.cuda.synchronize()
                 assert torch.equal(out, want), names
     del graph
+
+
+# ------------------------------------------------- what an adapted linear takes --
+
+def shapes():
+    """(selection, x's shape, how x is made from a tensor of that shape) for K 64."""
+    two, one = ["a", None], ["b"]
+    yield "3d", two, lambda r: r(2, 5, 64)
+    yield "slice of a batch", two, lambda r: r(2, 9, 64)[:, 4:]
+    yield "transposed", two, lambda r: r(5, 2, 64).transpose(0, 1)
+    yield "columns", two, lambda r: r(2, 5, 67)[..., 3:]
+    yield "columns of aligned rows", two, lambda r: r(2, 5, 80)[..., 4:68]
+    yield "4d", two, lambda r: r(2, 3, 4, 64)
+    yield "4d slice", two, lambda r: r(2, 3, 4, 64)[:, 1:, ::2]
+    yield "expanded", two, lambda r: r(1, 1, 64).expand(2, 5, 64)
+    yield "a row per sequence", two, lambda r: r(2, 64)
+    yield "rows of one sequence", one, lambda r: r(7, 64)
+    yield "one row", one, lambda r: r(64)
+    yield "nothing", two, lambda r: r(2, 0, 64)
+
+
+def check_adapted(m, base, stack, x, names):
+    """Against the adapters' definition in float64, one sequence at a time.
+
+    The bound: fp32 sums of K and of R products, off by at most F32 of the sum of magnitudes per addition (16 more for
+    the join of chunks, scale and base); h enters the second product as two bf16 terms, HALF^2 of it; the result
+    is rounded once, to bf16 or fp32.  The linear's own output is in both sides."""
+    with torch.no_grad():
+        m.route.select(names)
+        got, want = m(x), base(x)
+        assert got.shape == want.shape and got.dtype == want.dtype
+        rows, index = want.double().reshape(len(names), -1, want.shape[-1]).clone(), m.route.index.tolist()
+        xs, bound = x.double().reshape(len(names), -1, x.shape[-1]), torch.zeros_like(rows)
+        for i, a in enumerate(index):
+            if a >= 0:
+                down, up, scale = stack.down[a].double().T, stack.up[a].double().T, float(stack.scale[a])
+                rows[i] += scale * (xs[i] @ down) @ up
+                bound[i] = ((x.shape[-1] + up.shape[0] + 16) * R.F32 + R.HALF ** 2) * scale * (xs[i].abs() @ down.abs()) @ up.abs()
+        half = R.F32 if got.dtype == torch.float32 else R.HALF
+        bound += half * (rows.abs() + bound)
+        assert ((got.double().reshape(rows.shape) - rows).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("case", shapes(), ids=lambda c: c[0])
+def test_an_adapted_linear_takes_what_the_linear_takes(case):
+    _, names, make = case
+    m, base, _, stack = adapted()
+    g = torch.Generator().manual_seed(3)
+    check_adapted(m, base, stack, make(lambda *s: torch.randn(*s, generator=g)), names)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", shapes(), ids=lambda c: c[0])
+def test_an_adapted_linear_takes_what_the_linear_takes_gpu(dev, case):
+    what, names, make = case
+    say("adapted linear:", what)
+    m, base, _, stack = adapted(dtype=torch.bfloat16, device=dev)
+    g = torch.Generator().manual_seed(3)
+    check_adapted(m, base, stack, make(lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)), names)
+
+
+@pytest.mark.gpu
+def test_an_adapted_linear_of_sizes_the_kernel_does_not_take(dev):
+    say("adapted linear: K 36, N 52")
+    m, base, _, stack = adapted(k=36, n=52, dtype=torch.bfloat16, device=dev)
+    x = bf16_randn(torch.Generator().manual_seed(3), (2, 5, 36)).to(dev)
+    check_adapted(m, base, stack, x, ["a", None])
+
+
+def test_rows_that_belong_to_no_sequence_are_refused():
+    m, _, route, _ = adapted()
+    route.select(["a", None])
+    for shape in ((3, 5, 64), (10, 64), (64,)):
+        with pytest.raises(ValueError, match="names 2 sequences"), torch.no_grad():
+            m(torch.randn(shape))
 
 
 # ----------------------------------------------- adapters beside some linears --
