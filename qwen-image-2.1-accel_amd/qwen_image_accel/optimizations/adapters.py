@@ -25,15 +25,18 @@ class AdapterRoute:
     A step reads a tensor that its selection wrote before ``select`` returned
     and that nothing writes again: a step already queued keeps its selection,
     and one started afterwards, on any stream, has the new one.  A step that is
-    captured into a graph reads ``index`` instead: each batch size has one such
-    tensor, kept from its first ``select`` on and written by the later ones of that batch size
+    captured into a graph reads a kept tensor instead (``index``, on the device the adapters were
+    installed on): each batch size has one, from its first ``select``
+    on, written by the later ones of that batch size
     on the current stream, as any other input of a graph is
     (order replays on another stream behind it, and ``select`` behind them)."""
 
     def __init__(self, names, device):
         self.names, self.device, self.index = tuple(names), torch.device(device), None
-        self._by_batch = {}
-        self._step, self._streams = None, set()
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self._kept = {self.device: {}}  # per device that a step ran on: batch size -> tensor
+        self._numbers, self._steps = None, {}
 
     def select(self, names):
         """``names``: one adapter name (or None) per sequence of the batch;
@@ -41,40 +44,56 @@ class AdapterRoute:
         size too.  (A step captured while nothing was selected has no adapters in
         it, whatever is selected later.)"""
         if names is None:
-            self.index = self._step = None
-            for kept in self._by_batch.values():
-                kept.fill_(NO_ADAPTER)
+            self.index, self._numbers, self._steps = None, None, {}
+            for by_batch in self._kept.values():
+                for kept in by_batch.values():
+                    kept.fill_(NO_ADAPTER)
             return
         numbers = []
         for name in names:
             if name is not None and name not in self.names:
                 raise ValueError(f"unknown adapter {name!r}; installed: {list(self.names)}")
             numbers.append(NO_ADAPTER if name is None else self.names.index(name))
-        self._step, self._streams = torch.tensor(numbers, dtype=torch.int32, device=self.device), set()
-        self.index = self._by_batch.get(len(numbers))
-        if self.index is None:
-            self.index = self._by_batch[len(numbers)] = self._step.clone()
-        else:
-            self.index.copy_(self._step)
+        self._numbers, self._steps = numbers, {}
+        for device in self._kept:
+            self._write(device)
+        self.index = self._kept[self.device][len(numbers)]
 
-    def step_index(self):
-        """The int32 (B,) tensor that a step started now reads, or None."""
-        step = self._step
-        if step is None or not step.is_cuda:
-            return step
-        if torch.cuda.is_current_stream_capturing():
-            return self.index
-        stream = _native.stream(step.device)
-        if stream not in self._streams:  # its memory outlives what this stream does with it
-            self._streams.add(stream)
-            step.record_stream(torch.cuda.current_stream(step.device))
+    def _write(self, device):
+        """The selection on `device`: its own tensor, and the kept one of its batch size."""
+        step, by_batch = torch.tensor(self._numbers, dtype=torch.int32, device=device), self._kept[device]
+        self._steps[device] = step, set()
+        if len(self._numbers) in by_batch:
+            by_batch[len(self._numbers)].copy_(step)
+        else:
+            by_batch[len(self._numbers)] = step.clone()
+
+    def step_index(self, device):
+        """The int32 (B,) tensor on `device` that a step started now reads, or None."""
+        if self._numbers is None:
+            return None
+        capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+        if device not in self._steps:  # the model was moved, or has linears on several devices
+            if capturing:
+                raise RuntimeError(f"run the adapted step once on {device} before it is captured")
+            self._kept.setdefault(device, {})
+            self._write(device)
+        if capturing:
+            return self._kept[device][len(self._numbers)]
+        step, streams = self._steps[device]
+        if device.type == "cuda":
+            stream = _native.stream(device)
+            if stream not in streams:  # its memory outlives what this stream does with it
+                streams.add(stream)
+                step.record_stream(torch.cuda.current_stream(device))
         return step
 
 
 class AdapterStack(nn.Module):
     """The adapters of one projection, stacked: down (A, parts * R, K), up (A, N,
     R) in bf16, scale (A,).  An adapter of a smaller rank is padded with zeros, one that
-    does not touch this projection is zeros with scale 0."""
+    does not touch this projection is zeros with scale 0.  The three keep their
+    types when the model around them is cast."""
 
     def __init__(self, down, up, scale, parts=1):
         super().__init__()
@@ -82,6 +101,15 @@ class AdapterStack(nn.Module):
         self.register_buffer("down", down, persistent=False)
         self.register_buffer("up", up, persistent=False)
         self.register_buffer("scale", scale, persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        kept = dict(self.named_buffers(recurse=False))
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            moved = getattr(self, name)
+            if moved.dtype != t.dtype:
+                setattr(self, name, t.to(moved.device))
+        return self
 
     @classmethod
     def of(cls, triples, out_features, in_features, device):
@@ -145,7 +173,7 @@ class AdaptedLinear(nn.Module):
         return getattr(self, ADAPTED_BASE)
 
     def forward(self, x):
-        y, index = self.base(x), self.route.step_index()
+        y, index = self.base(x), self.route.step_index(x.device)
         return y if index is None else self.stack.add(x, y, index)
 
 

@@ -108,7 +108,7 @@ def _adapted_qkv(attn, x):
     adapters, stacked = getattr(attn, "_adapter_qkv", None), getattr(attn, "_mx_qkv", None)
     if adapters is None or stacked is None or x.dim() != 3 or not x.is_contiguous():
         return None
-    index = attn.to_q.route.step_index()
+    index = attn.to_q.route.step_index(x.device)
     y = mx_matmul(quantize(x.reshape(-1, x.shape[-1]), tiled=True), *stacked, weight_tiled=True).view(*x.shape[:2], -1)
     if index is not None:
         y = adapters.add(x, y, index)

@@ -272,3 +272,60 @@ def test_mxfp8_block_with_adapters_beside_one_linear(dev, path, monkeypatch):
     assert torch.equal(got[0], none[0])         # the request without an adapter
     delta, change = got[1] - bare[1], want[1] - bare[1]
     assert float((delta * change).sum() / (delta.norm() * change.norm())) > 0.9
+
+
+# ------------------------------------------------ moved, cast, saved and loaded --
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_adapters_keep_their_types_when_the_model_is_cast(dtype):
+    m, _, route, stack = adapted()
+    down, up, scale = stack.down.clone(), stack.up.clone(), stack.scale.clone()
+    m.to(dtype)
+    assert next(m.base.parameters()).dtype == dtype
+    for got, want in ((stack.down, down), (stack.up, up), (stack.scale, scale)):
+        assert got.dtype == want.dtype and torch.equal(got, want)
+    route.select(["a", None])
+    with torch.no_grad():
+        assert m(torch.randn(2, 3, 64).to(dtype)).dtype == dtype
+
+
+@pytest.mark.gpu
+def test_adapters_move_and_cast_with_the_model(dev):
+    """Installed on the host, selected, moved to the GPU, cast, run, captured."""
+    say("moved adapters")
+    m, base, route, stack = adapted(k=128, n=128)
+    route.select(["b", "a"])
+    m.to(dev).to(torch.bfloat16)
+    x = bf16_randn(torch.Generator().manual_seed(3), (2, 5, 128)).to(dev)
+    check_adapted(m, base, stack, x, ["a", None])
+    with torch.no_grad():
+        want = m(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        for names in (["a", None], ["b", "b"]):
+            route.select(names)
+            want = m(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+    del graph
+
+
+@pytest.mark.gpu
+def test_a_capture_on_a_device_no_step_ran_on_is_refused(dev):
+    say("capture before any step")
+    m, _, route, _ = adapted(k=128, n=128)
+    route.select(["b", "a"])
+    m.to(dev).to(torch.bfloat16)
+    x = bf16_randn(torch.Generator().manual_seed(3), (2, 5, 128)).to(dev)
+    with torch.no_grad():
+        m.base(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            m.base(x)
+            with pytest.raises(RuntimeError, match="before it is captured"):
+                m(x)
+    del graph
