@@ -160,7 +160,8 @@ class AdapterStack(nn.Module):
 
 
 class AdaptedLinear(nn.Module):
-    """A linear (nn.Linear or MXFP8Linear) with adapters beside it."""
+    """A linear (nn.Linear or MXFP8Linear) with adapters beside it.  A state dict
+    holds the linear under its own path, as without adapters."""
 
     def __init__(self, base, stack, route):
         super().__init__()
@@ -175,6 +176,15 @@ class AdaptedLinear(nn.Module):
     def forward(self, x):
         y, index = self.base(x), self.route.step_index(x.device)
         return y if index is None else self.stack.add(x, y, index)
+
+    def state_dict(self, *args, **kwargs):
+        return self.base.state_dict(*args, **kwargs)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        inner = f"{prefix}{ADAPTED_BASE}."
+        for key in [k for k in state_dict if k.startswith(prefix) and not k.startswith(inner)]:
+            state_dict[inner + key[len(prefix):]] = state_dict.pop(key)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
 
 def _stacked_qkv(linears):

@@ -329,3 +329,43 @@ def test_a_capture_on_a_device_no_step_ran_on_is_refused(dev):
             with pytest.raises(RuntimeError, match="before it is captured"):
                 m(x)
     del graph
+
+
+def block_with_adapters(mxfp8=()):
+    """A block, bf16 but for zero MXFP8 linears at the paths `mxfp8`, and the same with adapters on two of its linears."""
+    t = fq.make_transformer(n_blocks=1)
+    for path in mxfp8:
+        parent, _, leaf = path.rpartition(".")
+        m = t.transformer_blocks[0].get_submodule(path)
+        codes = torch.arange(m.weight.numel(), dtype=torch.int64).remainder(120).to(torch.uint8).view(m.weight.shape)
+        scales = torch.full((m.weight.numel() // 32,), 120, dtype=torch.uint8)
+        setattr(t.transformer_blocks[0].get_submodule(parent), leaf,
+                MXFP8Linear.from_quantized(m.in_features, m.out_features, codes, scales))
+    both = copy.deepcopy(t)
+    route = install.install_adapters(both, {"a": {f"transformer_blocks.0.{p}": (torch.randn(4, 256), torch.randn(256, 4), 1.0)
+                                                  for p in ("attn.to_q", "attn.to_out.0")}})
+    return t, both, route
+
+
+@pytest.mark.parametrize("mxfp8", [(), ("attn.to_q", "attn.to_k")])
+def test_state_dicts_are_those_of_the_model_without_adapters(mxfp8):
+    plain, both, _ = block_with_adapters(mxfp8)
+    a, b = plain.transformer_blocks.state_dict(), both.transformer_blocks.state_dict()
+    assert list(a) == list(b) and a._metadata.keys() >= {"0.attn.to_q", "0.attn.to_out.0"} and a._metadata["0.attn.to_q"] == b._metadata["0.attn.to_q"]
+    same = lambda s, t: all(torch.equal(s[k].reshape(-1).view(torch.uint8), t[k].reshape(-1).view(torch.uint8)) for k in s)
+    assert same(a, b)
+    linear = both.transformer_blocks[0].attn.to_q
+    assert list(linear.state_dict()) == list(plain.transformer_blocks[0].attn.to_q.state_dict())
+    # Other values, loaded into each from the other.
+    other = {k: (v.reshape(-1).view(torch.uint8) ^ 1).view(v.dtype).view(v.shape) for k, v in a.items()}
+    both.transformer_blocks.load_state_dict(other)
+    assert same(both.transformer_blocks.state_dict(), other)
+    plain.transformer_blocks.load_state_dict(both.transformer_blocks.state_dict())
+    assert same(plain.transformer_blocks.state_dict(), other)
+    key = "0.attn.to_q.weight_fp8" if mxfp8 else "0.attn.to_q.weight"
+    linear.load_state_dict({k.removeprefix("0.attn.to_q."): v for k, v in a.items() if k.startswith("0.attn.to_q.")})
+    assert same(both.transformer_blocks.state_dict(), {**other, **{k: a[k] for k in a if k.startswith("0.attn.to_q.")}})
+    with pytest.raises(RuntimeError, match="Missing key"):
+        both.transformer_blocks.load_state_dict({k: v for k, v in a.items() if k != key})
+    with pytest.raises(RuntimeError, match="Unexpected key"):
+        both.transformer_blocks.load_state_dict({**a, "0.attn.to_q.other": a[key]})
