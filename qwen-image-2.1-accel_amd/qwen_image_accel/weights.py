@@ -155,7 +155,8 @@ def save_mxfp8(transformer, path):
 def load_mxfp8(transformer, path, device=None):
     """Replace the linears named in a ``save_mxfp8`` file by ``MXFP8Linear`` s
     holding the saved bytes (no quantization), and restore the interleaved
-    gate/up weights.  Returns the converted module paths."""
+    gate/up weights.  Adapters installed beside them stay.  Returns the
+    converted module paths."""
     from safetensors import safe_open
     with safe_open(path, framework="pt", device="cpu") as f:
         meta = f.metadata() or {}
@@ -167,13 +168,15 @@ def load_mxfp8(transformer, path, device=None):
         loaded = []
         for name, (k, n) in sorted(json.loads(meta["layers"]).items()):
             old = _resolve(transformer, name)
+            place = f"{name}.{ADAPTED_BASE}" if hasattr(old, ADAPTED_BASE) else name
+            old = getattr(old, ADAPTED_BASE, old)
             if not isinstance(old, (nn.Linear, MXFP8Linear)) or (old.in_features, old.out_features) != (k, n):
                 raise ValueError(f"{path}: {name} is not a ({n}, {k}) linear in this model")
             dev = device if device is not None else next(old.buffers(), next(old.parameters(), None)).device
             bias = f.get_tensor(f"{name}.bias").to(dev) if f"{name}.bias" in keys else None
             new = MXFP8Linear.from_quantized(k, n, f.get_tensor(f"{name}.codes").to(dev),
                                              f.get_tensor(f"{name}.scales").to(dev), bias)
-            _set(transformer, name, new)
+            _set(transformer, place, new)
             loaded.append(name)
         for key in json.loads(meta["fused"]):
             name, _, attr = key.rpartition(".")
@@ -181,6 +184,7 @@ def load_mxfp8(transformer, path, device=None):
                 raise ValueError(f"{path}: unknown fused weight {key}")
             mod = _resolve(transformer, name)
             ref = mod.gate_layer if attr == "_mx_gate_up" else mod.to_q
+            ref = getattr(ref, ADAPTED_BASE, ref)
             dev = ref.weight_tiled.device
             setattr(mod, attr, (f.get_tensor(f"{key}.codes").to(dev).view(ref.weight_tiled.dtype),
                                 f.get_tensor(f"{key}.scales").to(dev).view(ref.weight_scale.dtype)))

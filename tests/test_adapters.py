@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch import nn
 
-from qwen_image_accel import pipeline
+from qwen_image_accel import pipeline, weights
 from qwen_image_accel.optimizations import adapters as install
 from qwen_image_accel.optimizations import decode
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
@@ -369,3 +369,26 @@ def test_state_dicts_are_those_of_the_model_without_adapters(mxfp8):
         both.transformer_blocks.load_state_dict({k: v for k, v in a.items() if k != key})
     with pytest.raises(RuntimeError, match="Unexpected key"):
         both.transformer_blocks.load_state_dict({**a, "0.attn.to_q.other": a[key]})
+
+
+def test_mxfp8_weights_load_beside_adapters(tmp_path):
+    """A file saved with or without adapters loads into a transformer with adapters installed, over bf16 and over MXFP8
+    linears, the stacked Q/K/V weight among what it restores; the adapters stay."""
+    linears = ("attn.to_q", "attn.to_k", "attn.to_v")
+    saved, both, route = block_with_adapters(linears)
+    weights.fuse_qkv(saved.transformer_blocks[0].attn)
+    path = str(tmp_path / "w.safetensors")
+    names = weights.save_mxfp8(saved, path)
+    assert names == sorted(f"transformer_blocks.0.{p}" for p in linears)
+    _, bf16, _ = block_with_adapters()
+    for t in (both, bf16):
+        attn = t.transformer_blocks[0].attn
+        stack = attn.to_q.stack
+        assert weights.load_mxfp8(t, path) == names
+        assert isinstance(attn.to_q, install.AdaptedLinear) and attn.to_q.stack is stack
+        assert isinstance(attn.to_q.base, MXFP8Linear) and isinstance(attn.to_k, MXFP8Linear)
+        assert torch.equal(attn.to_q.base.weight_tiled.view(torch.uint8),
+                           saved.transformer_blocks[0].attn.to_q.weight_tiled.view(torch.uint8))
+        assert torch.equal(attn._mx_qkv[0].view(torch.uint8), saved.transformer_blocks[0].attn._mx_qkv[0].view(torch.uint8))
+    again = str(tmp_path / "again.safetensors")
+    assert weights.save_mxfp8(both, again) == names and weights.load_mxfp8(saved, again) == names
