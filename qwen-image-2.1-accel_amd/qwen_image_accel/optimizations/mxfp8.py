@@ -149,7 +149,10 @@ def _replace(block, path, module):
 
 def quantize_transformer(transformer, skip_blocks=None, layers=None):
     """Swap the planned linears for MXFP8Linear (everything else stays bf16)
-    and return their module paths ("transformer_blocks.<i>.<path>")."""
+    and return their module paths ("transformer_blocks.<i>.<path>").  Adapters
+    (optimizations/adapters.py) are installed afterwards."""
+    if getattr(transformer, "_qw_adapters", None) is not None:
+        raise RuntimeError("linears with adapters beside them are not converted; remove_adapters first")
     plan = conversion_plan(transformer, skip_blocks, layers)
     blocks = transformer.transformer_blocks
     with torch.no_grad():

@@ -10,7 +10,7 @@ from torch import nn
 from qwen_image_accel import pipeline, weights
 from qwen_image_accel.optimizations import adapters as install
 from qwen_image_accel.optimizations import decode
-from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
+from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear, quantize_transformer
 from tests import fake_qwen21 as fq
 from tests import requests_ref as R
 from tests.helpers import bf16_randn
@@ -392,3 +392,15 @@ def test_mxfp8_weights_load_beside_adapters(tmp_path):
         assert torch.equal(attn._mx_qkv[0].view(torch.uint8), saved.transformer_blocks[0].attn._mx_qkv[0].view(torch.uint8))
     again = str(tmp_path / "again.safetensors")
     assert weights.save_mxfp8(both, again) == names and weights.load_mxfp8(saved, again) == names
+
+
+def test_linears_with_adapters_are_not_silently_left_out_of_the_conversion():
+    """quantize_transformer converts linears; with adapters in front of them it would find none of those."""
+    _, both, _ = block_with_adapters()
+    with pytest.raises(RuntimeError, match="remove_adapters"):
+        quantize_transformer(both, skip_blocks="")
+    with pytest.raises(RuntimeError, match="remove_adapters"):
+        pipeline.install_hot_path(both, "mxfp8", validate=False)
+    assert type(both.transformer_blocks[0].attn.to_k) is nn.Linear and getattr(both, "_qw_hot_path", None) is None
+    install.remove_adapters(both)
+    assert quantize_transformer(both, skip_blocks="0") == []
