@@ -210,7 +210,7 @@ def install_adapters(transformer, adapters):
     ``select`` names adapters the model runs without them."""
     if getattr(transformer, "_qw_adapters", None) is not None:
         raise RuntimeError("adapters are installed once per transformer; remove_adapters first")
-    if not adapters:
+    if not any(adapters.values()):
         raise ValueError("no adapters given")
     names = list(adapters)
     blocks = transformer.transformer_blocks

@@ -404,3 +404,14 @@ def test_linears_with_adapters_are_not_silently_left_out_of_the_conversion():
     assert type(both.transformer_blocks[0].attn.to_k) is nn.Linear and getattr(both, "_qw_hot_path", None) is None
     install.remove_adapters(both)
     assert quantize_transformer(both, skip_blocks="0") == []
+
+
+def test_adapters_of_no_linear_are_refused():
+    t = fq.make_transformer(n_blocks=1)
+    for adapters in ({"a": {}}, {"a": {}, "b": {}}):
+        with pytest.raises(ValueError, match="no adapters"):
+            install.install_adapters(t, adapters)
+    assert getattr(t, "_qw_adapters", None) is None
+    ok = (torch.zeros(4, 256), torch.zeros(256, 4), 1.0)
+    route = install.install_adapters(t, {"a": {"transformer_blocks.0.attn.to_q": ok}, "none": {}})   # one of the two is
+    route.select(["none"])
