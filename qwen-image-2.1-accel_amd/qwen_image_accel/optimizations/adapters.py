@@ -68,9 +68,14 @@ class AdapterRoute:
         else:
             by_batch[len(self._numbers)] = step.clone()
 
+    @property
+    def off(self):
+        """Whether nothing is selected."""
+        return self._numbers is None
+
     def step_index(self, device):
         """The int32 (B,) tensor on `device` that a step started now reads, or None."""
-        if self._numbers is None:
+        if self.off:
             return None
         capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
         if device not in self._steps:  # the model was moved, or has linears on several devices
@@ -187,6 +192,13 @@ class AdaptedLinear(nn.Module):
         super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
 
+def running(linear):
+    """The module that a step started now runs at a linear's place: the linear
+    itself while nothing is selected, so that the paths which fuse several MXFP8
+    linears or their neighbours see them as without adapters."""
+    return linear.base if isinstance(linear, AdaptedLinear) and linear.route.off else linear
+
+
 def _stacked_qkv(linears):
     """One AdapterStack over the stacked Q/K/V projection, or None where the
     three do not stack."""
@@ -206,8 +218,11 @@ def install_adapters(transformer, adapters):
     ``adapters``: {name: {path: (down (r, K), up (N, r), scale)}}, ``path`` as
     ``quantize_transformer`` returns them ("transformer_blocks.<i>.attn.to_q";
     any of LAYER_GROUPS["all"]), scale the factor on up @ down (alpha / rank).
-    Ranks up to 128 may differ.  Returns the ``AdapterRoute``; until its
-    ``select`` names adapters the model runs without them."""
+    Ranks up to 128 may differ; down and up are held in bf16.  Returns the ``AdapterRoute``; until its
+    ``select`` names adapters the model runs without them, as before.  With a selection
+    the mxfp8 profile's steps around an adapted linear run one by one: its
+    input is normalised in bf16 and quantized for it, gate and up are two
+    GEMMs and a SwiGLU, the attention's output is bf16."""
     if getattr(transformer, "_qw_adapters", None) is not None:
         raise RuntimeError("adapters are installed once per transformer; remove_adapters first")
     if not any(adapters.values()):
@@ -251,4 +266,4 @@ def remove_adapters(transformer):
     transformer._qw_adapters = None
 
 
-__all__ = ["AdapterRoute", "AdapterStack", "AdaptedLinear", "install_adapters", "remove_adapters"]
+__all__ = ["AdapterRoute", "AdapterStack", "AdaptedLinear", "running", "install_adapters", "remove_adapters"]

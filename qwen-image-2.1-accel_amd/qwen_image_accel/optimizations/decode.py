@@ -38,6 +38,7 @@ from qwen_image_accel.kernels.epilogue import layer_norm_scale_quantize, swiglu_
 from qwen_image_accel.kernels.gemm import mx_matmul
 from qwen_image_accel.kernels.layernorm import layer_norm_scale
 from qwen_image_accel.kernels.mxfp8 import Quantized, quantize
+from qwen_image_accel.optimizations.adapters import running
 from qwen_image_accel.optimizations.attention_call import attention, qim_backend
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear
 from qwen_image_accel.optimizations.prefix_cache import QuantizedLayerCache
@@ -85,7 +86,7 @@ def shared_activation(x, consumers):
 
 def project_qkv(attn, x, quantized):
     """(q, k, v), each (B, S, heads, head_dim)."""
-    linears = (attn.to_q, attn.to_k, attn.to_v)
+    linears = tuple(running(p) for p in (attn.to_q, attn.to_k, attn.to_v))
     shared = shared_activation(x, linears) if quantized else None
     if shared is None:
         adapted = _adapted_qkv(attn, x) if quantized else None
@@ -103,15 +104,14 @@ def project_qkv(attn, x, quantized):
 
 def _adapted_qkv(attn, x):
     """Q, K, V of MXFP8 projections with adapters beside all three
-    (optimizations/adapters.py): the stacked GEMM on x quantized once, and the
-    three adapters in one call on its output.  None where that does not apply."""
+    (optimizations/adapters.py) of which some are selected: the stacked GEMM on x
+    quantized once, and the three adapters in one call on its output.  None where
+    that does not apply."""
     adapters, stacked = getattr(attn, "_adapter_qkv", None), getattr(attn, "_mx_qkv", None)
     if adapters is None or stacked is None or x.dim() != 3 or not x.is_contiguous():
         return None
-    index = attn.to_q.route.step_index(x.device)
     y = mx_matmul(quantize(x.reshape(-1, x.shape[-1]), tiled=True), *stacked, weight_tiled=True).view(*x.shape[:2], -1)
-    if index is not None:
-        y = adapters.add(x, y, index)
+    y = adapters.add(x, y, attn.to_q.route.step_index(x.device))
     return y.unflatten(-1, (3, attn.heads, -1)).unbind(-3)
 
 
@@ -142,7 +142,7 @@ def attention_inputs(attn, q, k, v, freqs, layer_cache):
 
 
 def attend_and_project(attn, q, k, v, mask, native):
-    out_proj, dropout = attn.to_out[0], attn.to_out[1]
+    out_proj, dropout = running(attn.to_out[0]), attn.to_out[1]
     if isinstance(out_proj, MXFP8Linear) and qim_backend(q, k, v, mask):
         # This build's attention core writes the MXFP8 out-projection's input
         # itself: the bytes MXFP8Linear.forward would quantize from its output.
@@ -201,20 +201,21 @@ class QuantizedSwiGLU:
 
     def __call__(self, x):
         mlp = self.mlp
-        shared = shared_activation(x, (mlp.gate_layer, mlp.proj))
+        gate_layer, proj, out = running(mlp.gate_layer), running(mlp.proj), running(mlp.out)
+        shared = shared_activation(x, (gate_layer, proj))
         if shared is None:
-            return mlp.out(swiglu(mlp.gate_layer(x), mlp.proj(x)))
+            return out(swiglu(gate_layer(x), proj(x)))
         lead = shared.shape[:-1]
-        to_mxfp8 = isinstance(mlp.out, MXFP8Linear)
+        to_mxfp8 = isinstance(out, MXFP8Linear)
         gate_up = getattr(mlp, "_mx_gate_up", None)
         if gate_up is not None and to_mxfp8:
             act = mx_matmul(shared, *gate_up, epilogue="swiglu_quant", weight_tiled=True, out_tiled=True)
-            return mlp.out.matmul(act).view(*lead, -1)
-        gate, value = mlp.gate_layer.matmul(shared), mlp.proj.matmul(shared)
+            return out.matmul(act).view(*lead, -1)
+        gate, value = gate_layer.matmul(shared), proj.matmul(shared)
         act = swiglu_quantize(gate, value, tiled=True) if to_mxfp8 else None
         if act is None:
-            return mlp.out(swiglu(gate, value).view(*lead, -1))
-        return mlp.out.matmul(act).view(*lead, -1)
+            return out(swiglu(gate, value).view(*lead, -1))
+        return out.matmul(act).view(*lead, -1)
 
 
 # ---------------------------------------------------------------- block --
@@ -227,7 +228,7 @@ class DecodeBlock:
         self.block, self.eager, self.terms, self.quantized = block, block.forward, terms, quantized
 
     def normalize(self, h, scale, norm, consumers):
-        if self.quantized and all_mxfp8(*consumers):
+        if self.quantized and all_mxfp8(*(running(m) for m in consumers)):
             x = layer_norm_scale_quantize(h, scale, norm, tiled=True)
             if x is not None:
                 return x

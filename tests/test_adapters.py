@@ -7,7 +7,7 @@ import pytest
 import torch
 from torch import nn
 
-from qwen_image_accel import pipeline, weights
+from qwen_image_accel import _native, pipeline, weights
 from qwen_image_accel.optimizations import adapters as install
 from qwen_image_accel.optimizations import decode
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear, quantize_transformer
@@ -415,3 +415,39 @@ def test_adapters_of_no_linear_are_refused():
     ok = (torch.zeros(4, 256), torch.zeros(256, 4), 1.0)
     route = install.install_adapters(t, {"a": {"transformer_blocks.0.attn.to_q": ok}, "none": {}})   # one of the two is
     route.select(["none"])
+
+
+# ------------------------------------------------------------- nothing selected --
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("profile", ["fused", "mxfp8"])
+def test_the_model_runs_without_adapters_while_nothing_is_selected(dev, profile, monkeypatch):
+    """The same bits from the same launches as before install_adapters, before a selection and after select(None)."""
+    say("nothing selected", profile)
+    monkeypatch.setenv("QW21_MXFP8_SKIP_BLOCKS", "")
+    monkeypatch.setenv("QW21_ATTENTION_BACKEND", "qim")
+    t = fq.make_transformer(dim=512, heads=4, ffn=1024, device=dev)
+    h, mod, freqs, layer = fq.make_inputs(dim=512, heads=4, tokens=96, prefix=37, batch=2, device=dev)
+
+    def run():
+        before, x = dict(_native.calls), h
+        for b in t.transformer_blocks:
+            x = b(hidden_states=x, modulation=mod, rotary_emb=freqs, layer_cache=layer, kv_cache_mode="cached")
+        return x, {k: n - before.get(k, 0) for k, n in _native.calls.items() if n != before.get(k, 0)}
+    with torch.no_grad():
+        pipeline.install_hot_path(t, profile, validate=False)
+        bare, launches = run()
+        bare, launches = run()
+        ad = {}
+        for i, block in enumerate(t.transformer_blocks):
+            for path in install.LAYER_GROUPS["all"]:
+                m = block.get_submodule(path)
+                ad[f"transformer_blocks.{i}.{path}"] = (torch.randn(8, m.in_features), torch.randn(m.out_features, 8), 0.1)
+        route = install.install_adapters(t, {"a": ad})
+        for names in (None, ["a", None], None):
+            route.select(names)
+            out, used = run()
+            if names is None:
+                assert torch.equal(out, bare) and used == launches
+            else:
+                assert not torch.equal(out, bare) and used["qim_low_rank"] > 0
