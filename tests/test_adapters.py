@@ -451,3 +451,32 @@ def test_the_model_runs_without_adapters_while_nothing_is_selected(dev, profile,
                 assert torch.equal(out, bare) and used == launches
             else:
                 assert not torch.equal(out, bare) and used["qim_low_rank"] > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("profile", ["fused", "mxfp8"])
+def test_a_request_without_adapters_does_not_see_its_neighbours(dev, profile, monkeypatch):
+    """Every linear adapted: the request without an adapter gives the same bits whatever the others have, none among them."""
+    say("no adapter beside adapters", profile)
+    monkeypatch.setenv("QW21_MXFP8_SKIP_BLOCKS", "")
+    t = fq.make_transformer(dim=512, heads=4, ffn=1024, device=dev)
+    h, mod, freqs, layer = fq.make_inputs(dim=512, heads=4, tokens=96, prefix=37, batch=3, device=dev)
+    g, ad = torch.Generator().manual_seed(8), {"a": {}, "b": {}}
+    for i, block in enumerate(t.transformer_blocks):
+        for path in install.LAYER_GROUPS["all"]:
+            m = block.get_submodule(path)
+            for name, r in (("a", 8), ("b", 24)):
+                ad[name][f"transformer_blocks.{i}.{path}"] = (bf16_randn(g, (r, m.in_features)), bf16_randn(g, (m.out_features, r)), 0.1)
+    with torch.no_grad():
+        pipeline.install_hot_path(t, profile, validate=False)
+        route = install.install_adapters(t, ad)
+        outs = []
+        for names in ([None, None, None], ["a", None, "b"], ["b", None, "b"], ["a", None, None]):
+            route.select(names)
+            x = h
+            for b in t.transformer_blocks:
+                x = b(hidden_states=x, modulation=mod, rotary_emb=freqs, layer_cache=layer, kv_cache_mode="cached")
+            outs.append(x)
+    for out in outs[1:]:
+        assert torch.equal(out[1], outs[0][1]) and not torch.equal(out[0], outs[0][0])
+    assert torch.equal(outs[3][2], outs[0][2]) and torch.equal(outs[1][2], outs[2][2])
