@@ -131,7 +131,7 @@ extern "C" int qim_cache_write(const void *k, int64_t ldkb, int64_t ldk, const v
     QIM_REQUIRE(k && v, QIM_ERR_ARG, "qim_cache_write: null pointer");
     if (int rc = cache_common("qim_cache_write", kc, ks, vc, vs, B, S, C, H, D)) return rc;
     const int64_t W = H * D;
-    QIM_REQUIRE(start || (first >= 0 && first + S <= C), QIM_ERR_ARG,
+    QIM_REQUIRE(start || (first >= 0 && first <= C - S), QIM_ERR_ARG,
                 "qim_cache_write: %lld rows from position %lld of %lld", (long long)S, (long long)first, (long long)C);
     QIM_REQUIRE(ldk >= W && ldv >= W && ldkb >= 0 && ldvb >= 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldkb % 8 == 0 &&
                     ldvb % 8 == 0 && aligned16(k) && aligned16(v),

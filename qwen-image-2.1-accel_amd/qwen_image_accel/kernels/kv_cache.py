@@ -104,6 +104,8 @@ def write_cache(cache, k, v, start=0, count=None):
         starts, first = per_sequence("write_cache", "start", start, b, device), 0
     else:
         starts, first = None, int(start)
+        if not 0 <= first <= c - s:
+            raise _native.QimError("write_cache", _native.QIM_ERR_ARG, f"{s} rows from position {first} of {c}")
     _native.call_on(device, "qim_cache_write", k.data_ptr(), *strides[:2], v.data_ptr(), *strides[2:],
                     cache.k.data_ptr(), cache.k_exponent.data_ptr(), cache.v.data_ptr(), cache.v_exponent.data_ptr(), starts, first, counts, b, s, c, h, d)
 
