@@ -329,7 +329,7 @@ int qim_qk_norm_rope_pack_cached(const void *q, const void *k, const void *v, co
 /* Attention of a few tokens over such a cache, D = 128: o[b, i, h] =
  * softmax(q[b, i, h] K[b]^T * scale) V[b] over the keys t < lengths[b] of K/V
  * head h / (H / HK).  lengths: device int32 (B,), values outside [0, C] count as
- * the nearest of the two.  tree: NULL, or truth bytes (0 or 1) with tree_b
+ * the nearest of the two.  tree: NULL, or truth bytes (0 for false) with tree_b
  * bytes between sequences (0: shared by all), (S, S) each: of the last
  * S keys, at lengths[b] - S + j, query i sees only those with
  * tree[i * S + j] != 0 (drafted tokens: itself and its ancestors).  A row that

@@ -98,8 +98,9 @@ __device__ __forceinline__ uint64_t ca_tree_bits(const CacheAttnArgs &p, int b, 
     }
 #pragma unroll
     for (int i = 0; i < CA_MAX_S / 4; ++i) {
-        // Bytes of 0 or 1 to 4 bits.
-        const uint32_t four = ((w[i] & 0x01010101u) * 0x01020408u) >> 24;
+        // The bytes that are not 0, as 1 in each, to 4 bits.
+        const uint32_t ones = ((((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) >> 7) & 0x01010101u;
+        const uint32_t four = (ones * 0x01020408u) >> 24;
         bits |= (uint64_t)four << (4 * i + 4 <= p.S ? 4 * i : p.S - 4 > 0 ? p.S - 4 : 0);
     }
     return bits;

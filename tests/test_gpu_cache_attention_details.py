@@ -1,5 +1,5 @@
-"""How far the attention over the MXFP8 cache may be from float64: the output is
-rounded to bf16 once, and nothing before it is held in that few bits."""
+"""Attention over the MXFP8 cache: how far from float64 it may be -- the output is
+rounded to bf16 once, and nothing before it is held in that few bits -- and its masks' bytes."""
 import pytest
 import torch
 
@@ -40,3 +40,18 @@ def test_only_the_output_is_rounded_to_bf16(dev, b, s, h, hk, c, lengths, drafte
     want, bound = tight_bound(q, *(t.cpu() for t in kv_cache.read_cache(cache)), n, tree)
     err = (out.double().cpu() - want).abs()
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("s", [1, 2, 3, 4, 5, 7, 24, 64])
+def test_tree_bytes_other_than_one_are_true(dev, s):
+    """A mask of bytes viewed as bool: every byte that is not 0 shows its key, however many tokens there are."""
+    print("[case] tree bytes", s, flush=True)
+    g = torch.Generator().manual_seed(s)
+    q = bf16_randn(g, (2, s, 4, 128)).to(dev)
+    cache = kv_cache.empty_cache(2, 90, 2, 128, dev)
+    kv_cache.write_cache(cache, bf16_randn(g, (2, 90, 2, 128)).to(dev), bf16_randn(g, (2, 90, 2, 128)).to(dev))
+    n = torch.tensor([90, 70], dtype=torch.int32, device=dev)
+    values = torch.tensor([0, 0, 0, 1, 2, 64, 128, 254, 255], dtype=torch.uint8)
+    tree = values[torch.randint(0, 9, (2, s, s), generator=g)].to(dev)
+    want = attention.attention_cached(q, cache, n, tree=tree != 0)
+    assert torch.equal(attention.attention_cached(q, cache, n, tree=tree.view(torch.bool)), want)
