@@ -107,7 +107,7 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
     of the two.  ``tree``: None (every key is seen), or bool (B, S, S) or
     (S, S): of the last S keys, query i sees key j only where tree[..., i, j]
     (drafted tokens: itself and its ancestors; a causal step: the lower
-    triangle).  A row that sees no key is zeros.  scale defaults to
+    triangle).  A row that sees no key is zeros (all are, of a cache of no positions).  scale defaults to
     1/sqrt(128).  Returns (B, S, H, 128) bf16 (``out``, if given: contiguous, apart from q).  For the queries of a whole image,
     stage the prefix (``prepare_attention_inputs_quantized``) and use
     ``attention``."""
@@ -133,6 +133,10 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
         raise ValueError(f"out must be a contiguous bf16 {tuple(q.shape)} tensor on {device}")
     if not (b and s and h and d):
         return out
+    if c == 0:
+        if d != 128 or s > 64 or kv == 0 or h % kv:
+            raise _native.Unsupported("attention_cached", _native.QIM_ERR_SHAPE, f"{s} tokens, {h} heads of {d} on {kv} K/V heads")
+        return out.zero_()
     nbytes = _native.bytes_on(device, "qim_attention_cached_workspace_bytes", b, s, c, h, kv)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     _native.call_on(device, "qim_attention_cached", q.data_ptr(), *strides, cache.k.data_ptr(),

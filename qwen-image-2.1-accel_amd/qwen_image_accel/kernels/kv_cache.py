@@ -102,6 +102,8 @@ def write_cache(cache, k, v, start=0, count=None):
     counts = None if count is None else per_sequence("write_cache", "count", count, b, device)
     if isinstance(start, torch.Tensor):
         starts, first = per_sequence("write_cache", "start", start, b, device), 0
+        if c == 0:
+            return
     else:
         starts, first = None, int(start)
         if not 0 <= first <= c - s:

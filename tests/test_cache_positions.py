@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from qwen_image_accel import _native
-from qwen_image_accel.kernels import kv_cache
+from qwen_image_accel.kernels import attention, kv_cache
 from tests.helpers import bf16_randn
 
 
@@ -31,3 +31,24 @@ def test_a_start_that_no_64_bits_hold_is_refused(dev, start):
         kv_cache.write_cache(cache, x, x, start=start)
     torch.cuda.synchronize()
     assert all(bool((t.view(torch.uint8) == 0x38).all()) for t in cache)
+
+
+@pytest.mark.gpu
+def test_a_cache_of_no_positions(dev):
+    """No key to see, nowhere to write, nothing to read: zeros, nothing, empty; a host start does not fit."""
+    say("no positions")
+    cache = kv_cache.empty_cache(2, 0, 2, 128, dev)
+    x = bf16_randn(torch.Generator().manual_seed(0), (2, 3, 2, 128)).to(dev)
+    n = torch.tensor([5, 0], dtype=torch.int32, device=dev)
+    kv_cache.write_cache(cache, x, x, start=n)
+    with pytest.raises(_native.QimError):
+        kv_cache.write_cache(cache, x, x, start=0)
+    assert [t.shape for t in kv_cache.read_cache(cache)] == [(2, 0, 2, 128)] * 2
+    tree = torch.ones(3, 3, dtype=torch.bool, device=dev)
+    out = torch.full_like(x, 7.0)
+    assert attention.attention_cached(x, cache, n, tree=tree, out=out) is out and not out.any()
+    assert not attention.attention_cached(x[:, :1], cache, n).any()
+    with pytest.raises(_native.Unsupported):
+        attention.attention_cached(torch.zeros(2, 65, 2, 128, dtype=torch.bfloat16, device=dev), cache, n)
+    with pytest.raises(_native.Unsupported):
+        attention.attention_cached(torch.zeros(2, 1, 3, 128, dtype=torch.bfloat16, device=dev), cache, n)
