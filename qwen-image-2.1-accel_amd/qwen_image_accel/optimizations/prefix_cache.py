@@ -7,7 +7,16 @@ value for 2): pass its result as ``layer_cache``, and the cached-decode
 processors read it in the fused norm + RoPE + pack kernel.  There is no
 reference counterpart.
 """
-from qwen_image_accel.kernels.kv_cache import empty_cache, read_cache, write_cache
+import torch
+
+from qwen_image_accel.kernels.kv_cache import empty_cache, read_cache, token_strides, write_cache
+
+
+def _writable(t):
+    """t, or a copy where ``write_cache`` does not take its rows as they lie."""
+    strides = token_strides(t)
+    ok = strides is not None and strides[1] >= t.shape[2] * t.shape[3] and not (strides[0] % 8 or strides[1] % 8 or t.data_ptr() % 16)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 class QuantizedLayerCache:
@@ -19,7 +28,7 @@ class QuantizedLayerCache:
             raise ValueError(f"prefix K and V must both be (B, P, H, D), got {tuple(k.shape)} and {tuple(v.shape)}")
         b, p, h, d = k.shape
         self.quantized = empty_cache(b, p, h, d, k.device)
-        write_cache(self.quantized, k, v)
+        write_cache(self.quantized, _writable(k), _writable(v))
 
     def get(self):
         """The prefix in bf16, for a consumer that takes no MXFP8."""

@@ -1,10 +1,11 @@
 """Where rows of the MXFP8 K/V cache may be written and read: positions past what the
-arguments' types hold, and caches of no positions."""
+arguments' types hold, caches of no positions, and prefixes of any strides."""
 import pytest
 import torch
 
 from qwen_image_accel import _native
 from qwen_image_accel.kernels import attention, kv_cache
+from qwen_image_accel.optimizations.prefix_cache import QuantizedLayerCache
 from tests.helpers import bf16_randn
 
 
@@ -52,3 +53,18 @@ def test_a_cache_of_no_positions(dev):
         attention.attention_cached(torch.zeros(2, 65, 2, 128, dtype=torch.bfloat16, device=dev), cache, n)
     with pytest.raises(_native.Unsupported):
         attention.attention_cached(torch.zeros(2, 1, 3, 128, dtype=torch.bfloat16, device=dev), cache, n)
+
+
+@pytest.mark.gpu
+def test_a_prefix_of_any_strides_becomes_a_quantized_layer_cache(dev):
+    """Views whose heads are not packed, whose rows are not 16-byte aligned, or of one prompt for several sequences."""
+    say("strided prefixes")
+    g = torch.Generator().manual_seed(0)
+    wide = bf16_randn(g, (2, 4, 9, 132)).to(dev)          # (B, H, P, ...)
+    views = [wide[..., :128].transpose(1, 2), wide[..., 4:].transpose(1, 2), wide[:, :, :, :128].transpose(1, 2)[:, 2:7],
+             wide[:1, ..., :128].transpose(1, 2).expand(2, 9, 4, 128), bf16_randn(g, (2, 9, 516)).to(dev)[..., 4:].view(2, 9, 4, 128)]
+    for view in views:
+        got = QuantizedLayerCache(view, view * 2).quantized
+        want = QuantizedLayerCache(view.contiguous(), (view * 2).contiguous()).quantized
+        for a, b in zip(got, want):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
