@@ -115,10 +115,11 @@ static int cache_common(const char *who, const void *kc, const void *ks, const v
     return QIM_OK;
 }
 
-// Waves of 64 * CACHE_U vectors per token and tensor; 0 if the launch is too large.
+// Waves of 64 * CACHE_U vectors per token and tensor; 0 if the launch is too large
+// (2^32 threads or more).
 static int64_t cache_grid(int64_t tokens, int64_t W, uint32_t &groups, uint32_t &waves) {
     const int64_t g = (W / 8 + 64 * CACHE_U - 1) / (64 * CACHE_U);
-    if (tokens >= (1ll << 31) / (2 * g)) return 0;
+    if (tokens > ((1ll << 26) - 4) / (2 * g)) return 0;
     groups = (uint32_t)g;
     waves = (uint32_t)(tokens * 2 * g);
     return ((int64_t)waves + 3) / 4;

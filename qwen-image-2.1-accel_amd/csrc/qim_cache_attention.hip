@@ -552,7 +552,7 @@ using namespace qim;
 
 static bool ca_shape(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {
     return B > 0 && S > 0 && S <= CA_MAX_S && C > 0 && C < (1ll << 31) && HK > 0 && H > 0 && H % HK == 0 && H <= (1 << 16) && B < (1 << 20) &&
-           B * HK * ((S * (H / HK) + 15) / 16) < (1 << 25) && B * C < (1ll << 40) / HK && ca_plan(B, S, C, H, HK).grid() < (1ll << 31);
+           B * HK * ((S * (H / HK) + 15) / 16) < (1 << 25) && B * C < (1ll << 40) / HK && ca_plan(B, S, C, H, HK).grid() * (64 * CA_WAVES) < (1ll << 32);
 }
 
 extern "C" int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK) {

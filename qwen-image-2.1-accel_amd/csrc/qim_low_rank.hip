@@ -575,7 +575,8 @@ extern "C" int qim_low_rank(const void *x, int64_t ldx, const void *down, const 
     QIM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), QIM_ERR_ARG,
                 "%s: workspace of %lld bytes, this problem needs %lld", who, (long long)workspace_bytes, (long long)need);
     const int64_t up_tiles = (M + 16 * LR_MT - 1) / (16 * LR_MT);
-    QIM_REQUIRE(up_tiles * pl.nchunk * parts < (1ll << 31) && pl.tiles * pl.chunks < (1ll << 31) && pl.slots * pl.rblocks < 65536,
+    QIM_REQUIRE(up_tiles * pl.nchunk * parts < (1ll << 32) / 256 && pl.tiles * pl.chunks < (1ll << 32) / (64 * LR_WAVES) &&
+                    pl.slots * pl.rblocks < 65536,
                 QIM_ERR_SHAPE, "%s: too large", who);
     QIM_REQUIRE(!lr_shares(out, ldo, N, x, ldx, K, M) &&
                     (!base || (base == out && (ldb == ldo || M == 1)) || !lr_shares(out, ldo, N, base, ldb, N, M)),
