@@ -504,9 +504,9 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(CacheAttnArgs p, int64_
 // costs a round the time of its bytes, or that of a wave's work where rows share them
 // (8 waves a CU: 2100 with 16 rows, 3000 with 32); a round 1500 for its start;
 // chunks 5000 for the second launch and their partial results, written and read.
-// (5 sequences of up to 8040 keys, 64 rows a head, 32 heads: 182 us as 16 rows a wave,
-// 118 as 32; 14 of up to 428: 39 and 48.  Wider tiles gain nothing: 128 and 53 as 64
-// rows.  16 of up to 8392, one row: 5 rounds of chunks 168 us, 2.95 172, 2.1 200; 2 of up to
+// (With the join, 5 sequences of up to 8040 keys, 64 rows a head, 32 heads: 196 us as 16
+// rows a wave, 136 as 32; 14 of up to 428: 41 and 52.  64 rows a wave gained nothing:
+// 128 and 53 where 32 took 118 and 48, without the join and p's second term.  16 of up to 8392, one row: 5 rounds of chunks 168 us, 2.95 172, 2.1 200; 2 of up to
 // 131072, 8 heads: 249 chunks 88 us, 257 chunks 119.)
 struct CaPlan {
     int64_t rows, nr, ntile, wide, chunks, groups, B, HK;

@@ -520,9 +520,9 @@ static LrPlan lr_plan(int64_t M, int64_t seq, int64_t K, int64_t PR, int64_t wid
 
 // One launch (k_lr_small) for at most 16 rows whose adapter and own rows are few
 // values: every workgroup reads them (16 adapters of rank 16, a row each, K and N 4096:
-// 9.6 us).  One against two launches, us per call alone
-// on the GPU (N 4096; in a stream of calls the host's share of the second launch
-// adds 2.4): R 8, 8 rows each, K 1024 (16384 values) 4.6 / 6.8; R 16, 1 row, K 4096
+// 9.6 us).  The GPU's time decides, as in a replayed graph or behind other work: one
+// against two launches, us per call (N 4096; where the host is what is waited for, the second
+// launch costs 2.4 more): R 8, 8 rows each, K 1024 (16384 values) 4.6 / 6.8; R 16, 1 row, K 4096
 // (69632) 9.1 / 9.3; 4 rows each (81920) 8.8 / 7.8; R 16, 1 row, K 12288 (208896) 17.9 / 10.9.
 constexpr int64_t LR_SMALL = 72 * 1024;
 static bool lr_small(int64_t M, int64_t seq, int64_t K, int64_t R) {

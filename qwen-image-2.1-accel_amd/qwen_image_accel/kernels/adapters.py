@@ -52,10 +52,12 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     (zeros); ``out``: where the result goes, by default a new tensor; ``base`` itself is fine, else it
     shares no rows with ``base`` or ``x``.
     ``parts``: N is that many equal column blocks, and block j uses rows
-    [j * R, (j + 1) * R) of down: the adapters of a stacked projection (Q/K/V,
-    gate/up) in one call.  The sum is taken in fp32 and rounded once.  K, R and
+    [j * R, (j + 1) * R) of down: the adapters of a stacked projection (Q/K/V)
+    in one call.  The sum is taken in fp32 and rounded once.  K, R and
     N / parts are multiples of 8; rows may lie any multiple of 8 elements apart.
-    A row's result depends on its own x, base and adapter only.  No gradient is recorded."""
+    No value of another row enters a row.  Its bits are the same for the same number
+    of rows and sequence length; another of these may order the fp32 sums differently.
+    No gradient is recorded."""
     def refuse(why):
         raise _native.Unsupported("low_rank", _native.QIM_ERR_LAYOUT, why)
     device = x.device
