@@ -150,11 +150,13 @@ def _replace(block, path, module):
 def quantize_transformer(transformer, skip_blocks=None, layers=None):
     """Swap the planned linears for MXFP8Linear (everything else stays bf16)
     and return their module paths ("transformer_blocks.<i>.<path>").  Adapters
-    (optimizations/adapters.py) are installed afterwards."""
-    if getattr(transformer, "_qw_adapters", None) is not None:
-        raise RuntimeError("linears with adapters beside them are not converted; remove_adapters first")
+    beside these linears (optimizations/adapters.py) are installed afterwards."""
+    from qwen_image_accel.weights import ADAPTED_BASE
+    blocks, skip = transformer.transformer_blocks, skipped_blocks(skip_blocks)
+    for path in sorted(selected_layers(layers)):
+        if any(i not in skip and hasattr(block.get_submodule(path), ADAPTED_BASE) for i, block in enumerate(blocks)):
+            raise RuntimeError(f"{path} has adapters beside it and is not converted; remove_adapters first")
     plan = conversion_plan(transformer, skip_blocks, layers)
-    blocks = transformer.transformer_blocks
     with torch.no_grad():
         for i, path, linear in plan:
             _replace(blocks[i], path, MXFP8Linear(linear))

@@ -9,7 +9,7 @@ from torch import nn
 
 from qwen_image_accel import _native, pipeline, weights
 from qwen_image_accel.optimizations import adapters as install
-from qwen_image_accel.optimizations import decode
+from qwen_image_accel.optimizations import decode, mxfp8
 from qwen_image_accel.optimizations.mxfp8 import MXFP8Linear, quantize_transformer
 from tests import fake_qwen21 as fq
 from tests import requests_ref as R
@@ -394,16 +394,21 @@ def test_mxfp8_weights_load_beside_adapters(tmp_path):
     assert weights.save_mxfp8(both, again) == names and weights.load_mxfp8(saved, again) == names
 
 
-def test_linears_with_adapters_are_not_silently_left_out_of_the_conversion():
+def test_linears_with_adapters_are_not_silently_left_out_of_the_conversion(monkeypatch):
     """quantize_transformer converts linears; with adapters in front of them it would find none of those."""
     _, both, _ = block_with_adapters()
     with pytest.raises(RuntimeError, match="remove_adapters"):
         quantize_transformer(both, skip_blocks="")
+    monkeypatch.setenv("QW21_MXFP8_SKIP_BLOCKS", "")    # its default skips the only block there is
     with pytest.raises(RuntimeError, match="remove_adapters"):
         pipeline.install_hot_path(both, "mxfp8", validate=False)
     assert type(both.transformer_blocks[0].attn.to_k) is nn.Linear and getattr(both, "_qw_hot_path", None) is None
-    install.remove_adapters(both)
+    # Conversions of other linears are as without adapters.
     assert quantize_transformer(both, skip_blocks="0") == []
+    monkeypatch.setattr(mxfp8, "MXFP8Linear", HostMXFP8)
+    assert quantize_transformer(both, skip_blocks="", layers="mlp") == [f"transformer_blocks.0.img_mlp.{n}" for n in ("gate_layer", "out", "proj")]
+    install.remove_adapters(both)
+    assert len(quantize_transformer(both, skip_blocks="")) == 4
 
 
 def test_adapters_of_no_linear_are_refused():
