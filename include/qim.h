@@ -347,6 +347,48 @@ int qim_attention_cached(const void *q, int64_t ldqb, int64_t ldq, const void *k
                          int64_t HK, int64_t D, float scale, void *stream);
 int64_t qim_attention_cached_workspace_bytes(int64_t B, int64_t S, int64_t C, int64_t H, int64_t HK);
 
+/* Norms of qim_residual_norm. */
+enum qim_norm {
+    QIM_NORM_NONE = 0,
+    QIM_NORM_RMS = 1,    /* x / sqrt(mean(x^2) + eps), times a weight if there is one    */
+    QIM_NORM_LAYER = 2,  /* (x - mean) / sqrt(var + eps), the biased variance, no affine */
+};
+/* Flag of qim_residual_norm beside QIM_ADALN_ADD_ONE and QIM_ADALN_TILED: the eager operators' roundings. */
+#define QIM_NORM_EAGER 4
+
+/* The gated residual of a block with the norms on both of its sides, in one pass:
+ *   u = post(x),  h_out = h + alpha * gate * u,  z = norm(h_out) * (scale or 1 + scale) + shift
+ * h, x, h_out: (M, D) bf16, row strides ldh, ldx, ldho.  gate, scale, shift: bf16 (D,) vectors or NULL, that of row
+ * m at m / seq times gate_b, scale_b, shift_b elements (0: one for all).  post_weight, norm_weight: bf16 (D,) of
+ * an RMSNorm, or NULL.  z_scales NULL: z is (M, D) bf16, row stride ldz; else z holds the MXFP8 codes
+ * (Mp, D), row-major or tiled (QIM_ADALN_TILED), and z_scales their swizzled exponents, as
+ * qim_adaln_quantize writes them.  Computed in fp32 with row sums in float64 and rounded once, z from the
+ * unrounded h_out.  With QIM_NORM_EAGER (post none, norm LAYER, alpha 1, gate and scale present): the bits of
+ * qim_gated_residual followed by qim_adaln or qim_adaln_quantize on its result.  An output may be h or x
+ * itself (the same rows) and is else apart from the inputs and the other output; MXFP8 outputs are apart from all.  D a
+ * multiple of 8 up to 16384 (of 128 for MXFP8); strides multiples of 8, operands 16-byte aligned.  No
+ * reference counterpart. */
+int qim_residual_norm(const void *h, int64_t ldh, const void *x, int64_t ldx, int post, const void *post_weight,
+                      float post_eps, const void *gate, int64_t gate_b, float alpha, int norm,
+                      const void *norm_weight, float norm_eps, const void *scale, int64_t scale_b,
+                      const void *shift, int64_t shift_b, int flags, void *h_out, int64_t ldho, void *z, int64_t ldz,
+                      void *z_scales, int64_t M, int64_t D, int64_t seq, void *stream);
+
+/* Products of a few rows with 4-bit weights:
+ *   out[m, n] = sum_k x[m, k] W[n, k] (+ bias[n]),  or with a second weight silu(x W^T) * (x W2^T)
+ * in fp32, rounded once.  x: (M, K) bf16, row stride ldx (a multiple of 8); out: (M, N) bf16, or fp32 with out_f32,
+ * any row stride ldo, apart from x; bias: bf16 (N,) or NULL (none with a second weight).
+ * group 32, 64 or 128: W[n, k] = s (q - z) with codes q 0..15, a bf16 scale s and a zero point z (zeros NULL: 8) per
+ * group of k; group 0: W[n, k] = E2M1(code) 2^(e - 127), an exponent byte e per 32 of k.  K is a multiple of the group.
+ * The weight is laid out in tiles of 16 rows and steps of 128 k (N and K padded with zeros): codes (tiles, steps, 64, 16)
+ * bytes, where bytes 4j .. 4j + 3 of lane l hold row l % 16, k = 32 j + 8 (l / 16) + 0..7 of the step: for int4 byte i
+ * holds k i in its low and k i + 4 in its high half, for E2M1 k 2i and 2i + 1; scales and zeros (tiles,
+ * steps, 128 / group, 16) of bf16 and of bytes; exponents (tiles, steps, 16, 4) bytes.  All 16-byte aligned.  No
+ * reference counterpart. */
+int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const void *codes, const void *scales, const void *zeros,
+                       const void *codes2, const void *scales2, const void *zeros2, const void *bias, void *out,
+                       int64_t ldo, int out_f32, int64_t M, int64_t N, int64_t K, void *stream);
+
 /* Low-rank adapters of several requests beside one projection:
  *   out[m] = bf16(base[m] + scale[a] * up[a] (down[a] x[m])),  a = index[m / seq]
  * with the products and their sum in fp32.  x: (M, K) bf16, row stride ldx;

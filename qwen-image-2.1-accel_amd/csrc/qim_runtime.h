@@ -48,6 +48,22 @@ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Whether the bf16 rows of out, (M, N), share memory with the rows of t, (M, W): ranges that meet, other than
+// other columns of one buffer.
+inline bool rows_share(const void *out, int64_t ldo, int64_t N, const void *t, int64_t ldt, int64_t W, int64_t M) {
+    const int64_t d = (int64_t)((intptr_t)t - (intptr_t)out) / 2;  // both 16-byte aligned
+    if (d >= (M - 1) * ldo + N || -d >= (M - 1) * ldt + W) return false;
+    if (M == 1 || ldt != ldo) return true;
+    const int64_t col = (d % ldo + ldo) % ldo;
+    return col < N || col + W > ldo;
+}
+
+// Whether two ranges of bytes meet.
+inline bool bytes_share(const void *a, int64_t na, const void *b, int64_t nb) {
+    const intptr_t p = (intptr_t)a, q = (intptr_t)b;
+    return p < q + nb && q < p + na;
+}
+
 // Compute units of the current device, cached per device (0 if unknown).
 int device_cus();
 

@@ -16,7 +16,8 @@ LIB_PATH = os.environ.get("QIM_LIBRARY", os.path.join(os.path.dirname(os.path.ab
                                                        "libqim.so"))
 
 QIM_OK, QIM_ERR_ARG, QIM_ERR_SHAPE, QIM_ERR_LAYOUT, QIM_ERR_LAUNCH = range(5)
-ADALN_ADD_ONE, ADALN_TILED = 1, 2
+ADALN_ADD_ONE, ADALN_TILED, NORM_EAGER = 1, 2, 4
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
 GEMM_A_TILED, GEMM_B_TILED, GEMM_OUT_TILED, GEMM_OUT_F32, GEMM_OUT_F16 = 1, 2, 4, 8, 16
 EPI_NONE, EPI_BIAS, EPI_GATED_RESIDUAL, EPI_SWIGLU, EPI_SWIGLU_QUANT, EPI_QK_NORM_ROPE = range(6)
 SWIGLU_GROUP = 32
@@ -77,6 +78,9 @@ SIGNATURES = {
     "qim_attention_cached_workspace_bytes": (_I, [_I] * 5),
     "qim_low_rank": (_C, [_P, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _I] + [_I] * 7 + [_P]),
     "qim_low_rank_workspace_bytes": (_I, [_I] * 5),
+    "qim_residual_norm": (_C, [_P, _I, _P, _I, _C, _P, _F, _P, _I, _F, _C, _P, _F, _P, _I, _P, _I, _C, _P, _I, _P, _I, _P, _I, _I, _I,
+                               _P]),
+    "qim_fourbit_matmul": (_C, [_P, _I, _C] + [_P] * 8 + [_I, _C, _I, _I, _I, _P]),
     "qim_debug_e4m3_encode": (_C, [_P, _P, _I, _P]),
     "qim_debug_e4m3_encode_scaled": (_C, [_P, _C, _P, _I, _P]),
     "qim_debug_bf16_round": (_C, [_P, _P, _I, _P]),

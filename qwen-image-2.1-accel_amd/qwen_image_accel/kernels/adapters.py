@@ -13,7 +13,7 @@ from qwen_image_accel import _native
 MAX_RANK = 128
 
 
-def _rows(t):
+def row_layout(t):
     """(rows, width, row stride) of a (M, W) or (B, S, W) tensor whose rows lie
     one stride apart, else None.  An axis of one element may have any stride."""
     shape = t.shape
@@ -37,7 +37,7 @@ def _rows(t):
 def takes_rows(t):
     """Whether ``low_rank`` takes the rows of t as they lie: one multiple of 8
     elements apart, 16-byte aligned."""
-    rows = _rows(t)
+    rows = row_layout(t)
     return rows is not None and rows[2] >= rows[1] and rows[2] % 8 == 0 and t.data_ptr() % 16 == 0
 
 
@@ -63,7 +63,7 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     device = x.device
     if not x.is_cuda:
         refuse("expects tensors on the GPU")
-    xr = _rows(x)
+    xr = row_layout(x)
     bf16, lead = torch.bfloat16, x.shape[:-1]
     if x.dtype != bf16 or xr is None or xr[1] == 0:
         refuse("x is a bf16 (M, K) or (B, S, K) tensor, K > 0, with rows one stride apart")
@@ -81,7 +81,7 @@ def low_rank(x, down, up, index, *, scale=None, base=None, out=None, parts=1):
     shape = lead + (n,)
 
     def stride(t):
-        rows = _rows(t)
+        rows = row_layout(t)
         if rows is None or t.dtype != bf16 or t.shape != shape or t.device != device:
             refuse(f"base and out are bf16 {tuple(shape)} tensors on {device} with rows one stride apart")
         return rows[2]

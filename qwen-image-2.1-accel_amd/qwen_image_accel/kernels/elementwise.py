@@ -3,11 +3,15 @@
 Reference interface: src/qwen_image_accel/kernels/elementwise.py --
 ``residual(h, x, gate)`` (:26-34) and ``rope_qk(q, k, freqs)`` (:63-69).
 Kernels: libqim's ``qim_gated_residual`` and ``qim_rope_qk``.
+``residual_norm`` (no reference counterpart) is the residual with the norms on
+both sides of it in one pass: libqim's ``qim_residual_norm``.
 """
 import torch
 
 from qwen_image_accel import _native
+from qwen_image_accel.kernels.adapters import row_layout
 from qwen_image_accel.kernels.bf16 import HEAD_DIMS
+from qwen_image_accel.kernels.mxfp8 import empty_quantized
 
 
 def residual(h, x, gate):
@@ -26,6 +30,95 @@ def residual(h, x, gate):
                      _native.ptr(out), b * s, d, s, _native.stream(h.device))
         return out
     return h + gate * x
+
+
+def _norm_of(norm, d, device, refuse):
+    """(kind, weight or None, eps) of a norm over d values that ``residual_norm`` takes."""
+    if norm is None:
+        return _native.NORM_NONE, None, 0.0
+    weight, eps = getattr(norm, "weight", None), getattr(norm, "eps", None)
+    if eps is None or getattr(norm, "bias", None) is not None:
+        refuse("a norm has an eps and no bias")
+    shape = getattr(norm, "normalized_shape", None)
+    if shape is not None and tuple(shape) != (d,):
+        refuse(f"a norm over {tuple(shape)} of rows of {d}")
+    if shape is not None and not isinstance(norm, torch.nn.RMSNorm):
+        if weight is not None or getattr(norm, "elementwise_affine", False):
+            refuse("a LayerNorm has no affine")
+        return _native.NORM_LAYER, None, float(eps)
+    if weight is not None and (weight.shape != (d,) or weight.dtype != torch.bfloat16 or weight.device != device
+                               or not weight.is_contiguous()):
+        refuse(f"an RMSNorm's weight is a contiguous bf16 ({d},) tensor on {device}")
+    return _native.NORM_RMS, weight, float(eps)
+
+
+def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale=None, shift=None, add_one=False,
+                  quantized=False, tiled=False, rounding="once", out=None):
+    """The end of one block branch and the start of the next in one pass:
+
+        h' = h + residual_scale * gate * post(x),   z = norm(h') * scale + shift
+
+    Returns (h', z).  h, x: (B, S, D) or (M, D) bf16 on the GPU, rows any multiple of 8 elements apart, D
+    a multiple of 8 up to 16384.  ``norm`` and ``post`` (None: x itself): an RMSNorm (``weight`` bf16 or
+    None, ``eps``) or a LayerNorm without affine (``normalized_shape``, ``eps``).  ``gate``, ``scale``, ``shift``: None,
+    (B, 1, D) bf16, one vector per sequence at any stride that is a multiple of 8, or one for all, (1, 1, D) or (D,).
+    ``add_one``: 1 + scale instead of scale.  z is a new bf16 tensor, or with ``quantized`` a
+    ``mxfp8.Quantized`` (``tiled``: in the GEMM's layout; D a multiple of 128).  ``out``: where h' goes, by default a
+    new tensor; h or x itself is fine, else it shares no rows with them.
+
+    ``rounding="once"``: fp32 throughout, h' and z rounded at their ends (z from the unrounded h').
+    ``"eager"``: the bits of ``residual(h, x, gate)`` followed by ``layernorm.layer_norm_scale`` or
+    ``epilogue.layer_norm_scale_quantize`` on its result; for a gate and a scale, a LayerNorm, no post and a
+    residual_scale of 1.  No gradient is recorded."""
+    def refuse(why):
+        raise _native.Unsupported("residual_norm", _native.QIM_ERR_LAYOUT, why)
+    device, shape = h.device, h.shape
+    if not h.is_cuda:
+        refuse("expects tensors on the GPU")
+    if rounding not in ("once", "eager"):
+        raise ValueError(f"rounding={rounding!r}: once or eager")
+    if norm is None:
+        raise ValueError("residual_norm needs the norm that follows the residual")
+
+    def rows(t):
+        lay = row_layout(t) if t.dtype == torch.bfloat16 and t.shape == shape and t.device == device else None
+        if lay is None:
+            refuse(f"h, x and out are bf16 {tuple(shape)} tensors on {device} with rows one stride apart")
+        return lay
+    if len(shape) not in (2, 3):
+        refuse("h is a (B, S, D) or (M, D) tensor")
+    m, d, ldh = rows(h)
+    ldx = rows(x)[2]
+    batch = shape[0] if len(shape) == 3 else 1
+
+    def vector(t):
+        """(address, elements between sequences)"""
+        if t is None:
+            return None, 0
+        if t.dtype != torch.bfloat16 or t.device != device or t.shape not in ((batch, 1, d), (1, 1, d), (d,)) or (d > 1 and t.stride(-1) != 1):
+            refuse(f"gate, scale and shift are bf16 ({batch}, 1, {d}), (1, 1, {d}) or ({d},) tensors on {device}")
+        return t.data_ptr(), t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else 0
+    post_kind, post_w, post_eps = _norm_of(post, d, device, refuse)
+    norm_kind, norm_w, norm_eps = _norm_of(norm, d, device, refuse)
+    vectors = vector(gate) + vector(scale) + vector(shift)
+    if out is None:
+        out, ldo = torch.empty(shape, dtype=torch.bfloat16, device=device), d
+    else:
+        ldo = rows(out)[2]
+    if quantized:
+        z = empty_quantized(m, d, device, shape, tiled)
+        z_ptr, z_scales = z.values.data_ptr(), z.scales.data_ptr()
+    else:
+        z = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        z_ptr, z_scales = z.data_ptr(), None
+    if m == 0 or d == 0:
+        return out, z
+    flags = ((_native.ADALN_ADD_ONE if add_one and scale is not None else 0) | (_native.ADALN_TILED if quantized and tiled else 0)
+             | (_native.NORM_EAGER if rounding == "eager" else 0))
+    _native.call_on(device, "qim_residual_norm", h.data_ptr(), ldh, x.data_ptr(), ldx, post_kind, _native.ptr(post_w), post_eps,
+                    *vectors[:2], float(residual_scale), norm_kind, _native.ptr(norm_w), norm_eps, *vectors[2:], flags,
+                    out.data_ptr(), ldo, z_ptr, d, z_scales, m, d, shape[1] if len(shape) == 3 else m)
+    return out, z
 
 
 MOD_COPY, MOD_ONE_PLUS, MOD_TANH = 0, 1, 2
