@@ -389,6 +389,23 @@ int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const void *codes,
                        const void *codes2, const void *scales2, const void *zeros2, const void *bias, void *out,
                        int64_t ldo, int out_f32, int64_t M, int64_t N, int64_t K, void *stream);
 
+/* Attention of a few tokens of B requests that continue shared prefixes: qim_attention_cached over the keys of a prefix
+ * followed by those of the request's own cache, with a prefix read once for all of its requests.  pk, pks, pv, pvs: P
+ * prefixes of CP positions, kc, ks, vc, vs: B own caches of C (C may be 0, then none is read), both with HK heads.
+ * share: device int32 (B,), the prefix of each request (outside [0, P): none), or NULL for P = 1 (all requests on
+ * it); prefix_lengths: device int32 (P,), the keys of each prefix, or NULL (all CP); lengths: device int32 (B,), the
+ * own keys of each request; lengths outside the caches count as the nearest inside.  tree as in
+ * qim_attention_cached, over the last S own keys.  A row that sees no key is zeros.  P <= 4096.  workspace:
+ * qim_attention_shared_workspace_bytes(B, S, CP, C, H, HK, P, share != NULL) bytes, 16-byte aligned, not shared by calls
+ * that may overlap.  No reference counterpart. */
+int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, const void *pk, const void *pks, const void *pv,
+                         const void *pvs, const int32_t *prefix_lengths, const int32_t *share, const void *kc,
+                         const void *ks, const void *vc, const void *vs, const int32_t *lengths, const void *tree,
+                         int64_t tree_b, void *o, void *workspace, int64_t workspace_bytes, int64_t B, int64_t S,
+                         int64_t P, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t D, float scale, void *stream);
+int64_t qim_attention_shared_workspace_bytes(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P,
+                                             int shared);
+
 /* Low-rank adapters of several requests beside one projection:
  *   out[m] = bf16(base[m] + scale[a] * up[a] (down[a] x[m])),  a = index[m / seq]
  * with the products and their sum in fp32.  x: (M, K) bf16, row stride ldx;

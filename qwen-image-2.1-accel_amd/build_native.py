@@ -32,13 +32,14 @@ COMMON = [
 ]
 
 
-# Per-source additions.  qim_attention.hip and qim_cache_attention.hip: MFMA accumulators in architectural
+# Per-source additions.  The attention kernels: MFMA accumulators in architectural
 #   VGPRs (the "VGPR form"), operands in AGPRs, so the softmax reads the score
 #   tiles and the lazy O rescale multiplies O in place; the accumulation-
 #   register form copies every tile through v_accvgpr_read/write instead.
 EXTRA = {
     "qim_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "qim_cache_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "qim_shared_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1,0 +1,402 @@
+// Attention of a few tokens of many requests that continue shared prefixes: the prefixes and the requests' own keys in
+// MXFP8 caches (qim_cache.hip), head dim 128, query heads in groups of G that share a K/V head.
+//
+//   o[r] = (sum_prefix p_t V[t] + sum_own p_t V[t]) / (sum_prefix p_t + sum_own p_t),  p_t = 2^(c q_r . K[t] - m_r)
+//
+// The rows of all requests on one prefix (requests * S * G to a K/V head) are the columns of the same matrix products, so
+// that a prefix's codes are read and converted once for a tile of rows instead of once for every request.  Prefix and own
+// keys give partial results (numerator, maximum, sum; fp32) over chunks of keys, joined in a last launch.
+//
+// The rows of a prefix: its requests in the order of their numbers, S * G rows each.  Which requests those are is known on
+// the device only, so where a batch has several prefixes a first launch of one workgroup lists them.
+#include "qim_cache_attention.h"
+#include "qim_runtime.h"
+
+namespace qim {
+
+constexpr int SA_WAVES = 4;
+constexpr int SA_MAX_PREFIXES = 4096;
+
+// A space of key chunks: V sequences of up to C keys (own: a request and a tile of its rows; prefix: a tile of rows),
+// cut into `chunks` pieces more than there are sequences, at most.  Partial results by (piece, K/V head, row of the tile).
+struct SaSpace {
+    float *part_o;    // 128 values each
+    float2 *part_ml;  // (maximum, sum)
+    int2 *dir;        // per sequence: its first piece and their number
+    int V, chunks, rows;
+    uint32_t blocks;  // workgroups
+};
+struct SaArgs {
+    const uint16_t *q;
+    int64_t ldqb, ldq;
+    const uint8_t *pk, *pks, *pv, *pvs, *kc, *ks, *vc, *vs;
+    const int32_t *lengths, *plengths, *share;
+    const uint8_t *tree;
+    int64_t tree_b, CP, C;
+    uint16_t *o;
+    SaSpace pre, own;
+    int4 *tiles;      // per prefix tile: prefix, first of its requests in `order`, their rows, the tile's first row (share only)
+    int32_t *order;   // the requests by prefix
+    int2 *where;      // per request: its prefix's first tile (-1: none), its place among the prefix's requests
+    int B, S, H, HK, G, P, ntile;  // ntile: row tiles of a request's own keys
+    float scale_log2e;
+};
+
+__device__ __forceinline__ int64_t sa_clamp(int64_t n, int64_t most) { return n < 0 ? 0 : n > most ? most : n; }
+__device__ __forceinline__ int64_t sa_prefix_length(const SaArgs &p, int i) { return p.plengths ? sa_clamp(p.plengths[i], p.CP) : p.CP; }
+
+// Rows of a prefix tile.
+struct SaTile {
+    int prefix, first, rows, row0;
+};
+__device__ __forceinline__ SaTile sa_tile(const SaArgs &p, int i) {
+    if (!p.share) return SaTile{0, 0, p.B * p.S * p.G, i * p.pre.rows};
+    const int4 t = p.tiles[i];
+    return SaTile{t.x, t.y, t.z, t.w};
+}
+
+// The requests of each prefix, in their order, and the prefix's tiles of rows.  One workgroup; a wave per prefix counts and
+// lists with ballots, 64 requests at a time.
+__global__ __launch_bounds__(1024) void k_shared_plan(SaArgs p) {
+    extern __shared__ int32_t lds[];  // count, then first request, and first tile, of each prefix
+    int32_t *const first = lds, *const tile = lds + p.P;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = wave; i < p.P; i += 16) {
+        int n = 0;
+        for (int b = 0; b < p.B; b += 64)
+            n += (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(b + lane < p.B && p.share[b + lane] == i));
+        if (lane == 0) first[i] = n;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int requests = 0, tiles = 0;
+        for (int i = 0; i < p.P; i += 64) {
+            const int n = i + lane < p.P ? first[i + lane] : 0, t = (n * p.S * p.G + p.pre.rows - 1) / p.pre.rows;
+            const int ns = ca_scan(n, lane), ts = ca_scan(t, lane);
+            if (i + lane < p.P) {
+                first[i + lane] = requests + ns - n;
+                tile[i + lane] = tiles + ts - t;
+            }
+            requests += __builtin_amdgcn_readlane(ns, 63);
+            tiles += __builtin_amdgcn_readlane(ts, 63);
+        }
+        // Tiles that no prefix needs hold no rows.
+        for (int i = tiles + lane; i < p.pre.V; i += 64) p.tiles[i] = make_int4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < p.B; b += 1024)
+        if (p.share[b] < 0 || p.share[b] >= p.P) p.where[b] = make_int2(-1, 0);
+    for (int i = wave; i < p.P; i += 16) {
+        int n = 0;
+        for (int b = 0; b < p.B; b += 64) {
+            const bool mine = b + lane < p.B && p.share[b + lane] == i;
+            const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
+            if (mine) {
+                const int at = n + (int)__builtin_popcountll(all & ((1ull << lane) - 1));
+                p.order[first[i] + at] = b + lane;
+                p.where[b + lane] = make_int2(tile[i], at);
+            }
+            n += (int)__builtin_popcountll(all);
+        }
+        const int rows = n * p.S * p.G;
+        for (int t = lane; t * p.pre.rows < rows; t += 64) p.tiles[tile[i] + t] = make_int4(i, first[i], rows, t * p.pre.rows);
+    }
+}
+
+template <bool PRE>
+__device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
+    if constexpr (PRE) {
+        const SaTile t = sa_tile(p, i);
+        return t.rows ? sa_prefix_length(p, t.prefix) : 0;
+    }
+    return sa_clamp(p.lengths[i / p.ntile], p.C);
+}
+
+// Which piece this is: sequence v, its blocks [blk0, blk0 + per).  All sequences' blocks are cut into pieces of `per`, the
+// smallest of which there are at most chunks + V.  The first workgroup also writes the space's dir.
+template <bool PRE>
+__device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int64_t &blk0, int64_t &per) {
+    const int lane = threadIdx.x & 63;
+    auto blocks = [&](int i) { return i < sp.V ? (int)((sa_length<PRE>(p, i) + CA_KB - 1) / CA_KB) : 0; };
+    int64_t total = 0;
+    for (int i = 0; i < sp.V; i += 64) total += __builtin_amdgcn_readlane(ca_scan(blocks(i + lane), lane), 63);
+    const int64_t each = (total + sp.chunks - 1) / sp.chunks;
+    per = each > 1 ? each : 1;
+    uint32_t first = 0;
+    bool found = false;
+    for (int i = 0; i < sp.V && !(found && !writes); i += 64) {
+        const int n = (int)((blocks(i + lane) + per - 1) / per), last = ca_scan(n, lane);
+        const uint32_t from = first + last - n;
+        if (writes && i + lane < sp.V) sp.dir[i + lane] = make_int2((int)from, n);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(piece >= from && piece < from + n);
+        if (here) {
+            const int at = (int)__builtin_ctzll(here);
+            v = i + at;
+            blk0 = (int64_t)(piece - (uint32_t)__builtin_amdgcn_readlane((int)from, at)) * per;
+            found = true;
+        }
+        first += (uint32_t)__builtin_amdgcn_readlane(last, 63);
+    }
+    return found;
+}
+
+// One wave: a piece of keys of one K/V head for a tile of 16 * NR rows.
+template <bool PRE, int NR>
+__device__ __forceinline__ void sa_wave(const SaArgs &p, const SaSpace &sp, uint32_t block, uint8_t *vt) {
+    const int lane = threadIdx.x & 63, lr = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wide = (uint32_t)(p.HK + SA_WAVES - 1) / SA_WAVES, q8 = block >> 3, grp = q8 / wide;
+    const uint32_t piece = grp * 8 + (block & 7);  // the heads of a piece to one XCD
+    const int h = (int)((q8 - grp * wide) * SA_WAVES) + wave;
+    int v = 0;
+    int64_t blk0 = 0, per = 1;
+    if (!sa_piece<PRE>(p, sp, piece, block == 0 && wave == 0, v, blk0, per)) return;
+    if (h >= p.HK) return;
+    const int64_t len = sa_length<PRE>(p, v), W = (int64_t)p.HK * CA_D, C = PRE ? p.CP : p.C;
+    const SaTile tile = PRE ? sa_tile(p, v) : SaTile{v / p.ntile, 0, p.S * p.G, (v % p.ntile) * sp.rows};
+    const int64_t base = (int64_t)tile.prefix * C * W + h * CA_D;
+    const CaKeys keys{(PRE ? p.pk : p.kc) + base, (PRE ? p.pks : p.ks) + base / 32, (PRE ? p.pv : p.vc) + base,
+                      (PRE ? p.pvs : p.vs) + base / 32, C, W, len};
+    const int64_t nblk = (len + CA_KB - 1) / CA_KB, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
+    f32x4_t o[NR][8];
+    float m[NR], l[NR];
+    ca_wave<NR>(keys, blk0, blk1, p.scale_log2e, !PRE && p.tree ? len - p.S : len, vt,
+                [&](int t, uint64_t &bits) {
+                    int r = tile.row0 + 16 * t + lr;
+                    r = r < tile.rows ? r : tile.rows - 1;  // rows past the end: computed, not stored
+                    const int sg = p.S * p.G, i = PRE ? r / sg : 0, in = r - i * sg, s = in / p.G;
+                    const int b = PRE ? (p.share ? p.order[tile.first + i] : i) : tile.prefix;
+                    bits = PRE ? 0 : ca_tree_bits(p.tree ? p.tree + b * p.tree_b + s * p.S : nullptr, p.S);
+                    return p.q + b * p.ldqb + s * p.ldq + (h * p.G + (in - s * p.G)) * CA_D;
+                },
+                o, m, l);
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        float lt = l[t] + __shfl_xor(l[t], 16, 64);
+        lt += __shfl_xor(lt, 32, 64);
+        if (tile.row0 + 16 * t + lr >= tile.rows) continue;
+        const int64_t at = ((int64_t)piece * p.HK + h) * sp.rows + 16 * t + lr;
+        float *dst = sp.part_o + at * CA_D + 4 * kg;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4_t *>(dst + 16 * dt) = o[t][dt];
+        if (kg == 0) sp.part_ml[at] = make_float2(m[t], lt);
+    }
+}
+
+template <int NP, int NO>
+__global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_attn(SaArgs p) {
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[SA_WAVES * CA_VTILE];
+    uint8_t *const vt = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * CA_VTILE;
+    if (blockIdx.x < p.pre.blocks) sa_wave<true, NP>(p, p.pre, blockIdx.x, vt);
+    else sa_wave<false, NO>(p, p.own, blockIdx.x - p.pre.blocks, vt);
+}
+
+// Join the pieces of a row: GP groups of 32 lanes (4 head dims each) take them in turn, four loads at a time, and join in
+// LDS.  A row's pieces are its prefix's, then its own.
+template <int GP>
+__global__ __launch_bounds__(256) void k_shared_join(SaArgs p, int64_t nrows) {
+    __shared__ float4 so[8][32];
+    __shared__ float2 sml[8];
+    const int grp = threadIdx.x >> 5, ln = threadIdx.x & 31;
+    const int64_t g = (int64_t)blockIdx.x * (8 / GP) + grp / GP;
+    const bool live = g < nrows;
+    const int sg = p.S * p.G;
+    const int64_t row = live ? g : 0, item = row / sg;
+    const int r = (int)(row - item * sg), b = (int)(item / p.HK), h = (int)(item - (int64_t)b * p.HK);
+    const int2 od = p.own.dir[b * p.ntile + r / p.own.rows];
+    const int2 w = p.share ? p.where[b] : make_int2(0, b);
+    int2 pd = make_int2(0, 0);
+    int pr = 0;
+    if (w.x >= 0) {
+        const int64_t rr = (int64_t)w.y * sg + r;
+        pd = p.pre.dir[w.x + (int)(rr / p.pre.rows)];
+        pr = (int)(rr % p.pre.rows);
+    }
+    const int64_t pstep = (int64_t)p.HK * p.pre.rows, ostep = (int64_t)p.HK * p.own.rows;
+    const int64_t pfirst = pd.x * pstep + (int64_t)h * p.pre.rows + pr, ofirst = od.x * ostep + (int64_t)h * p.own.rows + r % p.own.rows;
+    const int n = pd.y + od.y;
+    const float ninf = -__builtin_inff();
+    float M = ninf, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = grp % GP; i < n; i += 4 * GP) {
+        float2 ml[4];
+        float4 f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = i + j * GP < n ? i + j * GP : i;
+            const bool pre = c < pd.y;
+            const int64_t at = pre ? pfirst + c * pstep : ofirst + (c - pd.y) * ostep;
+            ml[j] = (pre ? p.pre : p.own).part_ml[at];
+            f[j] = *reinterpret_cast<const float4 *>((pre ? p.pre : p.own).part_o + at * CA_D + 4 * ln);
+            if (i + j * GP >= n) ml[j] = make_float2(ninf, 0.f);
+        }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) Mn = ca_max(Mn, ml[j].x);
+        const float ref = Mn == ninf ? 0.f : Mn, sc = __builtin_amdgcn_exp2f(M - ref);
+        L *= sc;
+        acc = make_float4(acc.x * sc, acc.y * sc, acc.z * sc, acc.w * sc);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e = __builtin_amdgcn_exp2f(ml[j].x - ref);
+            if (i + j * GP < n) {  // (a repeated piece may hold NaN)
+                L += ml[j].y * e;
+                acc = make_float4(acc.x + f[j].x * e, acc.y + f[j].y * e, acc.z + f[j].z * e, acc.w + f[j].w * e);
+            }
+        }
+        M = Mn;
+    }
+    if constexpr (GP > 1) {
+        so[grp][ln] = acc;
+        if (ln == 0) sml[grp] = make_float2(M, L);
+        __syncthreads();
+        if (grp % GP) return;
+        M = ninf;
+#pragma unroll
+        for (int j = 0; j < GP; ++j) M = ca_max(M, sml[grp + j].x);
+        const float ref = M == ninf ? 0.f : M;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        L = 0.f;
+#pragma unroll
+        for (int j = 0; j < GP; ++j) {
+            const float e = __builtin_amdgcn_exp2f(sml[grp + j].x - ref);
+            const float4 f = so[grp + j][ln];
+            L += sml[grp + j].y * e;
+            acc = make_float4(acc.x + f.x * e, acc.y + f.y * e, acc.z + f.z * e, acc.w + f.w * e);
+        }
+    }
+    if (!live) return;
+    const float inv = L == 0.f ? 0.f : 1.0f / L;  // no visible key: zeros
+    const int s = r / p.G, head = h * p.G + (r - s * p.G);
+    uint16_t *dst = p.o + (((int64_t)b * p.S + s) * p.H + head) * CA_D + 4 * ln;
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// Row tiles and the pieces' numbers.
+struct SaPlan {
+    int64_t np, no, ntile, vp, vo, cp, co, gp, go, wide;  // 16-row tiles a wave; sequences, pieces beyond one each, pieces
+    int64_t HK, B;
+    bool shared;
+    static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
+    int64_t blocks_p() const { return (gp + 7) / 8 * 8 * wide; }
+    int64_t blocks_o() const { return (go + 7) / 8 * 8 * wide; }
+    int64_t rows_p() const { return gp * HK * np * 16; }
+    int64_t rows_o() const { return go * HK * no * 16; }
+    int64_t bytes() const {
+        return up(rows_p() * CA_D * 4) + up(rows_o() * CA_D * 4) + up(rows_p() * 8) + up(rows_o() * 8) + up(vp * 8) + up(vo * 8) +
+               (shared ? up(vp * 16) + up(B * 4) + up(B * 8) : 0);
+    }
+};
+static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P, bool shared) {
+    SaPlan pl;
+    const int64_t sg = S * (H / HK), rows = B * sg, cus = device_cus() > 0 ? device_cus() : 256;
+    pl.HK = HK;
+    pl.B = B;
+    pl.shared = shared;
+    pl.np = (rows + P - 1) / P > 16 ? 2 : 1;
+    pl.no = sg > 16 ? 2 : 1;
+    pl.wide = (HK + SA_WAVES - 1) / SA_WAVES;
+    pl.ntile = (sg + 16 * pl.no - 1) / (16 * pl.no);
+    pl.vo = B * pl.ntile;
+    // Several prefixes: each may end with a tile that is not full.
+    pl.vp = (rows + 16 * pl.np - 1) / (16 * pl.np) + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
+    const int64_t bp = (CP + CA_KB - 1) / CA_KB, bo = (C + CA_KB - 1) / CA_KB;
+    const int64_t at_once = 2 * cus / pl.wide > 8 ? 2 * cus / pl.wide : 8;  // pieces that run at a time
+    const int64_t wp = bp * pl.vp, wo = bo * pl.vo, slots = 2 * at_once;
+    auto pieces = [&](int64_t w, int64_t v, int64_t blocks) {
+        int64_t n = slots * w / (wp + wo > 0 ? wp + wo : 1) - v;
+        n = n < 1 ? 1 : n;
+        return n + v < v * blocks ? n : v * blocks - v > 1 ? v * blocks - v : 1;
+    };
+    pl.cp = pieces(wp, pl.vp, bp);
+    pl.co = pieces(wo, pl.vo, bo);
+    pl.gp = bp ? (pl.cp + pl.vp < pl.vp * bp ? pl.cp + pl.vp : pl.vp * bp) : 0;
+    pl.go = bo ? (pl.co + pl.vo < pl.vo * bo ? pl.co + pl.vo : pl.vo * bo) : 0;
+    // Pieces are numbered past their bound only where a space is empty; dir is written by its first workgroup.
+    if (pl.gp == 0) pl.gp = 1;
+    if (pl.go == 0) pl.go = 1;
+    return pl;
+}
+
+}  // namespace qim
+
+using namespace qim;
+
+static bool sa_shape(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P, int shared) {
+    if (!(B > 0 && S > 0 && S <= CA_MAX_S && P > 0 && P <= SA_MAX_PREFIXES && (shared || P == 1) && CP > 0 && C >= 0 && CP < (1ll << 31) &&
+          C < (1ll << 31) && HK > 0 && H > 0 && H % HK == 0 && H <= (1 << 16) && B < (1 << 20) && B * S * (H / HK) < (1 << 24) &&
+          B * C < (1ll << 40) / HK && P * CP < (1ll << 40) / HK))
+        return false;
+    const SaPlan pl = sa_plan(B, S, CP, C, H, HK, P, shared);
+    return (pl.blocks_p() + pl.blocks_o()) * (64 * SA_WAVES) < (1ll << 32) && B * S * H < (1ll << 26) && pl.vp * ((CP + 31) / 32) < (1ll << 31) &&
+           pl.vo * ((C + 31) / 32) < (1ll << 31);
+}
+
+extern "C" int64_t qim_attention_shared_workspace_bytes(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P,
+                                                        int shared) {
+    return sa_shape(B, S, CP, C, H, HK, P, shared) ? sa_plan(B, S, CP, C, H, HK, P, shared).bytes() : 0;
+}
+
+extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, const void *pk, const void *pks, const void *pv,
+                                    const void *pvs, const int32_t *prefix_lengths, const int32_t *share, const void *kc,
+                                    const void *ks, const void *vc, const void *vs, const int32_t *lengths, const void *tree,
+                                    int64_t tree_b, void *o, void *workspace, int64_t workspace_bytes, int64_t B, int64_t S,
+                                    int64_t P, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t D, float scale, void *stream) {
+    const char *who = "qim_attention_shared";
+    QIM_REQUIRE(q && pk && pks && pv && pvs && kc && ks && vc && vs && lengths && o && workspace, QIM_ERR_ARG, "%s: null pointer", who);
+    QIM_REQUIRE(D == CA_D, QIM_ERR_SHAPE, "%s: head dim %lld (128 only)", who, (long long)D);
+    QIM_REQUIRE(scale > 0.0f && scale < 1e30f, QIM_ERR_ARG, "%s: scale must be positive and finite", who);
+    QIM_REQUIRE(sa_shape(B, S, CP, C, H, HK, P, share ? 1 : 0), QIM_ERR_SHAPE,
+                "%s: B %lld, S %lld (1..64), %lld prefixes of %lld (one without share), C %lld, %lld heads on %lld K/V heads", who,
+                (long long)B, (long long)S, (long long)P, (long long)CP, (long long)C, (long long)H, (long long)HK);
+    QIM_REQUIRE(ldq >= H * D && ldqb >= 0 && ldq % 8 == 0 && ldqb % 8 == 0 && tree_b >= 0 && aligned16(q) && aligned16(pk) &&
+                    aligned16(pks) && aligned16(pv) && aligned16(pvs) && aligned16(kc) && aligned16(ks) && aligned16(vc) && aligned16(vs) &&
+                    aligned16(o) && aligned16(workspace) && ((reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(prefix_lengths) |
+                    reinterpret_cast<uintptr_t>(share)) & 3u) == 0,
+                QIM_ERR_LAYOUT, "%s: rows and the workspace must be 16-byte aligned", who);
+    const SaPlan pl = sa_plan(B, S, CP, C, H, HK, P, share != nullptr);
+    QIM_REQUIRE(workspace_bytes >= pl.bytes(), QIM_ERR_ARG, "%s: workspace of %lld bytes, this problem needs %lld", who,
+                (long long)workspace_bytes, (long long)pl.bytes());
+    QIM_REQUIRE(!bytes_share(o, 2 * B * S * H * D, q, 2 * ((B - 1) * ldqb + (S - 1) * ldq + H * D)), QIM_ERR_ARG, "%s: o overlaps q", who);
+    uint8_t *at = static_cast<uint8_t *>(workspace);
+    auto take = [&](int64_t n) {
+        uint8_t *r = at;
+        at += SaPlan::up(n);
+        return r;
+    };
+    SaArgs a{};
+    a.q = (const uint16_t *)q;
+    a.ldqb = ldqb;
+    a.ldq = ldq;
+    a.pk = (const uint8_t *)pk, a.pks = (const uint8_t *)pks, a.pv = (const uint8_t *)pv, a.pvs = (const uint8_t *)pvs;
+    a.kc = (const uint8_t *)kc, a.ks = (const uint8_t *)ks, a.vc = (const uint8_t *)vc, a.vs = (const uint8_t *)vs;
+    a.lengths = lengths, a.plengths = prefix_lengths, a.share = share;
+    a.tree = (const uint8_t *)tree;
+    a.tree_b = tree_b, a.CP = CP, a.C = C;
+    a.o = (uint16_t *)o;
+    a.pre.part_o = (float *)take(pl.rows_p() * CA_D * 4);
+    a.own.part_o = (float *)take(pl.rows_o() * CA_D * 4);
+    a.pre.part_ml = (float2 *)take(pl.rows_p() * 8);
+    a.own.part_ml = (float2 *)take(pl.rows_o() * 8);
+    a.pre.dir = (int2 *)take(pl.vp * 8);
+    a.own.dir = (int2 *)take(pl.vo * 8);
+    if (share) {
+        a.tiles = (int4 *)take(pl.vp * 16);
+        a.order = (int32_t *)take(B * 4);
+        a.where = (int2 *)take(B * 8);
+    }
+    a.pre.V = (int)pl.vp, a.pre.chunks = (int)pl.cp, a.pre.rows = (int)(16 * pl.np), a.pre.blocks = (uint32_t)pl.blocks_p();
+    a.own.V = (int)pl.vo, a.own.chunks = (int)pl.co, a.own.rows = (int)(16 * pl.no), a.own.blocks = (uint32_t)pl.blocks_o();
+    a.B = (int)B, a.S = (int)S, a.H = (int)H, a.HK = (int)HK, a.G = (int)(H / HK), a.P = (int)P, a.ntile = (int)pl.ntile;
+    a.scale_log2e = scale * 1.4426950408889634f;
+    hipStream_t st = as_stream(stream);
+    if (share) launch(k_shared_plan, dim3(1), dim3(1024), (size_t)(8 * P), st, a);
+    const dim3 grid(a.pre.blocks + a.own.blocks);
+    launch(pl.np == 2 ? (pl.no == 2 ? k_shared_attn<2, 2> : k_shared_attn<2, 1>) : (pl.no == 2 ? k_shared_attn<1, 2> : k_shared_attn<1, 1>), grid,
+           dim3(64 * SA_WAVES), 0, st, a);
+    const int64_t nrows = B * HK * S * a.G, each = pl.gp / pl.vp + pl.go / pl.vo;
+    const int64_t gp = each > 16 ? 8 : each > 4 ? 2 : 1;
+    launch(gp == 8 ? k_shared_join<8> : gp == 2 ? k_shared_join<2> : k_shared_join<1>, dim3((unsigned)((nrows * gp + 7) / 8)), dim3(256), 0, st,
+           a, nrows);
+    return check_launch(who);
+}

@@ -81,6 +81,8 @@ SIGNATURES = {
     "qim_residual_norm": (_C, [_P, _I, _P, _I, _C, _P, _F, _P, _I, _F, _C, _P, _F, _P, _I, _P, _I, _C, _P, _I, _P, _I, _P, _I, _I, _I,
                                _P]),
     "qim_fourbit_matmul": (_C, [_P, _I, _C] + [_P] * 8 + [_I, _C, _I, _I, _I, _P]),
+    "qim_attention_shared": (_C, [_P, _I, _I] + [_P] * 12 + [_I, _P, _P, _I] + [_I] * 8 + [_F, _P]),
+    "qim_attention_shared_workspace_bytes": (_I, [_I] * 7 + [_C]),
     "qim_debug_e4m3_encode": (_C, [_P, _P, _I, _P]),
     "qim_debug_e4m3_encode_scaled": (_C, [_P, _C, _P, _I, _P]),
     "qim_debug_bf16_round": (_C, [_P, _P, _I, _P]),

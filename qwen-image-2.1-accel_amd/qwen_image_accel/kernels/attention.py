@@ -146,6 +146,60 @@ def attention_cached(q, cache, lengths, *, tree=None, scale=None, out=None):
     return out
 
 
+def attention_shared(q, prefix, cache, lengths, *, share=None, prefix_lengths=None, tree=None, scale=None, out=None):
+    """``attention_cached`` of requests that continue shared prefixes, each prefix read once for all of its
+    requests: softmax(q [Kp; K]^T * scale) [Vp; V], libqim's ``qim_attention_shared``.
+
+    q: (B, S, H, 128) bf16, S <= 64, packed heads, any token and batch stride.  ``prefix``: P prefixes of CP positions
+    (CP > 0), ``cache``: the B requests' own keys, both ``kv_cache.QuantizedCache`` with HK heads.  ``share``: int32
+    (B,) device tensor, the prefix of each request (any other number, -1 by convention: none), or None where P
+    is 1 and every request continues it.  ``prefix_lengths``: int32 (P,) device tensor, the keys of each prefix, or None
+    (all CP); ``lengths``: int32 (B,) device tensor, the own keys of each request, its S tokens among them
+    when they attend to themselves.  Lengths outside the caches count as the nearest inside.
+    ``tree``, ``scale`` and ``out`` as for ``attention_cached``; the tree's keys are the last S own ones.  A row that
+    sees no key is zeros.  Returns (B, S, H, 128) bf16."""
+    name = "attention_shared"
+
+    def refuse(why):
+        raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT, why)
+    p, cp, kv, d = kv_cache.check_cache(name, prefix)
+    b, c, own_kv, own_d = kv_cache.check_cache(name, cache)
+    device = cache.k.device
+    if (own_kv, own_d) != (kv, d) or prefix.k.device != device:
+        refuse(f"prefix and own cache have one number of heads and head dim, on {device}")
+    if not (p and cp and kv):
+        refuse("a prefix of no positions: use attention_cached")
+    shape = q.shape
+    strides = (kv_cache.token_strides(q) if len(shape) == 4 and q.dtype == torch.bfloat16 and q.device == device
+               and shape[0] == b and shape[3] == d else None)
+    if strides is None:
+        refuse(f"q is a bf16 ({b}, S, H, {d}) tensor with packed heads on {device}")
+    s, h = shape[1], shape[2]
+    size = kv_cache.per_sequence(name, "lengths", lengths, b, device)
+    psize = None if prefix_lengths is None else kv_cache.per_sequence(name, "prefix_lengths", prefix_lengths, p, device)
+    if share is None and p != 1:
+        refuse(f"share names the prefix of each request where there are {p}")
+    which = None if share is None else kv_cache.per_sequence(name, "share", share, b, device)
+    mask, mask_b = None, 0
+    if tree is not None:
+        if tree.dtype != torch.bool or tree.device != device or tree.shape not in ((s, s), (b, s, s)) or not tree.is_contiguous():
+            refuse(f"tree is a contiguous bool ({b}, {s}, {s}) or ({s}, {s}) tensor on {device}")
+        mask, mask_b = tree.data_ptr(), s * s if tree.dim() == 3 else 0
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous bf16 {tuple(shape)} tensor on {device}")
+    if not (b and s and h):
+        return out
+    own = [(t if c else u).data_ptr() for t, u in zip(cache, prefix)]   # an empty cache has no address; it is not read
+    nbytes = _native.bytes_on(device, "qim_attention_shared_workspace_bytes", b, s, cp, c, h, kv, p, int(share is not None))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    _native.call_on(device, "qim_attention_shared", q.data_ptr(), *strides, *(t.data_ptr() for t in prefix), psize, which,
+                    *own, size, mask, mask_b, out.data_ptr(), ws.data_ptr(), nbytes, b, s, p, cp, c, h, kv, d,
+                    float(scale if scale is not None else d ** -0.5))
+    return out
+
+
 def workspace(b, s, t, h, device, d=128):
     """A workspace for ``attention`` / ``attention_mxfp8`` of this shape (room
     for V^T tiles first, then the split items' partial results)."""
