@@ -29,8 +29,9 @@ class FourBitWeight(NamedTuple):
     """A weight (N, K) in the kernels' layout: rows in tiles of 16, k in steps of 128 (the last of each padded)."""
 
     codes: torch.Tensor             # (tiles, steps, 64, 16) uint8: 16 bytes of each lane
-    scales: torch.Tensor            # int4: (tiles, steps, 128 / group, 16) bf16; mxfp4: (tiles, steps, 16, 4) uint8
-    zeros: Optional[torch.Tensor]   # int4: (tiles, steps, 128 / group, 16) uint8, or None
+    scales: torch.Tensor            # int4: (tiles, steps, 4, 128 / group, 4) bf16, row 4 a + c of a tile at (a, :, c); mxfp4:
+                                    # (tiles, steps, 16, 4) uint8
+    zeros: Optional[torch.Tensor]   # int4: (tiles, steps, 16, 128 / group) uint8, or None
     rows: int                       # N
     width: int                      # K
     group: int                      # 32, 64 or 128
@@ -77,10 +78,12 @@ def pack_weight(codes, scales, *, zeros=None):
     c = c.reshape(tiles, TILE, steps, 4, 4, 4).permute(0, 2, 4, 1, 3, 5).reshape(tiles, steps, 64, 16).contiguous()
     per = STEP // group
 
-    def by_group(t):
-        t = _padded(t, tiles * TILE, steps * per).view(tiles, TILE, steps, per)
-        return t.permute((0, 2, 1, 3) if mx else (0, 2, 3, 1)).contiguous()
-    return FourBitWeight(c, by_group(scales), None if zeros is None else by_group(zeros), n, k, group)
+    def by_step(t):
+        return _padded(t, tiles * TILE, steps * per).view(tiles, TILE, steps, per).permute(0, 2, 1, 3).contiguous()
+    s = by_step(scales)
+    if not mx:
+        s = s.view(tiles, steps, 4, 4, per).transpose(3, 4).contiguous()
+    return FourBitWeight(c, s, None if zeros is None else by_step(zeros), n, k, group)
 
 
 def unpack_weight(weight):
@@ -95,11 +98,9 @@ def unpack_weight(weight):
         c = (c[:, 0::2] | c[:, 1::2] << 4).view(tiles * TILE, steps * STEP // 2)
 
     def by_row(t):
-        if t is None:
-            return None
-        t = t.permute((0, 2, 1, 3) if mx else (0, 3, 1, 2)).reshape(tiles * TILE, steps * per)
-        return t[:n, :k // weight.group].contiguous()
-    return c[:n, :k // 2].contiguous(), by_row(weight.scales), by_row(weight.zeros)
+        return t.permute(0, 2, 1, 3).reshape(tiles * TILE, steps * per)[:n, :k // weight.group].contiguous()
+    s = weight.scales if mx else weight.scales.transpose(3, 4).reshape(tiles, steps, TILE, per)
+    return c[:n, :k // 2].contiguous(), by_row(s), None if weight.zeros is None else by_row(weight.zeros)
 
 
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
@@ -166,10 +167,11 @@ def quantize_weight(w, kind="int4", group=64, *, symmetric=False):
 def _check_weight(name, w, device):
     """The addresses of a weight's tensors, checked against its sizes."""
     tiles, steps, per = (w.rows + TILE - 1) // TILE, (w.width + STEP - 1) // STEP, STEP // w.group if w.group in GROUPS else 0
-    shape = (tiles, steps, TILE, 4) if w.scales.dtype == torch.uint8 else (tiles, steps, per, TILE)
+    by_row = (tiles, steps, TILE, per)
+    shape = by_row if w.scales.dtype == torch.uint8 else (tiles, steps, 4, per, 4)
     if not (per and w.rows > 0 and w.width > 0 and w.codes.shape == (tiles, steps, 64, 16) and w.codes.dtype == torch.uint8
             and w.scales.shape == shape and w.scales.dtype in (torch.bfloat16, torch.uint8)
-            and (w.zeros is None or (w.zeros.shape == shape and w.zeros.dtype == torch.uint8 and w.scales.dtype == torch.bfloat16))
+            and (w.zeros is None or (w.zeros.shape == by_row and w.zeros.dtype == torch.uint8 and w.scales.dtype == torch.bfloat16))
             and all(t is None or (t.device == device and t.is_contiguous()) for t in w[:3])):
         raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT, f"expects a FourBitWeight of pack_weight or quantize_weight on {device}")
     return w.codes.data_ptr(), w.scales.data_ptr(), _native.ptr(w.zeros)
