@@ -270,15 +270,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_fourbit(FourBitArgs p, uint32
     }
 }
 
-// More rows: a workgroup of four waves and 64 x 64 values of output; of each step of 128 k, staged in LDS, wave j takes the
-// k 32 j .. 32 j + 31, so that every operand is read from LDS, and every code made an operand, once.  Three stages: one
-// multiplied, two on their way.
-constexpr int FT_NR = 4, FT_NT = 4, FT_X = FT_NR * 16 * 256;
-template <int G>
+// More rows: a workgroup of eight waves and 16 NR x 64 values of output; of each step of 128 k, staged in LDS, wave w takes
+// the k 32 (w % 4) .. + 31 for half of the columns, so that every code is made an operand once.  Two stages: one
+// multiplied, one on its way; a stage's 16-byte chunk c of row r of x lies at c ^ (r % 16), so that the 16 rows of an operand
+// lie in different banks.
+constexpr int FT_WAVES = 8, FT_NT = 4;  // 16-column tiles of W: two for each half of the waves
+template <int G, int NR>
 struct FtStage {
     static constexpr int SB = G ? 32 * G : 64, ZB = 16 * G;  // bytes of a tile's scales or exponents, and of its zero points
-    static constexpr int CODES = FT_X, SCALES = CODES + FT_NT * 1024, ZEROS = SCALES + FT_NT * SB, BYTES = ZEROS + FT_NT * ZB;
-    static constexpr int LOADS = FT_NR + 1 + 1 + (G ? 1 : 0);  // of a wave: its quarter of x, and one tile of W
+    static constexpr int CODES = NR * 16 * 256, SCALES = CODES + FT_NT * 1024, ZEROS = SCALES + FT_NT * SB, BYTES = ZEROS + FT_NT * ZB;
+    static constexpr int JOIN = 4 * 2 * NR * 64 * 16;        // four waves' partial sums of half of the output
+    static constexpr int TABLES = 2 * BYTES > JOIN ? 2 * BYTES : JOIN, LDS = TABLES + (G ? 256 : 0);
 };
 
 // LDS DMA that the compiler does not see as a write of LDS (it would wait for all of them before every read): lane i's 16
@@ -287,89 +289,103 @@ struct FtStage {
 __device__ __forceinline__ void ft_dma(const uint8_t *base, uint32_t off, uint32_t lds) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void ft_wait() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
-template <int G, bool SWIGLU>
-__global__ __launch_bounds__(256, 2) void k_fourbit_tile(FourBitArgs p, uint32_t ncol) {
-    using St = FtStage<G>;
-    constexpr int JOIN = FT_NT * FT_NR / 2 * 64 * 16 * 4;    // half the blocks of four waves
-    constexpr int LDS = 3 * St::BYTES > JOIN ? 3 * St::BYTES : JOIN;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[LDS + (G ? 256 : 0)];
-    uint4 *const tables = reinterpret_cast<uint4 *>(lds + LDS);
+template <int G, int NR, bool SWIGLU>
+__global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p, uint32_t ncol) {
+    using St = FtStage<G, NR>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    uint4 *const tables = reinterpret_cast<uint4 *>(lds + St::TABLES);
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = wave & 3, half = wave >> 2;
     const uint32_t rowblock = blockIdx.x / ncol, col = blockIdx.x - rowblock * ncol;
-    const int row0 = (int)rowblock * 16 * FT_NR;
+    const int row0 = (int)rowblock * 16 * NR;
     constexpr int OT = SWIGLU ? FT_NT / 2 : FT_NT;
     if constexpr (G > 0) {
         if (tid < 16) tables[tid] = make_uint4(fb_table(tid, 0), fb_table(tid, 4), fb_table(tid, 8), fb_table(tid, 12));
     }
-    // This wave's part of a stage: 16 rows of x, 4 a load (16-byte chunk c of row r at c ^ (r % 16), so that the 16
-    // rows of an operand lie in different banks), and the step of tile `wave`.  Rows and tiles past the last are the last, and of
-    // k past the end others come: nothing multiplies with them.
-    const int ntiles = (p.N + 15) / 16, mine = (int)col * OT + (SWIGLU ? wave >> 1 : wave);
-    const FourBitWeight &fw = p.w[SWIGLU ? wave & 1 : 0];
+    // This wave's part of a stage: 1 KiB pieces of x, 4 rows each, and of tile j of W the codes (the first four waves) or the
+    // scales and zero points.  Rows and tiles past the last are the last, and of k past the end others come: nothing
+    // multiplies with them.
+    const int ntiles = (p.N + 15) / 16, mine = (int)col * OT + (SWIGLU ? j >> 1 : j);
+    const FourBitWeight &fw = p.w[SWIGLU ? j & 1 : 0];
     const int64_t tile = mine < ntiles ? mine : ntiles - 1;
     const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x + row0 * p.ldx);
     const uint8_t *const wc = fw.codes + tile * p.KT * 1024, *const ws = fw.scales + tile * p.KT * St::SB;
     const uint8_t *const wz = G && fw.zeros ? fw.zeros + tile * p.KT * St::ZB : wc;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds;
-    uint32_t xrow[FT_NR], xk[FT_NR];
+    constexpr int PIECES = (4 * NR + FT_WAVES - 1) / FT_WAVES;
+    uint32_t xoff[PIECES];
+    auto piece = [&](int i) { return wave + FT_WAVES * i < 4 * NR ? wave + FT_WAVES * i : wave; };  // (a piece brought twice)
 #pragma unroll
-    for (int i = 0; i < FT_NR; ++i) {
-        const int r = wave * 16 + 4 * i + kg, last = p.M - 1 - row0;
-        xrow[i] = (uint32_t)(r < last ? r : last) * (uint32_t)(2 * p.ldx);
-        xk[i] = 16 * (lr ^ (r & 15));
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = 4 * piece(i) + kg, last = p.M - 1 - row0;
+        xoff[i] = (uint32_t)(r < last ? r : last) * (uint32_t)(2 * p.ldx) + 16 * (lr ^ (r & 15));
     }
     auto issue = [&](int t, int slot) {
         const uint32_t to = lds0 + slot * St::BYTES;
-        const uint32_t left = (uint32_t)(2 * p.K) - 256 * (uint32_t)t;  // bytes of a row from this step on
+        const uint8_t *const xt = x0 + (int64_t)t * 256;
+        const bool whole = 128 * t + 128 <= p.K;
 #pragma unroll
-        for (int i = 0; i < FT_NR; ++i) ft_dma(x0 + (int64_t)t * 256, xrow[i] + (xk[i] < left ? xk[i] : 0), to + (wave * 4 + i) * 1024);
-        ft_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + wave * 1024);
-        if (lane < St::SB / 16) ft_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + wave * St::SB);
-        if constexpr (G > 0) {
-            if (lane < St::ZB / 16) ft_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + wave * St::ZB);
+        for (int i = 0; i < PIECES; ++i) {
+            uint32_t off = xoff[i];
+            if (!whole) {
+                const int k = 8 * (lr ^ ((4 * piece(i) + kg) & 15));
+                off -= 128 * t + k < p.K ? 0 : 2 * k;
+            }
+            ft_dma(xt, off, to + piece(i) * 1024);
+        }
+        if (half == 0) {
+            ft_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + j * 1024);
+        } else {
+            if (lane < St::SB / 16) ft_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + j * St::SB);
+            if constexpr (G > 0) {
+                if (lane < St::ZB / 16) ft_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + j * St::ZB);
+            }
         }
     };
 
-    f32x4_t acc[FT_NT][FT_NR];
+    f32x4_t acc[2][NR];
 #pragma unroll
-    for (int i = 0; i < FT_NT; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < FT_NR; ++r) acc[i][r] = f32x4_t{};
-    const int g = G ? wave * G / 4 : 0;  // the group of this wave's k
+        for (int r = 0; r < NR; ++r) acc[i][r] = f32x4_t{};
+    const int g = G ? j * G / 4 : 0;  // the group of this wave's k
+    const uint32_t zmask = fw.zeros ? 0xffu : 0u, znone = fw.zeros ? 0u : 8u;
     issue(0, 0);
-    issue(p.KT > 1 ? 1 : 0, 1);
-    int slot = 0;
     for (int t = 0; t < p.KT; ++t) {
-        ft_wait<St::LOADS>();                                            // this wave's part of the stage is there
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // every wave's is, and the third slot has been read
-        const int third = slot == 0 ? 2 : slot - 1;
-        issue(t + 2 < p.KT ? t + 2 : p.KT - 1, third);                   // (past the end: not multiplied)
-        const uint8_t *const st = lds + slot * St::BYTES;
-        if (128 * t + 32 * wave < p.K) {
-            bf16x8_t x[FT_NR];
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is there, the other has been read
+        if (t + 1 < p.KT) issue(t + 1, (t + 1) & 1);
+        const uint8_t *const st = lds + (t & 1) * St::BYTES;
+        if (128 * t + 32 * j < p.K) {
+            uint32_t c[2];
+            uint2 s2[2];
+            uint4 tab[2];
+            uint32_t e[2];
 #pragma unroll
-            for (int r = 0; r < FT_NR; ++r)
-                x[r] = *reinterpret_cast<const bf16x8_t *>(st + (16 * r + lr) * 256 + (((4 * wave + kg) ^ lr) << 4));
-#pragma unroll
-            for (int i = 0; i < FT_NT; ++i) {
-                const uint32_t c = *reinterpret_cast<const uint32_t *>(st + St::CODES + i * 1024 + lane * 16 + 4 * wave);
+            for (int i = 0; i < 2; ++i) {
+                const int n = 2 * half + i;
+                c[i] = *reinterpret_cast<const uint32_t *>(st + St::CODES + n * 1024 + lane * 16 + 4 * j);
                 if constexpr (G == 0) {
-                    const bf16x8_t w = fb_e2m1(c, mx_scale_operand(st[St::SCALES + i * St::SB + lr * 4 + wave]));
-#pragma unroll
-                    for (int r = 0; r < FT_NR; ++r) acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[r], acc[i][r], 0, 0, 0);
+                    e[i] = st[St::SCALES + n * St::SB + lr * 4 + j];
                 } else {
-                    const uint2 s2 = *reinterpret_cast<const uint2 *>(st + St::SCALES + i * St::SB + (kg * G + g) * 8);
-                    const float s[4] = {bf_lo(s2.x), bf_hi(s2.x), bf_lo(s2.y), bf_hi(s2.y)};
-                    const int z = fw.zeros ? st[St::ZEROS + i * St::ZB + lr * G + g] : 8;
-                    const bf16x8_t w = fb_int4(c, tables[z]);
+                    s2[i] = *reinterpret_cast<const uint2 *>(st + St::SCALES + n * St::SB + (kg * G + g) * 8);
+                    tab[i] = tables[(st[St::ZEROS + n * St::ZB + lr * G + g] & zmask) | znone];
+                }
+            }
+            bf16x8_t x[NR];
 #pragma unroll
-                    for (int r = 0; r < FT_NR; ++r) {
+            for (int r = 0; r < NR; ++r) x[r] = *reinterpret_cast<const bf16x8_t *>(st + (16 * r + lr) * 256 + (((4 * j + kg) ^ lr) << 4));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if constexpr (G == 0) {
+                    const bf16x8_t w = fb_e2m1(c[i], mx_scale_operand((int)e[i]));
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[r], acc[i][r], 0, 0, 0);
+                } else {
+                    const float s[4] = {bf_lo(s2[i].x), bf_hi(s2[i].x), bf_lo(s2[i].y), bf_hi(s2[i].y)};
+                    const bf16x8_t w = fb_int4(c[i], tab[i]);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
                         const f32x4_t a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[r], f32x4_t{}, 0, 0, 0);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) acc[i][r][n] = __builtin_fmaf(s[n], a[n], acc[i][r][n]);
@@ -377,51 +393,68 @@ __global__ __launch_bounds__(256, 2) void k_fourbit_tile(FourBitArgs p, uint32_t
                 }
             }
         }
-        slot = slot == 2 ? 0 : slot + 1;
     }
-    ft_wait<0>();
-    f32x4_t(*const part)[FT_NT * FT_NR / 2][64] = reinterpret_cast<f32x4_t(*)[FT_NT * FT_NR / 2][64]>(lds);
+    // The join, the columns of one half of the waves after those of the other.
+    f32x4_t(*const part)[2 * NR][64] = reinterpret_cast<f32x4_t(*)[2 * NR][64]>(lds);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int h = 0; h < 2; ++h) {
         __syncthreads();
+        if (half == h) {
 #pragma unroll
-        for (int i = 0; i < FT_NT / 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < FT_NR; ++r) part[wave][i * FT_NR + r][lane] = acc[half * FT_NT / 2 + i][r];
+                for (int r = 0; r < NR; ++r) part[j][i * NR + r][lane] = acc[i][r];
+        }
         __syncthreads();
-        constexpr int HT = OT / 2;
+        constexpr int BLOCKS = SWIGLU ? NR : 2 * NR;
 #pragma unroll
-        for (int i = 0; i < HT * FT_NR / 4; ++i) {
-            const int blk = wave * (HT * FT_NR / 4) + i, ot = blk / FT_NR, r = blk - ot * FT_NR;
+        for (int i = 0; i < (BLOCKS + FT_WAVES - 1) / FT_WAVES; ++i) {
+            const int blk = wave + FT_WAVES * i, ot = SWIGLU ? 0 : blk / NR, r = blk - ot * NR;
+            if (blk >= BLOCKS) break;
             f32x4_t y = {}, u = {};
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                y += part[v][(SWIGLU ? 2 * ot : ot) * FT_NR + r][lane];
-                if (SWIGLU) u += part[v][(2 * ot + 1) * FT_NR + r][lane];
+                y += part[v][blk][lane];
+                if (SWIGLU) u += part[v][NR + blk][lane];
             }
-            const int64_t n0 = ((int64_t)col * OT + half * HT + ot) * 16 + 4 * kg;
+            const int64_t n0 = ((int64_t)col * OT + h * (OT / 2) + ot) * 16 + 4 * kg;
             const int row = row0 + 16 * r + lr;
             if (row < p.M && n0 < p.N) fb_store<SWIGLU>(p, row, n0, y, u);
         }
     }
 }
 
-#ifndef FB_BIG
-#define FB_BIG 0
-#endif
+template <int G, int NR, bool SWIGLU>
+static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
+    constexpr int OT = SWIGLU ? FT_NT / 2 : FT_NT, bytes = FtStage<G, NR>::LDS;
+    static std::atomic<bool> done[QIM_MAX_DEVICES];
+    if (bytes > 65536) {
+        const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit_tile<G, NR, SWIGLU>), bytes, done, "qim_fourbit_matmul");
+        if (rc != QIM_OK) return rc;
+    }
+    const uint32_t ncol = (uint32_t)(((a.N + 15) / 16 + OT - 1) / OT);
+    launch(k_fourbit_tile<G, NR, SWIGLU>, dim3(ncol * (unsigned)((a.M + 16 * NR - 1) / (16 * NR))), dim3(64 * FT_WAVES), bytes, st, a, ncol);
+    return QIM_OK;
+}
+
 template <int G, bool SWIGLU>
-static void launch_fourbit(const FourBitArgs &a, hipStream_t st) {
+static int launch_fourbit(const FourBitArgs &a, hipStream_t st) {
     const int64_t ntiles = (a.N + 15) / 16;
     auto go = [&](auto fn, int nt, int nr, int waves) {
         const int ot = SWIGLU ? nt / 2 : nt;
         const uint32_t ncol = (uint32_t)((ntiles + ot - 1) / ot);
         launch(fn, dim3(ncol * (unsigned)((a.M + 16 * nr - 1) / (16 * nr))), dim3(64 * waves), 0, st, a, ncol);
+        return QIM_OK;
     };
     constexpr int ONE = SWIGLU ? 2 : 1;
-    if (a.M <= 16) go(k_fourbit<G, ONE, 1, SWIGLU, 8>, ONE, 1, 8);
-    else if (a.M <= 32) go(k_fourbit<G, 2, 2, SWIGLU, 8>, 2, 2, 8);
-    else if (FB_BIG) go(k_fourbit<G, FB_BIG ? FB_BIG : 2, 4, SWIGLU, 4>, FB_BIG, 4, 4);
-    else go(k_fourbit_tile<G, SWIGLU>, FT_NT, FT_NR, 4);
+#ifdef FT_FORCE
+    return launch_fourbit_tile<G, FT_FORCE, SWIGLU>(a, st);
+#endif
+    if (a.M <= 16) return go(k_fourbit<G, ONE, 1, SWIGLU, 8>, ONE, 1, 8);
+    if (a.M <= 32) return go(k_fourbit<G, 2, 2, SWIGLU, 8>, 2, 2, 8);
+    if (a.M <= 64) return launch_fourbit_tile<G, 4, SWIGLU>(a, st);
+    if (a.M <= 160) return launch_fourbit_tile<G, 5, SWIGLU>(a, st);
+    return launch_fourbit_tile<G, 8, SWIGLU>(a, st);
 }
 
 }  // namespace qim
@@ -452,15 +485,16 @@ extern "C" int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const v
                   (const uint16_t *)bias, out, ldo, (int)M, (int)N, (int)K, (int)((K + 127) / 128), out_f32,
                   ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * size - 1)) == 0};
     hipStream_t st = as_stream(stream);
+    int rc;
     switch ((codes2 ? 4 : 0) + (group ? 128 / group == 4 ? 3 : 128 / group : 0)) {
-        case 0: launch_fourbit<0, false>(a, st); break;
-        case 1: launch_fourbit<1, false>(a, st); break;
-        case 2: launch_fourbit<2, false>(a, st); break;
-        case 3: launch_fourbit<4, false>(a, st); break;
-        case 4: launch_fourbit<0, true>(a, st); break;
-        case 5: launch_fourbit<1, true>(a, st); break;
-        case 6: launch_fourbit<2, true>(a, st); break;
-        default: launch_fourbit<4, true>(a, st); break;
+        case 0: rc = launch_fourbit<0, false>(a, st); break;
+        case 1: rc = launch_fourbit<1, false>(a, st); break;
+        case 2: rc = launch_fourbit<2, false>(a, st); break;
+        case 3: rc = launch_fourbit<4, false>(a, st); break;
+        case 4: rc = launch_fourbit<0, true>(a, st); break;
+        case 5: rc = launch_fourbit<1, true>(a, st); break;
+        case 6: rc = launch_fourbit<2, true>(a, st); break;
+        default: rc = launch_fourbit<4, true>(a, st); break;
     }
-    return check_launch(who);
+    return rc != QIM_OK ? rc : check_launch(who);
 }
