@@ -91,183 +91,174 @@ __device__ __forceinline__ void fb_store(const FourBitArgs &p, int64_t row, int6
     }
 }
 
-// What the waves of a workgroup read in a step beside x; the next step's is on its way while one is multiplied.
-template <int G, int NT>
-struct FbStep {
-    uint4 w[NT], s[NT][G == 4 ? 2 : 1];  // s: the scales of rows 4 kg .. 4 kg + 3 of the tile, by group (G 1: half of it)
-    uint32_t z[NT];                      // mxfp4: the exponents, by j; int4: the zero points, by group
-};
 __device__ __forceinline__ uint32_t fb_word(const uint4 &u, int j) { return j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w; }
 
-// One workgroup: NT tiles of 16 columns of W (SWIGLU: NT / 2 of each weight) and 16 NR rows.  G: groups of int4 in a
-// step, 0 for mxfp4.
-template <int G, int NT, int NR, bool SWIGLU, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_fourbit(FourBitArgs p, uint32_t ncol) {
-    __shared__ f32x4_t part[WAVES][NT * NR][64];
-    uint4 *const tables = reinterpret_cast<uint4 *>(part);  // until the waves join
+// LDS DMA that the compiler does not see as a write of LDS (it would wait for all of them before every read): lane i's 16
+// bytes land at lds + 16 i.  The stages' own waits and barriers order them; the s_nop covers the wait state between the
+// write of M0 and its use.
+__device__ __forceinline__ void fb_dma(const uint8_t *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void fb_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Up to 4 RX rows: NT tiles of 16 columns of W (SWIGLU: NT / 2 of each weight) a workgroup, whose waves take the steps of k
+// in turn.  G: groups of int4 in a step, 0 for mxfp4.  Everything goes through a ring of S stages in LDS of the wave's own:
+// S steps are on their way without registers held for them, and x, whose rows an operand takes from 16 places at
+// once, arrives in whole 256-byte rows (read by the operands' lanes themselves, 16 bytes here and there, it cost four
+// times as many requests as bytes and more time than W).  No barrier stands in the loop.
+template <int G, int NT, int RX, int WAVES, int S>
+struct FbRing {
+    static constexpr int SB = G ? 32 * G : 64, ZB = 16 * G;  // bytes of a tile's scales or exponents, and of its zero points
+    static constexpr int CODES = RX * 1024, SCALES = CODES + NT * 1024, ZEROS = SCALES + NT * SB, BYTES = (ZEROS + NT * ZB + 15) / 16 * 16;
+    static constexpr int LOADS = RX + NT * (G ? 3 : 2);
+    static constexpr int JOIN = WAVES * NT * 1024, TABLES = WAVES * S * BYTES > JOIN ? WAVES * S * BYTES : JOIN, LDS = TABLES + (G ? 256 : 0);
+};
+template <int G, int NT, int RX, int WAVES, int S, bool SWIGLU>
+__global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
+    using Ring = FbRing<G, NT, RX, WAVES, S>;
+    constexpr int OT = SWIGLU ? NT / 2 : NT;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    uint4 *const tables = reinterpret_cast<uint4 *>(lds + Ring::TABLES);
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t rowblock = blockIdx.x / ncol, col = blockIdx.x - rowblock * ncol;
-    const int row0 = (int)rowblock * 16 * NR;
-    constexpr int OT = SWIGLU ? NT / 2 : NT;  // tiles of output columns
+    const int ntiles = (p.N + 15) / 16;
+    const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x);
+    const uint8_t *const ring = lds + wave * (S * Ring::BYTES);
+    const uint32_t ring0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)ring;
+    // Rows and tiles past the last are the last (computed, not stored); a 16-byte chunk c of row r of x lies at c ^ r, so that
+    // the rows of an operand lie in different banks.
+    uint32_t xoff[RX];
+#pragma unroll
+    for (int i = 0; i < RX; ++i) {
+        const int r = 4 * i + kg;
+        xoff[i] = (uint32_t)(r < p.M ? r : p.M - 1) * (uint32_t)(2 * p.ldx) + 16 * (lr ^ r);
+    }
+    auto issue = [&](int t, int slot) {
+        const uint32_t to = ring0 + slot * Ring::BYTES;
+        const uint8_t *const xt = x0 + (int64_t)t * 256;
+        const bool whole = 128 * t + 128 <= p.K;
+#pragma unroll
+        for (int i = 0; i < RX; ++i) {
+            uint32_t off = xoff[i];
+            if (!whole) {  // k past the end: others come, and nothing multiplies with them
+                const int k = 8 * (lr ^ (4 * i + kg));
+                off -= 128 * t + k < p.K ? 0 : 2 * k;
+            }
+            fb_dma(xt, off, to + i * 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const FourBitWeight &w = p.w[SWIGLU ? i & 1 : 0];
+            const int tl = (int)blockIdx.x * OT + (SWIGLU ? i >> 1 : i);
+            const int64_t at = (int64_t)(tl < ntiles ? tl : ntiles - 1) * p.KT + t;
+            fb_dma(w.codes + at * 1024, lane * 16, to + Ring::CODES + i * 1024);
+            if (lane < Ring::SB / 16) fb_dma(w.scales + at * Ring::SB, lane * 16, to + Ring::SCALES + i * Ring::SB);
+            if constexpr (G > 0) {
+                const uint8_t *z = w.zeros ? w.zeros + at * Ring::ZB : w.codes;
+                if (lane < Ring::ZB / 16) fb_dma(z, lane * 16, to + Ring::ZEROS + i * Ring::ZB);
+            }
+        }
+    };
+    const int steps = wave < p.KT ? (p.KT - wave + WAVES - 1) / WAVES : 0;  // of this wave: wave, wave + WAVES, ...
+    auto step = [&](int i) { return wave + WAVES * (i < steps ? i : 0); };   // (past the last: the first again, not multiplied)
+    if (steps) {
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) issue(step(i), i);
+    }
     if constexpr (G > 0) {
         if (tid < 16) tables[tid] = make_uint4(fb_table(tid, 0), fb_table(tid, 4), fb_table(tid, 8), fb_table(tid, 12));
-        __syncthreads();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (not __syncthreads: that waits for the loads too)
     }
-
-    // Wave-uniform bases and 32-bit offsets of the lanes.  Tiles past the last are the last, rows past the last row too:
-    // computed, not stored.
-    const int ntiles = (p.N + 15) / 16;
-    auto tile_of = [&](int i) {
-        const int tl = (int)col * OT + (SWIGLU ? i >> 1 : i);
-        return tl < ntiles ? tl : ntiles - 1;
-    };
-    auto weight_of = [&](int i) -> const FourBitWeight & { return p.w[SWIGLU ? i & 1 : 0]; };
-    const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x + row0 * p.ldx);
-    uint32_t xoff[NR];
+    const uint32_t zmask = p.w[0].zeros ? 0xffffffffu : 0u, znone = p.w[0].zeros ? 0u : 0x08080808u;
+    f32x4_t acc[NT], a[NT];
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        const int row = 16 * r + lr, last = p.M - 1 - row0;
-        xoff[r] = (uint32_t)(row < last ? row : last) * (uint32_t)(2 * p.ldx) + 16 * kg;
-    }
-    auto load_x = [&](uint4 (&v)[NR], int t, int j) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) v[r] = *reinterpret_cast<const uint4 *>(x0 + (int64_t)t * 256 + (xoff[r] + 64 * j));
-    };
-    auto load = [&](FbStep<G, NT> &v, int t) {
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4_t{};
+    constexpr int PER = G ? 4 / G : 1;  // matrix steps of a group
+    const int xrow = lr & (4 * RX - 1);
+    int slot = 0;
+    for (int n = 0; n < steps; ++n) {
+        // The slot that is filled next was read in the step before: those reads have returned (what they fed has been multiplied).
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue(step(n + S - 1), slot == 0 ? S - 1 : slot - 1);
+        fb_wait<(S - 1) * Ring::LOADS>();
+        const uint8_t *const st = ring + slot * Ring::BYTES;
+        slot = slot == S - 1 ? 0 : slot + 1;
+        uint4 c[NT], s[NT][G == 4 ? 2 : 1], x[4];
+        uint32_t z[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-            const FourBitWeight &w = weight_of(i);
-            const int64_t at = (int64_t)tile_of(i) * p.KT + t;
-            v.w[i] = *reinterpret_cast<const uint4 *>(w.codes + at * 1024 + (uint32_t)lane * 16);
             if constexpr (G == 0) {
-                v.z[i] = *reinterpret_cast<const uint32_t *>(w.scales + at * 64 + (uint32_t)lr * 4);
+                z[i] = *reinterpret_cast<const uint32_t *>(st + Ring::SCALES + i * Ring::SB + lr * 4);
             } else {
-                const uint8_t *sc = w.scales + at * (32 * G) + (uint32_t)kg * (8 * G);
+                const uint8_t *zp = st + Ring::ZEROS + i * Ring::ZB + lr * G, *sp = st + Ring::SCALES + i * Ring::SB + kg * (8 * G);
+                z[i] = G == 4 ? *reinterpret_cast<const uint32_t *>(zp) : G == 2 ? *reinterpret_cast<const uint16_t *>(zp) : *zp;
+                z[i] = (z[i] & zmask) | znone;
                 if constexpr (G == 1) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(sc);
-                    v.s[i][0] = make_uint4(u.x, u.y, 0, 0);
+                    const uint2 u = *reinterpret_cast<const uint2 *>(sp);
+                    s[i][0] = make_uint4(u.x, u.y, 0, 0);
                 } else {
 #pragma unroll
-                    for (int g = 0; g < G / 2; ++g) v.s[i][g] = reinterpret_cast<const uint4 *>(sc)[g];
-                }
-                v.z[i] = 0x08080808u;
-                if (w.zeros) {
-                    const uint8_t *z = w.zeros + at * (16 * G) + (uint32_t)lr * G;
-                    v.z[i] = G == 4 ? *reinterpret_cast<const uint32_t *>(z) : G == 2 ? *reinterpret_cast<const uint16_t *>(z) : *z;
+                    for (int g = 0; g < G / 2; ++g) s[i][g] = reinterpret_cast<const uint4 *>(sp)[g];
                 }
             }
+            c[i] = *reinterpret_cast<const uint4 *>(st + Ring::CODES + i * 1024 + lane * 16);
         }
-    };
-
-    f32x4_t acc[NT][NR];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+        for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4 *>(st + xrow * 256 + (((4 * j + kg) ^ xrow) << 4));
+        const int left = p.K - 128 * step(n);  // of k: whole groups, a step but for the last
 #pragma unroll
-        for (int r = 0; r < NR; ++r) acc[i][r] = f32x4_t{};
-    constexpr int PER = G ? 4 / G : 1;  // matrix steps of a group
-    f32x4_t a[NT][NR];
-    auto multiply = [&](const FbStep<G, NT> &v, const uint4 (&x)[NR], int j) {
+        for (int j = 0; j < 4; ++j) {
+            if (32 * j >= left) break;
+            const bf16x8_t xv = __builtin_bit_cast(bf16x8_t, x[j]);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            bf16x8_t w;
-            if constexpr (G == 0) {
-                w = fb_e2m1(fb_word(v.w[i], j), mx_scale_operand((int)((v.z[i] >> (8 * j)) & 0xffu)));
-            } else {
-                w = fb_int4(fb_word(v.w[i], j), tables[(v.z[i] >> (8 * (j / PER))) & 0xffu]);
-            }
-#pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                f32x4_t &to = G == 0 ? acc[i][r] : a[i][r];
-                to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(bf16x8_t, x[r]), G > 0 && j % PER == 0 ? f32x4_t{} : to, 0, 0, 0);
-            }
-            if constexpr (G > 0) {
-                if (j % PER == PER - 1) {
+            for (int i = 0; i < NT; ++i) {
+                if constexpr (G == 0) {
+                    const bf16x8_t w = fb_e2m1(fb_word(c[i], j), mx_scale_operand((int)((z[i] >> (8 * j)) & 0xffu)));
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xv, acc[i], 0, 0, 0);
+                } else {
                     const int g = j / PER;
-                    const uint32_t s0 = fb_word(v.s[i][g / 2], 2 * (g & 1)), s1 = fb_word(v.s[i][g / 2], 2 * (g & 1) + 1);
-                    const float s[4] = {bf_lo(s0), bf_hi(s0), bf_lo(s1), bf_hi(s1)};
+                    const bf16x8_t w = fb_int4(fb_word(c[i], j), tables[(z[i] >> (8 * g)) & 0xffu]);
+                    a[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xv, j % PER ? a[i] : f32x4_t{}, 0, 0, 0);
+                    if (j % PER == PER - 1) {
+                        const uint32_t s0 = fb_word(s[i][g / 2], 2 * (g & 1)), s1 = fb_word(s[i][g / 2], 2 * (g & 1) + 1);
+                        const float f[4] = {bf_lo(s0), bf_hi(s0), bf_lo(s1), bf_hi(s1)};
 #pragma unroll
-                    for (int r = 0; r < NR; ++r)
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) acc[i][r][n] = __builtin_fmaf(s[n], a[i][r][n], acc[i][r][n]);
+                        for (int v = 0; v < 4; ++v) acc[i][v] = __builtin_fmaf(f[v], a[i][v], acc[i][v]);
+                    }
                 }
             }
         }
-    };
-    // Whole steps.  x is loaded a step ahead where a step is little work, else a quarter of a step ahead.
-    const int full = p.K / 128;
-    constexpr bool AHEAD = NT * NR <= 4;
-    int t = wave;
-    if (t < full) {
-        FbStep<G, NT> cur, next;
-        load(cur, t);
-        if constexpr (AHEAD) {
-            uint4 x[4][NR], xn[4][NR];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) load_x(x[j], t, j);
-            for (;;) {
-                const int ahead = t + WAVES < full ? t + WAVES : t;  // (the last step again: not multiplied)
-                load(next, ahead);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) load_x(xn[j], ahead, j);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) multiply(cur, x[j], j);
-                t += WAVES;
-                if (t >= full) break;
-                cur = next;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) x[j][r] = xn[j][r];
-            }
-        } else {
-            uint4 x[2][NR];
-            load_x(x[0], t, 0);
-            for (;;) {
-                const int ahead = t + WAVES < full ? t + WAVES : t;
-                load(next, ahead);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    load_x(x[(j + 1) & 1], j < 3 ? t : ahead, (j + 1) & 3);
-                    multiply(cur, x[j & 1], j);
-                }
-                t += WAVES;
-                if (t >= full) break;
-                cur = next;
-            }
-        }
     }
-    // The rest of k (a multiple of 32, whole groups), with the wave whose turn it is.
-    if (t == full && full < p.KT) {
-        FbStep<G, NT> v;
-        load(v, t);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-            if (128 * t + 32 * j < p.K) {
-                uint4 x[NR];
-                load_x(x, t, j);
-                multiply(v, x, j);
-            }
-        }
-    }
-    if constexpr (G > 0) __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) part[wave][i * NR + r][lane] = acc[i][r];
+    fb_wait<0>();
     __syncthreads();
-    for (int i = tid; i < OT * NR * 64; i += 64 * WAVES) {  // 16 x 16 blocks of output
-        const int blk = i >> 6, l = i & 63, ot = blk / NR, r = blk - ot * NR;
-        f32x4_t y = {}, u = {};
+    f32x4_t(*const part)[NT][64] = reinterpret_cast<f32x4_t(*)[NT][64]>(lds);
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
-            y += part[v][SWIGLU ? 2 * ot * NR + r : blk][l];
-            if (SWIGLU) u += part[v][(2 * ot + 1) * NR + r][l];
-        }
-        const int64_t n0 = ((int64_t)col * OT + ot) * 16 + 4 * (l >> 4);
-        const int row = row0 + 16 * r + (l & 15);
-        if (row < p.M && n0 < p.N) fb_store<SWIGLU>(p, row, n0, y, u);
+    for (int i = 0; i < NT; ++i) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= OT) return;
+    f32x4_t y = {}, u = {};
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
+        y += part[v][SWIGLU ? 2 * wave : wave][lane];
+        if (SWIGLU) u += part[v][2 * wave + 1][lane];
     }
+    const int64_t n0 = ((int64_t)blockIdx.x * OT + wave) * 16 + 4 * kg;
+    if (lr < p.M && n0 < p.N) fb_store<SWIGLU>(p, lr, n0, y, u);
+}
+
+template <int G, int NT, int RX, int WAVES, int S, bool SWIGLU>
+static int launch_fourbit_ring(const FourBitArgs &a, hipStream_t st) {
+    constexpr int OT = SWIGLU ? NT / 2 : NT, bytes = FbRing<G, NT, RX, WAVES, S>::LDS;
+    static std::atomic<bool> done[QIM_MAX_DEVICES];
+    if (bytes > 65536) {
+        const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit<G, NT, RX, WAVES, S, SWIGLU>), bytes, done, "qim_fourbit_matmul");
+        if (rc != QIM_OK) return rc;
+    }
+    launch(k_fourbit<G, NT, RX, WAVES, S, SWIGLU>, dim3((unsigned)(((a.N + 15) / 16 + OT - 1) / OT)), dim3(64 * WAVES), bytes, st, a);
+    return QIM_OK;
 }
 
 // More rows: a workgroup of eight waves and 16 NR x 64 values of output; of each step of 128 k, staged in LDS, wave w takes
@@ -282,13 +273,6 @@ struct FtStage {
     static constexpr int JOIN = 4 * 2 * NR * 64 * 16;        // four waves' partial sums of half of the output
     static constexpr int TABLES = 2 * BYTES > JOIN ? 2 * BYTES : JOIN, LDS = TABLES + (G ? 256 : 0);
 };
-
-// LDS DMA that the compiler does not see as a write of LDS (it would wait for all of them before every read): lane i's 16
-// bytes land at lds + 16 i.  The stages' own waits and barriers order them; the s_nop covers the wait state between the
-// write of M0 and its use.
-__device__ __forceinline__ void ft_dma(const uint8_t *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
 
 template <int G, int NR, bool SWIGLU>
 __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p, uint32_t ncol) {
@@ -332,14 +316,14 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
                 const int k = 8 * (lr ^ ((4 * piece(i) + kg) & 15));
                 off -= 128 * t + k < p.K ? 0 : 2 * k;
             }
-            ft_dma(xt, off, to + piece(i) * 1024);
+            fb_dma(xt, off, to + piece(i) * 1024);
         }
         if (half == 0) {
-            ft_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + j * 1024);
+            fb_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + j * 1024);
         } else {
-            if (lane < St::SB / 16) ft_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + j * St::SB);
+            if (lane < St::SB / 16) fb_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + j * St::SB);
             if constexpr (G > 0) {
-                if (lane < St::ZB / 16) ft_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + j * St::ZB);
+                if (lane < St::ZB / 16) fb_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + j * St::ZB);
             }
         }
     };
@@ -439,19 +423,15 @@ static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
 
 template <int G, bool SWIGLU>
 static int launch_fourbit(const FourBitArgs &a, hipStream_t st) {
-    const int64_t ntiles = (a.N + 15) / 16;
-    auto go = [&](auto fn, int nt, int nr, int waves) {
-        const int ot = SWIGLU ? nt / 2 : nt;
-        const uint32_t ncol = (uint32_t)((ntiles + ot - 1) / ot);
-        launch(fn, dim3(ncol * (unsigned)((a.M + 16 * nr - 1) / (16 * nr))), dim3(64 * waves), 0, st, a, ncol);
-        return QIM_OK;
-    };
     constexpr int ONE = SWIGLU ? 2 : 1;
-#ifdef FT_FORCE
-    return launch_fourbit_tile<G, FT_FORCE, SWIGLU>(a, st);
-#endif
-    if (a.M <= 16) return go(k_fourbit<G, ONE, 1, SWIGLU, 8>, ONE, 1, 8);
-    if (a.M <= 32) return go(k_fourbit<G, 2, 2, SWIGLU, 8>, 2, 2, 8);
+    if (a.M <= 4) return launch_fourbit_ring<G, ONE, 1, 8, 3, SWIGLU>(a, st);
+    if (a.M <= 16) {
+        // Many columns: two tiles share the reads of x, and two workgroups of four waves a CU take more of them at a time
+        // (16 rows, mxfp4: 4096 -> 12288 9.2 us against 11.6; 12288 -> 4096, 256 tiles, 14.6 against 9.0).
+        if (a.N >= 16 * 512) return launch_fourbit_ring<G, 2, 4, 4, 3, SWIGLU>(a, st);
+        return launch_fourbit_ring<G, ONE, 4, 8, 2, SWIGLU>(a, st);
+    }
+    if (a.M <= 32) return launch_fourbit_tile<G, 2, SWIGLU>(a, st);
     if (a.M <= 64) return launch_fourbit_tile<G, 4, SWIGLU>(a, st);
     if (a.M <= 160) return launch_fourbit_tile<G, 5, SWIGLU>(a, st);
     return launch_fourbit_tile<G, 8, SWIGLU>(a, st);
