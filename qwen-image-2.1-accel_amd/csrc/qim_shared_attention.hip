@@ -24,6 +24,7 @@ struct SaSpace {
     float2 *part_ml;  // (maximum, sum)
     int2 *dir;        // per sequence: its first piece and their number
     int V, chunks, rows;
+    int keys;         // of a block: pieces are whole blocks
     uint32_t blocks;  // workgroups
 };
 struct SaArgs {
@@ -58,8 +59,8 @@ __device__ __forceinline__ SaTile sa_tile(const SaArgs &p, int i) {
 // The requests of each prefix, in their order, and the prefix's tiles of rows.  One workgroup; a wave per prefix counts and
 // lists with ballots, 64 requests at a time.
 __global__ __launch_bounds__(1024) void k_shared_plan(SaArgs p) {
-    extern __shared__ int32_t lds[];  // count, then first request, and first tile, of each prefix
-    int32_t *const first = lds, *const tile = lds + p.P;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    int32_t *const first = reinterpret_cast<int32_t *>(lds), *const tile = first + p.P;  // of each prefix: count, then first request; first tile
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int i = wave; i < p.P; i += 16) {
         int n = 0;
@@ -117,7 +118,7 @@ __device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
 template <bool PRE>
 __device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int64_t &blk0, int64_t &per) {
     const int lane = threadIdx.x & 63;
-    auto blocks = [&](int i) { return i < sp.V ? (int)((sa_length<PRE>(p, i) + CA_KB - 1) / CA_KB) : 0; };
+    auto blocks = [&](int i) { return i < sp.V ? (int)((sa_length<PRE>(p, i) + sp.keys - 1) / sp.keys) : 0; };
     int64_t total = 0;
     for (int i = 0; i < sp.V; i += 64) total += __builtin_amdgcn_readlane(ca_scan(blocks(i + lane), lane), 63);
     const int64_t each = (total + sp.chunks - 1) / sp.chunks;
@@ -189,6 +190,225 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_attn(SaArgs p) {
     uint8_t *const vt = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * CA_VTILE;
     if (blockIdx.x < p.pre.blocks) sa_wave<true, NP>(p, p.pre, blockIdx.x, vt);
     else sa_wave<false, NO>(p, p.own, blockIdx.x - p.pre.blocks, vt);
+}
+
+// Many rows to a prefix: a workgroup of four waves takes 32 RG rows and blocks of 64 keys; a wave 32 rows and, of each
+// block, all keys (RG 4) or one half of them (RG 2).  The block's codes become bf16 once, in LDS (two buffers; K with
+// 16-byte chunk c of key r at c ^ (r % 16), V with 32-byte unit n of key r at n ^ (r % 8), for the transposing reads),
+// where the wave above converts for 16 or 32 rows of its own.  Two blocks are on their way in registers.  Waves of the same
+// rows join in LDS.
+constexpr int ST_KEYS = 64, ST_BUF = ST_KEYS * 512;                       // bytes of K and V of a block
+constexpr int ST_LDS = 2 * ST_BUF;                                        // (also the join's: 2 waves x 16.25 KiB)
+template <int RG, int NO>
+__global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
+    constexpr int KQ = 4 / RG;                                            // waves of the same rows
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[ST_LDS];
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wave % RG, kq = wave / RG;
+    if (blockIdx.x >= p.pre.blocks) {
+        sa_wave<false, NO>(p, p.own, blockIdx.x - p.pre.blocks, lds + wave * CA_VTILE);
+        return;
+    }
+    const uint32_t q8 = blockIdx.x >> 3, grp = q8 / (uint32_t)p.HK, piece = grp * 8 + (blockIdx.x & 7);
+    const int h = (int)(q8 - grp * (uint32_t)p.HK);
+    int v = 0;
+    int64_t blk0 = 0, per = 1;
+    if (!sa_piece<true>(p, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per)) return;
+    const SaTile tile = sa_tile(p, v);
+    const int64_t len = sa_prefix_length(p, tile.prefix), W = (int64_t)p.HK * CA_D, base = (int64_t)tile.prefix * p.CP * W + h * CA_D;
+    const int64_t nblk = (len + ST_KEYS - 1) / ST_KEYS, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
+    const float c = p.scale_log2e, ninf = -__builtin_inff();
+
+    // A thread's share of a block: 16 codes of K and of V of keys tid / 8 and tid / 8 + 32.
+    const int ck = tid >> 3, cc = tid & 7;
+    struct Raw {
+        uint4 k[2], v[2];
+        uint32_t ke[2], ve[2];
+    };
+    auto load = [&](Raw &w, int64_t blk) {
+        blk = blk < blk1 ? blk : blk1 - 1;  // (past the end: not converted)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int64_t key = blk * ST_KEYS + 32 * i + ck;
+            key = key < p.CP ? key : p.CP - 1;
+            const int64_t at = base + key * W + 16 * cc;
+            w.k[i] = *reinterpret_cast<const uint4 *>(p.pk + at);
+            w.v[i] = *reinterpret_cast<const uint4 *>(p.pv + at);
+            w.ke[i] = p.pks[at >> 5];
+            w.ve[i] = p.pvs[at >> 5];
+        }
+    };
+    Raw raw[2];
+    load(raw[0], blk0);
+    load(raw[1], blk0 + 1);
+
+    bf16x8_t qf[2][4];  // d [64 j + 16 kg + 8 half, + 8) in step 2 j + half
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        int r = tile.row0 + 32 * rg + 16 * t + lr;
+        r = r < tile.rows ? r : tile.rows - 1;
+        const int sg = p.S * p.G, i = r / sg, in = r - i * sg, sq = in / p.G;
+        const int b = p.share ? p.order[tile.first + i] : i;
+        const uint16_t *qr = p.q + b * p.ldqb + sq * p.ldq + (h * p.G + (in - sq * p.G)) * CA_D + 16 * kg;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[t][j] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * (j >> 1) + 8 * (j & 1));
+    }
+    f32x4_t o[2][8];
+    float m[2], l[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        m[t] = ninf;
+        l[t] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) o[t][dt] = f32x4_t{};
+    }
+    const bool idle = tile.row0 + 32 * rg >= tile.rows;  // no rows of this wave's: it only converts
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    auto convert = [&](const Raw &w, int64_t blk, int buf) {
+        uint8_t *const kb = lds + buf * ST_BUF, *const vb = kb + ST_KEYS * 256;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int key = 32 * i + ck;
+            const float ks = mx_scale_operand((int)w.ke[i]);
+            *reinterpret_cast<bf16x8_t *>(kb + key * 256 + (((2 * cc) ^ (key & 15)) << 4)) = ca_operand(w.k[i].x, w.k[i].y, ks);
+            *reinterpret_cast<bf16x8_t *>(kb + key * 256 + (((2 * cc + 1) ^ (key & 15)) << 4)) = ca_operand(w.k[i].z, w.k[i].w, ks);
+            uint4 x = w.v[i];
+            uint32_t e = w.ve[i];
+            if (blk * ST_KEYS + key >= len) {  // V past the last key is zeros, whatever the cache holds there
+                x = make_uint4(0, 0, 0, 0);
+                e = 0;
+            }
+            const float vs = mx_scale_operand((int)e);
+            uint8_t *at = vb + key * 256 + ((cc ^ (key & 7)) << 5);
+            *reinterpret_cast<bf16x8_t *>(at) = ca_operand(x.x, x.y, vs);
+            *reinterpret_cast<bf16x8_t *>(at + 16) = ca_operand(x.z, x.w, vs);
+        }
+    };
+    // 32 keys of the block in a buffer, from its key `first` on, for the wave's 32 rows; `left` keys are there.
+    auto attend = [&](int buf, int first, int64_t left) {
+        const uint8_t *const kb = lds + buf * ST_BUF;
+        const int vkey = first + 4 * kg + (lr >> 2);
+        f32x4_t s[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int key = first + 16 * u + lr;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int ch = 8 * (j >> 1) + 2 * kg + (j & 1);
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(kb + key * 256 + ((ch ^ lr) << 4));
+#pragma unroll
+                for (int t = 0; t < 2; ++t) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], j == 0 ? f32x4_t{} : s[t][u], 0, 0, 0);
+            }
+        }
+        u32x4_t pw[2], pl[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (left < 32) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[t][u][i] = 16 * u + 4 * kg + i < (int)left ? s[t][u][i] : ninf;
+            }
+            float mx = ca_max(ca_max(ca_max(s[t][0][0], s[t][0][1]), ca_max(s[t][0][2], s[t][0][3])),
+                              ca_max(ca_max(s[t][1][0], s[t][1][1]), ca_max(s[t][1][2], s[t][1][3])));
+            {
+                const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = ca_swap_max(ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1]))) * c;
+            }
+            const float mn = ca_max(m[t], mx), ref = mn == ninf ? 0.f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m[t] - ref);
+            m[t] = mn;
+            float e[8], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], c, -ref));
+                sum += e[i];
+            }
+            l[t] = l[t] * alpha + sum;
+            // p as two bf16 terms, as in ca_wave.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pw[t][i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+                pl[t][i] = pack_bf16x2(e[2 * i] - bf_lo(pw[t][i]), e[2 * i + 1] - bf_hi(pw[t][i]));
+            }
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
+            }
+        }
+        const uint32_t vrow = lds0 + (uint32_t)(buf * ST_BUF + ST_KEYS * 256 + vkey * 256 + (lr & 3) * 8);
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            typedef __attribute__((address_space(3))) i16x4_t *ptr_t;
+            const uint32_t at = vrow + ((dt ^ (vkey & 7)) << 5);
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)at));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)(at + 16 * CA_D * 2)));
+            const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8_t, pl[t]), o[t][dt], 0, 0, 0);
+                o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8_t, pw[t]), o[t][dt], 0, 0, 0);
+            }
+        }
+    };
+    auto block = [&](Raw &w, int64_t blk, int buf) {
+        convert(w, blk, buf);
+        __syncthreads();
+        load(w, blk + 2);
+        if (idle) return;
+#pragma unroll
+        for (int i = 0; i < 2 / KQ; ++i) {
+            const int first = 32 * (kq + i);
+            const int64_t left = len - (blk * ST_KEYS + first);
+            if (left > 0) attend(buf, first, left);
+        }
+    };
+    for (int64_t blk = blk0; blk < blk1; blk += 2) {
+        block(raw[0], blk, 0);
+        if (blk + 1 < blk1) block(raw[1], blk + 1, 1);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+    }
+    // The second wave of the same rows joins with the first.
+    if constexpr (KQ == 2) {
+        f32x4_t *const so = reinterpret_cast<f32x4_t *>(lds) + rg * (16 * 64);
+        float2 *const sml = reinterpret_cast<float2 *>(lds + RG * (32 * CA_D * 4)) + rg * 32;
+        __syncthreads();
+        if (kq) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) so[(t * 8 + dt) * 64 + lane] = o[t][dt];
+                if (kg == 0) sml[t * 16 + lr] = make_float2(m[t], l[t]);
+            }
+        }
+        __syncthreads();
+        if (kq) return;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const float2 other = sml[t * 16 + lr];
+            const float M = ca_max(m[t], other.x), ref = M == ninf ? 0.f : M;
+            const float w0 = __builtin_amdgcn_exp2f(m[t] - ref), w1 = __builtin_amdgcn_exp2f(other.x - ref);
+            m[t] = M;
+            l[t] = l[t] * w0 + other.y * w1;
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt) o[t][dt] = o[t][dt] * w0 + so[(t * 8 + dt) * 64 + lane] * w1;
+        }
+    }
+    if (idle) return;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int r = 32 * rg + 16 * t + lr;
+        if (tile.row0 + r >= tile.rows) continue;
+        const int64_t at = ((int64_t)piece * p.HK + h) * p.pre.rows + r;
+        float *dst = p.pre.part_o + at * CA_D + 4 * kg;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4_t *>(dst + 16 * dt) = o[t][dt];
+        if (kg == 0) p.pre.part_ml[at] = make_float2(m[t], l[t]);
+    }
 }
 
 // Join the pieces of a row: GP groups of 32 lanes (4 head dims each) take them in turn, four loads at a time, and join in
@@ -274,45 +494,56 @@ __global__ __launch_bounds__(256) void k_shared_join(SaArgs p, int64_t nrows) {
 
 // Row tiles and the pieces' numbers.
 struct SaPlan {
-    int64_t np, no, ntile, vp, vo, cp, co, gp, go, wide;  // 16-row tiles a wave; sequences, pieces beyond one each, pieces
+    int64_t rg, np, no, ntile, tr, keys;  // rg: row groups of a tile (0: tiles of 16 np rows, a wave each); tr: rows of a prefix tile
+    int64_t vp, vo, cp, co, gp, go;       // sequences, pieces beyond one each, pieces
+    int64_t wp, wo;                       // workgroups of a piece's heads
     int64_t HK, B;
     bool shared;
     static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
-    int64_t blocks_p() const { return (gp + 7) / 8 * 8 * wide; }
-    int64_t blocks_o() const { return (go + 7) / 8 * 8 * wide; }
-    int64_t rows_p() const { return gp * HK * np * 16; }
+    int64_t blocks_p() const { return (gp + 7) / 8 * 8 * wp; }
+    int64_t blocks_o() const { return (go + 7) / 8 * 8 * wo; }
+    int64_t rows_p() const { return gp * HK * tr; }
     int64_t rows_o() const { return go * HK * no * 16; }
     int64_t bytes() const {
         return up(rows_p() * CA_D * 4) + up(rows_o() * CA_D * 4) + up(rows_p() * 8) + up(rows_o() * 8) + up(vp * 8) + up(vo * 8) +
                (shared ? up(vp * 16) + up(B * 4) + up(B * 8) : 0);
     }
 };
+#ifndef SA_ROUNDS
+#define SA_ROUNDS 1
+#endif
 static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P, bool shared) {
     SaPlan pl;
     const int64_t sg = S * (H / HK), rows = B * sg, cus = device_cus() > 0 ? device_cus() : 256;
+    const int64_t each = ((B + P - 1) / P) * sg;  // rows of a prefix, if they are alike
     pl.HK = HK;
     pl.B = B;
     pl.shared = shared;
-    pl.np = (rows + P - 1) / P > 16 ? 2 : 1;
+    pl.rg = each <= 32 ? 0 : (each - 1) % 128 < 64 ? 2 : 4;
+    pl.np = each > 16 ? 2 : 1;
+    pl.tr = pl.rg ? 32 * pl.rg : 16 * pl.np;
+    pl.keys = pl.rg ? ST_KEYS : CA_KB;
     pl.no = sg > 16 ? 2 : 1;
-    pl.wide = (HK + SA_WAVES - 1) / SA_WAVES;
+    pl.wo = (HK + SA_WAVES - 1) / SA_WAVES;
+    pl.wp = pl.rg ? HK : pl.wo;
     pl.ntile = (sg + 16 * pl.no - 1) / (16 * pl.no);
     pl.vo = B * pl.ntile;
     // Several prefixes: each may end with a tile that is not full.
-    pl.vp = (rows + 16 * pl.np - 1) / (16 * pl.np) + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
-    const int64_t bp = (CP + CA_KB - 1) / CA_KB, bo = (C + CA_KB - 1) / CA_KB;
-    const int64_t at_once = 2 * cus / pl.wide > 8 ? 2 * cus / pl.wide : 8;  // pieces that run at a time
-    const int64_t wp = bp * pl.vp, wo = bo * pl.vo, slots = 2 * at_once;
-    auto pieces = [&](int64_t w, int64_t v, int64_t blocks) {
-        int64_t n = slots * w / (wp + wo > 0 ? wp + wo : 1) - v;
+    pl.vp = (rows + pl.tr - 1) / pl.tr + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
+    const int64_t bp = (CP + pl.keys - 1) / pl.keys, bo = (C + CA_KB - 1) / CA_KB;
+    // Work in ns of a workgroup, two to a CU: a block of a prefix tile 1500 or 2500, a block of a wave's 2100 or 3000.
+    const int64_t tp = bp * pl.vp * pl.wp * (pl.rg == 4 ? 2500 : pl.rg == 2 ? 1500 : pl.np == 1 ? 2100 : 3000), to = bo * pl.vo * pl.wo * (pl.no == 1 ? 2100 : 3000);
+    const int64_t slots = 2 * SA_ROUNDS * cus;
+    auto pieces = [&](int64_t w, int64_t v, int64_t blocks, int64_t wide) {
+        int64_t n = slots * w / (tp + to > 0 ? tp + to : 1) / wide - v;
         n = n < 1 ? 1 : n;
         return n + v < v * blocks ? n : v * blocks - v > 1 ? v * blocks - v : 1;
     };
-    pl.cp = pieces(wp, pl.vp, bp);
-    pl.co = pieces(wo, pl.vo, bo);
+    pl.cp = pieces(tp, pl.vp, bp, pl.wp);
+    pl.co = pieces(to, pl.vo, bo, pl.wo);
     pl.gp = bp ? (pl.cp + pl.vp < pl.vp * bp ? pl.cp + pl.vp : pl.vp * bp) : 0;
     pl.go = bo ? (pl.co + pl.vo < pl.vo * bo ? pl.co + pl.vo : pl.vo * bo) : 0;
-    // Pieces are numbered past their bound only where a space is empty; dir is written by its first workgroup.
+    // A space without keys still has its first workgroup, which writes dir.
     if (pl.gp == 0) pl.gp = 1;
     if (pl.go == 0) pl.go = 1;
     return pl;
@@ -385,15 +616,20 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
         a.order = (int32_t *)take(B * 4);
         a.where = (int2 *)take(B * 8);
     }
-    a.pre.V = (int)pl.vp, a.pre.chunks = (int)pl.cp, a.pre.rows = (int)(16 * pl.np), a.pre.blocks = (uint32_t)pl.blocks_p();
-    a.own.V = (int)pl.vo, a.own.chunks = (int)pl.co, a.own.rows = (int)(16 * pl.no), a.own.blocks = (uint32_t)pl.blocks_o();
+    a.pre.V = (int)pl.vp, a.pre.chunks = (int)pl.cp, a.pre.rows = (int)pl.tr, a.pre.keys = (int)pl.keys, a.pre.blocks = (uint32_t)pl.blocks_p();
+    a.own.V = (int)pl.vo, a.own.chunks = (int)pl.co, a.own.rows = (int)(16 * pl.no), a.own.keys = CA_KB, a.own.blocks = (uint32_t)pl.blocks_o();
     a.B = (int)B, a.S = (int)S, a.H = (int)H, a.HK = (int)HK, a.G = (int)(H / HK), a.P = (int)P, a.ntile = (int)pl.ntile;
     a.scale_log2e = scale * 1.4426950408889634f;
     hipStream_t st = as_stream(stream);
     if (share) launch(k_shared_plan, dim3(1), dim3(1024), (size_t)(8 * P), st, a);
     const dim3 grid(a.pre.blocks + a.own.blocks);
-    launch(pl.np == 2 ? (pl.no == 2 ? k_shared_attn<2, 2> : k_shared_attn<2, 1>) : (pl.no == 2 ? k_shared_attn<1, 2> : k_shared_attn<1, 1>), grid,
-           dim3(64 * SA_WAVES), 0, st, a);
+    if (pl.rg) {
+        launch(pl.rg == 4 ? (pl.no == 2 ? k_shared_tile<4, 2> : k_shared_tile<4, 1>) : (pl.no == 2 ? k_shared_tile<2, 2> : k_shared_tile<2, 1>), grid,
+               dim3(64 * SA_WAVES), 0, st, a);
+    } else {
+        launch(pl.np == 2 ? (pl.no == 2 ? k_shared_attn<2, 2> : k_shared_attn<2, 1>) : (pl.no == 2 ? k_shared_attn<1, 2> : k_shared_attn<1, 1>),
+               grid, dim3(64 * SA_WAVES), 0, st, a);
+    }
     const int64_t nrows = B * HK * S * a.G, each = pl.gp / pl.vp + pl.go / pl.vo;
     const int64_t gp = each > 16 ? 8 : each > 4 ? 2 : 1;
     launch(gp == 8 ? k_shared_join<8> : gp == 2 ? k_shared_join<2> : k_shared_join<1>, dim3((unsigned)((nrows * gp + 7) / 8)), dim3(256), 0, st,
