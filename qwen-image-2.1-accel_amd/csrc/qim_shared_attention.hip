@@ -17,13 +17,13 @@ namespace qim {
 constexpr int SA_WAVES = 4;
 constexpr int SA_MAX_PREFIXES = 4096;
 
-// A space of key chunks: V sequences of up to C keys (own: a request and a tile of its rows; prefix: a tile of rows),
-// cut into `chunks` pieces more than there are sequences, at most.  Partial results by (piece, K/V head, row of the tile).
+// A space of keys: V sequences (own: a request and a tile of its rows; prefix: a tile of rows) cut into at most `most` pieces
+// (V or more).  Partial results by (piece, K/V head, row of the tile).
 struct SaSpace {
     float *part_o;    // 128 values each
     float2 *part_ml;  // (maximum, sum)
     int2 *dir;        // per sequence: its first piece and their number
-    int V, chunks, rows;
+    int V, most, rows;
     int keys;         // of a block: pieces are whole blocks
     uint32_t blocks;  // workgroups
 };
@@ -113,16 +113,26 @@ __device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
     return sa_clamp(p.lengths[i / p.ntile], p.C);
 }
 
-// Which piece this is: sequence v, its blocks [blk0, blk0 + per).  All sequences' blocks are cut into pieces of `per`, the
-// smallest of which there are at most chunks + V.  The first workgroup also writes the space's dir.
+// Which piece this is: sequence v, its blocks [blk0, blk0 + per).  All sequences' blocks are cut into pieces of `per`, of
+// which there are at most sp.most.  The first workgroup also writes the space's dir.
 template <bool PRE>
 __device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int64_t &blk0, int64_t &per) {
     const int lane = threadIdx.x & 63;
     auto blocks = [&](int i) { return i < sp.V ? (int)((sa_length<PRE>(p, i) + sp.keys - 1) / sp.keys) : 0; };
     int64_t total = 0;
     for (int i = 0; i < sp.V; i += 64) total += __builtin_amdgcn_readlane(ca_scan(blocks(i + lane), lane), 63);
-    const int64_t each = (total + sp.chunks - 1) / sp.chunks;
-    per = each > 1 ? each : 1;
+    // The smallest `per` that is sure to give at most `most` pieces, or a smaller one that happens to.
+    auto pieces = [&](int64_t of) {
+        int n = 0;
+        for (int i = 0; i < sp.V; i += 64) n += __builtin_amdgcn_readlane(ca_scan((int)((blocks(i + lane) + of - 1) / of), lane), 63);
+        return n;
+    };
+    const int spare = sp.most - sp.V > 1 ? sp.most - sp.V : 1;
+    const int64_t sure = (total + spare - 1) / spare;
+    per = (total + sp.most - 1) / sp.most;
+    per = per > 1 ? per : 1;
+    while (per < sure && pieces(per) > sp.most) per = per + per / 8 + 1;
+    per = per < sure || sure < 1 ? per : sure;
     uint32_t first = 0;
     bool found = false;
     for (int i = 0; i < sp.V && !(found && !writes); i += 64) {
@@ -209,39 +219,40 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         sa_wave<false, NO>(p, p.own, blockIdx.x - p.pre.blocks, lds + wave * CA_VTILE);
         return;
     }
-    const uint32_t q8 = blockIdx.x >> 3, grp = q8 / (uint32_t)p.HK, piece = grp * 8 + (blockIdx.x & 7);
-    const int h = (int)(q8 - grp * (uint32_t)p.HK);
+    // Eight heads of a piece to one XCD: they read neighbouring lines, and the same ones of exponents.
+    const uint32_t q8 = blockIdx.x >> 3, unit = (q8 >> 3) * 8 + (blockIdx.x & 7), units = (uint32_t)(p.HK + 7) / 8;
+    const uint32_t piece = unit / units;
+    const int h = (int)(unit - piece * units) * 8 + (int)(q8 & 7);
     int v = 0;
     int64_t blk0 = 0, per = 1;
-    if (!sa_piece<true>(p, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per)) return;
+    if (!sa_piece<true>(p, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per) || h >= p.HK) return;
     const SaTile tile = sa_tile(p, v);
     const int64_t len = sa_prefix_length(p, tile.prefix), W = (int64_t)p.HK * CA_D, base = (int64_t)tile.prefix * p.CP * W + h * CA_D;
     const int64_t nblk = (len + ST_KEYS - 1) / ST_KEYS, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
     const float c = p.scale_log2e, ninf = -__builtin_inff();
 
-    // A thread's share of a block: 16 codes of K and of V of keys tid / 8 and tid / 8 + 32.
+    // A thread's share of a block: 16 codes of K and of V of keys tid / 8 and tid / 8 + 32.  Wave-uniform bases and
+    // 32-bit offsets; only a block that reaches past the cache's end clamps its keys to the last.
     const int ck = tid >> 3, cc = tid & 7;
     struct Raw {
         uint4 k[2], v[2];
         uint32_t ke[2], ve[2];
     };
+    const uint32_t w32 = (uint32_t)W;
+    const uint8_t *const pk = p.pk + base, *const pv = p.pv + base, *const pks = p.pks + base / 32, *const pvs = p.pvs + base / 32;
     auto load = [&](Raw &w, int64_t blk) {
         blk = blk < blk1 ? blk : blk1 - 1;  // (past the end: not converted)
+        const int64_t k0 = blk * ST_KEYS, b8 = k0 * W, b5 = k0 * (W / 32);
+        const int last = p.CP - k0 < ST_KEYS ? (int)(p.CP - k0) - 1 : ST_KEYS - 1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            int64_t key = blk * ST_KEYS + 32 * i + ck;
-            key = key < p.CP ? key : p.CP - 1;
-            const int64_t at = base + key * W + 16 * cc;
-            w.k[i] = *reinterpret_cast<const uint4 *>(p.pk + at);
-            w.v[i] = *reinterpret_cast<const uint4 *>(p.pv + at);
-            w.ke[i] = p.pks[at >> 5];
-            w.ve[i] = p.pvs[at >> 5];
+            const uint32_t key = 32 * i + ck < last ? 32 * i + ck : last, at = key * w32 + 16 * cc, ae = key * (w32 / 32) + (cc >> 1);
+            w.k[i] = *reinterpret_cast<const uint4 *>(pk + b8 + at);
+            w.v[i] = *reinterpret_cast<const uint4 *>(pv + b8 + at);
+            w.ke[i] = (pks + b5)[ae];
+            w.ve[i] = (pvs + b5)[ae];
         }
     };
-    Raw raw[2];
-    load(raw[0], blk0);
-    load(raw[1], blk0 + 1);
-
     bf16x8_t qf[2][4];  // d [64 j + 16 kg + 8 half, + 8) in step 2 j + half
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -253,6 +264,14 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[t][j] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * (j >> 1) + 8 * (j & 1));
     }
+    Raw raw[2];
+    load(raw[0], blk0);
+    load(raw[1], blk0 + 1);
+    // Q is waited for here: a wait inside the loop would be one for all loads before the last, the second block's too.
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(qf[t][j]));
     f32x4_t o[2][8];
     float m[2], l[2];
 #pragma unroll
@@ -263,6 +282,14 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         for (int dt = 0; dt < 8; ++dt) o[t][dt] = f32x4_t{};
     }
     const bool idle = tile.row0 + 32 * rg >= tile.rows;  // no rows of this wave's: it only converts
+    // Places of this lane's operands in a buffer: K's chunks of row lr, V's units of key 4 kg + lr / 4.
+    const int vkey = 4 * kg + (lr >> 2);
+    uint32_t kat[4], vat[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kat[j] = (32 * kq + lr) * 256 + (((8 * (j >> 1) + 2 * kg + (j & 1)) ^ lr) << 4);
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) vat[dt] = ST_KEYS * 256 + (32 * kq + vkey) * 256 + (lr & 3) * 8 + ((dt ^ (vkey & 7)) << 5);
+    typedef __attribute__((address_space(3))) i16x4_t *tr_t;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     auto convert = [&](const Raw &w, int64_t blk, int buf) {
         uint8_t *const kb = lds + buf * ST_BUF, *const vb = kb + ST_KEYS * 256;
@@ -284,22 +311,17 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
             *reinterpret_cast<bf16x8_t *>(at + 16) = ca_operand(x.z, x.w, vs);
         }
     };
-    // 32 keys of the block in a buffer, from its key `first` on, for the wave's 32 rows; `left` keys are there.
-    auto attend = [&](int buf, int first, int64_t left) {
-        const uint8_t *const kb = lds + buf * ST_BUF;
-        const int vkey = first + 4 * kg + (lr >> 2);
+    // 32 keys of the block in a buffer, the wave's first or (RG 4) second 32, for its 32 rows; `left` keys are there.
+    auto attend = [&](int place, int64_t left) {
         f32x4_t s[2][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int key = first + 16 * u + lr;
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int ch = 8 * (j >> 1) + 2 * kg + (j & 1);
-                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(kb + key * 256 + ((ch ^ lr) << 4));
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(lds + kat[j] + (place + u * 4096));
 #pragma unroll
                 for (int t = 0; t < 2; ++t) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], j == 0 ? f32x4_t{} : s[t][u], 0, 0, 0);
             }
-        }
         u32x4_t pw[2], pl[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -311,38 +333,39 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
             }
             float mx = ca_max(ca_max(ca_max(s[t][0][0], s[t][0][1]), ca_max(s[t][0][2], s[t][0][3])),
                               ca_max(ca_max(s[t][1][0], s[t][1][1]), ca_max(s[t][1][2], s[t][1][3])));
-            {
+            // m follows the row's maximum when a score has passed it by more than 2^8 (in a row of the wave's, then in
+            // all of them): till then p is at most 2^8, which numerator and sum hold as well.
+            mx *= c;
+            if (__builtin_amdgcn_ballot_w64(!(mx <= m[t] + 8.0f))) {
                 const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = ca_swap_max(ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1]))) * c;
+                mx = ca_swap_max(ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+                const float mn = ca_max(m[t], mx);
+                const float alpha = __builtin_amdgcn_exp2f(m[t] - (mn == ninf ? 0.f : mn));
+                m[t] = mn;
+                l[t] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
             }
-            const float mn = ca_max(m[t], mx), ref = mn == ninf ? 0.f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m[t] - ref);
-            m[t] = mn;
+            const float ref = m[t] == ninf ? 0.f : m[t];
             float e[8], sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i >> 2][i & 3], c, -ref));
                 sum += e[i];
             }
-            l[t] = l[t] * alpha + sum;
+            l[t] += sum;
             // p as two bf16 terms, as in ca_wave.
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 pw[t][i] = pack_bf16x2(e[2 * i], e[2 * i + 1]);
                 pl[t][i] = pack_bf16x2(e[2 * i] - bf_lo(pw[t][i]), e[2 * i + 1] - bf_hi(pw[t][i]));
             }
-            if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) o[t][dt] *= alpha;
-            }
         }
-        const uint32_t vrow = lds0 + (uint32_t)(buf * ST_BUF + ST_KEYS * 256 + vkey * 256 + (lr & 3) * 8);
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            typedef __attribute__((address_space(3))) i16x4_t *ptr_t;
-            const uint32_t at = vrow + ((dt ^ (vkey & 7)) << 5);
-            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)at));
-            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<ptr_t>((uintptr_t)(at + 16 * CA_D * 2)));
+            const uint32_t at = lds0 + vat[dt] + place;
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tr_t>((uintptr_t)at));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tr_t>((uintptr_t)(at + 16 * CA_D * 2)));
             const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -358,9 +381,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         if (idle) return;
 #pragma unroll
         for (int i = 0; i < 2 / KQ; ++i) {
-            const int first = 32 * (kq + i);
-            const int64_t left = len - (blk * ST_KEYS + first);
-            if (left > 0) attend(buf, first, left);
+            const int64_t left = len - (blk * ST_KEYS + 32 * (kq + i));
+            if (left > 0) attend(buf * ST_BUF + i * (32 * 256), left);
         }
     };
     for (int64_t blk = blk0; blk < blk1; blk += 2) {
@@ -495,12 +517,12 @@ __global__ __launch_bounds__(256) void k_shared_join(SaArgs p, int64_t nrows) {
 // Row tiles and the pieces' numbers.
 struct SaPlan {
     int64_t rg, np, no, ntile, tr, keys;  // rg: row groups of a tile (0: tiles of 16 np rows, a wave each); tr: rows of a prefix tile
-    int64_t vp, vo, cp, co, gp, go;       // sequences, pieces beyond one each, pieces
+    int64_t vp, vo, gp, go;               // sequences, pieces (at most)
     int64_t wp, wo;                       // workgroups of a piece's heads
     int64_t HK, B;
     bool shared;
     static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
-    int64_t blocks_p() const { return (gp + 7) / 8 * 8 * wp; }
+    int64_t blocks_p() const { return rg ? (gp * ((HK + 7) / 8) + 7) / 8 * 64 : (gp + 7) / 8 * 8 * wp; }
     int64_t blocks_o() const { return (go + 7) / 8 * 8 * wo; }
     int64_t rows_p() const { return gp * HK * tr; }
     int64_t rows_o() const { return go * HK * no * 16; }
@@ -519,7 +541,7 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     pl.HK = HK;
     pl.B = B;
     pl.shared = shared;
-    pl.rg = each <= 32 ? 0 : (each - 1) % 128 < 64 ? 2 : 4;
+    pl.rg = each <= 32 ? 0 : each <= 64 ? 2 : 4;
     pl.np = each > 16 ? 2 : 1;
     pl.tr = pl.rg ? 32 * pl.rg : 16 * pl.np;
     pl.keys = pl.rg ? ST_KEYS : CA_KB;
@@ -531,21 +553,22 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     // Several prefixes: each may end with a tile that is not full.
     pl.vp = (rows + pl.tr - 1) / pl.tr + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
     const int64_t bp = (CP + pl.keys - 1) / pl.keys, bo = (C + CA_KB - 1) / CA_KB;
-    // Work in ns of a workgroup, two to a CU: a block of a prefix tile 1500 or 2500, a block of a wave's 2100 or 3000.
-    const int64_t tp = bp * pl.vp * pl.wp * (pl.rg == 4 ? 2500 : pl.rg == 2 ? 1500 : pl.np == 1 ? 2100 : 3000), to = bo * pl.vo * pl.wo * (pl.no == 1 ? 2100 : 3000);
+    // Work in ns of a workgroup, two to a CU.
+#ifndef SA_T
+#define SA_T 2300, 1400, 1000, 1500
+#endif
+    constexpr int64_t T[4] = {SA_T};
+    const int64_t tp = bp * pl.vp * pl.wp * (pl.rg == 4 ? T[0] : pl.rg == 2 ? T[1] : pl.np == 1 ? T[2] : T[3]), to = bo * pl.vo * pl.wo * (pl.no == 1 ? T[2] : T[3]);
     const int64_t slots = 2 * SA_ROUNDS * cus;
+    // At least a piece a sequence (also where a space holds no keys: its first workgroup writes dir), at most one a block.
     auto pieces = [&](int64_t w, int64_t v, int64_t blocks, int64_t wide) {
-        int64_t n = slots * w / (tp + to > 0 ? tp + to : 1) / wide - v;
-        n = n < 1 ? 1 : n;
-        return n + v < v * blocks ? n : v * blocks - v > 1 ? v * blocks - v : 1;
+        int64_t n = (slots * w / (tp + to > 0 ? tp + to : 1) + wide / 2) / wide;
+        const int64_t most = v * blocks;
+        if (n < 4 * v) n = n / v * v;  // (whole pieces of sequences that are alike)
+        return n < v || most < v ? v : n < most ? n : most;
     };
-    pl.cp = pieces(tp, pl.vp, bp, pl.wp);
-    pl.co = pieces(to, pl.vo, bo, pl.wo);
-    pl.gp = bp ? (pl.cp + pl.vp < pl.vp * bp ? pl.cp + pl.vp : pl.vp * bp) : 0;
-    pl.go = bo ? (pl.co + pl.vo < pl.vo * bo ? pl.co + pl.vo : pl.vo * bo) : 0;
-    // A space without keys still has its first workgroup, which writes dir.
-    if (pl.gp == 0) pl.gp = 1;
-    if (pl.go == 0) pl.go = 1;
+    pl.gp = pieces(tp, pl.vp, bp, pl.wp);
+    pl.go = pieces(to, pl.vo, bo, pl.wo);
     return pl;
 }
 
@@ -616,8 +639,8 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
         a.order = (int32_t *)take(B * 4);
         a.where = (int2 *)take(B * 8);
     }
-    a.pre.V = (int)pl.vp, a.pre.chunks = (int)pl.cp, a.pre.rows = (int)pl.tr, a.pre.keys = (int)pl.keys, a.pre.blocks = (uint32_t)pl.blocks_p();
-    a.own.V = (int)pl.vo, a.own.chunks = (int)pl.co, a.own.rows = (int)(16 * pl.no), a.own.keys = CA_KB, a.own.blocks = (uint32_t)pl.blocks_o();
+    a.pre.V = (int)pl.vp, a.pre.most = (int)pl.gp, a.pre.rows = (int)pl.tr, a.pre.keys = (int)pl.keys, a.pre.blocks = (uint32_t)pl.blocks_p();
+    a.own.V = (int)pl.vo, a.own.most = (int)pl.go, a.own.rows = (int)(16 * pl.no), a.own.keys = CA_KB, a.own.blocks = (uint32_t)pl.blocks_o();
     a.B = (int)B, a.S = (int)S, a.H = (int)H, a.HK = (int)HK, a.G = (int)(H / HK), a.P = (int)P, a.ntile = (int)pl.ntile;
     a.scale_log2e = scale * 1.4426950408889634f;
     hipStream_t st = as_stream(stream);
