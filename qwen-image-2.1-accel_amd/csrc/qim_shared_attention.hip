@@ -116,34 +116,48 @@ __device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
 // Which piece this is: sequence v, its blocks [blk0, blk0 + per).  All sequences' blocks are cut into pieces of `per`, of
 // which there are at most sp.most.  The first workgroup also writes the space's dir.
 template <bool PRE>
-__device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int64_t &blk0, int64_t &per) {
+__device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int &blk0, int &per) {
     const int lane = threadIdx.x & 63;
-    auto blocks = [&](int i) { return i < sp.V ? (int)((sa_length<PRE>(p, i) + sp.keys - 1) / sp.keys) : 0; };
-    int64_t total = 0;
-    for (int i = 0; i < sp.V; i += 64) total += __builtin_amdgcn_readlane(ca_scan(blocks(i + lane), lane), 63);
+    if (PRE && !p.share) {  // sequences alike: the same pieces of each
+        const int n = (int)(((uint32_t)sa_prefix_length(p, 0) + sp.keys - 1) / (uint32_t)sp.keys), each = sp.most / sp.V;
+        const int size = n > each ? (n + each - 1) / each : 1, count = (n + size - 1) / size;
+        per = size;
+        if (writes)
+            for (int i = lane; i < sp.V; i += 64) sp.dir[i] = make_int2(i * count, count);
+        if (!count || piece >= (uint32_t)(sp.V * count)) return false;
+        v = (int)(piece / (uint32_t)count);
+        blk0 = ((int)piece - v * count) * size;
+        return true;
+    }
+    auto blocks = [&](int i) { return i < sp.V ? (int)(((uint32_t)sa_length<PRE>(p, i) + sp.keys - 1) / (uint32_t)sp.keys) : 0; };
+    const int head = blocks(lane);  // the first 64 sequences' stay in a register
+    auto blocks_from = [&](int i) { return i ? blocks(i + lane) : head; };
+    uint32_t total = 0;  // (all spaces have fewer than 2^31 blocks)
+    for (int i = 0; i < sp.V; i += 64) total += (uint32_t)__builtin_amdgcn_readlane(ca_scan(blocks_from(i), lane), 63);
     // The smallest `per` that is sure to give at most `most` pieces, or a smaller one that happens to.
-    auto pieces = [&](int64_t of) {
+    auto pieces = [&](uint32_t of) {
         int n = 0;
-        for (int i = 0; i < sp.V; i += 64) n += __builtin_amdgcn_readlane(ca_scan((int)((blocks(i + lane) + of - 1) / of), lane), 63);
+        for (int i = 0; i < sp.V; i += 64) n += __builtin_amdgcn_readlane(ca_scan((int)((blocks_from(i) + of - 1) / of), lane), 63);
         return n;
     };
     const int spare = sp.most - sp.V > 1 ? sp.most - sp.V : 1;
-    const int64_t sure = (total + spare - 1) / spare;
-    per = (total + sp.most - 1) / sp.most;
-    per = per > 1 ? per : 1;
-    while (per < sure && pieces(per) > sp.most) per = per + per / 8 + 1;
-    per = per < sure || sure < 1 ? per : sure;
+    const uint32_t sure = (total + spare - 1) / (uint32_t)spare;
+    uint32_t of = (total + sp.most - 1) / (uint32_t)sp.most;
+    of = of > 1 ? of : 1;
+    while (of < sure && pieces(of) > sp.most) of = of + of / 8 + 1;
+    of = of < sure || sure < 1 ? of : sure;
+    per = (int)of;
     uint32_t first = 0;
     bool found = false;
     for (int i = 0; i < sp.V && !(found && !writes); i += 64) {
-        const int n = (int)((blocks(i + lane) + per - 1) / per), last = ca_scan(n, lane);
+        const int n = (int)((blocks_from(i) + of - 1) / of), last = ca_scan(n, lane);
         const uint32_t from = first + last - n;
         if (writes && i + lane < sp.V) sp.dir[i + lane] = make_int2((int)from, n);
         const uint64_t here = __builtin_amdgcn_ballot_w64(piece >= from && piece < from + n);
         if (here) {
             const int at = (int)__builtin_ctzll(here);
             v = i + at;
-            blk0 = (int64_t)(piece - (uint32_t)__builtin_amdgcn_readlane((int)from, at)) * per;
+            blk0 = (int)(piece - (uint32_t)__builtin_amdgcn_readlane((int)from, at)) * per;
             found = true;
         }
         first += (uint32_t)__builtin_amdgcn_readlane(last, 63);
@@ -160,7 +174,7 @@ __device__ __forceinline__ void sa_wave(const SaArgs &p, const SaSpace &sp, uint
     const uint32_t piece = grp * 8 + (block & 7);  // the heads of a piece to one XCD
     const int h = (int)((q8 - grp * wide) * SA_WAVES) + wave;
     int v = 0;
-    int64_t blk0 = 0, per = 1;
+    int blk0 = 0, per = 1;
     if (!sa_piece<PRE>(p, sp, piece, block == 0 && wave == 0, v, blk0, per)) return;
     if (h >= p.HK) return;
     const int64_t len = sa_length<PRE>(p, v), W = (int64_t)p.HK * CA_D, C = PRE ? p.CP : p.C;
@@ -168,7 +182,7 @@ __device__ __forceinline__ void sa_wave(const SaArgs &p, const SaSpace &sp, uint
     const int64_t base = (int64_t)tile.prefix * C * W + h * CA_D;
     const CaKeys keys{(PRE ? p.pk : p.kc) + base, (PRE ? p.pks : p.ks) + base / 32, (PRE ? p.pv : p.vc) + base,
                       (PRE ? p.pvs : p.vs) + base / 32, C, W, len};
-    const int64_t nblk = (len + CA_KB - 1) / CA_KB, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
+    const int nblk = (int)((len + CA_KB - 1) / CA_KB), blk1 = blk0 + per < nblk ? blk0 + per : nblk;
     f32x4_t o[NR][8];
     float m[NR], l[NR];
     ca_wave<NR>(keys, blk0, blk1, p.scale_log2e, !PRE && p.tree ? len - p.S : len, vt,
@@ -224,11 +238,11 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
     const uint32_t piece = unit / units;
     const int h = (int)(unit - piece * units) * 8 + (int)(q8 & 7);
     int v = 0;
-    int64_t blk0 = 0, per = 1;
+    int blk0 = 0, per = 1;
     if (!sa_piece<true>(p, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per) || h >= p.HK) return;
     const SaTile tile = sa_tile(p, v);
     const int64_t len = sa_prefix_length(p, tile.prefix), W = (int64_t)p.HK * CA_D, base = (int64_t)tile.prefix * p.CP * W + h * CA_D;
-    const int64_t nblk = (len + ST_KEYS - 1) / ST_KEYS, blk1 = blk0 + per < nblk ? blk0 + per : nblk;
+    const int nblk = (int)((len + ST_KEYS - 1) / ST_KEYS), blk1 = blk0 + per < nblk ? blk0 + per : nblk;
     const float c = p.scale_log2e, ninf = -__builtin_inff();
 
     // A thread's share of a block: 16 codes of K and of V of keys tid / 8 and tid / 8 + 32.  Wave-uniform bases and
@@ -240,9 +254,9 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
     };
     const uint32_t w32 = (uint32_t)W;
     const uint8_t *const pk = p.pk + base, *const pv = p.pv + base, *const pks = p.pks + base / 32, *const pvs = p.pvs + base / 32;
-    auto load = [&](Raw &w, int64_t blk) {
+    auto load = [&](Raw &w, int blk) {
         blk = blk < blk1 ? blk : blk1 - 1;  // (past the end: not converted)
-        const int64_t k0 = blk * ST_KEYS, b8 = k0 * W, b5 = k0 * (W / 32);
+        const int64_t k0 = (int64_t)blk * ST_KEYS, b8 = k0 * W, b5 = k0 * (W / 32);
         const int last = p.CP - k0 < ST_KEYS ? (int)(p.CP - k0) - 1 : ST_KEYS - 1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -291,7 +305,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
     for (int dt = 0; dt < 8; ++dt) vat[dt] = ST_KEYS * 256 + (32 * kq + vkey) * 256 + (lr & 3) * 8 + ((dt ^ (vkey & 7)) << 5);
     typedef __attribute__((address_space(3))) i16x4_t *tr_t;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    auto convert = [&](const Raw &w, int64_t blk, int buf) {
+    auto convert = [&](const Raw &w, int blk, int buf) {
+        const int live = len - (int64_t)blk * ST_KEYS < ST_KEYS ? (int)(len - (int64_t)blk * ST_KEYS) : ST_KEYS;
         uint8_t *const kb = lds + buf * ST_BUF, *const vb = kb + ST_KEYS * 256;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -301,7 +316,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
             *reinterpret_cast<bf16x8_t *>(kb + key * 256 + (((2 * cc + 1) ^ (key & 15)) << 4)) = ca_operand(w.k[i].z, w.k[i].w, ks);
             uint4 x = w.v[i];
             uint32_t e = w.ve[i];
-            if (blk * ST_KEYS + key >= len) {  // V past the last key is zeros, whatever the cache holds there
+            if (key >= live) {  // V past the last key is zeros, whatever the cache holds there
                 x = make_uint4(0, 0, 0, 0);
                 e = 0;
             }
@@ -374,18 +389,18 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
             }
         }
     };
-    auto block = [&](Raw &w, int64_t blk, int buf) {
+    auto block = [&](Raw &w, int blk, int buf) {
         convert(w, blk, buf);
         __syncthreads();
         load(w, blk + 2);
         if (idle) return;
 #pragma unroll
         for (int i = 0; i < 2 / KQ; ++i) {
-            const int64_t left = len - (blk * ST_KEYS + 32 * (kq + i));
+            const int64_t left = len - ((int64_t)blk * ST_KEYS + 32 * (kq + i));
             if (left > 0) attend(buf * ST_BUF + i * (32 * 256), left);
         }
     };
-    for (int64_t blk = blk0; blk < blk1; blk += 2) {
+    for (int blk = blk0; blk < blk1; blk += 2) {
         block(raw[0], blk, 0);
         if (blk + 1 < blk1) block(raw[1], blk + 1, 1);
     }
