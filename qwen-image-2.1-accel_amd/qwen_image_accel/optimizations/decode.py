@@ -23,7 +23,8 @@ stacked Q/K/V and interleaved gate/up weights were built):
                which also writes an MXFP8 out-projection's input
     mlp        img_mlp (SwiGLU hook)            gate/up GEMM with the SwiGLU -> MXFP8
                                                 epilogue, or two GEMMs + swiglu_quantize
-    residual   residual(h, branch, tanh g)
+    residual   residual(h, branch, tanh g); after the attention together with norm2 in one
+               pass (residual_norm in its eager form: the same bits)
 
 Prefill (any ``kv_cache_mode`` other than "cached") runs the block's own
 forward and the attention processor it replaced.
@@ -33,10 +34,10 @@ import torch
 from qwen_image_accel.kernels.attention import (attention_mxfp8, prepare_attention_inputs,
                                                 prepare_attention_inputs_quantized)
 from qwen_image_accel.kernels.bf16 import swiglu
-from qwen_image_accel.kernels.elementwise import residual, rope_qk
+from qwen_image_accel.kernels.elementwise import residual, residual_norm, rope_qk
 from qwen_image_accel.kernels.epilogue import layer_norm_scale_quantize, swiglu_quantize
 from qwen_image_accel.kernels.gemm import mx_matmul
-from qwen_image_accel.kernels.layernorm import layer_norm_scale
+from qwen_image_accel.kernels.layernorm import layer_norm_scale, native_supported
 from qwen_image_accel.kernels.mxfp8 import Quantized, quantize
 from qwen_image_accel.optimizations.adapters import running
 from qwen_image_accel.optimizations.attention_call import attention, qim_backend
@@ -46,6 +47,9 @@ from qwen_image_accel.weights import fuse_gate_up, fuse_qkv
 
 # Keyword arguments of a block call that the attention module does not take.
 BLOCK_ONLY = frozenset({"hidden_states", "modulation", "target_token_mask"})
+
+# Rows from which the residual and the norm behind it run as two launches (the joined one has a workgroup a row).
+MAX_JOINED_ROWS = (1 << 22) - 128
 
 
 class StepTerms:
@@ -234,6 +238,18 @@ class DecodeBlock:
                 return x
         return layer_norm_scale(h, scale, norm)
 
+    def add_and_normalize(self, h, branch, gate, scale, norm, consumers):
+        """(h + gate * branch, its normalisation for ``consumers``): in one pass where the kernel takes the
+        operands, with the bits of the two."""
+        quantized = self.quantized and all_mxfp8(*(running(m) for m in consumers))
+        if (gate is not None and branch.shape == h.shape and branch.is_contiguous() and branch.device == h.device
+                and branch.dtype == h.dtype and native_supported(h, scale, norm, gate=gate)
+                and h.shape[0] * h.shape[1] < MAX_JOINED_ROWS and (not quantized or h.shape[-1] % 128 == 0)):
+            return residual_norm(h, branch, norm, gate=gate, scale=scale, quantized=quantized, tiled=quantized,
+                                 rounding="eager")
+        h = residual(h, branch, gate)
+        return h, self.normalize(h, scale, norm, consumers)
+
     def __call__(self, *args, **kwargs):
         if kwargs.get("kv_cache_mode") != "cached":
             return self.eager(*args, **kwargs)
@@ -242,8 +258,8 @@ class DecodeBlock:
         scale1, gate1, scale2, gate2 = self.terms(kwargs["modulation"])
         attn_kwargs = {name: value for name, value in kwargs.items() if name not in BLOCK_ONLY}
         x = self.normalize(h, scale1, blk.img_norm1, (blk.attn.to_q, blk.attn.to_k, blk.attn.to_v))
-        h = residual(h, blk.attn(hidden_states=x, **attn_kwargs), gate1)
-        x = self.normalize(h, scale2, blk.img_norm2, (blk.img_mlp.gate_layer, blk.img_mlp.proj))
+        h, x = self.add_and_normalize(h, blk.attn(hidden_states=x, **attn_kwargs), gate1, scale2, blk.img_norm2,
+                                      (blk.img_mlp.gate_layer, blk.img_mlp.proj))
         return residual(h, blk.img_mlp(x), gate2)
 
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from qwen_image_accel import _native
-from qwen_image_accel.kernels import elementwise, fourbit
+from qwen_image_accel.kernels import attention, elementwise, fourbit, kv_cache
 
 ARG, SHAPE, LAYOUT = _native.QIM_ERR_ARG, _native.QIM_ERR_SHAPE, _native.QIM_ERR_LAYOUT
 FAR = 1 << 30
@@ -23,7 +23,20 @@ def four(x=FAR, ldx=256, group=64, codes=16, scales=16, zeros=None, codes2=None,
     return ("qim_fourbit_matmul", (x, ldx, group, codes, scales, zeros, codes2, scales2, zeros2, bias, out, ldo, f32, m, n, k, None))
 
 
+def share(q=FAR, ldq=512, pk=16, plens=16, which=16, kc=16, lengths=16, tree=None, o=2 * FAR, ws=16, nbytes=1 << 40, b=2, s=1, p=3, cp=64,
+          c=32, h=4, hk=2, d=128, scale=0.1):
+    return ("qim_attention_shared", (q, 512, ldq, pk, 16, 16, 16, plens, which, kc, 16, 16, 16, lengths, tree, 0, o, ws, nbytes, b, s, p, cp, c,
+                                     h, hk, d, scale, None))
+
+
 @pytest.mark.parametrize("call,code", [
+    (share(q=None), ARG), (share(pk=None), ARG), (share(kc=None), ARG), (share(lengths=None), ARG), (share(o=None), ARG), (share(ws=None), ARG),
+    (share(scale=0.0), ARG), (share(scale=float("nan")), ARG), (share(scale=1e31), ARG), (share(nbytes=64), ARG), (share(o=FAR + 512), ARG),
+    (share(which=None), SHAPE), (share(p=0), SHAPE), (share(p=4097), SHAPE), (share(cp=0), SHAPE), (share(c=-1), SHAPE), (share(s=65), SHAPE),
+    (share(s=0), SHAPE), (share(b=0), SHAPE), (share(h=3), SHAPE), (share(d=64), SHAPE), (share(cp=1 << 31), SHAPE), (share(b=1 << 20), SHAPE),
+    (share(h=1 << 17, hk=1), SHAPE), (share(b=1 << 19, s=64, p=1), SHAPE), (share(cp=1 << 30, p=4096), SHAPE),
+    (share(q=FAR + 8), LAYOUT), (share(ldq=500), LAYOUT), (share(ldq=256), LAYOUT), (share(pk=24), LAYOUT), (share(o=2 * FAR + 8), LAYOUT),
+    (share(ws=24), LAYOUT), (share(lengths=18), LAYOUT), (share(which=18), LAYOUT), (share(plens=17), LAYOUT),
     (norm(h=None), ARG), (norm(x=None), ARG), (norm(ho=None), ARG), (norm(z=None), ARG), (norm(post=3), ARG), (norm(norm=0), ARG),
     (norm(norm=3), ARG), (norm(flags=8), ARG), (norm(post_w=16), ARG), (norm(norm_w=16), ARG), (norm(scale=None, flags=1), ARG),
     (norm(flags=4, gate=None), ARG), (norm(flags=4, scale=None), ARG), (norm(flags=4, alpha=0.5), ARG), (norm(flags=4, norm=1), ARG),
@@ -50,6 +63,13 @@ def test_entry_points_refuse(call, code):
     assert _native.lib().qim_last_error()
 
 
+def test_workspace_sizes():
+    size = _native.lib().qim_attention_shared_workspace_bytes
+    assert size(2, 1, 64, 32, 4, 2, 1, 0) > 0 and size(2, 1, 64, 0, 4, 2, 1, 0) > 0      # an own cache of no positions
+    assert size(2, 65, 64, 32, 4, 2, 1, 0) == 0 and size(2, 1, 64, 32, 4, 2, 2, 0) == 0  # not shapes it takes
+    assert size(48, 1, 32768, 640, 32, 8, 5, 1) >= 48 * 32 * 2 * 128 * 4                 # a prefix's and an own result of every row
+
+
 def test_wrappers_refuse_host_tensors():
     x = torch.zeros(2, 128, dtype=torch.bfloat16)
     w = fourbit.quantize_weight(torch.ones(16, 128))
@@ -57,5 +77,8 @@ def test_wrappers_refuse_host_tensors():
         fourbit.matmul(x, w)
     with pytest.raises(_native.Unsupported):
         fourbit.swiglu(x, w, w)
+    cache = kv_cache.empty_cache(1, 8, 2, 128, "cpu")
+    with pytest.raises(_native.Unsupported):
+        attention.attention_shared(torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16), cache, cache, torch.ones(1, dtype=torch.int32))
     with pytest.raises(_native.Unsupported):
         elementwise.residual_norm(x, x, types.SimpleNamespace(weight=None, eps=1e-6))
