@@ -3,8 +3,8 @@
 //   int4:   W[n, k] = s[n, k / g] (q[n, k] - z[n, k / g]),  q 0..15, z 0..15 (8 if there are none), s bf16, g 32, 64 or 128
 //   mxfp4:  W[n, k] = E2M1(c[n, k]) 2^(e[n, k / 32] - 127)
 //
-// Up to some 32 rows the weights' bytes bound it: half a byte a weight, read once; beyond, the vector instructions that
-// make operands of codes.  W is laid out once in the order in which the matrix cores take it
+// Up to some 16 rows the weights' bytes bound it: half a byte a weight, read once; beyond, the vector instructions that make
+// operands of codes and, for int4, take the groups' scales in.  W is laid out once in the order in which the matrix cores take it
 // (v_mfma_f32_16x16x32_bf16, W the A operand, x the B operand): a tile of 16 rows of W and a step of 128 k is 1 KiB, lane
 // l's 16 bytes the row n = l % 16 and, in its dword j, k = 32 j + 8 (l / 16) + 0..7.  Codes become bf16 in registers, exactly:
 // E2M1 by the scaled conversion with the block's exponent; q - z by a table of the 16 E4M3 codes of 0 - z .. 15 - z (|q - z| is
@@ -13,8 +13,11 @@
 // group's scale.  (Taking q for q - z and z times the sum of x away again in fp32 costs less per code and
 // more per group and row; it also makes NaN of infinities.)
 //
-// The waves of a workgroup take the steps of k in turn, each for the whole tile of output, and join in LDS: nothing is
-// shared and no barrier stands in the loop, and every operand made of codes serves all of the tile's rows.
+// Two kernels.  k_fourbit, few rows or few columns: the waves of a workgroup take the steps of k in turn, each for the whole
+// tile of output and through a ring in LDS of its own, and join at the end; no barrier stands in the loop.  k_fourbit_tile,
+// the others: stages in LDS that eight waves share, and up to 128 rows for every operand made of codes.
+// Measured (weights in HBM, launches from a graph), int4 g 128, 1 row, 4096 -> 12288: 9.5 us; mxfp4, 16 rows, 12288 -> 4096: 8.9 us;
+// int4 g 32, 154 rows, 4096 -> 12288: 39.9 us, 390 TFLOP/s; mxfp4, 1024 rows, 4096 -> 4096: 37.6 us, 914 TFLOP/s.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -104,7 +107,7 @@ __device__ __forceinline__ void fb_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// Up to 4 RX rows: NT tiles of 16 columns of W (SWIGLU: NT / 2 of each weight) a workgroup, whose waves take the steps of k
+// 4 RX rows and NT tiles of 16 columns of W (SWIGLU: NT / 2 of each weight) a workgroup, whose waves take the steps of k
 // in turn.  G: groups of int4 in a step, 0 for mxfp4.  Everything goes through a ring of S stages in LDS of the wave's own:
 // S steps are on their way without registers held for them, and x, whose rows an operand takes from 16 places at
 // once, arrives in whole 256-byte rows (read by the operands' lanes themselves, 16 bytes here and there, it cost four
@@ -125,7 +128,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ntiles = (p.N + 15) / 16;
-    const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x);
+    const int row0 = (int)blockIdx.y * 4 * RX, rows = p.M - row0;
+    const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x + row0 * p.ldx);
     const uint8_t *const ring = lds + wave * (S * Ring::BYTES);
     const uint32_t ring0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)ring;
     // Rows and tiles past the last are the last (computed, not stored); a 16-byte chunk c of row r of x lies at c ^ r, so that
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
 #pragma unroll
     for (int i = 0; i < RX; ++i) {
         const int r = 4 * i + kg;
-        xoff[i] = (uint32_t)(r < p.M ? r : p.M - 1) * (uint32_t)(2 * p.ldx) + 16 * (lr ^ r);
+        xoff[i] = (uint32_t)(r < rows ? r : rows - 1) * (uint32_t)(2 * p.ldx) + 16 * (lr ^ r);
     }
     auto issue = [&](int t, int slot) {
         const uint32_t to = ring0 + slot * Ring::BYTES;
@@ -208,6 +212,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4 *>(st + xrow * 256 + (((4 * j + kg) ^ xrow) << 4));
+        uint4 tab[NT][G ? G : 1];
+        if constexpr (G > 0) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int g = 0; g < G; ++g) tab[i][g] = tables[(z[i] >> (8 * g)) & 0xffu];
+        }
+        __builtin_amdgcn_sched_barrier(0);  // all reads are on their way before the first result is used
         const int left = p.K - 128 * step(n);  // of k: whole groups, a step but for the last
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -220,7 +232,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
                     acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xv, acc[i], 0, 0, 0);
                 } else {
                     const int g = j / PER;
-                    const bf16x8_t w = fb_int4(fb_word(c[i], j), tables[(z[i] >> (8 * g)) & 0xffu]);
+                    const bf16x8_t w = fb_int4(fb_word(c[i], j), tab[i][g]);
                     a[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, xv, j % PER ? a[i] : f32x4_t{}, 0, 0, 0);
                     if (j % PER == PER - 1) {
                         const uint32_t s0 = fb_word(s[i][g / 2], 2 * (g & 1)), s1 = fb_word(s[i][g / 2], 2 * (g & 1) + 1);
@@ -246,7 +258,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
         if (SWIGLU) u += part[v][2 * wave + 1][lane];
     }
     const int64_t n0 = ((int64_t)blockIdx.x * OT + wave) * 16 + 4 * kg;
-    if (lr < p.M && n0 < p.N) fb_store<SWIGLU>(p, lr, n0, y, u);
+    if (lr < 4 * RX && lr < rows && n0 < p.N) fb_store<SWIGLU>(p, row0 + lr, n0, y, u);
 }
 
 template <int G, int NT, int RX, int WAVES, int S, bool SWIGLU>
@@ -257,7 +269,7 @@ static int launch_fourbit_ring(const FourBitArgs &a, hipStream_t st) {
         const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit<G, NT, RX, WAVES, S, SWIGLU>), bytes, done, "qim_fourbit_matmul");
         if (rc != QIM_OK) return rc;
     }
-    launch(k_fourbit<G, NT, RX, WAVES, S, SWIGLU>, dim3((unsigned)(((a.N + 15) / 16 + OT - 1) / OT)), dim3(64 * WAVES), bytes, st, a);
+    launch(k_fourbit<G, NT, RX, WAVES, S, SWIGLU>, dim3((unsigned)(((a.N + 15) / 16 + OT - 1) / OT), (unsigned)((a.M + 4 * RX - 1) / (4 * RX))), dim3(64 * WAVES), bytes, st, a);
     return QIM_OK;
 }
 
@@ -299,7 +311,7 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds;
     constexpr int PIECES = (4 * NR + FT_WAVES - 1) / FT_WAVES;
     uint32_t xoff[PIECES];
-    auto piece = [&](int i) { return wave + FT_WAVES * i < 4 * NR ? wave + FT_WAVES * i : wave; };  // (a piece brought twice)
+    auto piece = [&](int i) { return (wave + FT_WAVES * i) % (4 * NR); };  // (some come twice, where 2 does not divide NR)
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int r = 4 * piece(i) + kg, last = p.M - 1 - row0;
@@ -421,20 +433,34 @@ static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
     return QIM_OK;
 }
 
+// Which kernel.  At 4096 columns of x (and alike at others) the tile kernel takes about 12.5 us and 3.5 + 2.75 NR more for each
+// workgroup that a CU has to take, the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16: the first is held up
+// by the barrier of its steps while it has a workgroup or two a CU, the other makes operands of all codes again for every 16 rows.
+// int4, group 64, tile against ring: 32 x 4096 18.2 us and 9.7, 64 x 4096 18.3 and 12.7, 128 x 4096 19.3 and 21.7,
+// 24 x 24576 26.0 and 33.1, 16 x 65536 44.4 and 48.2; mxfp4: 64 x 4096 17.1 and 8.9, 16 x 65536 31.7 and 39.0.
 template <int G, bool SWIGLU>
 static int launch_fourbit(const FourBitArgs &a, hipStream_t st) {
-    constexpr int ONE = SWIGLU ? 2 : 1;
+    constexpr int ONE = SWIGLU ? 2 : 1, OT = SWIGLU ? FT_NT / 2 : FT_NT;
     if (a.M <= 4) return launch_fourbit_ring<G, ONE, 1, 8, 3, SWIGLU>(a, st);
-    if (a.M <= 16) {
-        // Many columns: two tiles share the reads of x, and two workgroups of four waves a CU take more of them at a time
-        // (16 rows, mxfp4: 4096 -> 12288 9.2 us against 11.6; 12288 -> 4096, 256 tiles, 14.6 against 9.0).
-        if (a.N >= 16 * 512) return launch_fourbit_ring<G, 2, 4, 4, 3, SWIGLU>(a, st);
+    const int64_t ntiles = (a.N + 15) / 16, ncol = (ntiles + OT - 1) / OT;
+    auto cost = [&](int nr) { return (ncol * ((a.M + 16 * nr - 1) / (16 * nr)) + 255) / 256 * (10 * nr + 13); };  // of 0.275 us
+    int nr = 8;
+    for (int n : {5, 4, 2, 1})
+        if (cost(n) < cost(nr)) nr = n;
+    const int64_t blocks = (a.M + 15) / 16 * ntiles;
+    if (a.M <= 16 * 65535 && 10 * ONE * blocks < 256 * (35 + cost(nr))) {  // (a grid of no more than 65535 blocks of rows)
+        // From one and a half tiles a CU on two of them share the reads of x, and two workgroups of four waves a CU take more of
+        // them at a time (16 rows, mxfp4: 4096 -> 12288 9.2 us against 11.6; 12288 -> 4096, 256 tiles, 14.6 against 9.0).
+        if (blocks >= 384) return launch_fourbit_ring<G, 2, 4, 4, 3, SWIGLU>(a, st);
         return launch_fourbit_ring<G, ONE, 4, 8, 2, SWIGLU>(a, st);
     }
-    if (a.M <= 32) return launch_fourbit_tile<G, 2, SWIGLU>(a, st);
-    if (a.M <= 64) return launch_fourbit_tile<G, 4, SWIGLU>(a, st);
-    if (a.M <= 160) return launch_fourbit_tile<G, 5, SWIGLU>(a, st);
-    return launch_fourbit_tile<G, 8, SWIGLU>(a, st);
+    switch (nr) {
+        case 1: return launch_fourbit_tile<G, 1, SWIGLU>(a, st);
+        case 2: return launch_fourbit_tile<G, 2, SWIGLU>(a, st);
+        case 4: return launch_fourbit_tile<G, 4, SWIGLU>(a, st);
+        case 5: return launch_fourbit_tile<G, 5, SWIGLU>(a, st);
+        default: return launch_fourbit_tile<G, 8, SWIGLU>(a, st);
+    }
 }
 
 }  // namespace qim

@@ -76,6 +76,24 @@ def test_swiglu(dev, m, n, k, kind, group, zeros):
     check(fourbit.swiglu(x, pack(a), pack(b)), y, e)
 
 
+# Rows and columns of a plain product (of a SwiGLU: half the columns) for each height of the shared tiles: 16, 32, 64, 80 and 128 rows.
+TILES = [(15, 65530), (30, 24600), (100, 8100), (150, 8100), (1020, 4090)]
+
+
+@pytest.mark.parametrize("kind,group,k", [("int4", 32, 160), ("int4", 64, 192), ("int4", 128, 384), ("mxfp4", 32, 224)])
+@pytest.mark.parametrize("m,n", TILES)
+def test_many_columns(dev, m, n, kind, group, k):
+    say("many columns", m, n, k, kind, group)
+    raw = random_weight(dev, n, k, kind, group, kind == "int4", seed=m)
+    x = bf16_randn(torch.Generator().manual_seed(k), (m, k)).to(dev)
+    bias = bf16_randn(torch.Generator().manual_seed(1), (n,)).to(dev)
+    w = pack(raw)
+    check(fourbit.matmul(x, w, bias=bias), *R.four_bit(x, *raw, bias=bias))
+    a, b = (tuple(None if t is None else t[h::2].contiguous() for t in raw) for h in (0, 1))
+    x = 0.3 * x
+    check(fourbit.swiglu(x, pack(a), pack(b)), *R.swiglu(R.four_bit(x, *a), R.four_bit(x, *b)))
+
+
 def test_every_code(dev):
     """A weight of each code alone, times powers of two: exact."""
     say("every code")
