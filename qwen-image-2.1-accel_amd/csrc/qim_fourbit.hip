@@ -273,45 +273,45 @@ static int launch_fourbit_ring(const FourBitArgs &a, hipStream_t st) {
     return QIM_OK;
 }
 
-// More rows: a workgroup of eight waves and 16 NR x 64 values of output; of each step of 128 k, staged in LDS, wave w takes
-// the k 32 (w % 4) .. + 31 for half of the columns, so that every code is made an operand once.  Two stages: one
-// multiplied, one on its way; a stage's 16-byte chunk c of row r of x lies at c ^ (r % 16), so that the 16 rows of an operand
-// lie in different banks.
-constexpr int FT_WAVES = 8, FT_NT = 4;  // 16-column tiles of W: two for each half of the waves
-template <int G, int NR>
+// More rows: a workgroup of WAVES = 8 or 4 waves and 16 NR x 64 or 32 values of output; of each step of 128 k, staged in LDS,
+// wave w takes the k 32 (w % 4) .. + 31 for 32 of the columns, so that every code is made an operand once.  Two
+// stages: one multiplied, one on its way (a third was slower: the step's chain of reads, operands and products holds it
+// up); a stage's 16-byte chunk c of row r of x lies at c ^ (r % 16), so that the 16 rows of an operand lie in different banks.
+template <int G, int NR, int WAVES>
 struct FtStage {
+    static constexpr int NT = WAVES / 2;  // 16-column tiles of W: two for each four waves
     static constexpr int SB = G ? 32 * G : 64, ZB = 16 * G;  // bytes of a tile's scales or exponents, and of its zero points
-    static constexpr int CODES = NR * 16 * 256, SCALES = CODES + FT_NT * 1024, ZEROS = SCALES + FT_NT * SB, BYTES = ZEROS + FT_NT * ZB;
+    static constexpr int CODES = NR * 16 * 256, SCALES = CODES + NT * 1024, ZEROS = SCALES + NT * SB, BYTES = ZEROS + NT * ZB;
     static constexpr int JOIN = 4 * 2 * NR * 64 * 16;        // four waves' partial sums of half of the output
     static constexpr int TABLES = 2 * BYTES > JOIN ? 2 * BYTES : JOIN, LDS = TABLES + (G ? 256 : 0);
 };
 
-template <int G, int NR, bool SWIGLU>
-__global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p, uint32_t ncol) {
-    using St = FtStage<G, NR>;
+template <int G, int NR, int WAVES, bool SWIGLU>
+__global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, uint32_t ncol) {
+    using St = FtStage<G, NR, WAVES>;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     uint4 *const tables = reinterpret_cast<uint4 *>(lds + St::TABLES);
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = wave & 3, half = wave >> 2;
     const uint32_t rowblock = blockIdx.x / ncol, col = blockIdx.x - rowblock * ncol;
     const int row0 = (int)rowblock * 16 * NR;
-    constexpr int OT = SWIGLU ? FT_NT / 2 : FT_NT;
+    constexpr int OT = SWIGLU ? St::NT / 2 : St::NT;
     if constexpr (G > 0) {
         if (tid < 16) tables[tid] = make_uint4(fb_table(tid, 0), fb_table(tid, 4), fb_table(tid, 8), fb_table(tid, 12));
     }
     // This wave's part of a stage: 1 KiB pieces of x, 4 rows each, and of tile j of W the codes (the first four waves) or the
     // scales and zero points.  Rows and tiles past the last are the last, and of k past the end others come: nothing
     // multiplies with them.
-    const int ntiles = (p.N + 15) / 16, mine = (int)col * OT + (SWIGLU ? j >> 1 : j);
-    const FourBitWeight &fw = p.w[SWIGLU ? j & 1 : 0];
+    const int ntiles = (p.N + 15) / 16, of = wave % St::NT, mine = (int)col * OT + (SWIGLU ? of >> 1 : of);
+    const FourBitWeight &fw = p.w[SWIGLU ? of & 1 : 0];
     const int64_t tile = mine < ntiles ? mine : ntiles - 1;
     const uint8_t *const x0 = reinterpret_cast<const uint8_t *>(p.x + row0 * p.ldx);
     const uint8_t *const wc = fw.codes + tile * p.KT * 1024, *const ws = fw.scales + tile * p.KT * St::SB;
     const uint8_t *const wz = G && fw.zeros ? fw.zeros + tile * p.KT * St::ZB : wc;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t *)lds;
-    constexpr int PIECES = (4 * NR + FT_WAVES - 1) / FT_WAVES;
+    constexpr int PIECES = (4 * NR + WAVES - 1) / WAVES;
     uint32_t xoff[PIECES];
-    auto piece = [&](int i) { return (wave + FT_WAVES * i) % (4 * NR); };  // (some come twice, where 2 does not divide NR)
+    auto piece = [&](int i) { return (wave + WAVES * i) % (4 * NR); };  // (some come twice, where 2 does not divide NR)
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
         const int r = 4 * piece(i) + kg, last = p.M - 1 - row0;
@@ -330,12 +330,12 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
             }
             fb_dma(xt, off, to + piece(i) * 1024);
         }
-        if (half == 0) {
-            fb_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + j * 1024);
+        if (wave < St::NT) {
+            fb_dma(wc + (int64_t)t * 1024, lane * 16, to + St::CODES + of * 1024);
         } else {
-            if (lane < St::SB / 16) fb_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + j * St::SB);
+            if (lane < St::SB / 16) fb_dma(ws + (int64_t)t * St::SB, lane * 16, to + St::SCALES + of * St::SB);
             if constexpr (G > 0) {
-                if (lane < St::ZB / 16) fb_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + j * St::ZB);
+                if (lane < St::ZB / 16) fb_dma(wz + (int64_t)t * St::ZB, lane * 16, to + St::ZEROS + of * St::ZB);
             }
         }
     };
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
     // The join, the columns of one half of the waves after those of the other.
     f32x4_t(*const part)[2 * NR][64] = reinterpret_cast<f32x4_t(*)[2 * NR][64]>(lds);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < WAVES / 4; ++h) {
         __syncthreads();
         if (half == h) {
 #pragma unroll
@@ -404,8 +404,8 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
         __syncthreads();
         constexpr int BLOCKS = SWIGLU ? NR : 2 * NR;
 #pragma unroll
-        for (int i = 0; i < (BLOCKS + FT_WAVES - 1) / FT_WAVES; ++i) {
-            const int blk = wave + FT_WAVES * i, ot = SWIGLU ? 0 : blk / NR, r = blk - ot * NR;
+        for (int i = 0; i < (BLOCKS + WAVES - 1) / WAVES; ++i) {
+            const int blk = wave + WAVES * i, ot = SWIGLU ? 0 : blk / NR, r = blk - ot * NR;
             if (blk >= BLOCKS) break;
             f32x4_t y = {}, u = {};
 #pragma unroll
@@ -413,53 +413,70 @@ __global__ __launch_bounds__(64 * FT_WAVES, 4) void k_fourbit_tile(FourBitArgs p
                 y += part[v][blk][lane];
                 if (SWIGLU) u += part[v][NR + blk][lane];
             }
-            const int64_t n0 = ((int64_t)col * OT + h * (OT / 2) + ot) * 16 + 4 * kg;
+            const int64_t n0 = ((int64_t)col * OT + h * (SWIGLU ? 1 : 2) + ot) * 16 + 4 * kg;
             const int row = row0 + 16 * r + lr;
             if (row < p.M && n0 < p.N) fb_store<SWIGLU>(p, row, n0, y, u);
         }
     }
 }
 
-template <int G, int NR, bool SWIGLU>
+template <int G, int NR, int WAVES, bool SWIGLU>
 static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
-    constexpr int OT = SWIGLU ? FT_NT / 2 : FT_NT, bytes = FtStage<G, NR>::LDS;
+    using St = FtStage<G, NR, WAVES>;
+    constexpr int OT = SWIGLU ? St::NT / 2 : St::NT, bytes = St::LDS;
     static std::atomic<bool> done[QIM_MAX_DEVICES];
     if (bytes > 65536) {
-        const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit_tile<G, NR, SWIGLU>), bytes, done, "qim_fourbit_matmul");
+        const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit_tile<G, NR, WAVES, SWIGLU>), bytes, done, "qim_fourbit_matmul");
         if (rc != QIM_OK) return rc;
     }
     const uint32_t ncol = (uint32_t)(((a.N + 15) / 16 + OT - 1) / OT);
-    launch(k_fourbit_tile<G, NR, SWIGLU>, dim3(ncol * (unsigned)((a.M + 16 * NR - 1) / (16 * NR))), dim3(64 * FT_WAVES), bytes, st, a, ncol);
+    launch(k_fourbit_tile<G, NR, WAVES, SWIGLU>, dim3(ncol * (unsigned)((a.M + 16 * NR - 1) / (16 * NR))), dim3(64 * WAVES), bytes, st, a, ncol);
     return QIM_OK;
 }
 
 // Which kernel.  At 4096 columns of x (and alike at others) the tile kernel takes about 12.5 us and 3.5 + 2.75 NR more for each
-// workgroup that a CU has to take, the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16: the first is held up
-// by the barrier of its steps while it has a workgroup or two a CU, the other makes operands of all codes again for every 16 rows.
-// int4, group 64, tile against ring: 32 x 4096 18.2 us and 9.7, 64 x 4096 18.3 and 12.7, 128 x 4096 19.3 and 21.7,
-// 24 x 24576 26.0 and 33.1, 16 x 65536 44.4 and 48.2; mxfp4: 64 x 4096 17.1 and 8.9, 16 x 65536 31.7 and 39.0.
+// workgroup of eight waves that a CU has to take, the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16: the
+// first is held up by the chain of its steps while a CU has few workgroups, the other makes operands of all codes again for
+// every 16 rows.  int4, group 64, tile against ring: 32 x 4096 18.2 us and 9.7, 64 x 4096 18.3 and 12.7, 128 x 4096 19.3 and
+// 21.7, 24 x 24576 26.0 and 33.1, 16 x 65536 44.4 and 48.2; mxfp4: 64 x 4096 17.1 and 8.9, 16 x 65536 31.7 and 39.0.
+// Up to one and a half workgroups of eight waves a CU int4 takes workgroups of four instead, which divide the CUs more evenly and
+// wait for fewer at a barrier (us, eight waves and four: 24 x 12288 SwiGLU 26.6, 23.8; 154 x 12288, group 32, 39.8, 35.1; 128 x
+// 4096 20.3, 18.0; but 300 x 12288, three a CU, 60.9 and 67.4, and mxfp4 154 x 12288 24.4 and 25.5).
 template <int G, bool SWIGLU>
 static int launch_fourbit(const FourBitArgs &a, hipStream_t st) {
-    constexpr int ONE = SWIGLU ? 2 : 1, OT = SWIGLU ? FT_NT / 2 : FT_NT;
+    constexpr int ONE = SWIGLU ? 2 : 1, OT = 4 / ONE;
     if (a.M <= 4) return launch_fourbit_ring<G, ONE, 1, 8, 3, SWIGLU>(a, st);
     const int64_t ntiles = (a.N + 15) / 16, ncol = (ntiles + OT - 1) / OT;
-    auto cost = [&](int nr) { return (ncol * ((a.M + 16 * nr - 1) / (16 * nr)) + 255) / 256 * (10 * nr + 13); };  // of 0.275 us
+    auto wgs = [&](int nr) { return ncol * ((a.M + 16 * nr - 1) / (16 * nr)); };  // of eight waves
+    auto four = [&](int nr) { return G > 0 && nr > 1 && nr < 8 && wgs(nr) <= 384; };
+    auto cost = [&](int nr) {  // of 0.14 us; (four waves on a CU issue no faster than half of eight do)
+        return (four(nr) && wgs(nr) > 256 ? 3 : (wgs(nr) + 255) / 256 * 2) * (10 * nr + 13);
+    };
     int nr = 8;
     for (int n : {5, 4, 2, 1})
         if (cost(n) < cost(nr)) nr = n;
     const int64_t blocks = (a.M + 15) / 16 * ntiles;
-    if (a.M <= 16 * 65535 && 10 * ONE * blocks < 256 * (35 + cost(nr))) {  // (a grid of no more than 65535 blocks of rows)
+    if (a.M <= 16 * 65535 && 20 * ONE * blocks < 256 * (70 + cost(nr))) {  // (a grid of no more than 65535 blocks of rows)
         // From one and a half tiles a CU on two of them share the reads of x, and two workgroups of four waves a CU take more of
         // them at a time (16 rows, mxfp4: 4096 -> 12288 9.2 us against 11.6; 12288 -> 4096, 256 tiles, 14.6 against 9.0).
         if (blocks >= 384) return launch_fourbit_ring<G, 2, 4, 4, 3, SWIGLU>(a, st);
         return launch_fourbit_ring<G, ONE, 4, 8, 2, SWIGLU>(a, st);
     }
+    if constexpr (G > 0) {
+        if (four(nr)) {
+            switch (nr) {
+                case 2: return launch_fourbit_tile<G, 2, 4, SWIGLU>(a, st);
+                case 4: return launch_fourbit_tile<G, 4, 4, SWIGLU>(a, st);
+                default: return launch_fourbit_tile<G, 5, 4, SWIGLU>(a, st);
+            }
+        }
+    }
     switch (nr) {
-        case 1: return launch_fourbit_tile<G, 1, SWIGLU>(a, st);
-        case 2: return launch_fourbit_tile<G, 2, SWIGLU>(a, st);
-        case 4: return launch_fourbit_tile<G, 4, SWIGLU>(a, st);
-        case 5: return launch_fourbit_tile<G, 5, SWIGLU>(a, st);
-        default: return launch_fourbit_tile<G, 8, SWIGLU>(a, st);
+        case 1: return launch_fourbit_tile<G, 1, 8, SWIGLU>(a, st);
+        case 2: return launch_fourbit_tile<G, 2, 8, SWIGLU>(a, st);
+        case 4: return launch_fourbit_tile<G, 4, 8, SWIGLU>(a, st);
+        case 5: return launch_fourbit_tile<G, 5, 8, SWIGLU>(a, st);
+        default: return launch_fourbit_tile<G, 8, 8, SWIGLU>(a, st);
     }
 }
 
