@@ -546,9 +546,6 @@ struct SaPlan {
                (shared ? up(vp * 16) + up(B * 4) + up(B * 8) : 0);
     }
 };
-#ifndef SA_ROUNDS
-#define SA_ROUNDS 1
-#endif
 static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P, bool shared) {
     SaPlan pl;
     const int64_t sg = S * (H / HK), rows = B * sg, cus = device_cus() > 0 ? device_cus() : 256;
@@ -568,16 +565,13 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     // Several prefixes: each may end with a tile that is not full.
     pl.vp = (rows + pl.tr - 1) / pl.tr + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
     const int64_t bp = (CP + pl.keys - 1) / pl.keys, bo = (C + CA_KB - 1) / CA_KB;
-    // Work in ns of a workgroup, two to a CU.
-#ifndef SA_T
-#define SA_T 2300, 1400, 1000, 1500
-#endif
-    constexpr int64_t T[4] = {SA_T};
-    const int64_t tp = bp * pl.vp * pl.wp * (pl.rg == 4 ? T[0] : pl.rg == 2 ? T[1] : pl.np == 1 ? T[2] : T[3]), to = bo * pl.vo * pl.wo * (pl.no == 1 ? T[2] : T[3]);
-    const int64_t slots = 2 * SA_ROUNDS * cus;
+    // The pieces of both spaces together: two workgroups a CU, divided by the time that the spaces' blocks take one
+    // (measured: 1.0 and 1.5 us for a wave's 16 and 32 rows, 1.4 and 2.3 us for tiles of 64 and 128).
+    const double wave[2] = {1.0, 1.5};
+    const double tp = (double)bp * pl.vp * pl.wp * (pl.rg == 4 ? 2.3 : pl.rg == 2 ? 1.4 : wave[pl.np - 1]), to = (double)bo * pl.vo * pl.wo * wave[pl.no - 1];
     // At least a piece a sequence (also where a space holds no keys: its first workgroup writes dir), at most one a block.
-    auto pieces = [&](int64_t w, int64_t v, int64_t blocks, int64_t wide) {
-        int64_t n = (slots * w / (tp + to > 0 ? tp + to : 1) + wide / 2) / wide;
+    auto pieces = [&](double w, int64_t v, int64_t blocks, int64_t wide) {
+        int64_t n = (int64_t)(2 * cus * w / (tp + to) / wide + 0.5);
         const int64_t most = v * blocks;
         if (n < 4 * v) n = n / v * v;  // (whole pieces of sequences that are alike)
         return n < v || most < v ? v : n < most ? n : most;
