@@ -16,8 +16,9 @@
 // Two kernels.  k_fourbit, few rows or few columns: the waves of a workgroup take the steps of k in turn, each for the whole
 // tile of output and through a ring in LDS of its own, and join at the end; no barrier stands in the loop.  k_fourbit_tile,
 // the others: stages in LDS that eight waves share, and up to 128 rows for every operand made of codes.
-// Measured (weights in HBM, launches from a graph), int4 g 128, 1 row, 4096 -> 12288: 9.5 us; mxfp4, 16 rows, 12288 -> 4096: 8.9 us;
-// int4 g 32, 154 rows, 4096 -> 12288: 39.9 us, 390 TFLOP/s; mxfp4, 1024 rows, 4096 -> 4096: 37.6 us, 914 TFLOP/s.
+// Measured (launches from a graph): int4 g 128, 1 row, 4096 -> 12288 9.1-9.9 us, 2.6 TB/s; mxfp4, 16 rows, 12288 -> 4096 8.9 us, 2.8
+// TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 24.0 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430 TFLOP/s; mxfp4, 1024
+// rows, 4096 -> 4096 38 us, 900 TFLOP/s.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int g = 0; g < G; ++g) tab[i][g] = tables[(z[i] >> (8 * g)) & 0xffu];
+                for (int g = 0; g < G; ++g) tab[i][g] = tables[(z[i] >> (8 * g)) & 15u];
         }
         __builtin_amdgcn_sched_barrier(0);  // all reads are on their way before the first result is used
         const int left = p.K - 128 * step(n);  // of k: whole groups, a step but for the last
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
 #pragma unroll
         for (int r = 0; r < NR; ++r) acc[i][r] = f32x4_t{};
     const int g = G ? j * G / 4 : 0;  // the group of this wave's k
-    const uint32_t zmask = fw.zeros ? 0xffu : 0u, znone = fw.zeros ? 0u : 8u;
+    const uint32_t zmask = fw.zeros ? 15u : 0u, znone = fw.zeros ? 0u : 8u;
     issue(0, 0);
     for (int t = 0; t < p.KT; ++t) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stage is there, the other has been read

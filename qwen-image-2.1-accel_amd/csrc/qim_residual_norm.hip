@@ -12,7 +12,9 @@
 //
 // Memory-bound: 8 bytes an element (7.03 with MXFP8) for about 20 vector operations.  A workgroup takes a
 // row; its lanes hold their 16-byte vectors of the row in registers from the loads to the stores, so the
-// reductions between (one for post, one for norm) cost no second read.
+// reductions between (one for post, one for norm) cost no second read.  Measured at D 4096: 2048 rows with gate, scale and
+// shift 14 us, 4.8 TB/s; 16384 rows with a norm on both sides 109-112 us, 4.8-4.9 TB/s, of the 5.1 that a 1 GiB copy reaches;
+// 16 rows 4.1 us, a launch and two reductions.
 #include "qim_device.h"
 #include "qim_runtime.h"
 

@@ -7,6 +7,11 @@
 // that a prefix's codes are read and converted once for a tile of rows instead of once for every request.  Prefix and own
 // keys give partial results (numerator, maximum, sum; fp32) over chunks of keys, joined in a last launch.
 //
+// Few rows: the cache's bytes and the launches' starts bound it; from some 64 rows on the vector instructions of the softmax and
+// the conversions, beside the matrix products.  Measured (launches from a graph): 4 requests, one row each on 32 heads, 1101 +
+// 96 keys 13.2 us (8.6 and the join's 4.9); 32 requests of 4 rows on 8 heads, 8392 + 1024 keys 30 us; 48 requests on 5
+// prefixes of up to 32768 keys 87 us, 3.6 TB/s; 8 requests of 24 rows on 32 heads, 8392 + 256 keys 74 us, 363 TFLOP/s.
+//
 // The rows of a prefix: its requests in the order of their numbers, S * G rows each.  Which requests those are is known on
 // the device only, so where a batch has several prefixes a first launch of one workgroup lists them.
 #include "qim_cache_attention.h"
