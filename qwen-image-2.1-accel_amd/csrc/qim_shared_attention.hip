@@ -10,7 +10,7 @@
 // Few rows: the cache's bytes and the launches' starts bound it; from some 64 rows on the vector instructions of the softmax and
 // the conversions, beside the matrix products.  Measured (launches from a graph): 4 requests, one row each on 32 heads, 1101 +
 // 96 keys 13.2 us (8.6 and the join's 4.9); 32 requests of 4 rows on 8 heads, 8392 + 1024 keys 30 us; 48 requests on 5
-// prefixes of up to 32768 keys 87 us, 3.6 TB/s; 8 requests of 24 rows on 32 heads, 8392 + 256 keys 74 us, 363 TFLOP/s.
+// prefixes of up to 32768 keys 88 us, 3.5 TB/s; 8 requests of 24 rows on 32 heads, 8392 + 256 keys 73 us, 370 TFLOP/s.
 //
 // The rows of a prefix: its requests in the order of their numbers, S * G rows each.  Which requests those are is known on
 // the device only, so where a batch has several prefixes a first launch of one workgroup lists them.
@@ -222,16 +222,19 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_attn(SaArgs p) {
 }
 
 // Many rows to a prefix: a workgroup of four waves takes 32 RG rows and blocks of 64 keys; a wave 32 rows and, of each
-// block, all keys (RG 4) or one half of them (RG 2).  The block's codes become bf16 once, in LDS (two buffers; K with
-// 16-byte chunk c of key r at c ^ (r % 16), V with 32-byte unit n of key r at n ^ (r % 8), for the transposing reads),
-// where the wave above converts for 16 or 32 rows of its own.  Two blocks are on their way in registers.  Waves of the same
-// rows join in LDS.
-constexpr int ST_KEYS = 64, ST_BUF = ST_KEYS * 512;                       // bytes of K and V of a block
-constexpr int ST_LDS = 2 * ST_BUF;                                        // (also the join's: 2 waves x 16.25 KiB)
+// block, all keys (RG 4) or one half of them (RG 2).  The block's codes become bf16 once, in LDS, where the wave above
+// converts for 16 or 32 rows of its own.  RG 2, bound by memory: two buffers, two blocks on their way in registers, two
+// workgroups a CU; waves of the same rows join in LDS.  RG 4, bound by the instructions that a wave issues one after
+// the other: one buffer and one block on its way, so that three workgroups' registers fit a CU; a request's own keys
+// go in tiles of 16 rows there, which fit too (with two of everything, us: 96 rows of 32 heads over 8392 keys 61 for
+// 46; 128 of 8 heads over 32768 59 for 49; but 64-row tiles of one buffer 93 for 87 over five long prefixes).
+// Rows of K are 16 bytes longer than a key, of V 32: a K operand's 16 rows, and the 8 rows that half a wave reads
+// transposed, lie in different banks, and every read is one address and a constant.
+constexpr int ST_KEYS = 64, ST_K = 2 * CA_D + 16, ST_V = 2 * CA_D + 32, ST_VAT = ST_KEYS * ST_K, ST_BUF = ST_VAT + ST_KEYS * ST_V;
 template <int RG, int NO>
-__global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
-    constexpr int KQ = 4 / RG;                                            // waves of the same rows
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[ST_LDS];
+__global__ __launch_bounds__(64 * SA_WAVES, RG == 4 ? 3 : 2) void k_shared_tile(SaArgs p) {
+    constexpr int KQ = 4 / RG, DEPTH = RG == 4 ? 1 : 2;                   // waves of the same rows; buffers
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];      // DEPTH * ST_BUF
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), rg = wave % RG, kq = wave / RG;
     if (blockIdx.x >= p.pre.blocks) {
@@ -283,9 +286,9 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[t][j] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * (j >> 1) + 8 * (j & 1));
     }
-    Raw raw[2];
-    load(raw[0], blk0);
-    load(raw[1], blk0 + 1);
+    Raw raw[DEPTH];
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) load(raw[i], blk0 + i);
     // Q is waited for here: a wait inside the loop would be one for all loads before the last, the second block's too.
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -303,22 +306,18 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
     const bool idle = tile.row0 + 32 * rg >= tile.rows;  // no rows of this wave's: it only converts
     // Places of this lane's operands in a buffer: K's chunks of row lr, V's units of key 4 kg + lr / 4.
     const int vkey = 4 * kg + (lr >> 2);
-    uint32_t kat[4], vat[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) kat[j] = (32 * kq + lr) * 256 + (((8 * (j >> 1) + 2 * kg + (j & 1)) ^ lr) << 4);
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) vat[dt] = ST_KEYS * 256 + (32 * kq + vkey) * 256 + (lr & 3) * 8 + ((dt ^ (vkey & 7)) << 5);
+    const uint8_t *const kat = lds + (32 * kq + lr) * ST_K + 32 * kg;
+    const uint32_t vat = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds + ST_VAT + (32 * kq + vkey) * ST_V + (lr & 3) * 8;
     typedef __attribute__((address_space(3))) i16x4_t *tr_t;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     auto convert = [&](const Raw &w, int blk, int buf) {
         const int live = len - (int64_t)blk * ST_KEYS < ST_KEYS ? (int)(len - (int64_t)blk * ST_KEYS) : ST_KEYS;
-        uint8_t *const kb = lds + buf * ST_BUF, *const vb = kb + ST_KEYS * 256;
+        uint8_t *const kb = lds + buf * ST_BUF + ck * ST_K + 32 * cc, *const vb = lds + buf * ST_BUF + ST_VAT + ck * ST_V + 32 * cc;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int key = 32 * i + ck;
             const float ks = mx_scale_operand((int)w.ke[i]);
-            *reinterpret_cast<bf16x8_t *>(kb + key * 256 + (((2 * cc) ^ (key & 15)) << 4)) = ca_operand(w.k[i].x, w.k[i].y, ks);
-            *reinterpret_cast<bf16x8_t *>(kb + key * 256 + (((2 * cc + 1) ^ (key & 15)) << 4)) = ca_operand(w.k[i].z, w.k[i].w, ks);
+            *reinterpret_cast<bf16x8_t *>(kb + 32 * i * ST_K) = ca_operand(w.k[i].x, w.k[i].y, ks);
+            *reinterpret_cast<bf16x8_t *>(kb + 32 * i * ST_K + 16) = ca_operand(w.k[i].z, w.k[i].w, ks);
             uint4 x = w.v[i];
             uint32_t e = w.ve[i];
             if (key >= live) {  // V past the last key is zeros, whatever the cache holds there
@@ -326,19 +325,18 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
                 e = 0;
             }
             const float vs = mx_scale_operand((int)e);
-            uint8_t *at = vb + key * 256 + ((cc ^ (key & 7)) << 5);
-            *reinterpret_cast<bf16x8_t *>(at) = ca_operand(x.x, x.y, vs);
-            *reinterpret_cast<bf16x8_t *>(at + 16) = ca_operand(x.z, x.w, vs);
+            *reinterpret_cast<bf16x8_t *>(vb + 32 * i * ST_V) = ca_operand(x.x, x.y, vs);
+            *reinterpret_cast<bf16x8_t *>(vb + 32 * i * ST_V + 16) = ca_operand(x.z, x.w, vs);
         }
     };
     // 32 keys of the block in a buffer, the wave's first or (RG 4) second 32, for its 32 rows; `left` keys are there.
-    auto attend = [&](int place, int64_t left) {
+    auto attend = [&](int buf, int half, int64_t left) {
         f32x4_t s[2][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(lds + kat[j] + (place + u * 4096));
+                const bf16x8_t kf = *reinterpret_cast<const bf16x8_t *>(kat + (buf * ST_BUF + (32 * half + 16 * u) * ST_K + 128 * (j >> 1) + 16 * (j & 1)));
 #pragma unroll
                 for (int t = 0; t < 2; ++t) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][j], j == 0 ? f32x4_t{} : s[t][u], 0, 0, 0);
             }
@@ -383,9 +381,9 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         }
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            const uint32_t at = lds0 + vat[dt] + place;
+            const uint32_t at = vat + (buf * ST_BUF + 32 * half * ST_V + 32 * dt);
             const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tr_t>((uintptr_t)at));
-            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tr_t>((uintptr_t)(at + 16 * CA_D * 2)));
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<tr_t>((uintptr_t)(at + 16 * ST_V)));
             const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -395,19 +393,21 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         }
     };
     auto block = [&](Raw &w, int blk, int buf) {
+        if (DEPTH == 1) __syncthreads();  // the block before has been read
         convert(w, blk, buf);
+        if (DEPTH == 1) load(w, blk + 1);
         __syncthreads();
-        load(w, blk + 2);
+        if (DEPTH == 2) load(w, blk + 2);
         if (idle) return;
 #pragma unroll
         for (int i = 0; i < 2 / KQ; ++i) {
             const int64_t left = len - ((int64_t)blk * ST_KEYS + 32 * (kq + i));
-            if (left > 0) attend(buf * ST_BUF + i * (32 * 256), left);
+            if (left > 0) attend(buf, i, left);
         }
     };
-    for (int blk = blk0; blk < blk1; blk += 2) {
+    for (int blk = blk0; blk < blk1; blk += DEPTH) {
         block(raw[0], blk, 0);
-        if (blk + 1 < blk1) block(raw[1], blk + 1, 1);
+        if (DEPTH == 2 && blk + 1 < blk1) block(raw[DEPTH - 1], blk + 1, 1);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -451,6 +451,18 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void k_shared_tile(SaArgs p) {
         for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4_t *>(dst + 16 * dt) = o[t][dt];
         if (kg == 0) p.pre.part_ml[at] = make_float2(m[t], l[t]);
     }
+}
+
+template <int RG, int NO>
+static int launch_shared_tile(const SaArgs &a, dim3 grid, hipStream_t st) {
+    constexpr int bytes = (RG == 4 ? 1 : 2) * ST_BUF;
+    static std::atomic<bool> done[QIM_MAX_DEVICES];
+    if (bytes > 65536) {
+        const int rc = reserve_lds(reinterpret_cast<const void *>(k_shared_tile<RG, NO>), bytes, done, "qim_attention_shared");
+        if (rc != QIM_OK) return rc;
+    }
+    launch(k_shared_tile<RG, NO>, grid, dim3(64 * SA_WAVES), bytes, st, a);
+    return QIM_OK;
 }
 
 // Join the pieces of a row: GP groups of 32 lanes (4 head dims each) take them in turn, four loads at a time, and join in
@@ -562,7 +574,7 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     pl.np = each > 16 ? 2 : 1;
     pl.tr = pl.rg ? 32 * pl.rg : 16 * pl.np;
     pl.keys = pl.rg ? ST_KEYS : CA_KB;
-    pl.no = sg > 16 ? 2 : 1;
+    pl.no = sg > 16 && pl.rg != 4 ? 2 : 1;
     pl.wo = (HK + SA_WAVES - 1) / SA_WAVES;
     pl.wp = pl.rg ? HK : pl.wo;
     pl.ntile = (sg + 16 * pl.no - 1) / (16 * pl.no);
@@ -571,16 +583,21 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     pl.vp = (rows + pl.tr - 1) / pl.tr + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
     const int64_t bp = (CP + pl.keys - 1) / pl.keys, bo = (C + CA_KB - 1) / CA_KB;
     // The pieces of both spaces together: two workgroups a CU, divided by the time that the spaces' blocks take one
-    // (measured: 1.0 and 1.5 us for a wave's 16 and 32 rows, 1.4 and 2.3 us for tiles of 64 and 128).
+    // (measured: 1.0 and 1.5 us for a wave's 16 and 32 rows, 1.4 and 2.3 us for tiles of 64 and 128).  Three of a CU's
+    // workgroups of 128 rows run at once; a third pays where a piece stays long beside its start and its results (8392 keys,
+    // requests of 24 rows on 32 heads, two and three a CU: 6 requests 73.8 and 68.8 us, 12 104 and 95.5; 4, pieces of 6 blocks,
+    // 46.4 and 48.9; 32 of 4 rows on 8 heads over 32768 keys 49.4 and 51.1).
     const double wave[2] = {1.0, 1.5};
     const double tp = (double)bp * pl.vp * pl.wp * (pl.rg == 4 ? 2.3 : pl.rg == 2 ? 1.4 : wave[pl.np - 1]), to = (double)bo * pl.vo * pl.wo * wave[pl.no - 1];
+    int64_t wgs = pl.rg == 4 ? 3 : 2;
     // At least a piece a sequence (also where a space holds no keys: its first workgroup writes dir), at most one a block.
     auto pieces = [&](double w, int64_t v, int64_t blocks, int64_t wide) {
-        int64_t n = (int64_t)(2 * cus * w / (tp + to) / wide + 0.5);
+        int64_t n = (int64_t)(wgs * cus * w / (tp + to) / wide + 0.5);
         const int64_t most = v * blocks;
         if (n < 4 * v) n = n / v * v;  // (whole pieces of sequences that are alike)
         return n < v || most < v ? v : n < most ? n : most;
     };
+    if (pl.rg == 4 && bp * pl.vp < 10 * pieces(tp, pl.vp, bp, pl.wp)) wgs = 2;
     pl.gp = pieces(tp, pl.vp, bp, pl.wp);
     pl.go = pieces(to, pl.vo, bo, pl.wo);
     return pl;
@@ -661,8 +678,8 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
     if (share) launch(k_shared_plan, dim3(1), dim3(1024), (size_t)(8 * P), st, a);
     const dim3 grid(a.pre.blocks + a.own.blocks);
     if (pl.rg) {
-        launch(pl.rg == 4 ? (pl.no == 2 ? k_shared_tile<4, 2> : k_shared_tile<4, 1>) : (pl.no == 2 ? k_shared_tile<2, 2> : k_shared_tile<2, 1>), grid,
-               dim3(64 * SA_WAVES), 0, st, a);
+        const int rc = pl.rg == 4 ? launch_shared_tile<4, 1>(a, grid, st) : pl.no == 2 ? launch_shared_tile<2, 2>(a, grid, st) : launch_shared_tile<2, 1>(a, grid, st);
+        if (rc != QIM_OK) return rc;
     } else {
         launch(pl.np == 2 ? (pl.no == 2 ? k_shared_attn<2, 2> : k_shared_attn<2, 1>) : (pl.no == 2 ? k_shared_attn<1, 2> : k_shared_attn<1, 1>),
                grid, dim3(64 * SA_WAVES), 0, st, a);
