@@ -186,14 +186,14 @@ def attention_shared(q, prefix, cache, lengths, *, share=None, prefix_lengths=No
             refuse(f"tree is a contiguous bool ({b}, {s}, {s}) or ({s}, {s}) tensor on {device}")
         mask, mask_b = tree.data_ptr(), s * s if tree.dim() == 3 else 0
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != torch.bfloat16 or out.shape != shape or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous bf16 {tuple(shape)} tensor on {device}")
     if not (b and s and h):
         return out
     own = [(t if c else u).data_ptr() for t, u in zip(cache, prefix)]   # an empty cache has no address; it is not read
     nbytes = _native.bytes_on(device, "qim_attention_shared_workspace_bytes", b, s, cp, c, h, kv, p, int(share is not None))
-    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    ws = q.new_empty(max(nbytes, 16), dtype=torch.uint8)
     _native.call_on(device, "qim_attention_shared", q.data_ptr(), *strides, *(t.data_ptr() for t in prefix), psize, which,
                     *own, size, mask, mask_b, out.data_ptr(), ws.data_ptr(), nbytes, b, s, p, cp, c, h, kv, d,
                     float(scale if scale is not None else d ** -0.5))

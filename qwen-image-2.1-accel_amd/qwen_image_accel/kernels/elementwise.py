@@ -102,14 +102,14 @@ def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale
     norm_kind, norm_w, norm_eps = _norm_of(norm, d, device, refuse)
     vectors = vector(gate) + vector(scale) + vector(shift)
     if out is None:
-        out, ldo = torch.empty(shape, dtype=torch.bfloat16, device=device), d
+        out, ldo = torch.empty_like(h, memory_format=torch.contiguous_format), d
     else:
         ldo = rows(out)[2]
     if quantized:
         z = empty_quantized(m, d, device, shape, tiled)
         z_ptr, z_scales = z.values.data_ptr(), z.scales.data_ptr()
     else:
-        z = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        z = torch.empty_like(h, memory_format=torch.contiguous_format)
         z_ptr, z_scales = z.data_ptr(), None
     if m == 0 or d == 0:
         return out, z

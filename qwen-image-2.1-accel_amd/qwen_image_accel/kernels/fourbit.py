@@ -201,7 +201,7 @@ def _product(name, x, first, second, bias, out, dtype):
         refuse(f"bias is a contiguous bf16 ({n},) tensor on {device}")
     shape = x.shape[:-1] + (n,)
     if out is None:
-        out, ldo = torch.empty(shape, dtype=dtype, device=device), n
+        out, ldo = x.new_empty(shape, dtype=dtype), n
     else:
         o = row_layout(out) if out.dtype == dtype and out.shape == shape and out.device == device else None
         if o is None:
