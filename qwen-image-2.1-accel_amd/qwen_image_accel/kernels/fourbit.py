@@ -155,7 +155,7 @@ def quantize_weight(w, kind="int4", group=64, *, symmetric=False):
         q = torch.where(s > 0, torch.round(g / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(g)).clamp(-8, 7) + 8
     else:
         lo, hi = g.amin(-1, keepdim=True).clamp(max=0), g.amax(-1, keepdim=True).clamp(min=0)
-        scales = ((hi - lo) / 15).squeeze(-1).to(torch.bfloat16)
+        scales = (hi / 15 - lo / 15).squeeze(-1).to(torch.bfloat16)   # (the span itself may pass fp32's range)
         s = scales.float().unsqueeze(-1)
         s = torch.where(s > 0, s, torch.ones_like(s))
         z = torch.round(-lo / s).clamp(0, 15)
@@ -170,7 +170,7 @@ def _check_weight(name, w, device):
     by_row = (tiles, steps, TILE, per)
     shape = by_row if w.scales.dtype == torch.uint8 else (tiles, steps, 4, per, 4)
     if not (per and w.rows > 0 and w.width > 0 and w.codes.shape == (tiles, steps, 64, 16) and w.codes.dtype == torch.uint8
-            and w.scales.shape == shape and w.scales.dtype in (torch.bfloat16, torch.uint8)
+            and w.scales.shape == shape and (w.scales.dtype == torch.bfloat16 or w.scales.dtype == torch.uint8 and w.group == MX_GROUP)
             and (w.zeros is None or (w.zeros.shape == by_row and w.zeros.dtype == torch.uint8 and w.scales.dtype == torch.bfloat16))
             and all(t is None or (t.device == device and t.is_contiguous()) for t in w[:3])):
         raise _native.Unsupported(name, _native.QIM_ERR_LAYOUT, f"expects a FourBitWeight of pack_weight or quantize_weight on {device}")
@@ -218,7 +218,7 @@ def matmul(x, weight, *, bias=None, out=None, dtype=torch.bfloat16):
     """``x @ W.T (+ bias)``: x (M, K) or (B, S, K) bf16 on the GPU, rows any multiple of 8 elements apart; W a
     ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if given (any row
     stride, apart from x).  The weights enter exactly, sums are fp32, the result is rounded once.  Meant for up to some hundred
-    rows; it takes any number.  No gradient is recorded."""
+    rows; it takes fewer than 2^20.  No gradient is recorded."""
     return _product("fourbit.matmul", x, weight, None, bias, out, dtype)
 
 

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from qwen_image_accel import _native
 from qwen_image_accel.kernels import fourbit
 
 
@@ -98,3 +99,24 @@ def test_refusals():
     for args in ((w, "int4", 64), (w, "int4", 48), (w, "nf4"), (w[0], "mxfp4"), (w[:, :40], "mxfp4"), (w * float("inf"), "mxfp4")):
         with pytest.raises(ValueError):
             fourbit.quantize_weight(*args)
+
+
+def test_a_weight_put_together_by_hand_is_checked():
+    """Sizes that do not belong to the tensors are refused before any address reaches a kernel."""
+    mx = fourbit.quantize_weight(torch.randn(20, 256), "mxfp4")
+    w = fourbit.quantize_weight(torch.randn(20, 256), "int4", 64)
+    cpu = mx.codes.device
+    fourbit._check_weight("test", mx, cpu), fourbit._check_weight("test", w, cpu)
+    wrong = [mx._replace(group=64), mx._replace(group=64, scales=mx.scales[..., :2].contiguous()), mx._replace(width=384), mx._replace(rows=33),
+             mx._replace(zeros=mx.scales), mx._replace(codes=mx.codes.transpose(0, 1)), w._replace(group=32), w._replace(group=48),
+             w._replace(rows=0), w._replace(scales=w.scales.view(torch.int16)), w._replace(zeros=w.zeros[..., :1])]
+    for bad in wrong:
+        with pytest.raises(_native.Unsupported):
+            fourbit._check_weight("test", bad, cpu)
+
+
+def test_a_group_whose_span_passes_fp32():
+    g = torch.zeros(16, 64)
+    g[:, 0], g[:, 1] = 3e38, -3e38
+    back = fourbit.dequantize_weight(fourbit.quantize_weight(g, "int4", 64))
+    assert back.isfinite().all() and (back - g).abs().max() <= 2.1e37   # half a step of 4e37 and the scale's own rounding, 2^-9 of 15 / 2 steps
