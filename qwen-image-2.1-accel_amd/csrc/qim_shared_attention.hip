@@ -351,13 +351,13 @@ __global__ __launch_bounds__(64 * SA_WAVES, RG == 4 ? 3 : 2) void k_shared_tile(
             }
             float mx = ca_max(ca_max(ca_max(s[t][0][0], s[t][0][1]), ca_max(s[t][0][2], s[t][0][3])),
                               ca_max(ca_max(s[t][1][0], s[t][1][1]), ca_max(s[t][1][2], s[t][1][3])));
-            // m follows the row's maximum when a score has passed it by more than 2^8 (in a row of the wave's, then in
-            // all of them): till then p is at most 2^8, which numerator and sum hold as well.
+            // m follows the row's maximum when a score has passed it by more than 2^8: till then p is at most 2^8, which
+            // numerator and sum hold as well.
             mx *= c;
             if (__builtin_amdgcn_ballot_w64(!(mx <= m[t] + 8.0f))) {
                 const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
                 mx = ca_swap_max(ca_max(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
-                const float mn = ca_max(m[t], mx);
+                const float mn = mx <= m[t] + 8.0f ? m[t] : ca_max(m[t], mx);  // (this row's own need, whoever else asked)
                 const float alpha = __builtin_amdgcn_exp2f(m[t] - (mn == ninf ? 0.f : mn));
                 m[t] = mn;
                 l[t] *= alpha;

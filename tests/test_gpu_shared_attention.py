@@ -114,6 +114,49 @@ def test_no_own_keys(dev):
     assert ((out.double().cpu() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("b", [3, 14, 20, 70])
+@pytest.mark.parametrize("falling", [False, True])
+def test_scores_that_rise_or_fall_along_the_keys(dev, b, falling):
+    """The row's maximum moves with every block of keys, by less and by more than what the sums leave room for."""
+    say("rising", b, falling)
+    h, hk, cp, c = 6, 2, 700, 40
+    q, prefix, cache = make(dev, b, 1, h, hk, 1, cp, c, seed=b)
+    g = torch.Generator().manual_seed(b + 1)
+    along = bf16_randn(g, (1, 1, 1, 128)).float()
+    steps = torch.linspace(-3, 3, cp)[None, :, None, None]
+    k = (along * (steps.flip(1) if falling else steps)).expand(1, cp, hk, 128).to(torch.bfloat16).contiguous().to(dev)
+    kv_cache.write_cache(prefix, k, bf16_randn(g, (1, cp, hk, 128)).to(dev))
+    q = (along * torch.linspace(0.1, 3, b * h).view(b, 1, h, 1)).to(torch.bfloat16).to(dev)
+    out = attention.attention_shared(q, prefix, cache, ints([c] * b, dev))
+    check(out, q, prefix, cache, [c] * b, [0] * b, [cp])
+
+
+@pytest.mark.parametrize("b", [2, 6, 14, 32])
+def test_a_row_has_its_bits_whatever_the_others_hold(dev, b):
+    """Other requests' large scores and NaN, over pieces of several blocks of keys."""
+    say("row bits", b)
+    q, prefix, cache = make(dev, b, 1, 64, 16, 1, 14000, 40, seed=b)
+    n = ints([40] * b, dev)
+    want = attention.attention_shared(q, prefix, cache, n)
+    for value in (40.0, float("nan")):
+        other = q.clone()
+        other[0, :, ::3] *= value
+        got = attention.attention_shared(other, prefix, cache, n)
+        assert torch.equal(got[1:], want[1:]), value
+        same = [h for h in range(64) if h % 3]
+        assert torch.equal(got[0, :, same], want[0, :, same]), value
+
+
+@pytest.mark.parametrize("b,s,p", [(130, 1, 40), (12, 24, 12), (60, 1, 3)])
+def test_all_requests_on_one_of_many_prefixes(dev, b, s, p):
+    """More rows on one prefix than the tiles were chosen for."""
+    say("skew", b, s, p)
+    q, prefix, cache = make(dev, b, s, 4, 2, p, 150, 30, seed=p)
+    share, lengths, plens = [p - 1] * b, [30 - i % 7 for i in range(b)], [150 - i for i in range(p)]
+    out = attention.attention_shared(q, prefix, cache, ints(lengths, dev), share=ints(share, dev), prefix_lengths=ints(plens, dev))
+    check(out, q, prefix, cache, lengths, share, plens)
+
+
 def test_what_lies_behind_a_length_is_not_read_into_a_row(dev):
     """NaN in positions past the lengths of prefixes and caches, and in a prefix of other requests."""
     say("nan behind")
@@ -198,6 +241,31 @@ def test_strides_streams_and_graphs(dev):
         want = attention.attention_shared(q, prefix, cache, n, **args)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want) and torch.equal(outs[1], want), i
+
+
+def test_two_graphs_of_one_memory_pool(dev):
+    """Captured steps whose workspaces may lie at the same place, replayed in turn with eager calls between."""
+    say("two graphs")
+    q, prefix, cache = make(dev, 40, 2, 4, 2, 2, 300, 40)
+    share, n = ints([i % 3 - 1 for i in range(40)], dev), ints([i for i in range(40)], dev)
+    few, one = q[:5].clone(), kv_cache.QuantizedCache(*(t[:1].clone() for t in prefix))
+    own, m = kv_cache.QuantizedCache(*(t[:5].clone() for t in cache)), ints([9, 0, 40, 3, 17], dev)
+    calls = (lambda: attention.attention_shared(q, prefix, cache, n, share=share), lambda: attention.attention_shared(few, one, own, m))
+    for f in calls:
+        f()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, f in zip(graphs, calls):
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if outs else None):
+            outs.append(f())
+    for i in range(3):
+        q.copy_(torch.randn_like(q.float()).to(torch.bfloat16))
+        few.copy_(torch.randn_like(few.float()).to(torch.bfloat16))
+        n.add_(1)
+        for graph, out, f in zip(graphs, outs, calls):
+            graph.replay()
+            want = f()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), i
 
 
 def test_agrees_with_attention_over_one_cache(dev):
