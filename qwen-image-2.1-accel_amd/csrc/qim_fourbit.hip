@@ -275,15 +275,18 @@ static int launch_fourbit_ring(const FourBitArgs &a, hipStream_t st) {
 }
 
 // More rows: a workgroup of WAVES = 8 or 4 waves and 16 NR x 64 or 32 values of output; of each step of 128 k, staged in LDS,
-// wave w takes the k 32 (w % 4) .. + 31 for 32 of the columns, so that every code is made an operand once.  Two
+// wave w takes the k 32 (w % 4) .. + 31 for 32 of the columns, so that every code is made an operand once; or, in groups of 64
+// or 128 k and up to 80 rows (KC 2), the k 64 (w % 2) .. + 63 for 16 columns: half of the scalings for twice the reads of x.  Two
 // stages: one multiplied, one on its way (a third was slower: the step's chain of reads, operands and products holds it
 // up); a stage's 16-byte chunk c of row r of x lies at c ^ (r % 16), so that the 16 rows of an operand lie in different banks.
 template <int G, int NR, int WAVES>
 struct FtStage {
-    static constexpr int NT = WAVES / 2;  // 16-column tiles of W: two for each four waves
+    static constexpr int NT = WAVES / 2;  // 16-column tiles of W
+    static constexpr int KC = (G == 1 || G == 2) && NR < 8 ? 2 : 1, KW = 4 / KC, TW = 2 / KC;  // a wave's steps of 32 k, waves along k, tiles a wave
+    static constexpr int TP = KC == 1 ? 2 : NT;  // tiles joined at a time
     static constexpr int SB = G ? 32 * G : 64, ZB = 16 * G;  // bytes of a tile's scales or exponents, and of its zero points
     static constexpr int CODES = NR * 16 * 256, SCALES = CODES + NT * 1024, ZEROS = SCALES + NT * SB, BYTES = ZEROS + NT * ZB;
-    static constexpr int JOIN = 4 * 2 * NR * 64 * 16;        // four waves' partial sums of half of the output
+    static constexpr int JOIN = KW * TP * NR * 64 * 16;        // the waves' partial sums of those
     static constexpr int TABLES = 2 * BYTES > JOIN ? 2 * BYTES : JOIN, LDS = TABLES + (G ? 256 : 0);
 };
 
@@ -293,7 +296,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     uint4 *const tables = reinterpret_cast<uint4 *>(lds + St::TABLES);
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = wave & 3, half = wave >> 2;
+    constexpr int KC = St::KC, TW = St::TW;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = KC * (wave % St::KW), part_of = wave / St::KW;  // first step of 32 k; of the columns
     const uint32_t rowblock = blockIdx.x / ncol, col = blockIdx.x - rowblock * ncol;
     const int row0 = (int)rowblock * 16 * NR;
     constexpr int OT = SWIGLU ? St::NT / 2 : St::NT;
@@ -341,9 +345,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
         }
     };
 
-    f32x4_t acc[2][NR];
+    f32x4_t acc[TW][NR];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < TW; ++i)
 #pragma unroll
         for (int r = 0; r < NR; ++r) acc[i][r] = f32x4_t{};
     const int g = G ? j * G / 4 : 0;  // the group of this wave's k
@@ -354,14 +358,20 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
         if (t + 1 < p.KT) issue(t + 1, (t + 1) & 1);
         const uint8_t *const st = lds + (t & 1) * St::BYTES;
         if (128 * t + 32 * j < p.K) {
-            uint32_t c[2];
-            uint2 s2[2];
-            uint4 tab[2];
-            uint32_t e[2];
+            uint32_t c[TW][KC];
+            uint2 s2[TW];
+            uint4 tab[TW];
+            uint32_t e[TW];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int n = 2 * half + i;
-                c[i] = *reinterpret_cast<const uint32_t *>(st + St::CODES + n * 1024 + lane * 16 + 4 * j);
+            for (int i = 0; i < TW; ++i) {
+                const int n = TW * part_of + i;
+                const uint8_t *const cp = st + St::CODES + n * 1024 + lane * 16 + 4 * j;
+                if constexpr (KC == 2) {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(cp);
+                    c[i][0] = u.x, c[i][1] = u.y;
+                } else {
+                    c[i][0] = *reinterpret_cast<const uint32_t *>(cp);
+                }
                 if constexpr (G == 0) {
                     e[i] = st[St::SCALES + n * St::SB + lr * 4 + j];
                 } else {
@@ -369,21 +379,27 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
                     tab[i] = tables[(st[St::ZEROS + n * St::ZB + lr * G + g] & zmask) | znone];
                 }
             }
-            bf16x8_t x[NR];
+            bf16x8_t x[KC][NR];
 #pragma unroll
-            for (int r = 0; r < NR; ++r) x[r] = *reinterpret_cast<const bf16x8_t *>(st + (16 * r + lr) * 256 + (((4 * j + kg) ^ lr) << 4));
+            for (int k = 0; k < KC; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+                for (int r = 0; r < NR; ++r) x[k][r] = *reinterpret_cast<const bf16x8_t *>(st + (16 * r + lr) * 256 + (((4 * (j + k) + kg) ^ lr) << 4));
+#pragma unroll
+            for (int i = 0; i < TW; ++i) {
                 if constexpr (G == 0) {
-                    const bf16x8_t w = fb_e2m1(c[i], mx_scale_operand((int)e[i]));
+                    const bf16x8_t w = fb_e2m1(c[i][0], mx_scale_operand((int)e[i]));
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[r], acc[i][r], 0, 0, 0);
+                    for (int r = 0; r < NR; ++r) acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[0][r], acc[i][r], 0, 0, 0);
                 } else {
                     const float s[4] = {bf_lo(s2[i].x), bf_hi(s2[i].x), bf_lo(s2[i].y), bf_hi(s2[i].y)};
-                    const bf16x8_t w = fb_int4(c[i], tab[i]);
+                    bf16x8_t w[KC];
+#pragma unroll
+                    for (int k = 0; k < KC; ++k) w[k] = fb_int4(c[i][k], tab[i]);
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
-                        const f32x4_t a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[r], f32x4_t{}, 0, 0, 0);
+                        f32x4_t a = f32x4_t{};
+#pragma unroll
+                        for (int k = 0; k < KC; ++k) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[k], x[k][r], a, 0, 0, 0);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) acc[i][r][n] = __builtin_fmaf(s[n], a[n], acc[i][r][n]);
                     }
@@ -391,30 +407,31 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
             }
         }
     }
-    // The join, the columns of one half of the waves after those of the other.
-    f32x4_t(*const part)[2 * NR][64] = reinterpret_cast<f32x4_t(*)[2 * NR][64]>(lds);
+    // The join, TP tiles at a time.
+    constexpr int TP = St::TP;
+    f32x4_t(*const part)[TP * NR][64] = reinterpret_cast<f32x4_t(*)[TP * NR][64]>(lds);
 #pragma unroll
-    for (int h = 0; h < WAVES / 4; ++h) {
+    for (int h = 0; h < St::NT / TP; ++h) {
         __syncthreads();
-        if (half == h) {
+        if (part_of * TW / TP == h) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < TW; ++i)
 #pragma unroll
-                for (int r = 0; r < NR; ++r) part[j][i * NR + r][lane] = acc[i][r];
+                for (int r = 0; r < NR; ++r) part[wave % St::KW][(part_of * TW % TP + i) * NR + r][lane] = acc[i][r];
         }
         __syncthreads();
-        constexpr int BLOCKS = SWIGLU ? NR : 2 * NR;
+        constexpr int OP = SWIGLU ? TP / 2 : TP, BLOCKS = OP * NR;
 #pragma unroll
         for (int i = 0; i < (BLOCKS + WAVES - 1) / WAVES; ++i) {
-            const int blk = wave + WAVES * i, ot = SWIGLU ? 0 : blk / NR, r = blk - ot * NR;
+            const int blk = wave + WAVES * i, ot = blk / NR, r = blk - ot * NR, first = (SWIGLU ? 2 * ot : ot) * NR + r;
             if (blk >= BLOCKS) break;
             f32x4_t y = {}, u = {};
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                y += part[v][blk][lane];
-                if (SWIGLU) u += part[v][NR + blk][lane];
+            for (int v = 0; v < St::KW; ++v) {
+                y += part[v][first][lane];
+                if (SWIGLU) u += part[v][first + NR][lane];
             }
-            const int64_t n0 = ((int64_t)col * OT + h * (SWIGLU ? 1 : 2) + ot) * 16 + 4 * kg;
+            const int64_t n0 = ((int64_t)col * OT + h * OP + ot) * 16 + 4 * kg;
             const int row = row0 + 16 * r + lr;
             if (row < p.M && n0 < p.N) fb_store<SWIGLU>(p, row, n0, y, u);
         }
