@@ -17,7 +17,7 @@
 // tile of output and through a ring in LDS of its own, and join at the end; no barrier stands in the loop.  k_fourbit_tile,
 // the others: stages in LDS that eight waves share, and up to 128 rows for every operand made of codes.
 // Measured (launches from a graph): int4 g 128, 1 row, 4096 -> 12288 9.1-9.9 us, 2.6 TB/s; mxfp4, 16 rows, 12288 -> 4096 8.9 us, 2.8
-// TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 24.0 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430 TFLOP/s; mxfp4, 1024
+// TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 22.0 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430 TFLOP/s; mxfp4, 1024
 // rows, 4096 -> 4096 38 us, 900 TFLOP/s.
 #include "qim_device.h"
 #include "qim_runtime.h"
@@ -452,11 +452,13 @@ static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
     return QIM_OK;
 }
 
-// Which kernel.  At 4096 columns of x (and alike at others) the tile kernel takes about 12.5 us and 3.5 + 2.75 NR more for each
-// workgroup of eight waves that a CU has to take, the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16: the
-// first is held up by the chain of its steps while a CU has few workgroups, the other makes operands of all codes again for
-// every 16 rows.  int4, group 64, tile against ring: 32 x 4096 18.2 us and 9.7, 64 x 4096 18.3 and 12.7, 128 x 4096 19.3 and
-// 21.7, 24 x 24576 26.0 and 33.1, 16 x 65536 44.4 and 48.2; mxfp4: 64 x 4096 17.1 and 8.9, 16 x 65536 31.7 and 39.0.
+// Which kernel.  At 4096 columns of x (and alike at others) the tile kernel takes about 3.5 + 2.75 NR us for each workgroup of
+// eight waves that a CU has to take (groups of 64 and 128, up to 80 rows: 4 + 2.2 NR), a third more where it takes one only,
+// and up to 10 us besides; the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16.  The first is held up by the
+// chain of its steps while a CU has few workgroups, the other makes operands of all codes again for every 16 rows.
+// int4, group 64, tile against ring: 32 x 4096 18.2 us and 9.7, 64 x 4096 18.3 and 12.7, 128 x 4096 16.7 and 21.7, 24 x 24576
+// 21.1 and 33.1, 16 x 65536 41.7 and 48.2; mxfp4: 64 x 4096 17.1 and 8.9, 16 x 65536 31.7 and 39.0.  Tiles of 64 rows
+// against 128, group 64: 512 x 4096 31.3 us and 38.5, 1024 x 4096 58.5 and 56.4.
 // Up to one and a half workgroups of eight waves a CU int4 takes workgroups of four instead, which divide the CUs more evenly and
 // wait for fewer at a barrier (us, eight waves and four: 24 x 12288 SwiGLU 26.6, 23.8; 154 x 12288, group 32, 39.8, 35.1; 128 x
 // 4096 20.3, 18.0; but 300 x 12288, three a CU, 60.9 and 67.4, and mxfp4 154 x 12288 24.4 and 25.5).
@@ -467,14 +469,16 @@ static int launch_fourbit(const FourBitArgs &a, hipStream_t st) {
     const int64_t ntiles = (a.N + 15) / 16, ncol = (ntiles + OT - 1) / OT;
     auto wgs = [&](int nr) { return ncol * ((a.M + 16 * nr - 1) / (16 * nr)); };  // of eight waves
     auto four = [&](int nr) { return G > 0 && nr > 1 && nr < 8 && wgs(nr) <= 384; };
-    auto cost = [&](int nr) {  // of 0.14 us; (four waves on a CU issue no faster than half of eight do)
-        return (four(nr) && wgs(nr) > 256 ? 3 : (wgs(nr) + 255) / 256 * 2) * (10 * nr + 13);
+    constexpr bool wide = G == 1 || G == 2;  // (FtStage's KC 2)
+    auto cost = [&](int nr) {  // of 0.0275 us
+        const int64_t n = wgs(nr);
+        return (n <= 256 ? four(nr) ? 11 : 13 : four(nr) ? 15 : (n + 255) / 256 * 10) * (wide && nr < 8 ? 8 * nr + 16 : 10 * nr + 13);
     };
     int nr = 8;
     for (int n : {5, 4, 2, 1})
         if (cost(n) < cost(nr)) nr = n;
     const int64_t blocks = (a.M + 15) / 16 * ntiles;
-    if (a.M <= 16 * 65535 && 20 * ONE * blocks < 256 * (70 + cost(nr))) {  // (a grid of no more than 65535 blocks of rows)
+    if (a.M <= 16 * 65535 && 100 * ONE * blocks < 256 * ((wide ? 190 : 350) + cost(nr))) {  // (a grid of no more than 65535 blocks of rows)
         // From one and a half tiles a CU on two of them share the reads of x, and two workgroups of four waves a CU take more of
         // them at a time (16 rows, mxfp4: 4096 -> 12288 9.2 us against 11.6; 12288 -> 4096, 256 tiles, 14.6 against 9.0).
         if (blocks >= 384) return launch_fourbit_ring<G, 2, 4, 4, 3, SWIGLU>(a, st);

@@ -78,7 +78,7 @@ def test_swiglu(dev, m, n, k, kind, group, zeros):
 
 # Rows and columns of a plain product (of a SwiGLU: half the columns) for each height of the shared tiles (16, 32, 64, 80 and
 # 128 rows) and, for int4, each of their widths.
-TILES = [(15, 65530), (30, 24600), (30, 14210), (40, 24610), (100, 8100), (150, 8100), (200, 8390), (1020, 4090)]
+TILES = [(15, 65530), (30, 24600), (30, 14210), (48, 12200), (40, 24610), (100, 8100), (150, 8100), (70, 20000), (200, 8390), (1020, 4090)]
 
 
 @pytest.mark.parametrize("kind,group,k", [("int4", 32, 160), ("int4", 64, 192), ("int4", 128, 384), ("mxfp4", 32, 224)])
