@@ -18,7 +18,7 @@
 // the others: stages in LDS that eight waves share, and up to 128 rows for every operand made of codes.
 // Measured (launches from a graph): int4 g 128, 1 row, 4096 -> 12288 9.1-9.9 us, 2.6 TB/s; mxfp4, 16 rows, 12288 -> 4096 8.9 us, 2.8
 // TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 22.0 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430 TFLOP/s; mxfp4, 1024
-// rows, 4096 -> 4096 38 us, 900 TFLOP/s.
+// rows, 4096 -> 4096 37-39 us, 900 TFLOP/s.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -276,8 +276,8 @@ static int launch_fourbit_ring(const FourBitArgs &a, hipStream_t st) {
 
 // More rows: a workgroup of WAVES = 8 or 4 waves and 16 NR x 64 or 32 values of output; of each step of 128 k, staged in LDS,
 // wave w takes the k 32 (w % 4) .. + 31 for 32 of the columns, so that every code is made an operand once; or, in groups of 64
-// or 128 k and up to 80 rows (KC 2), the k 64 (w % 2) .. + 63 for 16 columns: half of the scalings for twice the reads of x.  Two
-// stages: one multiplied, one on its way (a third was slower: the step's chain of reads, operands and products holds it
+// or 128 k and up to 80 rows (KC 2), the k 64 (w % 2) .. + 63 for 16 columns: half of the scalings for twice the reads of x (300
+// rows, 4096 -> 12288: 61.7 us and 52.1).  Two stages: one multiplied, one on its way (a third was slower: the step's chain of reads, operands and products holds it
 // up); a stage's 16-byte chunk c of row r of x lies at c ^ (r % 16), so that the 16 rows of an operand lie in different banks.
 template <int G, int NR, int WAVES>
 struct FtStage {
