@@ -10,10 +10,11 @@
 // Few rows: the cache's bytes and the launches' starts bound it; from some 64 rows on the vector instructions of the softmax and
 // the conversions, beside the matrix products.  Measured (launches from a graph): 4 requests, one row each on 32 heads, 1101 +
 // 96 keys 13.2 us (8.6 and the join's 4.9); 32 requests of 4 rows on 8 heads, 8392 + 1024 keys 30 us; 48 requests on 5
-// prefixes of up to 32768 keys 88 us, 3.5 TB/s; 8 requests of 24 rows on 32 heads, 8392 + 256 keys 73 us, 370 TFLOP/s.
+// prefixes of up to 32768 keys 86 us, 3.6 TB/s; 8 requests of 24 rows on 32 heads, 8392 + 256 keys 71-74 us, 370 TFLOP/s.
 //
 // The rows of a prefix: its requests in the order of their numbers, S * G rows each.  Which requests those are is known on
-// the device only, so where a batch has several prefixes a first launch of one workgroup lists them.
+// the device only.  Up to 64 requests and 16 prefixes every wave finds them itself, a request a lane (48 requests on 5
+// prefixes 3 us less than with a launch for it); of more, a first launch of one workgroup makes lists.
 #include "qim_cache_attention.h"
 #include "qim_runtime.h"
 
@@ -21,6 +22,7 @@ namespace qim {
 
 constexpr int SA_WAVES = 4;
 constexpr int SA_MAX_PREFIXES = 4096;
+constexpr int SA_FEW_PREFIXES = 16;
 
 // A space of keys: V sequences (own: a request and a tile of its rows; prefix: a tile of rows) cut into at most `most` pieces
 // (V or more).  Partial results by (piece, K/V head, row of the tile).
@@ -41,6 +43,7 @@ struct SaArgs {
     int64_t tree_b, CP, C;
     uint16_t *o;
     SaSpace pre, own;
+    int few;          // share: no lists, every wave has a request and a prefix tile a lane
     int4 *tiles;      // per prefix tile: prefix, first of its requests in `order`, their rows, the tile's first row (share only)
     int32_t *order;   // the requests by prefix
     int2 *where;      // per request: its prefix's first tile (-1: none), its place among the prefix's requests
@@ -59,6 +62,49 @@ __device__ __forceinline__ SaTile sa_tile(const SaArgs &p, int i) {
     if (!p.share) return SaTile{0, 0, p.B * p.S * p.G, i * p.pre.rows};
     const int4 t = p.tiles[i];
     return SaTile{t.x, t.y, t.z, t.w};
+}
+
+// What a lane holds of the plan where the batch is small: its request's prefix, and the prefix tile of its number.
+struct SaLanes {
+    int who;
+    SaTile tile;
+};
+template <class Each>
+__device__ __forceinline__ void sa_each_prefix(const SaArgs &p, int who, Each each) {  // (prefix, its requests, its first tile, tiles)
+    const int shift = __builtin_ctz((unsigned)p.pre.rows);
+    int first = 0;
+    for (int i = 0; i < p.P; ++i) {
+        const uint64_t all = __builtin_amdgcn_ballot_w64(who == i);
+        const int tiles = ((int)__builtin_popcountll(all) * p.S * p.G + p.pre.rows - 1) >> shift;
+        each(i, all, first, tiles);
+        first += tiles;
+    }
+}
+__device__ __forceinline__ SaLanes sa_lanes(const SaArgs &p) {
+    const int lane = threadIdx.x & 63;
+    SaLanes l{-1, SaTile{0, 0, 0, 0}};
+    if (!p.few) return l;
+    l.who = lane < p.B ? p.share[lane] : -1;
+    sa_each_prefix(p, l.who, [&](int i, uint64_t all, int first, int tiles) {
+        if (lane >= first && lane < first + tiles) l.tile = SaTile{i, 0, (int)__builtin_popcountll(all) * p.S * p.G, (lane - first) * p.pre.rows};
+    });
+    return l;
+}
+__device__ __forceinline__ SaTile sa_tile(const SaArgs &p, const SaLanes &l, int i) {
+    if (!p.few) return sa_tile(p, i);
+    return SaTile{__builtin_amdgcn_readlane(l.tile.prefix, i), 0, __builtin_amdgcn_readlane(l.tile.rows, i), __builtin_amdgcn_readlane(l.tile.row0, i)};
+}
+// The requests of a tile's prefix, one a lane, in their order (few only).
+__device__ __forceinline__ int sa_requests(const SaArgs &p, const SaLanes &l, int prefix) {
+    if (!p.few) return 0;
+    const int lane = threadIdx.x & 63;
+    const uint64_t all = __builtin_amdgcn_ballot_w64(l.who == prefix), below = (1ull << lane) - 1;
+    const int at = l.who == prefix ? (int)__builtin_popcountll(all & below) : (int)(__builtin_popcountll(all) + __builtin_popcountll(~all & below));
+    return __builtin_amdgcn_ds_permute(4 * at, lane);
+}
+__device__ __forceinline__ int sa_request(const SaArgs &p, const SaTile &t, int requests, int i) {
+    if (!p.share) return i;
+    return p.few ? __shfl(requests, i, 64) : p.order[t.first + i];
 }
 
 // The requests of each prefix, in their order, and the prefix's tiles of rows.  One workgroup; a wave per prefix counts and
@@ -110,9 +156,9 @@ __global__ __launch_bounds__(1024) void k_shared_plan(SaArgs p) {
 }
 
 template <bool PRE>
-__device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
+__device__ __forceinline__ int64_t sa_length(const SaArgs &p, const SaLanes &l, int i) {  // (few: i is the lane's own number)
     if constexpr (PRE) {
-        const SaTile t = sa_tile(p, i);
+        const SaTile t = p.few ? l.tile : sa_tile(p, i);
         return t.rows ? sa_prefix_length(p, t.prefix) : 0;
     }
     return sa_clamp(p.lengths[i / p.ntile], p.C);
@@ -121,7 +167,7 @@ __device__ __forceinline__ int64_t sa_length(const SaArgs &p, int i) {
 // Which piece this is: sequence v, its blocks [blk0, blk0 + per).  All sequences' blocks are cut into pieces of `per`, of
 // which there are at most sp.most.  The first workgroup also writes the space's dir.
 template <bool PRE>
-__device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uint32_t piece, bool writes, int &v, int &blk0, int &per) {
+__device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaLanes &l, const SaSpace &sp, uint32_t piece, bool writes, int &v, int &blk0, int &per) {
     const int lane = threadIdx.x & 63;
     if (PRE && !p.share) {  // sequences alike: the same pieces of each
         const int n = (int)(((uint32_t)sa_prefix_length(p, 0) + sp.keys - 1) / (uint32_t)sp.keys), each = sp.most / sp.V;
@@ -134,7 +180,7 @@ __device__ __forceinline__ bool sa_piece(const SaArgs &p, const SaSpace &sp, uin
         blk0 = ((int)piece - v * count) * size;
         return true;
     }
-    auto blocks = [&](int i) { return i < sp.V ? (int)(((uint32_t)sa_length<PRE>(p, i) + sp.keys - 1) / (uint32_t)sp.keys) : 0; };
+    auto blocks = [&](int i) { return i < sp.V ? (int)(((uint32_t)sa_length<PRE>(p, l, i) + sp.keys - 1) / (uint32_t)sp.keys) : 0; };
     const int head = blocks(lane);  // the first 64 sequences' stay in a register
     auto blocks_from = [&](int i) { return i ? blocks(i + lane) : head; };
     uint32_t total = 0;  // (all spaces have fewer than 2^31 blocks)
@@ -180,10 +226,13 @@ __device__ __forceinline__ void sa_wave(const SaArgs &p, const SaSpace &sp, uint
     const int h = (int)((q8 - grp * wide) * SA_WAVES) + wave;
     int v = 0;
     int blk0 = 0, per = 1;
-    if (!sa_piece<PRE>(p, sp, piece, block == 0 && wave == 0, v, blk0, per)) return;
+    const SaLanes lanes = PRE ? sa_lanes(p) : SaLanes{};
+    if (!sa_piece<PRE>(p, lanes, sp, piece, block == 0 && wave == 0, v, blk0, per)) return;
     if (h >= p.HK) return;
-    const int64_t len = sa_length<PRE>(p, v), W = (int64_t)p.HK * CA_D, C = PRE ? p.CP : p.C;
-    const SaTile tile = PRE ? sa_tile(p, v) : SaTile{v / p.ntile, 0, p.S * p.G, (v % p.ntile) * sp.rows};
+    const int64_t W = (int64_t)p.HK * CA_D, C = PRE ? p.CP : p.C;
+    const SaTile tile = PRE ? sa_tile(p, lanes, v) : SaTile{v / p.ntile, 0, p.S * p.G, (v % p.ntile) * sp.rows};
+    const int64_t len = PRE ? sa_prefix_length(p, tile.prefix) : sa_clamp(p.lengths[tile.prefix], p.C);
+    const int requests = PRE ? sa_requests(p, lanes, tile.prefix) : 0;
     const int64_t base = (int64_t)tile.prefix * C * W + h * CA_D;
     const CaKeys keys{(PRE ? p.pk : p.kc) + base, (PRE ? p.pks : p.ks) + base / 32, (PRE ? p.pv : p.vc) + base,
                       (PRE ? p.pvs : p.vs) + base / 32, C, W, len};
@@ -195,7 +244,7 @@ __device__ __forceinline__ void sa_wave(const SaArgs &p, const SaSpace &sp, uint
                     int r = tile.row0 + 16 * t + lr;
                     r = r < tile.rows ? r : tile.rows - 1;  // rows past the end: computed, not stored
                     const int sg = p.S * p.G, i = PRE ? r / sg : 0, in = r - i * sg, s = in / p.G;
-                    const int b = PRE ? (p.share ? p.order[tile.first + i] : i) : tile.prefix;
+                    const int b = PRE ? sa_request(p, tile, requests, i) : tile.prefix;
                     bits = PRE ? 0 : ca_tree_bits(p.tree ? p.tree + b * p.tree_b + s * p.S : nullptr, p.S);
                     return p.q + b * p.ldqb + s * p.ldq + (h * p.G + (in - s * p.G)) * CA_D;
                 },
@@ -247,8 +296,10 @@ __global__ __launch_bounds__(64 * SA_WAVES, RG == 4 ? 3 : 2) void k_shared_tile(
     const int h = (int)(unit - piece * units) * 8 + (int)(q8 & 7);
     int v = 0;
     int blk0 = 0, per = 1;
-    if (!sa_piece<true>(p, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per) || h >= p.HK) return;
-    const SaTile tile = sa_tile(p, v);
+    const SaLanes lanes = sa_lanes(p);
+    if (!sa_piece<true>(p, lanes, p.pre, piece, blockIdx.x == 0 && wave == 0, v, blk0, per) || h >= p.HK) return;
+    const SaTile tile = sa_tile(p, lanes, v);
+    const int requests = sa_requests(p, lanes, tile.prefix);
     const int64_t len = sa_prefix_length(p, tile.prefix), W = (int64_t)p.HK * CA_D, base = (int64_t)tile.prefix * p.CP * W + h * CA_D;
     const int nblk = (int)((len + ST_KEYS - 1) / ST_KEYS), blk1 = blk0 + per < nblk ? blk0 + per : nblk;
     const float c = p.scale_log2e, ninf = -__builtin_inff();
@@ -281,7 +332,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, RG == 4 ? 3 : 2) void k_shared_tile(
         int r = tile.row0 + 32 * rg + 16 * t + lr;
         r = r < tile.rows ? r : tile.rows - 1;
         const int sg = p.S * p.G, i = r / sg, in = r - i * sg, sq = in / p.G;
-        const int b = p.share ? p.order[tile.first + i] : i;
+        const int b = sa_request(p, tile, requests, i);
         const uint16_t *qr = p.q + b * p.ldqb + sq * p.ldq + (h * p.G + (in - sq * p.G)) * CA_D + 16 * kg;
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[t][j] = *reinterpret_cast<const bf16x8_t *>(qr + 64 * (j >> 1) + 8 * (j & 1));
@@ -478,7 +529,16 @@ __global__ __launch_bounds__(256) void k_shared_join(SaArgs p, int64_t nrows) {
     const int64_t row = live ? g : 0, item = row / sg;
     const int r = (int)(row - item * sg), b = (int)(item / p.HK), h = (int)(item - (int64_t)b * p.HK);
     const int2 od = p.own.dir[b * p.ntile + r / p.own.rows];
-    const int2 w = p.share ? p.where[b] : make_int2(0, b);
+    int2 w = make_int2(0, b);
+    if (p.few) {
+        const int mine = (threadIdx.x & 63) < p.B ? p.share[threadIdx.x & 63] : -1, prefix = p.share[b];
+        w.x = -1;
+        sa_each_prefix(p, mine, [&](int i, uint64_t all, int first, int) {
+            if (prefix == i) w = make_int2(first, (int)__builtin_popcountll(all & ((1ull << b) - 1)));
+        });
+    } else if (p.share) {
+        w = p.where[b];
+    }
     int2 pd = make_int2(0, 0);
     int pr = 0;
     if (w.x >= 0) {
@@ -552,7 +612,7 @@ struct SaPlan {
     int64_t vp, vo, gp, go;               // sequences, pieces (at most)
     int64_t wp, wo;                       // workgroups of a piece's heads
     int64_t HK, B;
-    bool shared;
+    bool shared, few;
     static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
     int64_t blocks_p() const { return rg ? (gp * ((HK + 7) / 8) + 7) / 8 * 64 : (gp + 7) / 8 * 8 * wp; }
     int64_t blocks_o() const { return (go + 7) / 8 * 8 * wo; }
@@ -560,7 +620,7 @@ struct SaPlan {
     int64_t rows_o() const { return go * HK * no * 16; }
     int64_t bytes() const {
         return up(rows_p() * CA_D * 4) + up(rows_o() * CA_D * 4) + up(rows_p() * 8) + up(rows_o() * 8) + up(vp * 8) + up(vo * 8) +
-               (shared ? up(vp * 16) + up(B * 4) + up(B * 8) : 0);
+               (shared && !few ? up(vp * 16) + up(B * 4) + up(B * 8) : 0);
     }
 };
 static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, int64_t HK, int64_t P, bool shared) {
@@ -581,6 +641,7 @@ static SaPlan sa_plan(int64_t B, int64_t S, int64_t CP, int64_t C, int64_t H, in
     pl.vo = B * pl.ntile;
     // Several prefixes: each may end with a tile that is not full.
     pl.vp = (rows + pl.tr - 1) / pl.tr + (shared && P > 1 ? (P - 1 < B ? P - 1 : B) : 0);
+    pl.few = shared && B <= 64 && P <= SA_FEW_PREFIXES && pl.vp <= 64;
     const int64_t bp = (CP + pl.keys - 1) / pl.keys, bo = (C + CA_KB - 1) / CA_KB;
     // The pieces of both spaces together: two workgroups a CU, divided by the time that the spaces' blocks take one
     // (measured: 1.0 and 1.5 us for a wave's 16 and 32 rows, 1.4 and 2.3 us for tiles of 64 and 128).  Three of a CU's
@@ -665,7 +726,8 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
     a.own.part_ml = (float2 *)take(pl.rows_o() * 8);
     a.pre.dir = (int2 *)take(pl.vp * 8);
     a.own.dir = (int2 *)take(pl.vo * 8);
-    if (share) {
+    a.few = pl.few;
+    if (share && !pl.few) {
         a.tiles = (int4 *)take(pl.vp * 16);
         a.order = (int32_t *)take(B * 4);
         a.where = (int2 *)take(B * 8);
@@ -675,7 +737,7 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
     a.B = (int)B, a.S = (int)S, a.H = (int)H, a.HK = (int)HK, a.G = (int)(H / HK), a.P = (int)P, a.ntile = (int)pl.ntile;
     a.scale_log2e = scale * 1.4426950408889634f;
     hipStream_t st = as_stream(stream);
-    if (share) launch(k_shared_plan, dim3(1), dim3(1024), (size_t)(8 * P), st, a);
+    if (share && !pl.few) launch(k_shared_plan, dim3(1), dim3(1024), (size_t)(8 * P), st, a);
     const dim3 grid(a.pre.blocks + a.own.blocks);
     if (pl.rg) {
         const int rc = pl.rg == 4 ? launch_shared_tile<4, 1>(a, grid, st) : pl.no == 2 ? launch_shared_tile<2, 2>(a, grid, st) : launch_shared_tile<2, 1>(a, grid, st);

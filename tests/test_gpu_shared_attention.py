@@ -65,7 +65,8 @@ def test_one_prefix(dev, b, s, h, hk, cp, c):
 
 @pytest.mark.parametrize("b,s,h,hk,p,cp,c", [
     (1, 1, 1, 1, 3, 40, 4), (6, 1, 2, 2, 2, 100, 8), (9, 5, 4, 2, 4, 130, 40), (48, 1, 8, 2, 5, 900, 33), (70, 1, 2, 1, 3, 257, 6),
-    (20, 1, 2, 2, 70, 65, 3), (5, 33, 4, 4, 2, 300, 60), (150, 1, 1, 1, 6, 64, 2), (30, 3, 4, 4, 1, 333, 9)])
+    (20, 1, 2, 2, 70, 65, 3), (5, 33, 4, 4, 2, 300, 60), (150, 1, 1, 1, 6, 64, 2), (30, 3, 4, 4, 1, 333, 9),
+    (64, 1, 4, 2, 16, 200, 9), (64, 3, 8, 2, 15, 130, 10), (65, 1, 2, 2, 16, 100, 5), (40, 1, 2, 2, 17, 90, 5), (40, 64, 4, 1, 2, 70, 64)])
 def test_several_prefixes(dev, b, s, h, hk, p, cp, c):
     """Prefixes of different lengths, some of them empty or of no request, and requests without a prefix."""
     say("prefixes", b, s, h, hk, p, cp, c)
