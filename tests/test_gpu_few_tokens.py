@@ -162,3 +162,32 @@ def test_cached_decode_keeps_its_bits(dev, profile, tokens, batch, monkeypatch):
     parts = run()
     assert _native.calls.get("qim_residual_norm", 0) == before + len(t.transformer_blocks)
     assert torch.equal(joined, parts)
+
+
+def test_two_calls_at_once(dev):
+    """The same operators on two streams at the same time, with inputs, weights and caches in common."""
+    say("two streams")
+    g = torch.Generator().manual_seed(5)
+    w = [fourbit.quantize_weight(bf16_randn(g, (1500, 1024)).to(dev).float(), "int4", 64) for _ in range(2)]
+    x, h = (bf16_randn(g, (2, 40, 1024)).to(dev) for _ in range(2))
+    caches = []
+    for b, c in ((2, 900), (40, 30)):
+        caches.append(kv_cache.empty_cache(b, c, 4, 128, dev))
+        kv_cache.write_cache(caches[-1], bf16_randn(g, (b, c, 4, 128)).to(dev), bf16_randn(g, (b, c, 4, 128)).to(dev))
+    q, n = bf16_randn(g, (40, 2, 8, 128)).to(dev), torch.full((40,), 30, dtype=torch.int32, device=dev)
+    share, norm = torch.arange(40, dtype=torch.int32, device=dev) % 3 - 1, torch.nn.RMSNorm(1024, eps=1e-6, device=dev, dtype=torch.bfloat16)
+
+    def step():
+        return (fourbit.swiglu(x, *w), fourbit.matmul(x[0, :3], w[0]), attention.attention_shared(q, *caches, n, share=share),
+                *elementwise.residual_norm(h, x, norm))
+    want = step()
+    streams, results = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for s, r in zip(streams, results):
+            with torch.cuda.stream(s):
+                r.append(step())
+    torch.cuda.synchronize()
+    for r in results:
+        assert all(torch.equal(a, b) for got in r for a, b in zip(got, want))
