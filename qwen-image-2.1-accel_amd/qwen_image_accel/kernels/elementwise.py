@@ -32,24 +32,46 @@ def residual(h, x, gate):
     return h + gate * x
 
 
+def norm_kind(norm):
+    """``NORM_LAYER``, ``NORM_RMS`` or ``NORM_NONE`` (None) of what ``residual_norm`` takes as a norm, else None.
+
+    A module counts by its class, since others with the same attributes compute other things: torch's LayerNorm, or one that is
+    named after it, and torch's RMSNorm with its own ``forward``, or a class named RMSNorm (Diffusers', x / rms times the weight).
+    Any other object holds a norm's parameters: with a ``normalized_shape`` a LayerNorm's, else an RMSNorm's."""
+    if norm is None:
+        return _native.NORM_NONE
+    shaped = getattr(norm, "normalized_shape", None) is not None
+    if not isinstance(norm, torch.nn.Module):
+        return _native.NORM_LAYER if shaped else _native.NORM_RMS
+    cls = type(norm)
+    if isinstance(norm, torch.nn.RMSNorm):
+        return _native.NORM_RMS if cls.forward is torch.nn.RMSNorm.forward else None
+    if isinstance(norm, torch.nn.LayerNorm) or (shaped and cls.__name__.endswith("LayerNorm")):
+        return _native.NORM_LAYER
+    return _native.NORM_RMS if cls.__name__ == "RMSNorm" and not shaped else None
+
+
 def _norm_of(norm, d, device, refuse):
     """(kind, weight or None, eps) of a norm over d values that ``residual_norm`` takes."""
-    if norm is None:
-        return _native.NORM_NONE, None, 0.0
+    kind = norm_kind(norm)
+    if kind == _native.NORM_NONE:
+        return kind, None, 0.0
+    if kind is None:
+        refuse(f"a {type(norm).__name__} is no LayerNorm or RMSNorm")
     weight, eps = getattr(norm, "weight", None), getattr(norm, "eps", None)
     if eps is None or getattr(norm, "bias", None) is not None:
         refuse("a norm has an eps and no bias")
     shape = getattr(norm, "normalized_shape", None)
     if shape is not None and tuple(shape) != (d,):
         refuse(f"a norm over {tuple(shape)} of rows of {d}")
-    if shape is not None and not isinstance(norm, torch.nn.RMSNorm):
+    if kind == _native.NORM_LAYER:
         if weight is not None or getattr(norm, "elementwise_affine", False):
             refuse("a LayerNorm has no affine")
-        return _native.NORM_LAYER, None, float(eps)
+        return kind, None, float(eps)
     if weight is not None and (weight.shape != (d,) or weight.dtype != torch.bfloat16 or weight.device != device
                                or not weight.is_contiguous()):
         refuse(f"an RMSNorm's weight is a contiguous bf16 ({d},) tensor on {device}")
-    return _native.NORM_RMS, weight, float(eps)
+    return kind, weight, float(eps)
 
 
 def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale=None, shift=None, add_one=False,
@@ -60,7 +82,8 @@ def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale
 
     Returns (h', z).  h, x: (B, S, D) or (M, D) bf16 on the GPU, rows any multiple of 8 elements apart, D
     a multiple of 8 up to 16384.  ``norm`` and ``post`` (None: x itself): an RMSNorm (``weight`` bf16 or
-    None, ``eps``) or a LayerNorm without affine (``normalized_shape``, ``eps``).  ``gate``, ``scale``, ``shift``: None,
+    None, ``eps``) or a LayerNorm without affine (``normalized_shape``, ``eps``); ``norm_kind`` says what counts as which, other
+    modules are refused.  ``gate``, ``scale``, ``shift``: None,
     (B, 1, D) bf16, one vector per sequence at any stride that is a multiple of 8, or one for all, (1, 1, D) or (D,).
     ``add_one``: 1 + scale instead of scale.  z is a new bf16 tensor, or with ``quantized`` a
     ``mxfp8.Quantized`` (``tiled``: in the GEMM's layout; D a multiple of 128).  ``out``: where h' goes, by default a

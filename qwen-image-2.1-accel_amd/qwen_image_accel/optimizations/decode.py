@@ -31,10 +31,11 @@ forward and the attention processor it replaced.
 """
 import torch
 
+from qwen_image_accel._native import NORM_LAYER
 from qwen_image_accel.kernels.attention import (attention_mxfp8, prepare_attention_inputs,
                                                 prepare_attention_inputs_quantized)
 from qwen_image_accel.kernels.bf16 import swiglu
-from qwen_image_accel.kernels.elementwise import residual, residual_norm, rope_qk
+from qwen_image_accel.kernels.elementwise import norm_kind, residual, residual_norm, rope_qk
 from qwen_image_accel.kernels.epilogue import layer_norm_scale_quantize, swiglu_quantize
 from qwen_image_accel.kernels.gemm import mx_matmul
 from qwen_image_accel.kernels.layernorm import layer_norm_scale, native_supported
@@ -243,7 +244,7 @@ class DecodeBlock:
         operands, with the bits of the two."""
         quantized = self.quantized and all_mxfp8(*(running(m) for m in consumers))
         if (gate is not None and branch.shape == h.shape and branch.is_contiguous() and branch.device == h.device
-                and branch.dtype == h.dtype and native_supported(h, scale, norm, gate=gate)
+                and branch.dtype == h.dtype and native_supported(h, scale, norm, gate=gate) and norm_kind(norm) == NORM_LAYER
                 and h.shape[0] * h.shape[1] < MAX_JOINED_ROWS and (not quantized or h.shape[-1] % 128 == 0)):
             return residual_norm(h, branch, norm, gate=gate, scale=scale, quantized=quantized, tiled=quantized,
                                  rounding="eager")
