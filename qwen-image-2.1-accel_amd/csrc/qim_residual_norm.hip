@@ -298,6 +298,16 @@ extern "C" int qim_residual_norm(const void *h, int64_t ldh, const void *x, int6
     } else {
         ok = ok && apart(z, ldz, h, ldh) && apart(z, ldz, x, ldx) && !rows_share(z, ldz, D, h_out, ldho, D, M);
     }
+    // Other workgroups still read the vectors.
+    const void *vectors[5] = {gate, scale, shift, post_weight, norm_weight};
+    const int64_t steps[5] = {gate_b, scale_b, shift_b, 0, 0}, nseq = (M - 1) / seq + 1;
+    for (int i = 0; i < 5; ++i) {
+        auto meets = [&](const void *out, int64_t ldo, int64_t n, int64_t rows) {
+            return rows_share_vectors(out, ldo, n, rows, vectors[i], steps[i], nseq, D);
+        };
+        ok = ok && !meets(h_out, ldho, D, M) && !(z_scales ? meets(z, pad * D / 2, pad * D / 2, 1) || meets(z_scales, pad * D / 64, pad * D / 64, 1)
+                                                           : meets(z, ldz, D, M));
+    }
     QIM_REQUIRE(ok, QIM_ERR_ARG, "%s: an output overlaps an input other than as the same rows, or the other output", who);
     ResNormArgs a{(const uint16_t *)h, (const uint16_t *)x, (const uint16_t *)post_weight, (const uint16_t *)gate,
                   (const uint16_t *)norm_weight, (const uint16_t *)scale, (const uint16_t *)shift, (uint16_t *)h_out,

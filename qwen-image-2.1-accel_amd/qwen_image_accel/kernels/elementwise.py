@@ -87,7 +87,7 @@ def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale
     (B, 1, D) bf16, one vector per sequence at any stride that is a multiple of 8, or one for all, (1, 1, D) or (D,).
     ``add_one``: 1 + scale instead of scale.  z is a new bf16 tensor, or with ``quantized`` a
     ``mxfp8.Quantized`` (``tiled``: in the GEMM's layout; D a multiple of 128).  ``out``: where h' goes, by default a
-    new tensor; h or x itself is fine, else it shares no rows with them.
+    new tensor; h or x itself is fine, else it shares no rows with them, and nothing with the vectors and weights.
 
     ``rounding="once"``: fp32 throughout, h' and z rounded at their ends (z from the unrounded h').
     ``"eager"``: the bits of ``residual(h, x, gate)`` followed by ``layernorm.layer_norm_scale`` or

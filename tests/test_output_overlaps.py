@@ -1,0 +1,54 @@
+"""Outputs of the few-token operators over inputs that other workgroups still read: refused before any launch (no GPU), and
+outputs between such inputs are taken (GPU)."""
+import pytest
+import torch
+
+from qwen_image_accel import _native
+from qwen_image_accel.kernels import elementwise
+from tests.helpers import bf16_randn
+from tests.test_few_tokens_refusals import ARG, FAR, norm
+
+FREE = 64 * FAR    # an address far from all others
+HO, Z = 3 * FAR, 4 * FAR
+
+
+@pytest.mark.parametrize("call", [
+    # h' over the vectors: the first, one of a later sequence, a part of one, one that begins in the gap before a row
+    norm(gate=HO), norm(gate=HO - 2 * 256), norm(gate=HO + 7 * 512), norm(scale=HO + 16), norm(shift=HO + 512), norm(gate=HO - 496, gate_b=0),
+    norm(gate=HO + 1024, ldho=512, gate_b=0), norm(gate=HO + 512 + 16, ldho=512, gate_b=0), norm(gate=HO - 1024, gate_b=512),
+    norm(norm=1, norm_w=HO + 512), norm(post=1, post_w=HO + 512),
+    # z over them, as rows and as codes and exponents
+    norm(gate=Z), norm(scale=Z + 7 * 512), norm(shift=Z - 496), norm(norm=1, norm_w=Z), norm(gate=Z, zs=FREE),
+    norm(shift=Z + 128 * 256 - 16, zs=FREE), norm(scale=FREE + 16, zs=FREE)])
+def test_residual_norm_refuses(call):
+    name, args = call
+    rc = getattr(_native.lib(), name)(*args)
+    assert rc == ARG, (rc, _native.lib().qim_last_error())
+
+
+@pytest.mark.gpu
+def test_vectors_beside_the_rows_of_one_buffer(dev):
+    """gate, scale and shift in other columns of the buffer that h' goes to, and behind its last row."""
+    print("[case] vectors beside rows", flush=True)
+    g = torch.Generator().manual_seed(1)
+    b, s, d = 3, 5, 264
+    h, x = (bf16_randn(g, (b, s, d)).to(dev) for _ in range(2))
+    layer = torch.nn.LayerNorm(d, eps=1e-6, elementwise_affine=False)
+    vectors = {k: bf16_randn(g, (b, 1, d)).to(dev) for k in ("gate", "scale", "shift")}
+    want = elementwise.residual_norm(h, x, layer, **vectors)
+    wide = torch.zeros(b * s + 1, 4 * d, dtype=torch.bfloat16, device=dev)
+    out = wide[:b * s].view(b, s, 4 * d)[..., :d]
+    places = {k: wide[:b * s].view(b, s, 4 * d)[:, 2:3, (i + 1) * d:(i + 2) * d] for i, k in enumerate(vectors)}
+    for k, v in vectors.items():
+        places[k].copy_(v)
+    got = elementwise.residual_norm(h, x, layer, out=out, **places)
+    assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+    assert all(torch.equal(places[k], v) for k, v in vectors.items())
+    last = wide[b * s, :d]
+    last.copy_(vectors["gate"][0, 0])
+    one = dict(vectors, gate=last)
+    want = elementwise.residual_norm(h, x, layer, **dict(vectors, gate=vectors["gate"][0, 0].clone()))
+    got = elementwise.residual_norm(h, x, layer, out=out, **one)
+    assert torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(_native.QimError):
+        elementwise.residual_norm(h, x, layer, out=out, **dict(vectors, gate=wide[1, :d]))
