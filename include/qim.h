@@ -395,7 +395,8 @@ int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const void *codes,
  * share: device int32 (B,), the prefix of each request (outside [0, P): none), or NULL for P = 1 (all requests on
  * it); prefix_lengths: device int32 (P,), the keys of each prefix, or NULL (all CP); lengths: device int32 (B,), the
  * own keys of each request; lengths outside the caches count as the nearest inside.  tree as in
- * qim_attention_cached, over the last S own keys.  A row that sees no key is zeros.  P <= 4096.  workspace:
+ * qim_attention_cached, over the last S own keys.  A row that sees no key is zeros.  P <= 4096.  o, (B, S, H, D) bf16, and the
+ * workspace are apart from each other and from all inputs.  workspace:
  * qim_attention_shared_workspace_bytes(B, S, CP, C, H, HK, P, share != NULL) bytes, 16-byte aligned, not shared by calls
  * that may overlap.  No reference counterpart. */
 int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, const void *pk, const void *pks, const void *pv,

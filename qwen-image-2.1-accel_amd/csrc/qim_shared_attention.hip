@@ -703,7 +703,17 @@ extern "C" int qim_attention_shared(const void *q, int64_t ldqb, int64_t ldq, co
     const SaPlan pl = sa_plan(B, S, CP, C, H, HK, P, share != nullptr);
     QIM_REQUIRE(workspace_bytes >= pl.bytes(), QIM_ERR_ARG, "%s: workspace of %lld bytes, this problem needs %lld", who,
                 (long long)workspace_bytes, (long long)pl.bytes());
-    QIM_REQUIRE(!bytes_share(o, 2 * B * S * H * D, q, 2 * ((B - 1) * ldqb + (S - 1) * ldq + H * D)), QIM_ERR_ARG, "%s: o overlaps q", who);
+    // Rows are written while others are still read, and the last launch reads lengths and workspace.
+    const struct {
+        const void *at;
+        int64_t bytes;
+    } inputs[] = {{q, 2 * ((B - 1) * ldqb + (S - 1) * ldq + H * D)}, {pk, P * CP * HK * D}, {pks, P * CP * HK * D / 32}, {pv, P * CP * HK * D},
+                  {pvs, P * CP * HK * D / 32}, {kc, B * C * HK * D}, {ks, B * C * HK * D / 32}, {vc, B * C * HK * D}, {vs, B * C * HK * D / 32},
+                  {prefix_lengths, 4 * P}, {share, 4 * B}, {lengths, 4 * B}, {tree, (B - 1) * tree_b + S * S}};
+    for (const auto &in : inputs)
+        QIM_REQUIRE(!in.at || !in.bytes || (!bytes_share(o, 2 * B * S * H * D, in.at, in.bytes) && !bytes_share(workspace, pl.bytes(), in.at, in.bytes)),
+                    QIM_ERR_ARG, "%s: o or the workspace overlaps an input", who);
+    QIM_REQUIRE(!bytes_share(o, 2 * B * S * H * D, workspace, pl.bytes()), QIM_ERR_ARG, "%s: o overlaps the workspace", who);
     uint8_t *at = static_cast<uint8_t *>(workspace);
     auto take = [&](int64_t n) {
         uint8_t *r = at;

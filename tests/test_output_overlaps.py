@@ -6,7 +6,7 @@ import torch
 from qwen_image_accel import _native
 from qwen_image_accel.kernels import elementwise
 from tests.helpers import bf16_randn
-from tests.test_few_tokens_refusals import ARG, FAR, norm
+from tests.test_few_tokens_refusals import ARG, FAR, norm, share
 
 FREE = 64 * FAR    # an address far from all others
 HO, Z = 3 * FAR, 4 * FAR
@@ -24,6 +24,33 @@ def test_residual_norm_refuses(call):
     name, args = call
     rc = getattr(_native.lib(), name)(*args)
     assert rc == ARG, (rc, _native.lib().qim_last_error())
+
+
+def attend(places, **kw):
+    """A call of qim_attention_shared whose operands lie far from each other, except for those placed here."""
+    name, args = share(**kw)
+    args = list(args)
+    for i, at in enumerate((0, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 16, 17)):
+        if args[at] is not None:
+            args[at] = (8 + 2 * i) * FAR
+    for at, value in places.items():
+        args[at] = value
+    return name, args
+
+
+Q, O, WS = 8 * FAR, (8 + 2 * 13) * FAR, (8 + 2 * 14) * FAR
+OUT = 2 * 2 * 1 * 4 * 128           # bytes of o
+CODES = 3 * 64 * 2 * 128            # of a prefix cache
+
+
+@pytest.mark.parametrize("places,kw", [
+    ({0: O}, {}), ({3: O}, {}), ({3: O - CODES + 16}, {}), ({4: O}, {}), ({4: O - CODES // 32 + 16}, {}), ({5: O + OUT - 16}, {}), ({6: O + 16}, {}),
+    ({7: O + OUT - 4}, {}), ({8: O - 4}, {}), ({9: O}, {}), ({10: O}, {}), ({11: O - 2 * 32 * 2 * 128 + 16}, {}), ({12: O + 32}, {}), ({13: O + 4}, {}),
+    ({14: O}, dict(tree=16)), ({17: O}, {}), ({16: WS + 4096}, {}), ({0: WS}, {}), ({3: WS + 256}, {}), ({13: WS + 8}, {}), ({8: WS + 512}, {})])
+def test_attention_shared_refuses(places, kw):
+    name, args = attend(places, **kw)
+    rc = getattr(_native.lib(), name)(*args)
+    assert rc == ARG and b"overlap" in _native.lib().qim_last_error(), (rc, _native.lib().qim_last_error())
 
 
 @pytest.mark.gpu
