@@ -377,7 +377,7 @@ int qim_residual_norm(const void *h, int64_t ldh, const void *x, int64_t ldx, in
 /* Products of a few rows with 4-bit weights:
  *   out[m, n] = sum_k x[m, k] W[n, k] (+ bias[n]),  or with a second weight silu(x W^T) * (x W2^T)
  * in fp32, rounded once.  x: (M, K) bf16, row stride ldx (a multiple of 8); out: (M, N) bf16, or fp32 with out_f32,
- * any row stride ldo, apart from x; bias: bf16 (N,) or NULL (none with a second weight).
+ * any row stride ldo, apart from all inputs; bias: bf16 (N,) or NULL (none with a second weight).
  * group 32, 64 or 128: W[n, k] = s (q - z) with codes q 0..15, a bf16 scale s and a zero point z (zeros NULL: 8) per
  * group of k; group 0: W[n, k] = E2M1(code) 2^(e - 127), an exponent byte e per 32 of k.  K is a multiple of the group.
  * The weight is laid out in tiles of 16 rows and steps of 128 k (N and K padded with zeros): codes (tiles, steps, 64, 16)

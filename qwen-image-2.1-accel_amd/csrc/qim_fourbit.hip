@@ -524,6 +524,16 @@ extern "C" int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const v
                 QIM_ERR_LAYOUT, "%s: rows of x must be 16-byte aligned and fewer than 2^24 elements apart", who);
     const int64_t size = out_f32 ? 4 : 2;
     QIM_REQUIRE(!bytes_share(out, size * ((M - 1) * ldo + N), x, 2 * ((M - 1) * ldx + K)), QIM_ERR_ARG, "%s: out overlaps x", who);
+    // (codes, scales or exponents, zero points: of 16 rows and 128 k)
+    const int64_t steps = (N + 15) / 16 * ((K + 127) / 128), per = group ? 128 / group : 0;
+    const struct {
+        const void *at;
+        int64_t bytes;
+    } inputs[] = {{codes, 1024 * steps}, {codes2, 1024 * steps}, {scales, (group ? 32 * per : 64) * steps}, {scales2, (group ? 32 * per : 64) * steps},
+                  {zeros, 16 * per * steps}, {zeros2, 16 * per * steps}, {bias, 2 * N}};
+    for (const auto &in : inputs)
+        QIM_REQUIRE(!rows_share_vectors(out, ldo * size / 2, N * size / 2, M, in.at, 0, 1, in.bytes / 2), QIM_ERR_ARG,
+                    "%s: out overlaps a weight or the bias", who);
     FourBitArgs a{(const uint16_t *)x, ldx,
                   {{(const uint8_t *)codes, (const uint8_t *)scales, (const uint8_t *)zeros},
                    {(const uint8_t *)codes2, (const uint8_t *)scales2, (const uint8_t *)zeros2}},

@@ -58,11 +58,12 @@ inline bool rows_share(const void *out, int64_t ldo, int64_t N, const void *t, i
     return col < N || col + W > ldo;
 }
 
-// Whether the bf16 rows of out, (M, N), share memory with n vectors of W values, `step` elements apart (0: one for all; NULL: none).
+// Whether the rows of out, (M, N), share memory with n vectors of W values, `step` elements apart (0: one for all; NULL: none); all in
+// elements of two bytes.
 inline bool rows_share_vectors(const void *out, int64_t ldo, int64_t N, int64_t M, const void *v, int64_t step, int64_t n, int64_t W) {
     if (!v) return false;
     if (step == 0) n = 1;
-    const int64_t d = (int64_t)((intptr_t)v - (intptr_t)out) / 2, end = (M - 1) * ldo + N;  // both 16-byte aligned
+    const int64_t d = (int64_t)((intptr_t)v - (intptr_t)out) / 2, end = (M - 1) * ldo + N;  // both even
     if (d >= end || -d >= (n - 1) * step + W) return false;
     for (int64_t i = 0; i < n; ++i) {
         const int64_t a = d + i * step;

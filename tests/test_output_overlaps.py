@@ -4,9 +4,9 @@ import pytest
 import torch
 
 from qwen_image_accel import _native
-from qwen_image_accel.kernels import elementwise
+from qwen_image_accel.kernels import elementwise, fourbit
 from tests.helpers import bf16_randn
-from tests.test_few_tokens_refusals import ARG, FAR, norm, share
+from tests.test_few_tokens_refusals import ARG, FAR, four, norm, share
 
 FREE = 64 * FAR    # an address far from all others
 HO, Z = 3 * FAR, 4 * FAR
@@ -51,6 +51,38 @@ def test_attention_shared_refuses(places, kw):
     name, args = attend(places, **kw)
     rc = getattr(_native.lib(), name)(*args)
     assert rc == ARG and b"overlap" in _native.lib().qim_last_error(), (rc, _native.lib().qim_last_error())
+
+
+# A weight of 100 rows and 256 k: 7 tiles of 2 steps.
+W4 = dict(m=4, n=100, k=256, ldo=100, zeros=5 * FAR, codes=6 * FAR, scales=7 * FAR)
+GATE_UP = dict(W4, codes2=8 * FAR, scales2=9 * FAR, zeros2=10 * FAR)
+
+
+@pytest.mark.parametrize("call", [
+    four(**W4 | dict(out=6 * FAR)), four(**W4 | dict(out=6 * FAR + 14 * 1024 - 16)), four(**W4 | dict(out=7 * FAR + 14 * 64 - 2)),
+    four(**W4 | dict(out=5 * FAR - 798)), four(**W4 | dict(out=5 * FAR + 14 * 32 - 16)), four(**GATE_UP | dict(out=8 * FAR)),
+    four(**GATE_UP | dict(out=9 * FAR - 2)), four(**GATE_UP | dict(out=10 * FAR)), four(**W4 | dict(bias=2 * FAR + 200)),
+    four(**W4 | dict(bias=2 * FAR + 799 - 1)), four(**W4 | dict(bias=2 * FAR - 198)), four(**W4 | dict(bias=2 * FAR + 4 * 396, ldo=300, f32=1)),
+    four(**dict(W4, zeros=None, group=0) | dict(out=7 * FAR + 14 * 64 - 2)), four(**dict(W4, group=32) | dict(out=7 * FAR + 14 * 128 - 2))])
+def test_fourbit_refuses(call):
+    name, args = call
+    rc = getattr(_native.lib(), name)(*args)
+    assert rc == ARG and b"overlap" in _native.lib().qim_last_error(), (rc, _native.lib().qim_last_error())
+
+
+@pytest.mark.gpu
+def test_a_bias_beside_the_rows_of_one_buffer(dev):
+    print("[case] bias beside rows", flush=True)
+    g = torch.Generator().manual_seed(1)
+    w = fourbit.quantize_weight(bf16_randn(g, (40, 128)).to(dev))
+    x, bias = bf16_randn(g, (6, 128)).to(dev), bf16_randn(g, (40,)).to(dev)
+    want = fourbit.matmul(x, w, bias=bias)
+    wide = torch.zeros(6, 100, dtype=torch.bfloat16, device=dev)
+    wide[3, 50:90] = bias
+    got = fourbit.matmul(x, w, bias=wide[3, 50:90], out=wide[:, 3:43])
+    assert torch.equal(got, want) and torch.equal(wide[3, 50:90], bias)
+    with pytest.raises(_native.QimError):
+        fourbit.matmul(x, w, bias=wide[3, 40:80], out=wide[:, 3:43])
 
 
 @pytest.mark.gpu
