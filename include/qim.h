@@ -384,7 +384,8 @@ int qim_residual_norm(const void *h, int64_t ldh, const void *x, int64_t ldx, in
  * bytes, where bytes 4j .. 4j + 3 of lane l hold row l % 16, k = 32 j + 8 (l / 16) + 0..7 of the step: for int4 byte i
  * holds k i in its low and k i + 4 in its high half, for E2M1 k 2i and 2i + 1; scales (tiles, steps, 4, 128 / group, 4)
  * bf16, that of row 4a + c of the tile at (a, group, c); zeros (tiles, steps, 16, 128 / group) bytes; exponents (tiles,
- * steps, 16, 4) bytes.  All 16-byte aligned; M < 2^20, N, K and ldx < 2^24.  No reference counterpart. */
+ * steps, 16, 4) bytes.  All 16-byte aligned; M < 2^20, N, K and ldx < 2^24, and a problem of fewer than 2^32 threads (some 4 * 10^10
+ * values of output, half as many with a second weight).  No reference counterpart. */
 int qim_fourbit_matmul(const void *x, int64_t ldx, int group, const void *codes, const void *scales, const void *zeros,
                        const void *codes2, const void *scales2, const void *zeros2, const void *bias, void *out,
                        int64_t ldo, int out_f32, int64_t M, int64_t N, int64_t K, void *stream);

@@ -442,13 +442,15 @@ template <int G, int NR, int WAVES, bool SWIGLU>
 static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
     using St = FtStage<G, NR, WAVES>;
     constexpr int OT = SWIGLU ? St::NT / 2 : St::NT, bytes = St::LDS;
+    const uint32_t ncol = (uint32_t)(((a.N + 15) / 16 + OT - 1) / OT);
+    const int64_t wgs = (int64_t)ncol * ((a.M + 16 * NR - 1) / (16 * NR));
+    QIM_REQUIRE(wgs * (64 * WAVES) < (1ll << 32), QIM_ERR_SHAPE, "qim_fourbit_matmul: M %d, N %d: too large", a.M, a.N);
     static std::atomic<bool> done[QIM_MAX_DEVICES];
     if (bytes > 65536) {
         const int rc = reserve_lds(reinterpret_cast<const void *>(k_fourbit_tile<G, NR, WAVES, SWIGLU>), bytes, done, "qim_fourbit_matmul");
         if (rc != QIM_OK) return rc;
     }
-    const uint32_t ncol = (uint32_t)(((a.N + 15) / 16 + OT - 1) / OT);
-    launch(k_fourbit_tile<G, NR, WAVES, SWIGLU>, dim3(ncol * (unsigned)((a.M + 16 * NR - 1) / (16 * NR))), dim3(64 * WAVES), bytes, st, a, ncol);
+    launch(k_fourbit_tile<G, NR, WAVES, SWIGLU>, dim3((unsigned)wgs), dim3(64 * WAVES), bytes, st, a, ncol);
     return QIM_OK;
 }
 

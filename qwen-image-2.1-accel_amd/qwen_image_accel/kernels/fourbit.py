@@ -218,7 +218,7 @@ def matmul(x, weight, *, bias=None, out=None, dtype=torch.bfloat16):
     """``x @ W.T (+ bias)``: x (M, K) or (B, S, K) bf16 on the GPU, rows any multiple of 8 elements apart; W a
     ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if given (any row
     stride, apart from x, weight and bias).  The weights enter exactly, sums are fp32, the result is rounded once.  Meant for up to some hundred
-    rows; it takes fewer than 2^20.  No gradient is recorded."""
+    rows; it takes fewer than 2^20, and fewer than some 4 * 10^10 values of output (half as many with ``swiglu``).  No gradient is recorded."""
     return _product("fourbit.matmul", x, weight, None, bias, out, dtype)
 
 
