@@ -20,6 +20,7 @@ import torch
 from qwen_image_accel import _native
 from qwen_image_accel.kernels.adapters import row_layout
 
+KINDS = ("int4", "mxfp4")
 GROUPS = (32, 64, 128)
 MX_GROUP = 32
 TILE, STEP = 16, 128   # rows of a weight tile, values of k of a step
@@ -123,7 +124,7 @@ def quantize_weight(w, kind="int4", group=64, *, symmetric=False):
     int4: the scale is a group's span / 15 with a zero point, or with ``symmetric`` its largest magnitude / 7; rounded to
     bf16 before the codes are taken.  mxfp4: the exponent that brings the largest magnitude to 4..8 (then at most 6), as the
     OCP MX formats define it, or the next one where that is nearer in squares.  Rows that hold infinities or NaN are refused."""
-    if kind not in ("int4", "mxfp4"):
+    if kind not in KINDS:
         raise ValueError(f"kind {kind!r}: int4 or mxfp4")
     group = MX_GROUP if kind == "mxfp4" else group
     if group not in GROUPS or w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0 or w.shape[1] % group:

@@ -12,8 +12,11 @@ from qwen_image_accel.kernels.adapters import takes_rows
 
 
 def convertible(linear, kind="int4", group=64):
-    """Whether ``linear`` becomes a FourBitLinear: in_features a multiple of the group."""
-    return isinstance(linear, nn.Linear) and linear.in_features % (fourbit.MX_GROUP if kind == "mxfp4" else group) == 0
+    """Whether ``linear`` becomes a FourBitLinear: a known kind and group, in_features a multiple of the group, a weight that is not
+    empty."""
+    group = fourbit.MX_GROUP if kind == "mxfp4" else group
+    return (kind in fourbit.KINDS and group in fourbit.GROUPS and isinstance(linear, nn.Linear) and linear.in_features % group == 0
+            and linear.weight.numel() > 0)
 
 
 class FourBitLinear(nn.Module):
@@ -69,16 +72,17 @@ class FourBitLinear(nn.Module):
 
 def quantize_linears(module, names, kind="int4", group=64, *, symmetric=False):
     """Replace the ``nn.Linear`` s of ``module`` at the given paths ("time_embed.linear_1", ...) by ``FourBitLinear`` s.
-    Returns the paths.  A path that is no convertible linear is refused before any is replaced."""
-    names = list(names)
+    Returns the paths, each once.  A path that is no convertible linear, or whose weight cannot be quantized, is refused before
+    any is replaced."""
+    names = list(dict.fromkeys(names))
     for name in names:
-        if not convertible(module.get_submodule(name), kind, group):
-            raise ValueError(f"{name} is not a linear whose in_features are a multiple of its {kind} group")
+        if not name or not convertible(module.get_submodule(name), kind, group):
+            raise ValueError(f"{name!r} is not a linear whose in_features are a multiple of its {kind} group ({group})")
     with torch.no_grad():
-        for name in names:
-            parent, _, leaf = name.rpartition(".")
-            owner = module.get_submodule(parent) if parent else module
-            setattr(owner, leaf, FourBitLinear(owner.get_submodule(leaf), kind, group, symmetric=symmetric))
+        made = [FourBitLinear(module.get_submodule(name), kind, group, symmetric=symmetric) for name in names]
+    for name, linear in zip(names, made):
+        parent, _, leaf = name.rpartition(".")
+        setattr(module.get_submodule(parent), leaf, linear)
     return names
 
 
