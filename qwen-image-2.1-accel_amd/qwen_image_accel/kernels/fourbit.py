@@ -123,15 +123,16 @@ def quantize_weight(w, kind="int4", group=64, *, symmetric=False):
 
     int4: the scale is a group's span / 15 with a zero point, or with ``symmetric`` its largest magnitude / 7; rounded to
     bf16 before the codes are taken.  mxfp4: the exponent that brings the largest magnitude to 4..8 (then at most 6), as the
-    OCP MX formats define it, or the next one where that is nearer in squares.  Rows that hold infinities or NaN are refused."""
+    OCP MX formats define it, or the next one where that is nearer in squares.  A weight that holds infinities or NaN, in fp32, is refused."""
     if kind not in KINDS:
         raise ValueError(f"kind {kind!r}: int4 or mxfp4")
     group = MX_GROUP if kind == "mxfp4" else group
     if group not in GROUPS or w.dim() != 2 or w.shape[0] == 0 or w.shape[1] == 0 or w.shape[1] % group:
         raise ValueError(f"a weight {tuple(w.shape)} in groups of {group}: (N, K), K a multiple of one of {GROUPS}")
+    w = w.detach().float()
     if not torch.isfinite(w).all():
-        raise ValueError("the weight holds infinities or NaN")
-    g = w.detach().float().unflatten(1, (-1, group))
+        raise ValueError("the weight holds infinities, NaN or values that fp32 does not")
+    g = w.unflatten(1, (-1, group))
     zeros = None
     if kind == "mxfp4":
         edges = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device=w.device)

@@ -1,8 +1,9 @@
-"""quantize_linears refuses before it replaces anything; convertible knows kinds and groups (no GPU)."""
+"""quantize_linears refuses before it replaces anything; convertible knows kinds and groups; weights of other types (no GPU)."""
 import pytest
 import torch
 from torch import nn
 
+from qwen_image_accel.kernels import fourbit
 from qwen_image_accel.optimizations.fourbit import FourBitLinear, convertible, quantize_linears
 
 
@@ -49,3 +50,13 @@ def test_convertible():
     assert all(convertible(linear, "int4", g) for g in (32, 64, 128)) and convertible(linear, "mxfp4", 7)
     assert not any(convertible(linear, "int4", g) for g in (0, -64, 16, 256)) and not convertible(linear, "nf4", 64)
     assert not convertible(nn.Linear(64, 0)) and not convertible(nn.Linear(0, 8))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(symmetric=True), dict(kind="mxfp4")])
+def test_float64_weights(kw):
+    w = torch.randn(16, 64, dtype=torch.float64, generator=torch.Generator().manual_seed(1))
+    for a, b in zip(fourbit.quantize_weight(w, **kw)[:3], fourbit.quantize_weight(w.float(), **kw)[:3]):
+        assert (a is None and b is None) or torch.equal(a, b)
+    w[3, 5] = 1e39                                            # finite, beyond fp32
+    with pytest.raises(ValueError):
+        fourbit.quantize_weight(w, **kw)
