@@ -84,7 +84,7 @@ __device__ __forceinline__ void rn_store_codes(const ResNormArgs &p, int64_t row
 
 // NV 16-byte vectors a lane; lane t holds the vectors t, t + blockDim, ...
 template <int NV, bool QUANT, bool EAGER>
-__global__ __launch_bounds__(64 * RN_MAX_WAVES) void k_residual_norm(ResNormArgs p) {
+__global__ __launch_bounds__(NV > 2 ? 256 : 64 * RN_MAX_WAVES) void k_residual_norm(ResNormArgs p) {
     __shared__ double red[2][2][RN_MAX_WAVES];
     const int tid = threadIdx.x, nthr = blockDim.x, nvec = p.D >> 3;
     const int64_t row = blockIdx.x;
@@ -247,6 +247,16 @@ static void launch_residual_norm(const ResNormArgs &a, hipStream_t st) {
     const int nvec = a.D / 8;
     const dim3 grid((unsigned)a.rows_pad);
     auto go = [&](auto fn, int nv) { launch(fn, grid, dim3(64 * ((nvec + 64 * nv - 1) / (64 * nv))), 0, st, a); };
+    // The eager form needs some 72 registers a lane: a row of more than 8 waves leaves a CU one or two workgroups, which wait at
+    // their barriers with nothing beside them.  From 4096 to 8192 values it takes four vectors a lane instead, and no more than four
+    // waves (4096 rows, us, the two separate calls, a vector a lane and four, bf16: D 4608 35.1, 38.2 and 30.7; 6144 44.7, 43.1 and
+    // 38.5; 8192 57.8, 68.1 and 50.1; MXFP8: 37.2, 37.9 and 32.6; 47.1, 44.9 and 40.5; 58.7, 67.5 and 52.3).
+    if constexpr (EAGER) {
+        if (nvec > 512 && nvec <= 1024) {
+            go(k_residual_norm<4, QUANT, EAGER>, 4);
+            return;
+        }
+    }
     if (nvec <= 64 * RN_MAX_WAVES) go(k_residual_norm<1, QUANT, EAGER>, 1);
     else go(k_residual_norm<2, QUANT, EAGER>, 2);
 }
