@@ -24,6 +24,7 @@ KINDS = ("int4", "mxfp4")
 GROUPS = (32, 64, 128)
 MX_GROUP = 32
 TILE, STEP = 16, 128   # rows of a weight tile, values of k of a step
+MAX_STRIDE = 1 << 24   # elements between rows of x that the kernels take
 
 
 class FourBitWeight(NamedTuple):
@@ -188,6 +189,9 @@ def _product(name, x, first, second, bias, out, dtype):
     lay = row_layout(x) if x.dtype == torch.bfloat16 else None
     if lay is None or lay[1] != first.width:
         refuse(f"x is a bf16 (M, {first.width}) or (B, S, {first.width}) tensor with rows one stride apart")
+    if lay[2] >= MAX_STRIDE:   # (a token of each of several long sequences; the kernels' offsets within a tile are 32-bit)
+        x = x.contiguous()
+        lay = row_layout(x)
     weights = _check_weight(name, first, device)
     if second is None:
         weights += (None, None, None)
@@ -217,8 +221,8 @@ def _product(name, x, first, second, bias, out, dtype):
 
 
 def matmul(x, weight, *, bias=None, out=None, dtype=torch.bfloat16):
-    """``x @ W.T (+ bias)``: x (M, K) or (B, S, K) bf16 on the GPU, rows any multiple of 8 elements apart; W a
-    ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if given (any row
+    """``x @ W.T (+ bias)``: x (M, K) or (B, S, K) bf16 on the GPU, rows any multiple of 8 elements apart (copied
+    if 2^24 or more); W a ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if given (any row
     stride, apart from x, weight and bias).  The weights enter exactly, sums are fp32, the result is rounded once.  Meant for up to some hundred
     rows; it takes fewer than 2^20, and fewer than some 4 * 10^10 values of output (half as many with ``swiglu``).  No gradient is recorded."""
     return _product("fourbit.matmul", x, weight, None, bias, out, dtype)
