@@ -10,7 +10,9 @@
 // E2M1 by the scaled conversion with the block's exponent; q - z by a table of the 16 E4M3 codes of 0 - z .. 15 - z (|q - z| is
 // at most 15, which 4 significand bits hold), looked up four codes at a time by v_perm, and the E4M3 conversion.  A
 // group of int4 is one to four steps of the product with an accumulator of its own, which enters the row's in fp32, times the
-// group's scale.  (Taking q for q - z and z times the sum of x away again in fp32 costs less per code and
+// group's scale.  q - z enters times 2^-11, which the last sum takes back (exact): a group's sum before its scale, up to
+// 15 * 128 times the row's largest value, then is in fp32 whatever x holds (and results below 2^-114 are off by some 2^-138).
+// (Taking q for q - z and z times the sum of x away again in fp32 costs less per code and
 // more per group and row; it also makes NaN of infinities.)
 //
 // Two kernels.  k_fourbit, few rows or few columns: the waves of a workgroup take the steps of k in turn, each for the whole
@@ -26,6 +28,8 @@ namespace qim {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr float FB_UNIT = 0x1p-11f;  // of int4's operands
 
 struct FourBitWeight {
     const uint8_t *codes, *scales, *zeros;
@@ -55,7 +59,7 @@ __device__ __forceinline__ bf16x8_t fb_int4(uint32_t w, const uint4 &t) {
         return __builtin_amdgcn_perm(__builtin_amdgcn_perm(t.w, t.z, low), __builtin_amdgcn_perm(t.y, t.x, low), half);
     };
     const uint32_t lo = look(w), hi = look(w >> 4);
-    const float s = 512.0f;
+    const float s = 512.0f * FB_UNIT;
     const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true);
     const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true);
     return bf16x8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
@@ -258,6 +262,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit(FourBitArgs p) {
         y += part[v][SWIGLU ? 2 * wave : wave][lane];
         if (SWIGLU) u += part[v][2 * wave + 1][lane];
     }
+    if (G) y *= 1.0f / FB_UNIT, u *= 1.0f / FB_UNIT;
     const int64_t n0 = ((int64_t)blockIdx.x * OT + wave) * 16 + 4 * kg;
     if (lr < 4 * RX && lr < rows && n0 < p.N) fb_store<SWIGLU>(p, row0 + lr, n0, y, u);
 }
@@ -431,6 +436,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
                 y += part[v][first][lane];
                 if (SWIGLU) u += part[v][first + NR][lane];
             }
+            if (G) y *= 1.0f / FB_UNIT, u *= 1.0f / FB_UNIT;
             const int64_t n0 = ((int64_t)col * OT + h * OP + ot) * 16 + 4 * kg;
             const int row = row0 + 16 * r + lr;
             if (row < p.M && n0 < p.N) fb_store<SWIGLU>(p, row, n0, y, u);

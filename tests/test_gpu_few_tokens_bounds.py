@@ -206,3 +206,22 @@ def test_the_ends_of_the_exponents(dev, m):
         y, e = B.four_bit(xs, *raw)
         got = fourbit.matmul(xs, fourbit.pack_weight(raw[0], raw[1], zeros=raw[2]), dtype=torch.float32)
         inside(got.double().cpu(), y, B.rounded(y, e, torch.float32), factor)
+
+
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, True), (128, False)])
+@pytest.mark.parametrize("m", [2, 16, 40, 300])
+def test_the_largest_values_of_x(dev, m, group, zeros):
+    """Rows of bf16's largest numbers, of one sign or both: a group's sum of q - z times them is far beyond fp32, the result is not."""
+    say("largest", m, group, zeros)
+    g = torch.Generator().manual_seed(m + group)
+    n, k = 100, 384
+    codes, _, z = random_weight("cpu", g, n, k, "int4", group, zeros)
+    scales = (torch.rand(n, k // group, generator=g) * 2.0 ** -20).to(torch.bfloat16)
+    x = torch.full((m, k), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16)
+    x[1::2] *= B.signs(g, x[1::2].shape).to(torch.bfloat16)
+    x = x.to(dev)
+    raw = [None if t is None else t.to(dev) for t in (codes, scales, z)]
+    y, e = B.four_bit(x, *raw)
+    w = fourbit.pack_weight(raw[0], raw[1], zeros=raw[2])
+    for dtype in (torch.float32, torch.bfloat16):
+        inside(fourbit.matmul(x, w, dtype=dtype).double().cpu(), y, B.rounded(y, e, dtype), dtype)
