@@ -366,8 +366,8 @@ enum qim_norm {
  * unrounded h_out.  With QIM_NORM_EAGER (post none, norm LAYER, alpha 1, gate and scale present): the bits of
  * qim_gated_residual followed by qim_adaln or qim_adaln_quantize on its result.  An output may be h or x
  * itself (the same rows) and is else apart from the inputs and the other output; MXFP8 outputs are apart from all.  D a
- * multiple of 8 up to 16384 (of 128 for MXFP8); strides multiples of 8, operands 16-byte aligned.  No
- * reference counterpart. */
+ * multiple of 8 up to 16384 (of 128 for MXFP8); M, for MXFP8 rounded up to 128, and seq below 2^22 and 2^31; strides
+ * multiples of 8, operands 16-byte aligned.  No reference counterpart. */
 int qim_residual_norm(const void *h, int64_t ldh, const void *x, int64_t ldx, int post, const void *post_weight,
                       float post_eps, const void *gate, int64_t gate_b, float alpha, int norm,
                       const void *norm_weight, float norm_eps, const void *scale, int64_t scale_b,

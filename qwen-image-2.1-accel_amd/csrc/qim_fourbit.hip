@@ -18,9 +18,9 @@
 // Two kernels.  k_fourbit, few rows or few columns: the waves of a workgroup take the steps of k in turn, each for the whole
 // tile of output and through a ring in LDS of its own, and join at the end; no barrier stands in the loop.  k_fourbit_tile,
 // the others: stages in LDS that eight waves share, and up to 128 rows for every operand made of codes.
-// Measured (launches from a graph): int4 g 128, 1 row, 4096 -> 12288 9.1-9.9 us, 2.6 TB/s; mxfp4, 16 rows, 12288 -> 4096 8.9 us, 2.8
-// TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 22.0 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430 TFLOP/s; mxfp4, 1024
-// rows, 4096 -> 4096 37-39 us, 900 TFLOP/s.
+// Measured (calls one behind the other; from a graph 1-3 us more): int4 g 128, 1 row, 4096 -> 12288 9.0 us, 2.9 TB/s; mxfp4, 16 rows,
+// 12288 -> 4096 9.1 us, 3.0 TB/s; int4 g 64, 24 rows, 4096 -> 12288 SwiGLU 20.8 us; int4 g 32, 154 rows, 4096 -> 12288 36 us, 430
+// TFLOP/s; mxfp4, 1024 rows, 4096 -> 4096 38.5 us, 890 TFLOP/s.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -309,8 +309,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void k_fourbit_tile(FourBitArgs p, u
     if constexpr (G > 0) {
         if (tid < 16) tables[tid] = make_uint4(fb_table(tid, 0), fb_table(tid, 4), fb_table(tid, 8), fb_table(tid, 12));
     }
-    // This wave's part of a stage: 1 KiB pieces of x, 4 rows each, and of tile j of W the codes (the first four waves) or the
-    // scales and zero points.  Rows and tiles past the last are the last, and of k past the end others come: nothing
+    // This wave's part of a stage: 1 KiB pieces of x, 4 rows each, and of tile `of` of W the codes (the first NT waves) or the
+    // scales and zero points (the others).  Rows and tiles past the last are the last, and of k past the end others come: nothing
     // multiplies with them.
     const int ntiles = (p.N + 15) / 16, of = wave % St::NT, mine = (int)col * OT + (SWIGLU ? of >> 1 : of);
     const FourBitWeight &fw = p.w[SWIGLU ? of & 1 : 0];
@@ -460,7 +460,7 @@ static int launch_fourbit_tile(const FourBitArgs &a, hipStream_t st) {
     return QIM_OK;
 }
 
-// Which kernel.  At 4096 columns of x (and alike at others) the tile kernel takes about 3.5 + 2.75 NR us for each workgroup of
+// Which kernel.  At 4096 columns of x (where the times were taken; other widths choose alike) the tile kernel takes about 3.5 + 2.75 NR us for each workgroup of
 // eight waves that a CU has to take (groups of 64 and 128, up to 80 rows: 4 + 2.2 NR), a third more where it takes one only,
 // and up to 10 us besides; the ring kernel 1.5 us and 2.75 for each of the CU's tiles of 16 x 16.  The first is held up by the
 // chain of its steps while a CU has few workgroups, the other makes operands of all codes again for every 16 rows.

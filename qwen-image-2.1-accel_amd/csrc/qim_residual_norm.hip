@@ -14,7 +14,8 @@
 // row; its lanes hold their 16-byte vectors of the row in registers from the loads to the stores, so the
 // reductions between (one for post, one for norm) cost no second read.  Measured at D 4096: 2048 rows with gate, scale and
 // shift 14 us, 4.8 TB/s; 16384 rows with a norm on both sides 109-112 us, 4.8-4.9 TB/s, of the 5.1 that a 1 GiB copy reaches;
-// 16 rows 4.1 us, a launch and two reductions.
+// 16 rows 4.1 us, a launch and two reductions.  The eager form beside the two launches that it replaces (D 4096, from a graph, bf16
+// and MXFP8): 16 rows 3.3 us for 5.2 and 3.7 for 6.0; 2048 17.1 for 18.6 and 16.8 for 18.9; 16384 98 for 109 and 99 for 108.
 #include "qim_device.h"
 #include "qim_runtime.h"
 
@@ -249,8 +250,8 @@ static void launch_residual_norm(const ResNormArgs &a, hipStream_t st) {
     auto go = [&](auto fn, int nv) { launch(fn, grid, dim3(64 * ((nvec + 64 * nv - 1) / (64 * nv))), 0, st, a); };
     // The eager form needs some 72 registers a lane: a row of more than 8 waves leaves a CU one or two workgroups, which wait at
     // their barriers with nothing beside them.  From 4096 to 8192 values it takes four vectors a lane instead, and no more than four
-    // waves (4096 rows, us, the two separate calls, a vector a lane and four, bf16: D 4608 35.1, 38.2 and 30.7; 6144 44.7, 43.1 and
-    // 38.5; 8192 57.8, 68.1 and 50.1; MXFP8: 37.2, 37.9 and 32.6; 47.1, 44.9 and 40.5; 58.7, 67.5 and 52.3).
+    // waves (4096 rows, us, the two separate calls, a vector a lane and four, bf16: D 4608 35.3, 38.2 and 30.4; 6144 44.6, 43.1 and
+    // 37.8; 8192 58.7, 68.1 and 48.3; MXFP8: 37.2, 37.9 and 32.3; 46.5, 44.9 and 40.6; 58.9, 67.5 and 51.5).
     if constexpr (EAGER) {
         if (nvec > 512 && nvec <= 1024) {
             go(k_residual_norm<4, QUANT, EAGER>, 4);

@@ -14,7 +14,9 @@
 //
 // The rows of a prefix: its requests in the order of their numbers, S * G rows each.  Which requests those are is known on
 // the device only.  Up to 64 requests and 16 prefixes every wave finds them itself, a request a lane (48 requests on 5
-// prefixes 3 us less than with a launch for it); of more, a first launch of one workgroup makes lists.
+// prefixes 3 us less than with a launch for it); of more, a first launch of one workgroup makes lists.  It looks at every
+// request for every prefix: 65 requests on 17 prefixes 3.6 us, 256 on 64 8.7, 1024 on 64 30, 1024 on 512 164, 4096 on 1024 1168,
+// which from some 512 prefixes on is as long as the attention itself (8 K/V heads, short prefixes).
 #include "qim_cache_attention.h"
 #include "qim_runtime.h"
 

@@ -80,11 +80,11 @@ def residual_norm(h, x, norm, *, gate=None, residual_scale=1.0, post=None, scale
 
         h' = h + residual_scale * gate * post(x),   z = norm(h') * scale + shift
 
-    Returns (h', z).  h, x: (B, S, D) or (M, D) bf16 on the GPU, rows any multiple of 8 elements apart, D
+    Returns (h', z).  h, x: (B, S, D) or (M, D) bf16 on the GPU, fewer than 2^22 rows any multiple of 8 elements apart, D
     a multiple of 8 up to 16384.  ``norm`` and ``post`` (None: x itself): an RMSNorm (``weight`` bf16 or
     None, ``eps``) or a LayerNorm without affine (``normalized_shape``, ``eps``); ``norm_kind`` says what counts as which, other
-    modules are refused.  ``gate``, ``scale``, ``shift``: None,
-    (B, 1, D) bf16, one vector per sequence at any stride that is a multiple of 8, or one for all, (1, 1, D) or (D,).
+    modules are refused.  ``gate``, ``scale``, ``shift``: None, (B, 1, D) bf16, one vector per sequence at any stride that is
+    a multiple of 8, or one for all, (1, 1, D) or (D,).
     ``add_one``: 1 + scale instead of scale.  z is a new bf16 tensor, or with ``quantized`` a
     ``mxfp8.Quantized`` (``tiled``: in the GEMM's layout; D a multiple of 128).  ``out``: where h' goes, by default a
     new tensor; h or x itself is fine, else it shares no rows with them, and nothing with the vectors and weights.

@@ -222,9 +222,10 @@ def _product(name, x, first, second, bias, out, dtype):
 
 def matmul(x, weight, *, bias=None, out=None, dtype=torch.bfloat16):
     """``x @ W.T (+ bias)``: x (M, K) or (B, S, K) bf16 on the GPU, rows any multiple of 8 elements apart (copied
-    if 2^24 or more); W a ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if given (any row
-    stride, apart from x, weight and bias).  The weights enter exactly, sums are fp32, the result is rounded once.  Meant for up to some hundred
-    rows; it takes fewer than 2^20, and fewer than some 4 * 10^10 values of output (half as many with ``swiglu``).  No gradient is recorded."""
+    if 2^24 or more); W a ``FourBitWeight`` (N, K); bias bf16 (N,).  Returns (..., N) of ``dtype`` (bf16 or fp32), in ``out`` if
+    given (any row stride, apart from x, weight and bias).  The weights enter exactly, sums are fp32, the result is rounded
+    once.  Meant for up to some hundred rows; it takes fewer than 2^20, and fewer than some 4 * 10^10 values of output (half as
+    many with ``swiglu``).  No gradient is recorded."""
     return _product("fourbit.matmul", x, weight, None, bias, out, dtype)
 
 
